@@ -18,6 +18,7 @@ from .sw import SoftSW, SoftSWAffine, SWResult, soft_sw, soft_sw_affine
 from .nw import NWResult, SoftNW, SoftNWAffine, soft_nw, soft_nw_affine
 from .dtw import DTWResult, SoftDTW, soft_dtw
 from .embed import embed_scores, soft_sw_embed
+from .encoder import attention, dropout_add, qk_norm_rope, relative_bucket_edges
 from . import ops
 from .engine import engine_counts, set_engine, use_engine
 
@@ -52,6 +53,7 @@ __version__ = "0.1.0"
 
 __all__ = [
     "soft_sw", "soft_sw_affine", "SWResult", "SoftSW", "SoftSWAffine", "ops", "embed_scores", "soft_sw_embed",
+    "attention", "qk_norm_rope", "dropout_add", "relative_bucket_edges",
     "soft_sw_float", "soft_sw_with_grads", "soft_sw_hvp", "soft_sw_param_jacobian", "soft_sw_backward_full",
     "soft_sw_affine_float", "soft_sw_affine_with_grads", "soft_sw_affine_hvp", "soft_sw_affine_param_jacobian",
     "soft_sw_affine_backward_full", "engine_counts", "set_engine", "use_engine",

@@ -1,0 +1,62 @@
+// enc_attn.cuh -- the arguments of an attention call as the kernels take them,
+// and the bucket of a relative position.
+#pragma once
+#include "enc_common.cuh"
+
+namespace d2pb {
+namespace enc {
+
+constexpr int kMaxEdges = 63;
+constexpr int kMaxReach = 1024;   // largest bucket edge: past it a side's last bucket is one constant
+
+struct Edges {
+    int n;                        // edges of one side; that side has n + 1 buckets
+    int two;                      // keys after the query take the second half of the buckets
+    int e[kMaxEdges];
+};
+
+struct AttnArgs {
+    const void *q, *k, *v;
+    long long qs[3], ks[3], vs[3];
+    const void* bias;
+    int bias_f32;
+    Edges edges;
+    const int* lengths;
+    int B, Lq, Lk, H, Hkv, D, causal;
+    float scale;                  // of the natural scores
+};
+
+__device__ __forceinline__ int bucket_of(const Edges& e, int d) {
+    const int n = e.two ? abs(d) : max(-d, 0);
+    int lo = 0, hi = e.n;         // the number of edges <= n
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (e.e[mid] <= n) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo + ((e.two && d > 0) ? e.n + 1 : 0);
+}
+__device__ __forceinline__ int n_buckets(const Edges& e) { return (e.n + 1) << e.two; }
+
+// bias of a bucket in base-2 units.  Finite values are held within 1e30 so that
+// a row of lowest values stays a row of equal finite scores
+template <class T>
+__device__ __forceinline__ float bias_log2(const AttnArgs& a, int bucket, int h) {
+    const size_t at = (size_t)bucket * a.H + h;
+    const float b = a.bias_f32 ? ((const float*)a.bias)[at] : to_f<T>(((const T*)a.bias)[at]);
+    return fabsf(b) < INFINITY ? fminf(fmaxf(b, -1e30f), 1e30f) * kLog2e : b;
+}
+
+__device__ __forceinline__ void problem_lengths(const AttnArgs& a, int b, int* lq, int* lk) {
+    *lq = a.Lq, *lk = a.Lk;
+    if (a.lengths) {
+        *lq = min(max(a.lengths[2 * b], 0), a.Lq);
+        *lk = min(max(a.lengths[2 * b + 1], 0), a.Lk);
+    }
+}
+
+// checks of the C entry points; fills *a
+int attn_args(const d2p_attention_args* p, AttnArgs* a);
+
+}  // namespace enc
+}  // namespace d2pb

@@ -970,13 +970,246 @@ Tensor embed_grad_scores_cuda(const Tensor& marginals, const Tensor& grad_value,
     return out;
 }
 
+// =============================================================================
+// encoder operators (no reference counterpart): attention with a bucketed
+// relative position bias and its gradients, head norms with the position
+// rotation, dropout with the residual
+// =============================================================================
+int enc_dtype(const Tensor& t, const char* what, bool f32) {
+    if (t.scalar_type() == at::kBFloat16) return D2P_DTYPE_BF16;
+    if (t.scalar_type() == at::kHalf) return D2P_DTYPE_F16;
+    TORCH_CHECK(f32 && t.scalar_type() == at::kFloat, what, ": unsupported dtype ", t.scalar_type());
+    return D2P_DTYPE_F32;
+}
+
+// a tensor at a 16-byte boundary (views into a larger buffer may be off one)
+Tensor at_16(const Tensor& t) {
+    return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) ? t.clone(at::MemoryFormat::Contiguous) : t;
+}
+Tensor packed16(const Tensor& t) { return at_16(t.contiguous()); }
+
+// [B, L, heads, D] rows the kernels can read in place: the last axis
+// contiguous, the other strides positive whole 16-byte units; else a copy
+Tensor rows16(const Tensor& t) {
+    const int64_t unit = 16 / t.element_size();
+    bool ok = (t.size(3) == 1 || t.stride(3) == 1);
+    for (int i = 0; i < 3; ++i)
+        ok = ok && (t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % unit == 0 && t.stride(i) < (int64_t(1) << 36)));
+    return ok ? at_16(t) : packed16(t);
+}
+void strides_of(const Tensor& t, long long* s) {   // of an axis of one element: any valid stride
+    const long long dense[3] = {t.size(1) * t.size(2) * t.size(3), t.size(2) * t.size(3), t.size(3)};
+    for (int i = 0; i < 3; ++i) s[i] = t.size(i) > 1 ? t.stride(i) : dense[i];
+}
+
+struct Attn {
+    d2p_attention_args a{};
+    Tensor q, k, v, bias, lengths;
+    std::vector<int> edges;
+};
+
+void attn_fill(Attn& f, const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& bias,
+               const c10::optional<Tensor>& lengths, at::IntArrayRef edges, double scale, bool causal) {
+    TORCH_CHECK(q.is_cuda() && k.is_cuda() && v.is_cuda(), "attention: q, k and v must be CUDA tensors");
+    TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && v.dim() == 4, "attention: q must be [B, Lq, H, D], k and v [B, Lk, Hkv, D]");
+    TORCH_CHECK(k.sizes() == v.sizes() && q.size(0) == k.size(0) && q.size(3) == k.size(3),
+                "attention: q must be [B, Lq, H, D], k and v [B, Lk, Hkv, D]");
+    TORCH_CHECK(q.scalar_type() == k.scalar_type() && q.scalar_type() == v.scalar_type(),
+                "attention: q, k and v must have the same dtype");
+    TORCH_CHECK(q.device() == k.device() && q.device() == v.device(), "attention: q, k and v must be on the same device");
+    TORCH_CHECK(k.size(2) > 0 && q.size(2) > 0 && q.size(2) % k.size(2) == 0,
+                "attention: the heads of q must be a multiple of those of k and v");
+    TORCH_CHECK(q.size(3) >= 8 && q.size(3) <= 128 && q.size(3) % 8 == 0,
+                "attention: the head size must be a multiple of 8, at most 128, got ", q.size(3));
+    d2p_attention_args& a = f.a;
+    a.dtype = enc_dtype(q, "attention", false);
+    a.B = checked_dim(q.size(0), "attention batch"), a.Lq = checked_dim(q.size(1), "attention Lq");
+    a.Lk = checked_dim(k.size(1), "attention Lk"), a.H = checked_dim(q.size(2), "attention heads");
+    a.Hkv = (int)k.size(2), a.D = (int)q.size(3);
+    a.causal = causal, a.scale = (float)scale;
+    f.q = rows16(q), f.k = rows16(k), f.v = rows16(v);
+    a.q = f.q.data_ptr(), a.k = f.k.data_ptr(), a.v = f.v.data_ptr();
+    strides_of(f.q, a.q_stride), strides_of(f.k, a.k_stride), strides_of(f.v, a.v_stride);
+    if (bias.has_value() && bias->defined()) {
+        const int64_t nb = (int64_t)(edges.size() + 1) * (causal ? 1 : 2);
+        TORCH_CHECK(bias->device() == q.device(), "attention: bias must be on the same device as q");
+        TORCH_CHECK(bias->dim() == 2 && bias->size(0) == nb && bias->size(1) == q.size(2),
+                    "attention: bias must be [", nb, ", ", q.size(2), "], got ", bias->sizes());
+        f.bias = bias->contiguous();
+        a.bias_dtype = enc_dtype(f.bias, "attention bias", true);
+        TORCH_CHECK(a.bias_dtype == D2P_DTYPE_F32 || a.bias_dtype == a.dtype, "attention: bias must be float32 or of q's dtype");
+        a.bias = f.bias.data_ptr();
+        f.edges.assign(edges.begin(), edges.end());
+        a.bucket_edges = f.edges.data(), a.n_edges = (int)f.edges.size();
+    }
+    if (lengths.has_value() && lengths->defined()) {
+        TORCH_CHECK(lengths->device() == q.device(), "attention: lengths must be on the same device as q");
+        TORCH_CHECK(lengths->scalar_type() == at::kInt && lengths->dim() == 2 && lengths->size(0) == q.size(0) &&
+                        lengths->size(1) == 2,
+                    "attention: lengths must be int32 [B, 2]");
+        f.lengths = lengths->contiguous();
+        a.lengths = f.lengths.data_ptr<int>();
+    }
+}
+
+std::tuple<Tensor, Tensor> attention_forward_cuda(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                  const c10::optional<Tensor>& bias, const c10::optional<Tensor>& lengths,
+                                                  at::IntArrayRef edges, double scale, bool causal, bool want_lse) {
+    TORCH_CHECK(q.is_cuda(), "attention: q, k and v must be CUDA tensors");
+    const c10::cuda::CUDAGuard guard(q.device());
+    Attn f;
+    attn_fill(f, q, k, v, bias, lengths, edges, scale, causal);
+    Tensor out = torch::empty({q.size(0), q.size(1), q.size(2), q.size(3)}, q.options());
+    Tensor lse = torch::empty({want_lse ? q.size(0) : 0, q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    check_rc(d2p_attention_forward(&f.a, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, cur_stream()),
+             "d2p_attention_forward");
+    return {out, lse};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(
+    const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& bias,
+    const c10::optional<Tensor>& lengths, at::IntArrayRef edges, double scale, bool causal, const Tensor& out,
+    const Tensor& lse, bool want_bias) {
+    TORCH_CHECK(q.is_cuda(), "attention: q, k and v must be CUDA tensors");
+    const c10::cuda::CUDAGuard guard(q.device());
+    Attn f;
+    attn_fill(f, q, k, v, bias, lengths, edges, scale, causal);
+    for (const Tensor* t : {&grad, &out})
+        TORCH_CHECK(t->sizes() == q.sizes() && t->scalar_type() == q.scalar_type() && t->device() == q.device(),
+                    "attention_backward: grad and out must have q's shape, dtype and device");
+    TORCH_CHECK(lse.scalar_type() == at::kFloat && lse.device() == q.device() && lse.dim() == 3 &&
+                    lse.size(0) == q.size(0) && lse.size(1) == q.size(2) && lse.size(2) == q.size(1),
+                "attention_backward: lse must be the forward's fp32 [B, H, Lq]");
+    TORCH_CHECK(!want_bias || f.bias.defined(), "attention_backward: no bias to take the gradient of");
+    const Tensor g = packed16(grad), o = packed16(out), L = lse.contiguous();
+    Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
+    Tensor dv = torch::empty(v.sizes(), v.options());
+    Tensor db = want_bias ? torch::empty(f.bias.sizes(), f.bias.options()) : torch::empty({0, 0}, q.options());
+    const size_t n = d2p_attention_backward_workspace_bytes(&f.a, want_bias);
+    TORCH_CHECK(n != static_cast<size_t>(-1), "attention_backward: problem not supported");
+    Tensor ws = torch::empty({static_cast<int64_t>(n > 0 ? n : 1)}, q.options().dtype(at::kByte));
+    check_rc(d2p_attention_backward(&f.a, o.data_ptr(), L.data_ptr<float>(), g.data_ptr(), dq.data_ptr(), dk.data_ptr(),
+                                    dv.data_ptr(), want_bias ? db.data_ptr() : nullptr, ws.data_ptr(), n, cur_stream()),
+             "d2p_attention_backward");
+    return {dq, dk, dv, db};
+}
+
+struct NormRope {
+    d2p_norm_rope_args a{};
+    Tensor q, k, qw, kw, cos, sin, pos;
+};
+void norm_rope_fill(NormRope& f, const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw, const Tensor& cos,
+                    const Tensor& sin, const c10::optional<Tensor>& positions, double eps) {
+    TORCH_CHECK(q.is_cuda() && k.is_cuda() && qw.is_cuda() && kw.is_cuda() && cos.is_cuda() && sin.is_cuda(),
+                "qk_norm_rope: all tensors must be CUDA tensors");
+    TORCH_CHECK(q.dim() == 4 && k.dim() == 4 && q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3),
+                "qk_norm_rope: q must be [B, L, H, D] and k [B, L, Hkv, D]");
+    TORCH_CHECK(q.scalar_type() == k.scalar_type(), "qk_norm_rope: q and k must have the same dtype");
+    for (const Tensor* t : {&k, &qw, &kw, &cos, &sin})
+        TORCH_CHECK(t->device() == q.device(), "qk_norm_rope: all tensors must be on the same device");
+    const int64_t D = q.size(3);
+    TORCH_CHECK(D >= 16 && D <= 256 && D % 16 == 0, "qk_norm_rope: the head size must be a multiple of 16, at most 256, got ", D);
+    TORCH_CHECK(qw.dim() == 1 && kw.dim() == 1 && qw.size(0) == D && kw.size(0) == D, "qk_norm_rope: weights must be [D]");
+    TORCH_CHECK(qw.scalar_type() == kw.scalar_type() && (qw.scalar_type() == at::kFloat || qw.scalar_type() == q.scalar_type()),
+                "qk_norm_rope: weights must both be float32 or of q's dtype");
+    TORCH_CHECK(cos.dim() == 2 && cos.sizes() == sin.sizes() && cos.scalar_type() == at::kFloat && sin.scalar_type() == at::kFloat,
+                "qk_norm_rope: cos and sin must be float32 [P, R / 2]");
+    TORCH_CHECK(2 * cos.size(1) <= D && cos.size(1) % 8 == 0, "qk_norm_rope: 2 * cos.shape[1] must be a multiple of 16, at most D");
+    d2p_norm_rope_args& a = f.a;
+    a.dtype = enc_dtype(q, "qk_norm_rope", true), a.weight_dtype = enc_dtype(qw, "qk_norm_rope weights", true);
+    a.B = checked_dim(q.size(0), "qk_norm_rope batch"), a.L = checked_dim(q.size(1), "qk_norm_rope L");
+    a.H = checked_dim(q.size(2), "qk_norm_rope heads"), a.Hkv = checked_dim(k.size(2), "qk_norm_rope key heads");
+    a.D = (int)D, a.R = (int)(2 * cos.size(1)), a.P = checked_dim(cos.size(0), "qk_norm_rope table"), a.eps = (float)eps;
+    f.q = rows16(q), f.k = rows16(k), f.qw = packed16(qw), f.kw = packed16(kw), f.cos = packed16(cos), f.sin = packed16(sin);
+    a.q = f.q.data_ptr(), a.k = f.k.data_ptr(), a.q_weight = f.qw.data_ptr(), a.k_weight = f.kw.data_ptr();
+    a.cos = f.cos.data_ptr<float>(), a.sin = f.sin.data_ptr<float>();
+    strides_of(f.q, a.q_stride), strides_of(f.k, a.k_stride);
+    if (positions.has_value() && positions->defined()) {
+        const Tensor& p = *positions;
+        TORCH_CHECK(p.device() == q.device() && (p.scalar_type() == at::kInt || p.scalar_type() == at::kLong),
+                    "qk_norm_rope: positions must be int32 or int64 on q's device");
+        TORCH_CHECK((p.dim() == 2 && p.size(0) == q.size(0) && p.size(1) == q.size(1)) || (p.dim() == 1 && p.size(0) == q.size(1)),
+                    "qk_norm_rope: positions must be [B, L] or [L]");
+        TORCH_CHECK(a.P > 0 || a.R == 0, "qk_norm_rope: cos and sin have no rows");
+        f.pos = p.contiguous();
+        a.positions = f.pos.data_ptr(), a.positions_int64 = p.scalar_type() == at::kLong;
+        a.position_batch_stride = p.dim() == 2 ? p.size(1) : 0;
+    } else {
+        TORCH_CHECK(a.R == 0 || a.L <= a.P, "qk_norm_rope: L = ", a.L, " positions but cos and sin have ", a.P, " rows");
+    }
+}
+
+std::tuple<Tensor, Tensor> qk_norm_rope_cuda(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
+                                             const Tensor& cos, const Tensor& sin, const c10::optional<Tensor>& positions,
+                                             double eps) {
+    TORCH_CHECK(q.is_cuda(), "qk_norm_rope: all tensors must be CUDA tensors");
+    const c10::cuda::CUDAGuard guard(q.device());
+    NormRope f;
+    norm_rope_fill(f, q, k, qw, kw, cos, sin, positions, eps);
+    Tensor yq = torch::empty(q.sizes(), q.options()), yk = torch::empty(k.sizes(), k.options());
+    check_rc(d2p_norm_rope_forward(&f.a, yq.data_ptr(), yk.data_ptr(), cur_stream()), "d2p_norm_rope_forward");
+    return {yq, yk};
+}
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rope_backward_cuda(
+    const Tensor& gq, const Tensor& gk, const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
+    const Tensor& cos, const Tensor& sin, const c10::optional<Tensor>& positions, double eps) {
+    TORCH_CHECK(q.is_cuda(), "qk_norm_rope: all tensors must be CUDA tensors");
+    const c10::cuda::CUDAGuard guard(q.device());
+    NormRope f;
+    norm_rope_fill(f, q, k, qw, kw, cos, sin, positions, eps);
+    TORCH_CHECK(gq.sizes() == q.sizes() && gk.sizes() == k.sizes() && gq.scalar_type() == q.scalar_type() &&
+                    gk.scalar_type() == q.scalar_type() && gq.device() == q.device() && gk.device() == q.device(),
+                "qk_norm_rope_backward: gradients must have the shape, dtype and device of q and k");
+    const Tensor g0 = packed16(gq), g1 = packed16(gk);
+    Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
+    Tensor dqw = torch::empty(qw.sizes(), qw.options()), dkw = torch::empty(kw.sizes(), kw.options());
+    const size_t n = d2p_norm_rope_workspace_bytes(&f.a);
+    TORCH_CHECK(n != static_cast<size_t>(-1), "qk_norm_rope_backward: problem not supported");
+    Tensor ws = torch::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte));
+    check_rc(d2p_norm_rope_backward(&f.a, g0.data_ptr(), g1.data_ptr(), dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(),
+                                    dkw.data_ptr(), ws.data_ptr(), n, cur_stream()),
+             "d2p_norm_rope_backward");
+    return {dq, dk, dqw, dkw};
+}
+
+Tensor dropout_add_cuda(const Tensor& x, const c10::optional<Tensor>& residual, double p, int64_t seed, int64_t offset) {
+    TORCH_CHECK(x.is_cuda(), "dropout_add: x must be a CUDA tensor");
+    TORCH_CHECK(p >= 0.0 && p < 1.0, "dropout_add: p must be in [0, 1), got ", p);
+    const int dt = enc_dtype(x, "dropout_add", true);
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor xc = x.contiguous();
+    Tensor rc;
+    if (residual.has_value() && residual->defined()) {
+        TORCH_CHECK(residual->sizes() == x.sizes() && residual->scalar_type() == x.scalar_type() &&
+                        residual->device() == x.device(),
+                    "dropout_add: residual must have x's shape, dtype and device");
+        rc = residual->contiguous();
+    }
+    Tensor y = torch::empty(x.sizes(), x.options());
+    check_rc(d2p_dropout_add(xc.data_ptr(), rc.defined() ? rc.data_ptr() : nullptr, dt, (unsigned long long)x.numel(), p,
+                             (unsigned long long)seed, (unsigned long long)offset, y.data_ptr(), cur_stream()),
+             "d2p_dropout_add");
+    return y;
+}
+
 TORCH_LIBRARY_FRAGMENT(d2p_b200, m) {
     m.def("embed_scores(Tensor x, Tensor y, float scale) -> Tensor");
     m.def("embed_grad_scores(Tensor marginals, Tensor grad_value, float scale) -> Tensor");
+    m.def("attention_forward(Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal, bool want_lse) -> (Tensor, Tensor)");
+    m.def("attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal, Tensor out, Tensor lse, bool want_bias) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("qk_norm_rope(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor)");
+    m.def("qk_norm_rope_backward(Tensor grad_q, Tensor grad_k, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("dropout_add(Tensor x, Tensor? residual, float p, int seed, int offset) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(d2p_b200, CUDA, m) {
     m.impl("embed_scores", embed_scores_cuda);
     m.impl("embed_grad_scores", embed_grad_scores_cuda);
+    m.impl("attention_forward", attention_forward_cuda);
+    m.impl("attention_backward", attention_backward_cuda);
+    m.impl("qk_norm_rope", qk_norm_rope_cuda);
+    m.impl("qk_norm_rope_backward", qk_norm_rope_backward_cuda);
+    m.impl("dropout_add", dropout_add_cuda);
 }
 
 TORCH_LIBRARY_FRAGMENT(d2p, m) {

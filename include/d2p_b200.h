@@ -46,6 +46,7 @@ extern "C" {
 
 #define D2P_DTYPE_F32 0
 #define D2P_DTYPE_BF16 1
+#define D2P_DTYPE_F16 2
 
 #define D2P_FAMILY_LINEAR 0
 #define D2P_FAMILY_AFFINE 1
@@ -301,6 +302,88 @@ D2P_API int d2p_embed_scores(const void* x, const void* y, int B, int L1, int L2
  * d2p_embed_scores). */
 D2P_API int d2p_embed_grad_scores(const float* marginals, const float* grad_value, int B, int L1, int L2, float scale,
                                   void* grad_scores_bf16, void* stream);
+
+/* ---- Encoder operators: what a network in front of the alignment runs to make
+ * its embeddings.  No operator of the reference corresponds (it takes the score
+ * plane as input, d2p/sw.py:247). ---- */
+
+/* Attention over a ragged batch.  q [B, Lq, H, D], k and v [B, Lk, Hkv, D] with
+ * element strides of batch, position and head (the last axis contiguous; base
+ * addresses and strides whole 16-byte units), bf16 or fp16; D a multiple of 8,
+ * at most 128; H a multiple of Hkv (query head h reads key head h / (H / Hkv)).
+ * lengths [B, 2] int32 (lq, lk), clamped to [0, Lq] x [0, Lk], or NULL.
+ * Query i stands at position i, or i + lk - lq when causal; with d = j - that
+ * position, key j is allowed where i < lq, j < lk and (not causal or d <= 0), and
+ *   score = scale q.k + bias[bucket(d), h],   out = softmax(score) v,
+ * rows with no allowed key (and rows past lq) exactly zero.  Values of q, k and v
+ * outside the lengths are never used, whatever they hold.
+ * bias [num_buckets, H] (contiguous, bias_dtype F32 or the inputs' type) or NULL.
+ * bucket_edges: host array of n_edges distances in [1, 1024], none below the one before; a
+ * distance n lies in bucket #{edges <= n} of its side.  Causal: n = max(-d, 0)
+ * and num_buckets = n_edges + 1.  Else n = |d|, num_buckets = 2 (n_edges + 1) and
+ * keys after the query (d > 0) take the second half.  n_edges at most 63. */
+typedef struct {
+    const void* q;
+    const void* k;
+    const void* v;
+    long long q_stride[3], k_stride[3], v_stride[3]; /* batch, position, head, in elements */
+    const void* bias;
+    const int* lengths;
+    const int* bucket_edges;
+    int n_edges, bias_dtype;
+    int B, Lq, Lk, H, Hkv, D;
+    int dtype; /* D2P_DTYPE_BF16 or D2P_DTYPE_F16 */
+    int causal;
+    float scale; /* positive */
+} d2p_attention_args;
+/* out [B, Lq, H, D] contiguous, the inputs' type; lse [B, H, Lq] fp32 or NULL:
+ * what the backward pass takes (log2 of the sum of exponentials, +inf in rows
+ * with no allowed key). */
+D2P_API int d2p_attention_forward(const d2p_attention_args* args, void* out, float* lse, void* stream);
+/* Gradients of the above with the probabilities recomputed: grad, out [B, Lq, H,
+ * D] contiguous, lse from the forward call; dq, dk, dv contiguous in the inputs'
+ * type (zero outside the lengths); dbias [num_buckets, H] in bias_dtype, or NULL.
+ * Deterministic: no atomics. */
+D2P_API size_t d2p_attention_backward_workspace_bytes(const d2p_attention_args* args, int want_dbias);
+D2P_API int d2p_attention_backward(const d2p_attention_args* args, const void* out, const float* lse, const void* grad,
+                                   void* dq, void* dk, void* dv, void* dbias, void* workspace, size_t workspace_bytes,
+                                   void* stream);
+
+/* RMS norms of queries and keys for each head with the position rotation.
+ * q [B, L, H, D], k [B, L, Hkv, D] with element strides of batch, position and
+ * head (last axis contiguous, 16-byte units); D a multiple of 16, at most 256.
+ * y = x / sqrt(mean(x^2) + eps) * weight, then the first R elements (R a multiple
+ * of 16) turned in pairs (d, d + R/2) by cos, sin [P, R/2] fp32 at the token's
+ * position: positions [B, L] (or [L]: position_batch_stride 0), int32 or int64,
+ * clamped to the tables, or NULL for 0 .. L - 1.  fp32, bf16 or fp16 rows;
+ * weights [D] F32 or the rows' type.  Outputs [B, L, heads, D] contiguous. */
+typedef struct {
+    const void* q;
+    const void* k;
+    long long q_stride[3], k_stride[3];
+    const void* q_weight;
+    const void* k_weight;
+    const float* cos;
+    const float* sin;
+    const void* positions;
+    long long position_batch_stride;
+    int positions_int64;
+    int P, B, L, H, Hkv, D, R;
+    int dtype, weight_dtype;
+    float eps;
+} d2p_norm_rope_args;
+D2P_API int d2p_norm_rope_forward(const d2p_norm_rope_args* args, void* q_out, void* k_out, void* stream);
+D2P_API size_t d2p_norm_rope_workspace_bytes(const d2p_norm_rope_args* args);
+D2P_API int d2p_norm_rope_backward(const d2p_norm_rope_args* args, const void* dq_out, const void* dk_out, void* dq,
+                                   void* dk, void* dq_weight, void* dk_weight, void* workspace,
+                                   size_t workspace_bytes, void* stream);
+
+/* y = residual + keep x / (1 - p) over n elements (residual may be NULL), fp32,
+ * bf16 or fp16.  Element e is kept where word e % 4 of Philox4x32-10 with counter
+ * (e / 4, offset) and key seed is at least floor(p 2^32); the backward pass is the
+ * same call on the gradient, without a residual. */
+D2P_API int d2p_dropout_add(const void* x, const void* residual, int dtype, unsigned long long n, double p,
+                            unsigned long long seed, unsigned long long offset, void* y, void* stream);
 
 /* Engine selection for the whole process (all devices): D2P_ENGINE_AUTO picks
  * per shape (the default, or what D2P_B200_ENGINE names at load: "plane",
