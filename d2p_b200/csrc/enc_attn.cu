@@ -48,35 +48,6 @@ __device__ const T* row_at(const void* p, const long long* s, int b, int l, int 
     return (const T*)p + b * s[0] + l * s[1] + h * s[2];
 }
 
-template <class T>
-__global__ void __launch_bounds__(32 * kRowWarps) attn_rows_kernel(const __grid_constant__ AttnArgs a, T* out, float* lse) {
-    const int lane = threadIdx.x & 31, i = blockIdx.x * kRowWarps + (threadIdx.x >> 5), h = blockIdx.y, b = blockIdx.z;
-    if (i >= a.Lq) return;
-    int lq, lk;
-    problem_lengths(a, b, &lq, &lk);
-    const int off = a.causal ? lk - lq : 0, kh = h / (a.H / a.Hkv);
-    const int end = i < lq ? (a.causal ? min(lk, i + off + 1) : lk) : 0;
-    Row<T> q, acc, k;
-    q.zero();
-    if (end > 0) q.load(row_at<T>(a.q, a.qs, b, i, h), a.D, lane);
-    acc.zero();
-    float m = -INFINITY, l = 0.f;
-    for (int j = 0; j < end; ++j) {
-        k.load(row_at<T>(a.k, a.ks, b, j, kh), a.D, lane);
-        float s = q.dot(k) * (a.scale * kLog2e);
-        if (a.bias) s += bias_log2<T>(a, bucket_of(a.edges, j - i - off), h);
-        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-        const float f = exp2f(m - base), p = exp2f(s - base);
-        l = l * f + p;
-        k.load(row_at<T>(a.v, a.vs, b, j, kh), a.D, lane);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) acc.v[t] = p > 0.f || p != p ? fmaf(p, k.v[t], acc.v[t] * f) : acc.v[t] * f;
-        m = mn;
-    }
-    acc.store(out + (((size_t)b * a.Lq + i) * a.H + h) * a.D, a.D, lane, l > 0.f || l != l ? 1.f / l : 0.f);
-    if (lse && lane == 0) lse[((size_t)b * a.H + h) * a.Lq + i] = l > 0.f || l != l ? m + log2f(l) : INFINITY;
-}
-
 // dq, delta and the row block's bucket sums
 template <class T>
 __global__ void __launch_bounds__(32 * kRowWarps) attn_dq_rows_kernel(const __grid_constant__ AttnArgs a, const T* out,
@@ -204,12 +175,6 @@ int attn_args(const d2p_attention_args* p, AttnArgs* a) {
 
 int row_blocks(int n) { return (n + kRowWarps - 1) / kRowWarps; }
 
-template <class T>
-int launch_forward(const AttnArgs& a, void* out, float* lse, cudaStream_t st) {
-    attn_rows_kernel<T><<<dim3(row_blocks(a.Lq), a.H, a.B), 32 * kRowWarps, 0, st>>>(a, (T*)out, lse);
-    return (int)cudaGetLastError();
-}
-
 size_t delta_bytes(const AttnArgs& a) { return (((size_t)a.B * a.H * a.Lq * sizeof(float)) + 255) & ~(size_t)255; }
 size_t part_bytes(const AttnArgs& a) {
     return (size_t)((a.edges.n + 1) << a.edges.two) * a.H * a.B * row_blocks(a.Lq) * sizeof(float);
@@ -249,8 +214,8 @@ int d2p_attention_forward(const d2p_attention_args* p, void* out, float* lse, vo
     if (rc) return rc;
     if (a.B == 0 || a.Lq == 0) return D2P_OK;
     if (!out) return D2P_ERR_INVALID_ARGUMENT;
-    return p->dtype == D2P_DTYPE_BF16 ? enc::launch_forward<__nv_bfloat16>(a, out, lse, (cudaStream_t)stream)
-                                      : enc::launch_forward<__half>(a, out, lse, (cudaStream_t)stream);
+    if ((uintptr_t)out & 15) return D2P_ERR_INVALID_ARGUMENT;
+    return enc::attn_forward_tiles(a, p->dtype, out, lse, (cudaStream_t)stream);
 }
 
 size_t d2p_attention_backward_workspace_bytes(const d2p_attention_args* p, int want_dbias) {

@@ -57,6 +57,8 @@ __device__ __forceinline__ void problem_lengths(const AttnArgs& a, int b, int* l
 
 // checks of the C entry points; fills *a
 int attn_args(const d2p_attention_args* p, AttnArgs* a);
+// out and lse (or null) by tiles of 128 query rows (enc_attn_fwd.cu)
+int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st);
 
 }  // namespace enc
 }  // namespace d2pb

@@ -1,0 +1,165 @@
+// enc_tc.cuh -- the pieces the attention kernels on the fifth-generation tensor
+// cores share: bounded mbarrier waits, TMA tile copies, tcgen05 products with
+// their descriptors, and TMEM loads and stores.
+//
+// Shared tiles are rows of 64 16-bit elements (128 bytes, 128-byte swizzle); a
+// head of up to 128 elements is one or two such chunks.  Columns past the
+// head's size and rows past the tensor are zero-filled by the copy.
+#pragma once
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include "enc_attn.cuh"
+
+namespace d2pb {
+namespace enc {
+
+constexpr int kWaitLimit = 1 << 21;   // polls before a wait gives up
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// waits for the phase of the given parity; *dead is the CTA's flag that some
+// wait gave up (then every other wait ends as well)
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
+    for (int it = 0; it < kWaitLimit; ++it) {
+        uint32_t done;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        if ((it & 255) == 255 && *dead) return false;
+    }
+    *dead = 1;
+    return false;
+}
+
+// the same for a whole warp, one answer for its lanes
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* dead) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity, dead));
+}
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int x, int row, int head, int b, uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+        "[%6];" ::"r"(dst),
+        "l"((unsigned long long)tm), "r"(x), "r"(row), "r"(head), "r"(b), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma_store(const CUtensorMap* tm, int x, int row, int head, int b, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                     (unsigned long long)tm),
+                 "r"(x), "r"(row), "r"(head), "r"(b), "r"(src)
+                 : "memory");
+}
+
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, int columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t tmem, int columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// shared-memory operand, the contraction along the 128-byte rows: 8-row groups 1024 bytes apart
+__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)2 << 61);
+}
+// shared-memory operand, the contraction down the rows: 8-row groups 1024 bytes
+// apart, the next 64 elements of the other extent one chunk further
+__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t chunk_bytes) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(chunk_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+// fp32 accumulator, both operands of type T; b_rows: operand B's contraction runs down its rows
+template <class T>
+__host__ __device__ constexpr uint32_t mma_desc(int m, int n, bool b_rows);
+template <>
+__host__ __device__ constexpr uint32_t mma_desc<__nv_bfloat16>(int m, int n, bool b_rows) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (b_rows ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+template <>
+__host__ __device__ constexpr uint32_t mma_desc<__half>(int m, int n, bool b_rows) {
+    return (1u << 4) | (b_rows ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        : "memory");
+}
+
+#define ENC_R8(v, o) "r"(v[o]), "r"(v[o + 1]), "r"(v[o + 2]), "r"(v[o + 3]), "r"(v[o + 4]), "r"(v[o + 5]), "r"(v[o + 6]), "r"(v[o + 7])
+#define ENC_W8(v, o) "=r"(v[o]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]), "=r"(v[o + 7])
+// 32 columns of this warp's 32 TMEM lanes, one lane a thread
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+        "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : ENC_W8(v, 0), ENC_W8(v, 8), ENC_W8(v, 16), ENC_W8(v, 24)
+        : "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::ENC_R8(v, 0),
+        ENC_R8(v, 8), ENC_R8(v, 16), ENC_R8(v, 24), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15};" ::ENC_R8(v, 0),
+        ENC_R8(v, 8), "r"(addr)
+        : "memory");
+}
+// the values of a load are used after its wait, not before (no instruction of its own)
+#define ENC_T8(v, o) "+r"(v[o]), "+r"(v[o + 1]), "+r"(v[o + 2]), "+r"(v[o + 3]), "+r"(v[o + 4]), "+r"(v[o + 5]), "+r"(v[o + 6]), "+r"(v[o + 7])
+__device__ __forceinline__ void tmem_tie32(uint32_t* v) {
+    asm volatile("" : ENC_T8(v, 0), ENC_T8(v, 8), ENC_T8(v, 16), ENC_T8(v, 24));
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The bias by relative position of one head, in shared memory: lut[d + E + kPad]
+// for d in [-(E + kPad), E + kPad], E the largest edge, so that a tile that
+// touches |d| < E reads it without clamping (a tile's positions span < kPad)
+constexpr int kPad = 256;
+__host__ __device__ inline int lut_size(int reach) { return 2 * (reach + kPad) + 1; }
+
+// [B, L, heads, D] rows with element strides s (batch, position, head) as a 4-D
+// tensor (D, position, head, batch) in boxes of 64 elements x rows
+bool rows_map(CUtensorMap* tm, int dtype, const void* base, int B, int L, int heads, int D, const long long* s, int rows);
+
+}  // namespace enc
+}  // namespace d2pb
