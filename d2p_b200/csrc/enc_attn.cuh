@@ -59,6 +59,13 @@ __device__ __forceinline__ void problem_lengths(const AttnArgs& a, int b, int* l
 int attn_args(const d2p_attention_args* p, AttnArgs* a);
 // out and lse (or null) by tiles of 128 query rows (enc_attn_fwd.cu)
 int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st);
+// the gradients (enc_attn_bwd.cu) and their workspace
+size_t attn_backward_bytes(const AttnArgs& a, bool dbias);
+int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const float* lse, const void* grad, void* dq,
+                        void* dk, void* dv, void* dbias, void* ws, cudaStream_t st);
+// CTAs of the current device one of whose bounded waits gave up, since the library was loaded
+int attn_forward_gave_up(unsigned long long* n);
+int attn_backward_gave_up(unsigned long long* n);
 
 }  // namespace enc
 }  // namespace d2pb

@@ -24,8 +24,6 @@ struct Softmax<__half> {
     static constexpr float kShift = 8.f, kSlack = 7.f;
 };
 
-__device__ unsigned long long g_gave_up;   // CTAs one of whose waits gave up
-
 namespace fwd {
 
 constexpr int kThreads = 160;   // a softmax warpgroup and the warp that copies and multiplies
@@ -80,7 +78,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     volatile int* const dead = reinterpret_cast<volatile int*>(bars + Sh::kBars);
     uint32_t* const slot = reinterpret_cast<uint32_t*>(bars + Sh::kBars) + 1;
     float* const lut = reinterpret_cast<float*>(bars + Sh::kBars + 2);
-    const int reach = BIAS && a.edges.n ? a.edges.e[a.edges.n - 1] : 0;
+    const int reach = BIAS ? reach_of(a.edges) : 0;
 
     if (tid == 0) {
         bar_init(barQ, 1), bar_init(barS, 1), bar_init(barP, 128), bar_init(barO, 1);
@@ -302,7 +300,7 @@ int launch(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st)
     else if (!rows_map(&k, dtype, a.k, a.B, a.Lk, a.Hkv, a.D, a.ks, kRows) ||
              !rows_map(&v, dtype, a.v, a.B, a.Lk, a.Hkv, a.D, a.vs, kRows))
         return D2P_ERR_INVALID_ARGUMENT;
-    const int lut = BIAS ? lut_size(a.edges.n ? a.edges.e[a.edges.n - 1] : 0) : 0;
+    const int lut = BIAS ? lut_size(reach_of(a.edges)) : 0;
     // at least a third of the SM's shared memory: no more than two CTAs (2 x 256 TMEM columns), so no allocation waits
     size_t smem = Sh::smem(lut);
     if (smem < 80 * 1024) smem = 80 * 1024;
@@ -343,6 +341,8 @@ bool rows_map(CUtensorMap* tm, int dtype, const void* base, int B, int L, int he
               const_cast<void*>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
+
+int attn_forward_gave_up(unsigned long long* n) { return (int)cudaMemcpyFromSymbol(n, g_gave_up, sizeof(*n)); }
 
 int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st) {
     return dtype == D2P_DTYPE_BF16 ? fwd::pick<__nv_bfloat16>(a, dtype, out, lse, st) : fwd::pick<__half>(a, dtype, out, lse, st);

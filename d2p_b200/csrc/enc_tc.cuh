@@ -14,6 +14,8 @@
 namespace d2pb {
 namespace enc {
 
+static __device__ unsigned long long g_gave_up;   // CTAs one of whose waits gave up (their rows are NaN)
+
 constexpr int kWaitLimit = 1 << 21;   // polls before a wait gives up
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -155,6 +157,7 @@ __device__ __forceinline__ float ex2(float x) {
 // for d in [-(E + kPad), E + kPad], E the largest edge, so that a tile that
 // touches |d| < E reads it without clamping (a tile's positions span < kPad)
 constexpr int kPad = 256;
+__host__ __device__ inline int reach_of(const Edges& e) { return e.n ? e.e[e.n - 1] : 1; }
 __host__ __device__ inline int lut_size(int reach) { return 2 * (reach + kPad) + 1; }
 
 // [B, L, heads, D] rows with element strides s (batch, position, head) as a 4-D

@@ -348,6 +348,10 @@ D2P_API size_t d2p_attention_backward_workspace_bytes(const d2p_attention_args* 
 D2P_API int d2p_attention_backward(const d2p_attention_args* args, const void* out, const float* lse, const void* grad,
                                    void* dq, void* dk, void* dv, void* dbias, void* workspace, size_t workspace_bytes,
                                    void* stream);
+/* CTAs of the attention kernels on the current device, since the library was
+ * loaded, one of whose bounded waits gave up; the rows such a CTA owns are NaN.
+ * Synchronises with the device. */
+D2P_API int d2p_attention_gave_up(unsigned long long* n);
 
 /* RMS norms of queries and keys for each head with the position rotation.
  * q [B, L, H, D], k [B, L, Hkv, D] with element strides of batch, position and
