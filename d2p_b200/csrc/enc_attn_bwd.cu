@@ -10,17 +10,20 @@
 // owned and Y1, Y2 the streamed rows (keys pass: K, V / Q, dO; query pass: Q, dO
 // / K, V) both are
 //   S = X1 Y1^T,  dP = X2 Y2^T  (two 64-column products into TMEM),
-//   P, dS in 16 bits over S's and dP's own columns (TMEM operands A),
+//   P, dS in 16 bits over S's and dP's own columns (TMEM operands A; each half
+//   of the columns over its own, so that no warp writes what another still reads),
 //   acc1 += P Y2 (keys pass: dV),  acc2 += dS Y1 (dK or dQ).
-// S and dP are double-buffered: one warpgroup works on even tiles, one on odd,
-// while the tensor cores run the products of the other.  The scores are formed
+// S and dP are double-buffered: two warpgroups work on even tiles (32 columns
+// each), two on odd, while the tensor cores run the products of the other.  The scores are formed
 // twice (7 products a tile pair rather than 5); in exchange dQ needs no
 // cross-CTA sums, whose order would change results from run to run.
 //
 // The query pass also sums dS by relative position.  Along a diagonal of a
-// warp's 32 x 64 block the sum moves one lane per column (one shuffle each), the
-// 95 sums are scanned, and each lane takes its buckets as differences of the
+// warp's 32 x 32 block the sum moves one lane per column (one shuffle each), the
+// 63 sums are scanned, and each lane takes its buckets as differences of the
 // scan: registers only, in a fixed order.
+#include <type_traits>
+
 #include "enc_tc.cuh"
 
 namespace d2pb {
@@ -28,7 +31,8 @@ namespace enc {
 
 namespace bwd {
 
-constexpr int kThreads = 320;   // two warpgroups, the products' warp, the copies' warp
+constexpr int kWork = 512;              // four warpgroups: two for a buffer of S and dP, half of its columns each
+constexpr int kThreads = kWork + 64;    // and the products' warp and the copies' warp
 constexpr int kOwn = 128, kStep = 64;
 constexpr int kColumns = 512;   // TMEM: S 2 x 64, dP 2 x 64, two accumulators of up to 128
 constexpr int kChunkX = kOwn * 128, kChunkY = kStep * 128;
@@ -44,11 +48,11 @@ struct Shape {
     static constexpr int kBars = 2 + 2 * kStages + 4;
     static constexpr size_t fixed() { return 1024 + 2 * (size_t)kX + (size_t)kStages * kStage + kBars * 8 + 16; }
 };
-// after the tiles: the bias by position (keys pass: one for each warpgroup, whose tiles may be of two heads), then
+// after the tiles: the bias by position (keys pass: one for each buffer, whose tiles may be of two heads), then
 // (query pass) the diagonals' stage of each warp and the buckets' ranges
 __host__ __device__ inline size_t extra(bool bias, bool dkv, int reach) {
     if (!bias) return 0;
-    return 4 * (size_t)lut_size(reach) * (dkv ? 2 : 1) + (dkv ? 0 : 4 * (size_t)(8 * 100 + 8 * kBuckets + 2 * kBuckets));
+    return 4 * (size_t)lut_size(reach) * (dkv ? 2 : 1) + (dkv ? 0 : 4 * (size_t)(16 * 72 + 16 * kBuckets + 2 * kBuckets));
 }
 // at least 116 KB: one CTA an SM, since it takes the whole TMEM (no allocation waits)
 template <int DP>
@@ -118,19 +122,19 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t* const slot = reinterpret_cast<uint32_t*>(bars + Sh::kBars) + 1;
     float* lut = reinterpret_cast<float*>(bars + Sh::kBars + 2);
     const int reach = BIAS ? reach_of(a.edges) : 0;
-    float* const diag = lut + lut_size(reach);               // [8][100] a warp's diagonals, scanned in place
-    float* const red = diag + 8 * 100;                       // [8][kBuckets]
-    int* const range = reinterpret_cast<int*>(red + 8 * kBuckets);   // [kBuckets][2] positions of a bucket
+    float* const diag = lut + lut_size(reach);                        // [16][72] a warp's diagonals, scanned in place
+    float* const red = diag + 16 * 72;                                // [16][kBuckets]
+    int* const range = reinterpret_cast<int*>(red + 16 * kBuckets);   // [kBuckets][2] positions of a bucket
     const bool sums = !DKV && BIAS && g.part;
 
     if (tid == 0) {
         bar_init(barX, 1), bar_init(barF, 1);
         for (int s = 0; s < NST; ++s) bar_init(barY + 8 * s, 1), bar_init(barE + 8 * s, 1);
-        for (int s = 0; s < 2; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 128);
+        for (int s = 0; s < 2; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 256);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *dead = 0;
     }
-    if (warp == 8) tmem_alloc(smem_addr(slot), kColumns);
+    if (warp == kWork / 32) tmem_alloc(smem_addr(slot), kColumns);
     if (BIAS && !DKV) {
         for (int i = tid; i < lut_size(reach); i += kThreads) lut[i] = bias_log2<T>(a, bucket_of(a.edges, i - reach - kPad), hx);
         if (sums)
@@ -146,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *slot, tA1 = tmem + 256, tA2 = tmem + 384;
 
-    if (warp == 9) {   // copies
+    if (warp == kWork / 32 + 1) {   // copies
         if (lane == 0) {
             auto copy = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, uint32_t bar, int chunk) {
 #pragma unroll
@@ -183,7 +187,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         __syncwarp();
-    } else if (warp == 8) {   // products
+    } else if (warp == kWork / 32) {   // products
         if (lane == 0) {
             constexpr uint32_t idS = mma_desc<T>(128, kStep, false), idA = mma_desc<T>(128, DP, true);
             auto scores = [&](int it) {
@@ -213,11 +217,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (DKV) {
 #pragma unroll
                     for (int k = 0; k < kStep / 16; ++k)
-                        mma_ts(tA1, p + 8 * k, desc_mn(y + Sh::kY + k * 2048, kChunkY), idA, (it | k) != 0);
+                        mma_ts(tA1, p + 32 * (k / 2) + 8 * (k % 2), desc_mn(y + Sh::kY + k * 2048, kChunkY), idA, (it | k) != 0);
                 }
 #pragma unroll
                 for (int k = 0; k < kStep / 16; ++k)
-                    mma_ts(tA2, p + 128 + 8 * k, desc_mn(y + k * 2048, kChunkY), idA, (it | k) != 0);
+                    mma_ts(tA2, p + 128 + 32 * (k / 2) + 8 * (k % 2), desc_mn(y + k * 2048, kChunkY), idA, (it | k) != 0);
                 tc_commit(barE + 8 * s);
                 if (it + 2 < n) ok = scores(it + 2);
             }
@@ -225,64 +229,67 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) atomicAdd(&g_gave_up, 1ull);
         }
         __syncwarp();
-    } else {   // two warpgroups: P and dS of even and odd tiles
-        const int wg = warp >> 2, r = tid & 127, x = x0 + r;
-        const uint32_t trow = (uint32_t)(32 * (warp & 3)) << 16;
+    } else {   // P and dS of a tile
+        const int buf = warp >> 3, half = (warp >> 2) & 1, w4 = warp & 3, r = tid & 127, x = x0 + r;
+        const uint32_t trow = (uint32_t)(32 * w4) << 16;
         const float c = a.scale * kLog2e;
         float rl = 0.f, rd = 0.f;
         if (!DKV) {
             const size_t at = ((size_t)b * a.H + hx) * g.Lp + x;   // Lp covers the tile
             rl = g.lse[at], rd = g.delta[at];
         }
-        float far[2] = {0.f, 0.f}, bsum[kBuckets / 32];
+        float far0 = 0.f, far1 = 0.f, bsum[kBuckets / 32];
 #pragma unroll
         for (int i = 0; i < kBuckets / 32; ++i) bsum[i] = 0.f;
         bool ok = true;
-        int filled = -1;   // keys pass: the head of the group whose bias is in the warpgroup's lut
-        if (BIAS && DKV && wg) lut += lut_size(reach);
-        for (int it = wg; it < n; it += 2) {
+        int filled = -1;   // keys pass: the head of the group whose bias is in the buffer's lut
+        if (BIAS && DKV && buf) lut += lut_size(reach);
+        float* const dw = diag + warp * 72;
+        for (int it = buf; it < n; it += 2) {
             const int s = it % NST, yb = y0 + (it % per) * kStep;
             if (BIAS && DKV && it / per != filled) {
                 filled = it / per;
-                asm volatile("bar.sync %0, 128;" ::"r"(3 + wg) : "memory");   // the last tile's reads are over
-                for (int i = r; i < lut_size(reach); i += 128)
+                asm volatile("bar.sync %0, 256;" ::"r"(3 + buf) : "memory");   // the last tile's reads are over
+                for (int i = tid & 255; i < lut_size(reach); i += 256)
                     lut[i] = bias_log2<T>(a, bucket_of(a.edges, i - reach - kPad), hx * group + filled);
-                asm volatile("bar.sync %0, 128;" ::"r"(3 + wg) : "memory");
+                asm volatile("bar.sync %0, 256;" ::"r"(3 + buf) : "memory");
             }
-            // (after a wait that gave up a warp still meets its warpgroup at the barriers above)
-            ok = ok && bar_wait_warp(barS + 8 * wg, (it >> 1) & 1, dead) && bar_wait_warp(barY + 8 * s, (it / NST) & 1, dead);
+            // (after a wait that gave up a warp still meets its partners at the barriers above)
+            ok = ok && bar_wait_warp(barS + 8 * buf, (it >> 1) & 1, dead) && bar_wait_warp(barY + 8 * s, (it / NST) & 1, dead);
             if (!ok) continue;
             tc_fence_after();
-            const uint32_t tS = tmem + trow + wg * kStep, tD = tS + 128;
-            const float* const st = reinterpret_cast<const float*>(gb + 2 * Sh::kX + s * Sh::kStage + 2 * Sh::kY);
-            // d of the tile's corner: key - position of query, of row r and column 0, then +-1 a column
-            const int d0 = DKV ? x - (yb + off) : yb - (x + off);
-            const int lo = DKV ? x0 - (yb + kStep - 1 + off) : yb - (x0 + kOwn - 1 + off), hi = lo + kOwn + kStep - 2;
+            const int col0 = 32 * half, yc = yb + col0;
+            const uint32_t tS = tmem + trow + buf * kStep, tD = tS + 128;
+            const float* const st = reinterpret_cast<const float*>(gb + 2 * Sh::kX + s * Sh::kStage + 2 * Sh::kY) + col0;
+            // d = key position - query position of this row and the block's first column; a column is one less or one more
+            const int d0 = DKV ? x - (yc + off) : yc - (x + off);
+            // the range of d in the warp's block of 32 x 32
+            const int lo = DKV ? x0 + 32 * w4 - (yc + 31 + off) : yc - (x0 + 32 * w4 + 31 + off), hi = lo + 62;
             const bool near = BIAS && lo < reach && hi > -reach;
-            const float* const lp = lut + (d0 + reach + kPad);
-            const float flat = BIAS ? (lo >= reach ? lut[lut_size(reach) - 1] : lut[0]) : 0.f;
             // columns this row meets: [c0, c1)
-            const bool edge = yb + kStep > ly || x0 + kOwn > lx || (a.causal && hi > 0);
-            int c0 = 0, c1 = x < lx ? min(kStep, ly - yb) : 0;
+            int c0 = 0, c1 = x < lx ? min(32, ly - yc) : 0;
             if (a.causal) {
                 if (DKV) c0 = max(0, d0);
                 else c1 = min(c1, 1 - d0);
             }
-            float run = 0.f, all = 0.f;
-            float* const dw = diag + warp * 100;
-#pragma unroll
-            for (int q = 0; q < kStep; q += 32) {
-                uint32_t sv[32], dv[32], p[16], ds[16];
-                tmem_ld32(tS + q, sv);
-                tmem_ld32(tD + q, dv);
+            const bool edge = __any_sync(0xffffffffu, c0 > 0 || c1 < 32);
+            float run = 0.f, all = 0.f;   // the diagonals under way; the sum of a block in one bucket
+            // (forms without the masks and without the bias by position: a block needs them rarely)
+            auto block = [&](auto edge_c, auto near_c) {
+                constexpr bool EDGE = decltype(edge_c)::value, NEAR = decltype(near_c)::value;
+                const float* const lp = lut + (d0 + reach + kPad);
+                const float flat = BIAS && !NEAR ? (lo >= reach ? lut[lut_size(reach) - 1] : lut[0]) : 0.f;
+                uint32_t sv[32], dv[32];
+                tmem_ld32(tS + col0, sv);
+                tmem_ld32(tD + col0, dv);
                 tmem_wait_ld();
                 tmem_tie32(sv), tmem_tie32(dv);
 #pragma unroll
                 for (int y = 0; y < 32; y += 4) {
                     float4 L, E;
                     if (DKV) {
-                        L = *reinterpret_cast<const float4*>(st + q + y);
-                        E = *reinterpret_cast<const float4*>(st + kStep + q + y);
+                        L = *reinterpret_cast<const float4*>(st + y);
+                        E = *reinterpret_cast<const float4*>(st + kStep + y);
                     } else {
                         L = make_float4(rl, rl, rl, rl), E = make_float4(rd, rd, rd, rd);
                     }
@@ -290,20 +297,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                     float pv[4], gv[4];
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
-                        const int col = q + y + z;
-                        const float raw_s = __uint_as_float(sv[y + z]);
-                        float t;
-                        if (!BIAS) t = fmaf(raw_s, c, -Lv[z]);
-                        else t = fmaf(raw_s, c, near ? (DKV ? lp[-col] : lp[col]) : flat) - Lv[z];
+                        const int col = y + z;
+                        const float raw_s = __uint_as_float(sv[col]);
+                        const float t = BIAS ? fmaf(raw_s, c, NEAR ? (DKV ? lp[-col] : lp[col]) : flat) - Lv[z] : fmaf(raw_s, c, -Lv[z]);
                         pv[z] = ex2(t);
-                        gv[z] = pv[z] * (__uint_as_float(dv[y + z]) - Ev[z]);
-                        if (edge) {
+                        gv[z] = pv[z] * (__uint_as_float(dv[col]) - Ev[z]);
+                        if (EDGE) {
                             const bool in = col >= c0 && col < c1;
                             pv[z] = in ? pv[z] : 0.f;
                             gv[z] = in ? gv[z] : 0.f;
                         }
-                        if (sums) {
-                            if (near) {
+                        if (BIAS && !DKV) {
+                            if (NEAR) {
                                 run = __shfl_up_sync(0xffffffffu, run, 1);
                                 run = (lane ? run : 0.f) + gv[z];
                                 if (lane == 31) dw[col] = run;
@@ -312,17 +317,24 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                     }
-                    p[y / 2] = pack2<T>(pv[0], pv[1]), p[y / 2 + 1] = pack2<T>(pv[2], pv[3]);
-                    ds[y / 2] = pack2<T>(gv[0], gv[1]), ds[y / 2 + 1] = pack2<T>(gv[2], gv[3]);
+                    sv[y / 2] = pack2<T>(pv[0], pv[1]), sv[y / 2 + 1] = pack2<T>(pv[2], pv[3]);
+                    dv[y / 2] = pack2<T>(gv[0], gv[1]), dv[y / 2 + 1] = pack2<T>(gv[2], gv[3]);
                 }
-                if (DKV) tmem_st16(tS + q / 2, p);
-                tmem_st16(tD + q / 2, ds);
+                if (DKV) tmem_st16(tS + col0, sv);
+                tmem_st16(tD + col0, dv);
+            };
+            if (BIAS && near) {
+                if (edge) block(std::true_type{}, std::true_type{});
+                else block(std::false_type{}, std::true_type{});
+            } else {
+                if (edge) block(std::true_type{}, std::false_type{});
+                else block(std::false_type{}, std::false_type{});
             }
             const int live = ly - yb;
             if (live < kStep) {   // rows of Y past the length to zero, for the products that sum over them
                 uint8_t* const y = gb + 2 * Sh::kX + s * Sh::kStage;
                 const int dead_units = (kStep - live) * 8;
-                for (int e = r; e < dead_units * Sh::kChunks * (DKV ? 2 : 1); e += 128) {
+                for (int e = tid & 255; e < dead_units * Sh::kChunks * (DKV ? 2 : 1); e += 256) {
                     const int ch = e / dead_units, o = e % dead_units;
                     *reinterpret_cast<uint4*>(y + ch * kChunkY + live * 128 + o * 16) = make_uint4(0, 0, 0, 0);
                 }
@@ -330,60 +342,60 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_wait_st();
             tc_fence_before();
-            bar_arrive(barP + 8 * wg);
+            bar_arrive(barP + 8 * buf);
             if (sums) {
                 if (near) {
-                    dw[94 - lane] = run;   // the diagonals still under way; lane 31's is in place
+                    dw[62 - lane] = run;   // the diagonals still under way; lane 31's is in place
                     __syncwarp();
-                    // inclusive scan of the 95 sums (and a zero): lane l takes 3 l .. 3 l + 2
-                    const float s0 = dw[3 * lane], s1 = s0 + dw[3 * lane + 1];
-                    const float s2 = s1 + (3 * lane + 2 < 95 ? dw[3 * lane + 2] : 0.f);
-                    float t = s2;
+                    // the 63 sums (and a zero) scanned: lane l takes 2 l and 2 l + 1
+                    const float s0 = dw[2 * lane], s1 = s0 + (lane < 31 ? dw[2 * lane + 1] : 0.f);
+                    float t = s1;
 #pragma unroll
                     for (int o = 1; o < 32; o <<= 1) {
                         const float u = __shfl_up_sync(0xffffffffu, t, o);
                         if (lane >= o) t += u;
                     }
-                    const float before = t - s2;
                     __syncwarp();
-                    dw[3 * lane + 1] = before + s0, dw[3 * lane + 2] = before + s1, dw[3 * lane + 3] = t;
+                    dw[2 * lane + 1] = t - s1 + s0, dw[2 * lane + 2] = t;
                     if (lane == 0) dw[0] = 0.f;
                     __syncwarp();
-                    // entry e holds the sum of the diagonals below d = dmin + e
-                    const int dmin = yb - (x0 + 32 * (warp & 3) + 31 + off), nb = n_buckets(a.edges);
+                    // entry e now holds the sum of the diagonals d in [lo, lo + e)
+                    const int nb = n_buckets(a.edges);
 #pragma unroll
                     for (int i = 0; i < kBuckets / 32; ++i) {
                         const int t2 = lane + 32 * i;
                         if (t2 < nb) {
-                            const int e0 = max(range[2 * t2] - dmin, 0), e1 = min(range[2 * t2 + 1] - dmin + 1, 95);
+                            const int e0 = max(range[2 * t2] - lo, 0), e1 = min(range[2 * t2 + 1] - lo + 1, 63);
                             if (e0 < e1) bsum[i] += dw[e1] - dw[e0];
                         }
                     }
                     __syncwarp();
+                } else if (lo >= reach) {
+                    far1 += all;
                 } else {
-                    if (lo >= reach) far[1] += all;
-                    else far[0] += all;
+                    far0 += all;
                 }
             }
         }
         ok = ok && bar_wait_warp(barF, 0, dead);
         tc_fence_after();
         // accumulators to the owned tiles' shared memory (their last use is over), swizzled as the copy out reads them:
-        // keys pass: a warpgroup each for dV and dK; query pass: half of dQ's columns each
+        // keys pass: half of dV's (buffer 0) or dK's columns a warpgroup; query pass: a quarter of dQ's
         const bool row = x < lx;
-        const float w = !ok ? NAN : (DKV && wg == 0 ? 1.f : a.scale);
-        const int f0 = DKV ? 0 : wg * (DP / 2), f1 = DKV ? DP : f0 + DP / 2;
-        const uint32_t acc = DKV && wg == 0 ? tA1 : tA2;
-        uint8_t* const stage = gb + (DKV && wg == 0 ? 0 : Sh::kX);
+        const bool first = DKV && buf == 0;
+        const float w = !ok ? NAN : (first ? 1.f : a.scale);
+        const int f0 = DKV ? half * (DP / 2) : (warp >> 2) * (DP / 4), f1 = f0 + (DKV ? DP / 2 : DP / 4);
+        const uint32_t acc = (first ? tA1 : tA2) + trow;
+        uint8_t* const stage = gb + (first ? 0 : Sh::kX);
 #pragma unroll 1
-        for (int f = f0; f < f1; f += 32) {
-            uint32_t o[32];
-            tmem_ld32(acc + trow + f, o);
+        for (int f = f0; f < f1; f += 16) {
+            uint32_t o[16];
+            tmem_ld16(acc + f, o);
             tmem_wait_ld();
-            tmem_tie32(o);
+            tmem_tie16(o);
             uint8_t* const rp = stage + (f / 64) * kChunkX + r * 128;
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
+            for (int y = 0; y < 2; ++y) {
                 uint32_t p[4];
 #pragma unroll
                 for (int z = 0; z < 4; ++z)
@@ -394,17 +406,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (sums) {
             const int nb = n_buckets(a.edges);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) far[i] += __shfl_xor_sync(0xffffffffu, far[i], o);
+            for (int o = 16; o > 0; o >>= 1) {
+                far0 += __shfl_xor_sync(0xffffffffu, far0, o);
+                far1 += __shfl_xor_sync(0xffffffffu, far1, o);
+            }
 #pragma unroll
             for (int i = 0; i < kBuckets / 32; ++i) {
                 const int t = lane + 32 * i;
-                if (t < nb) red[warp * kBuckets + t] = bsum[i] + (t == a.edges.n ? far[0] : 0.f) + (a.edges.two && t == nb - 1 ? far[1] : 0.f);
+                if (t < nb) red[warp * kBuckets + t] = bsum[i] + (t == a.edges.n ? far0 : 0.f) + (a.edges.two && t == nb - 1 ? far1 : 0.f);
             }
         }
         fence_async_smem();
-        asm volatile("bar.sync 2, 256;" ::: "memory");
+        asm volatile("bar.sync 1, 512;" ::: "memory");
         if (tid == 0) {
 #pragma unroll
             for (int ch = 0; ch < Sh::kChunks; ++ch) {
@@ -416,17 +429,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (sums) {
             const int nb = n_buckets(a.edges);
-            for (int t = tid; t < nb; t += 256) {
+            for (int t = tid; t < nb; t += kWork) {
                 float v = 0.f;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) v += red[k * kBuckets + t];
+                for (int k = 0; k < kWork / 32; ++k) v += red[k * kBuckets + t];
                 g.part[(((size_t)hx * nb + t) * a.B + b) * gridDim.x + blockIdx.x] = v;
             }
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) tmem_free(tmem, kColumns);
+    if (warp == kWork / 32) tmem_free(tmem, kColumns);
 }
 
 // delta = rowsum(dO O) and lse in rows padded to whole tiles: +inf and 0 where no key is met.  16 lanes a row

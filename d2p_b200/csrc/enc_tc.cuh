@@ -125,6 +125,13 @@ __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* v) {
         : "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t* v) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : ENC_W8(v, 0), ENC_W8(v, 8)
+        : "r"(addr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -144,6 +151,7 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
 __device__ __forceinline__ void tmem_tie32(uint32_t* v) {
     asm volatile("" : ENC_T8(v, 0), ENC_T8(v, 8), ENC_T8(v, 16), ENC_T8(v, 24));
 }
+__device__ __forceinline__ void tmem_tie16(uint32_t* v) { asm volatile("" : ENC_T8(v, 0), ENC_T8(v, 8)); }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
