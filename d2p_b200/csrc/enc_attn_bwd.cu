@@ -13,8 +13,10 @@
 //   P, dS in 16 bits over S's and dP's own columns (TMEM operands A; each half
 //   of the columns over its own, so that no warp writes what another still reads),
 //   acc1 += P Y2 (keys pass: dV),  acc2 += dS Y1 (dK or dQ).
-// S and dP are double-buffered: two warpgroups work on even tiles (32 columns
-// each), two on odd, while the tensor cores run the products of the other.  The scores are formed
+// S and dP have three buffers (two where the accumulators leave no third): two
+// warpgroups work on even tiles (32 columns each), two on odd, and find the next
+// S and dP ready.  A round from P to the next S takes ~1300 cycles of waits and
+// latencies besides the products, so with two buffers the tensor cores wait.  The scores are formed
 // twice (7 products a tile pair rather than 5); in exchange dQ needs no
 // cross-CTA sums, whose order would change results from run to run.
 //
@@ -31,12 +33,15 @@ namespace enc {
 
 namespace bwd {
 
-constexpr int kWork = 512;              // four warpgroups: two for a buffer of S and dP, half of its columns each
+constexpr int kWork = 512;              // four warpgroups: two for a tile, half of its columns each
 constexpr int kThreads = kWork + 64;    // and the products' warp and the copies' warp
 constexpr int kOwn = 128, kStep = 64;
-constexpr int kColumns = 512;   // TMEM: S 2 x 64, dP 2 x 64, two accumulators of up to 128
+constexpr int kColumns = 512;   // TMEM: buffers of 64 columns of S and 64 of dP, then the accumulators
 constexpr int kChunkX = kOwn * 128, kChunkY = kStep * 128;
 constexpr int kBuckets = 2 * (kMaxEdges + 1);
+
+template <int DP, bool DKV>
+__host__ __device__ constexpr int buffers() { return DKV && DP == 128 ? 2 : 3; }
 
 template <int DP>
 struct Shape {
@@ -44,11 +49,11 @@ struct Shape {
     static constexpr int kX = kChunks * kChunkX, kY = kChunks * kChunkY;
     static constexpr int kRowStats = 2 * kStep * 4;               // lse and delta of a streamed tile's queries
     static constexpr int kStage = 2 * kY + 1024;                  // keeps the tiles at 1024-byte boundaries
-    static constexpr int kStages = DP == 64 ? 4 : 3;
-    static constexpr int kBars = 2 + 2 * kStages + 4;
+    static constexpr int kStages = DP == 64 ? 8 : 4;
+    static constexpr int kBars = 2 + 2 * kStages + 6;
     static constexpr size_t fixed() { return 1024 + 2 * (size_t)kX + (size_t)kStages * kStage + kBars * 8 + 16; }
 };
-// after the tiles: the bias by position (keys pass: one for each buffer, whose tiles may be of two heads), then
+// after the tiles: the bias by position (keys pass: one for each pair of warpgroups, whose tiles may be of two heads), then
 // (query pass) the diagonals' stage of each warp and the buckets' ranges
 __host__ __device__ inline size_t extra(bool bias, bool dkv, int reach) {
     if (!bias) return 0;
@@ -79,7 +84,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ CUtensorMap tmD1, const __grid_constant__ CUtensorMap tmD2,
                     const __grid_constant__ Args g) {
     using Sh = Shape<DP>;
-    constexpr int NST = Sh::kStages;
+    constexpr int NST = Sh::kStages, NB = buffers<DP, DKV>();
     const AttnArgs& a = g.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     // causal: the first keys and the last queries have the most to do
@@ -117,7 +122,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr size_t kTiles = 2 * (size_t)Sh::kX + (size_t)NST * Sh::kStage;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(gb + kTiles);
     const uint32_t barX = smem_addr(bars), barF = barX + 8, barY = barX + 16, barE = barY + 8 * NST, barS = barE + 8 * NST,
-                   barP = barS + 16;
+                   barP = barS + 24;
     volatile int* const dead = reinterpret_cast<volatile int*>(bars + Sh::kBars);
     uint32_t* const slot = reinterpret_cast<uint32_t*>(bars + Sh::kBars) + 1;
     float* lut = reinterpret_cast<float*>(bars + Sh::kBars + 2);
@@ -130,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (tid == 0) {
         bar_init(barX, 1), bar_init(barF, 1);
         for (int s = 0; s < NST; ++s) bar_init(barY + 8 * s, 1), bar_init(barE + 8 * s, 1);
-        for (int s = 0; s < 2; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 256);
+        for (int s = 0; s < NB; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *dead = 0;
     }
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot, tA1 = tmem + 256, tA2 = tmem + 384;
+    const uint32_t tmem = *slot, tA1 = tmem + 128 * NB, tA2 = DKV ? tA1 + DP : tA1;
 
     if (warp == kWork / 32 + 1) {   // copies
         if (lane == 0) {
@@ -194,43 +199,40 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int s = it % NST;
                 if (!bar_wait(barY + 8 * s, (it / NST) & 1, dead)) return false;
                 tc_fence_after();
-                const uint32_t y = sY + s * Sh::kStage, d = tmem + (it & 1) * kStep;
+                const uint32_t d = tmem + (it % NB) * 128, dX = desc_along(sX1), dY = desc_along(sY + s * Sh::kStage);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t ox = (k / 4) * kChunkX + (k % 4) * 32, oy = (k / 4) * kChunkY + (k % 4) * 32;
-                    mma_ss(d, desc_k(sX1 + ox), desc_k(y + oy), idS, k != 0);
-                }
+                for (int w = 0; w < 2; ++w)
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t ox = (k / 4) * kChunkX + (k % 4) * 32, oy = (k / 4) * kChunkY + (k % 4) * 32;
-                    mma_ss(d + 128, desc_k(sX2 + ox), desc_k(y + Sh::kY + oy), idS, k != 0);
-                }
-                tc_commit(barS + 8 * (it & 1));
+                    for (int k = 0; k < DP / 16; ++k)
+                        mma_ss(d + 64 * w, dX + (w * Sh::kX + (k / 4) * kChunkX + (k % 4) * 32) / 16,
+                               dY + (w * Sh::kY + (k / 4) * kChunkY + (k % 4) * 32) / 16, idS, k != 0);
+                tc_commit(barS + 8 * (it % NB));
                 return true;
             };
-            bool ok = bar_wait(barX, 0, dead) && scores(0) && (n < 2 || scores(1));
+            bool ok = bar_wait(barX, 0, dead);
+            for (int it = 0; ok && it < NB && it < n; ++it) ok = scores(it);
             for (int it = 0; ok && it < n; ++it) {
                 const int s = it % NST;
-                if (!(ok = bar_wait(barP + 8 * (it & 1), (it >> 1) & 1, dead))) break;
+                if (!(ok = bar_wait(barP + 8 * (it % NB), (it / NB) & 1, dead))) break;
                 tc_fence_after();
-                const uint32_t y = sY + s * Sh::kStage, p = tmem + (it & 1) * kStep;
+                const uint32_t p = tmem + (it % NB) * 128, dY = desc_down(sY + s * Sh::kStage, kChunkY);
                 if (DKV) {
 #pragma unroll
                     for (int k = 0; k < kStep / 16; ++k)
-                        mma_ts(tA1, p + 32 * (k / 2) + 8 * (k % 2), desc_mn(y + Sh::kY + k * 2048, kChunkY), idA, (it | k) != 0);
+                        mma_ts(tA1, p + 32 * (k / 2) + 8 * (k % 2), dY + (Sh::kY + k * 2048) / 16, idA, (it | k) != 0);
                 }
 #pragma unroll
                 for (int k = 0; k < kStep / 16; ++k)
-                    mma_ts(tA2, p + 128 + 32 * (k / 2) + 8 * (k % 2), desc_mn(y + k * 2048, kChunkY), idA, (it | k) != 0);
+                    mma_ts(tA2, p + 64 + 32 * (k / 2) + 8 * (k % 2), dY + k * (2048 / 16), idA, (it | k) != 0);
                 tc_commit(barE + 8 * s);
-                if (it + 2 < n) ok = scores(it + 2);
+                if (it + NB < n) ok = scores(it + NB);
             }
             tc_commit(barF);
             if (!ok) atomicAdd(&g_gave_up, 1ull);
         }
         __syncwarp();
     } else {   // P and dS of a tile
-        const int buf = warp >> 3, half = (warp >> 2) & 1, w4 = warp & 3, r = tid & 127, x = x0 + r;
+        const int pair = warp >> 3, half = (warp >> 2) & 1, w4 = warp & 3, r = tid & 127, x = x0 + r;
         const uint32_t trow = (uint32_t)(32 * w4) << 16;
         const float c = a.scale * kLog2e;
         float rl = 0.f, rd = 0.f;
@@ -242,24 +244,28 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kBuckets / 32; ++i) bsum[i] = 0.f;
         bool ok = true;
-        int filled = -1;   // keys pass: the head of the group whose bias is in the buffer's lut
-        if (BIAS && DKV && buf) lut += lut_size(reach);
+        int filled = -1;   // keys pass: the head of the group whose bias is in the pair's lut
+        if (BIAS && DKV && pair) lut += lut_size(reach);
         float* const dw = diag + warp * 72;
-        for (int it = buf; it < n; it += 2) {
-            const int s = it % NST, yb = y0 + (it % per) * kStep;
-            if (BIAS && DKV && it / per != filled) {
-                filled = it / per;
-                asm volatile("bar.sync %0, 256;" ::"r"(3 + buf) : "memory");   // the last tile's reads are over
+        int head = 0, step = pair;   // of tile it: the head of the group and the tile of its rows
+        for (int it = pair; it < n; it += 2, step += 2) {
+            while (step >= per) step -= per, ++head;
+            const int s = it % NST, buf = it % NB, yb = y0 + step * kStep;
+            if (BIAS && DKV && head != filled) {
+                filled = head;
+                asm volatile("bar.sync %0, 256;" ::"r"(3 + pair) : "memory");   // the last tile's reads are over
                 for (int i = tid & 255; i < lut_size(reach); i += 256)
                     lut[i] = bias_log2<T>(a, bucket_of(a.edges, i - reach - kPad), hx * group + filled);
-                asm volatile("bar.sync %0, 256;" ::"r"(3 + buf) : "memory");
+                asm volatile("bar.sync %0, 256;" ::"r"(3 + pair) : "memory");
             }
             // (after a wait that gave up a warp still meets its partners at the barriers above)
-            ok = ok && bar_wait_warp(barS + 8 * buf, (it >> 1) & 1, dead) && bar_wait_warp(barY + 8 * s, (it / NST) & 1, dead);
+            // (the streamed tile's own barrier: the keys pass reads the row statistics that came with it)
+            ok = ok && (!DKV || bar_wait_warp(barY + 8 * s, (it / NST) & 1, dead)) &&
+                 bar_wait_warp(barS + 8 * buf, (it / NB) & 1, dead);
             if (!ok) continue;
             tc_fence_after();
             const int col0 = 32 * half, yc = yb + col0;
-            const uint32_t tS = tmem + trow + buf * kStep, tD = tS + 128;
+            const uint32_t tS = tmem + trow + buf * 128, tD = tS + 64;
             const float* const st = reinterpret_cast<const float*>(gb + 2 * Sh::kX + s * Sh::kStage + 2 * Sh::kY) + col0;
             // d = key position - query position of this row and the block's first column; a column is one less or one more
             const int d0 = DKV ? x - (yc + off) : yc - (x + off);
@@ -342,7 +348,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             tmem_wait_st();
             tc_fence_before();
-            bar_arrive(barP + 8 * buf);
+            bar_arrive_warp(barP + 8 * buf);
             if (sums) {
                 if (near) {
                     dw[62 - lane] = run;   // the diagonals still under way; lane 31's is in place
@@ -380,9 +386,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = ok && bar_wait_warp(barF, 0, dead);
         tc_fence_after();
         // accumulators to the owned tiles' shared memory (their last use is over), swizzled as the copy out reads them:
-        // keys pass: half of dV's (buffer 0) or dK's columns a warpgroup; query pass: a quarter of dQ's
+        // keys pass: half of dV's or dK's columns a warpgroup; query pass: a quarter of dQ's
         const bool row = x < lx;
-        const bool first = DKV && buf == 0;
+        const bool first = DKV && pair == 0;
         const float w = !ok ? NAN : (first ? 1.f : a.scale);
         const int f0 = DKV ? half * (DP / 2) : (warp >> 2) * (DP / 4), f1 = f0 + (DKV ? DP / 2 : DP / 4);
         const uint32_t acc = (first ? tA1 : tA2) + trow;

@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int reach = BIAS ? reach_of(a.edges) : 0;
 
     if (tid == 0) {
-        bar_init(barQ, 1), bar_init(barS, 1), bar_init(barP, 128), bar_init(barO, 1);
+        bar_init(barQ, 1), bar_init(barS, 1), bar_init(barP, 4), bar_init(barO, 1);
         for (int s = 0; s < NST; ++s) bar_init(barK + 8 * s, 1), bar_init(barV + 8 * s, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         *dead = 0;
@@ -115,10 +115,11 @@ __global__ void __launch_bounds__(kThreads, 2)
                 const uint32_t ph = (j / NST) & 1;
                 if (!(ok = bar_wait(barK + 8 * s, ph, dead))) break;
                 tc_fence_after();
+                const uint32_t dQ = desc_along(sQ), dK = desc_along(sK + s * Sh::kTile);
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t o = (k / 4) * kChunk + (k % 4) * 32;
-                    mma_ss(tmem, desc_k(sQ + o), desc_k(sK + s * Sh::kTile + o), idS, k != 0);
+                    const uint32_t o = ((k / 4) * kChunk + (k % 4) * 32) / 16;
+                    mma_ss(tmem, dQ + o, dK + o, idS, k != 0);
                 }
                 tc_commit(barS);
                 // S (and every product before it) done: its K tile is free, and V's of the tile before
@@ -130,9 +131,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (j + NST < tiles) load(sK + s * Sh::kTile, &tmK, (j + NST) * kRows, kh, barK + 8 * s);
                 if (!(ok = bar_wait(barV + 8 * s, ph, dead) && bar_wait(barP, j & 1, dead))) break;
                 tc_fence_after();
+                const uint32_t dV = desc_down(sV + s * Sh::kTile, kChunk);
 #pragma unroll
-                for (int k = 0; k < kRows / 16; ++k)
-                    mma_ts(tO, tmem + 8 * k, desc_mn(sV + s * Sh::kTile + k * 2048, kChunk), idO, (j | k) != 0);
+                for (int k = 0; k < kRows / 16; ++k) mma_ts(tO, tmem + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
                 tc_commit(barO);
             }
             if (!ok) {   // a wait gave up: what is in flight ends (bounded) before the CTA does
@@ -237,7 +238,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
             tmem_wait_st();
             tc_fence_before();
-            bar_arrive(barP);
+            bar_arrive_warp(barP);
         }
         ok = ok && bar_wait_warp(barO, (tiles - 1) & 1, dead);
         tc_fence_after();

@@ -29,6 +29,11 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// one arrival for a warp, after all its lanes (one for each lane would queue up on the barrier's word)
+__device__ __forceinline__ void bar_arrive_warp(uint32_t bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) bar_arrive(bar);
+}
 // waits for the phase of the given parity; *dead is the CTA's flag that some
 // wait gave up (then every other wait ends as well)
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
@@ -79,17 +84,14 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-// shared-memory operand, the contraction along the 128-byte rows: 8-row groups 1024 bytes apart
-__device__ __forceinline__ uint64_t desc_k(uint32_t saddr) {
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)2 << 61);
-}
-// shared-memory operand, the contraction down the rows: 8-row groups 1024 bytes
-// apart, the next 64 elements of the other extent one chunk further
-__device__ __forceinline__ uint64_t desc_mn(uint32_t saddr, uint32_t chunk_bytes) {
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | ((uint64_t)(chunk_bytes >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
+// Shared-memory operands, 128-byte rows and swizzle, 8-row groups 1024 bytes
+// apart.  The low words differ by address only, so a step along a tile is one
+// addition (in 16-byte units: addresses stay below 2^18); the high word is constant.
+// along: the contraction runs along the rows.  down: it runs down the rows, and
+// the next 64 elements of the other extent lie one chunk further.
+constexpr uint32_t kDescHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc_along(uint32_t saddr) { return (saddr >> 4) | (1u << 16); }
+__device__ __forceinline__ uint32_t desc_down(uint32_t saddr, uint32_t chunk_bytes) { return (saddr >> 4) | ((chunk_bytes >> 4) << 16); }
 // fp32 accumulator, both operands of type T; b_rows: operand B's contraction runs down its rows
 template <class T>
 __host__ __device__ constexpr uint32_t mma_desc(int m, int n, bool b_rows);
@@ -101,16 +103,19 @@ template <>
 __host__ __device__ constexpr uint32_t mma_desc<__half>(int m, int n, bool b_rows) {
     return (1u << 4) | (b_rows ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool acc) {
+// d (+)= A B: A from shared memory (ss) or TMEM (ts), B from shared memory, K = 16
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        "{\n .reg .pred p;\n .reg .b64 x, y;\n setp.ne.b32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool acc) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool acc) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc)
+        "{\n .reg .pred p;\n .reg .b64 y;\n setp.ne.b32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)acc), "n"(kDescHigh)
         : "memory");
 }
 
