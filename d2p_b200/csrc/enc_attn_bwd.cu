@@ -193,42 +193,46 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
     } else if (warp == kWork / 32) {   // products
-        if (lane == 0) {
+        {
+            // the whole warp runs this, so that the operands' words stay in uniform registers; one lane issues
+            const bool lead = elect_one();
+            const int nu = __shfl_sync(0xffffffffu, n, 0);
+            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), uA1 = tm + 128 * NB, uA2 = DKV ? uA1 + DP : uA1;
             constexpr uint32_t idS = mma_desc<T>(128, kStep, false), idA = mma_desc<T>(128, DP, true);
             auto scores = [&](int it) {
                 const int s = it % NST;
-                if (!bar_wait(barY + 8 * s, (it / NST) & 1, dead)) return false;
+                if (!bar_wait_warp(barY + 8 * s, (it / NST) & 1, dead)) return false;
                 tc_fence_after();
-                const uint32_t d = tmem + (it % NB) * 128, dX = desc_along(sX1), dY = desc_along(sY + s * Sh::kStage);
+                const uint32_t d = tm + (it % NB) * 128, dX = desc_along(sX1), dY = desc_along(sY + s * Sh::kStage);
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k)
-                        mma_ss(d + 64 * w, dX + (w * Sh::kX + (k / 4) * kChunkX + (k % 4) * 32) / 16,
+                        if (lead) mma_ss(d + 64 * w, dX + (w * Sh::kX + (k / 4) * kChunkX + (k % 4) * 32) / 16,
                                dY + (w * Sh::kY + (k / 4) * kChunkY + (k % 4) * 32) / 16, idS, k != 0);
-                tc_commit(barS + 8 * (it % NB));
+                if (lead) tc_commit(barS + 8 * (it % NB));
                 return true;
             };
-            bool ok = bar_wait(barX, 0, dead);
-            for (int it = 0; ok && it < NB && it < n; ++it) ok = scores(it);
-            for (int it = 0; ok && it < n; ++it) {
+            bool ok = bar_wait_warp(barX, 0, dead);
+            for (int it = 0; ok && it < NB && it < nu; ++it) ok = scores(it);
+            for (int it = 0; ok && it < nu; ++it) {
                 const int s = it % NST;
-                if (!(ok = bar_wait(barP + 8 * (it % NB), (it / NB) & 1, dead))) break;
+                if (!(ok = bar_wait_warp(barP + 8 * (it % NB), (it / NB) & 1, dead))) break;
                 tc_fence_after();
-                const uint32_t p = tmem + (it % NB) * 128, dY = desc_down(sY + s * Sh::kStage, kChunkY);
+                const uint32_t p = tm + (it % NB) * 128, dY = desc_down(sY + s * Sh::kStage, kChunkY);
                 if (DKV) {
 #pragma unroll
                     for (int k = 0; k < kStep / 16; ++k)
-                        mma_ts(tA1, p + 32 * (k / 2) + 8 * (k % 2), dY + (Sh::kY + k * 2048) / 16, idA, (it | k) != 0);
+                        if (lead) mma_ts(uA1, p + 32 * (k / 2) + 8 * (k % 2), dY + (Sh::kY + k * 2048) / 16, idA, (it | k) != 0);
                 }
 #pragma unroll
                 for (int k = 0; k < kStep / 16; ++k)
-                    mma_ts(tA2, p + 64 + 32 * (k / 2) + 8 * (k % 2), dY + k * (2048 / 16), idA, (it | k) != 0);
-                tc_commit(barE + 8 * s);
-                if (it + NB < n) ok = scores(it + NB);
+                    if (lead) mma_ts(uA2, p + 64 + 32 * (k / 2) + 8 * (k % 2), dY + k * (2048 / 16), idA, (it | k) != 0);
+                if (lead) tc_commit(barE + 8 * s);
+                if (it + NB < nu) ok = scores(it + NB);
             }
-            tc_commit(barF);
-            if (!ok) atomicAdd(&g_gave_up, 1ull);
+            if (lead) tc_commit(barF);
+            if (!ok && lead) atomicAdd(&g_gave_up, 1ull);
         }
         __syncwarp();
     } else {   // P and dS of a tile

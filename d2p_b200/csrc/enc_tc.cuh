@@ -56,6 +56,13 @@ __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, vol
     return __all_sync(0xffffffffu, bar_wait(bar, parity, dead));
 }
 
+// true in one lane of a converged warp
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+    return p != 0;
+}
+
 __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, int x, int row, int head, int b, uint32_t bar) {
     asm volatile(
         "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
