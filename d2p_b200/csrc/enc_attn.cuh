@@ -26,16 +26,6 @@ struct AttnArgs {
     float scale;                  // of the natural scores
 };
 
-__device__ __forceinline__ int bucket_of(const Edges& e, int d) {
-    const int n = e.two ? abs(d) : max(-d, 0);
-    int lo = 0, hi = e.n;         // the number of edges <= n
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (e.e[mid] <= n) lo = mid + 1;
-        else hi = mid;
-    }
-    return lo + ((e.two && d > 0) ? e.n + 1 : 0);
-}
 __device__ __forceinline__ int n_buckets(const Edges& e) { return (e.n + 1) << e.two; }
 
 // bias of a bucket in base-2 units.  Finite values are held within 1e30 so that

@@ -132,22 +132,49 @@ __global__ void __launch_bounds__(kThreads, 1)
     int* const range = reinterpret_cast<int*>(red + 16 * kBuckets);   // [kBuckets][2] positions of a bucket
     const bool sums = !DKV && BIAS && g.part;
 
-    if (tid == 0) {
-        bar_init(barX, 1), bar_init(barF, 1);
-        for (int s = 0; s < NST; ++s) bar_init(barY + 8 * s, 1), bar_init(barE + 8 * s, 1);
-        for (int s = 0; s < NB; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 8);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        *dead = 0;
-    }
-    if (warp == kWork / 32) tmem_alloc(smem_addr(slot), kColumns);
-    if (BIAS && !DKV) {
-        for (int i = tid; i < lut_size(reach); i += kThreads) lut[i] = bias_log2<T>(a, bucket_of(a.edges, i - reach - kPad), hx);
+    auto copy = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, uint32_t bar, int chunk) {
+#pragma unroll
+        for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * chunk, tm, 64 * c, row, head, b, bar);
+    };
+    auto stream = [&](int it) {
+        const int s = it % NST, head = DKV ? hx * group + it / per : hx / group, row = y0 + (it % per) * kStep;
+        const uint32_t dst = sY + s * Sh::kStage, bar = barY + 8 * s;
+        bar_expect(bar, 2 * Sh::kY + (DKV ? Sh::kRowStats : 0));
+        copy(dst, &tmY1, row, head, bar, kChunkY);
+        copy(dst + Sh::kY, &tmY2, row, head, bar, kChunkY);
+        if (DKV) {
+            const size_t at = ((size_t)b * a.H + head) * g.Lp + row;
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+                asm volatile(
+                    "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                        dst + 2 * Sh::kY + w * kStep * 4),
+                    "l"((w ? g.delta : g.lse) + at), "r"(kStep * 4), "r"(bar)
+                    : "memory");
+        }
+    };
+    if (warp == kWork / 32 + 1) {   // barriers, and the first copies before the CTA meets
+        if (lane == 0) {
+            bar_init(barX, 1), bar_init(barF, 1);
+            for (int s = 0; s < NST; ++s) bar_init(barY + 8 * s, 1), bar_init(barE + 8 * s, 1);
+            for (int s = 0; s < NB; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 8);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            fence_async_smem();
+            *dead = 0;
+            bar_expect(barX, 2 * Sh::kX);
+            copy(sX1, &tmX1, x0, hx, barX, kChunkX);
+            copy(sX2, &tmX2, x0, hx, barX, kChunkX);
+            for (int it = 0; it < NST && it < n; ++it) stream(it);
+        }
+        __syncwarp();
+    } else if (warp == kWork / 32) {
+        tmem_alloc(smem_addr(slot), kColumns);
+    } else if (BIAS && !DKV) {
+        fill_lut<T>(lut, a, hx, reach, warp, kWork / 32);
         if (sums)
-            for (int t = tid; t < n_buckets(a.edges); t += kThreads) {
-                const int side = a.edges.n + 1, u = t % side, far = 1 << 30;
-                const int lo = u ? a.edges.e[u - 1] : 0, hi = u < a.edges.n ? a.edges.e[u] - 1 : far;
-                range[2 * t] = t < side ? -hi : max(lo, 1);
-                range[2 * t + 1] = t < side ? -lo : hi;
+            for (int t = tid; t < n_buckets(a.edges); t += kWork) {
+                const int2 v = bucket_range(a.edges, t, 1 << 29);
+                range[2 * t] = v.x, range[2 * t + 1] = v.y;
             }
     }
     tc_fence_before();
@@ -157,33 +184,11 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     if (warp == kWork / 32 + 1) {   // copies
         if (lane == 0) {
-            auto copy = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, uint32_t bar, int chunk) {
-#pragma unroll
-                for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * chunk, tm, 64 * c, row, head, b, bar);
-            };
-            bar_expect(barX, 2 * Sh::kX);
-            copy(sX1, &tmX1, x0, hx, barX, kChunkX);
-            copy(sX2, &tmX2, x0, hx, barX, kChunkX);
             bool ok = true;
-            int it = 0;
+            int it = min(n, NST);
             for (; it < n; ++it) {
-                const int s = it % NST;
-                if (it >= NST && !(ok = bar_wait(barE + 8 * s, (it / NST - 1) & 1, dead))) break;
-                const int head = DKV ? hx * group + it / per : hx / group, row = y0 + (it % per) * kStep;
-                const uint32_t dst = sY + s * Sh::kStage, bar = barY + 8 * s;
-                bar_expect(bar, 2 * Sh::kY + (DKV ? Sh::kRowStats : 0));
-                copy(dst, &tmY1, row, head, bar, kChunkY);
-                copy(dst + Sh::kY, &tmY2, row, head, bar, kChunkY);
-                if (DKV) {
-                    const size_t at = ((size_t)b * a.H + head) * g.Lp + row;
-#pragma unroll
-                    for (int w = 0; w < 2; ++w)
-                        asm volatile(
-                            "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                                dst + 2 * Sh::kY + w * kStep * 4),
-                            "l"((w ? g.delta : g.lse) + at), "r"(kStep * 4), "r"(bar)
-                            : "memory");
-                }
+                if (!(ok = bar_wait(barE + 8 * (it % NST), (it / NST - 1) & 1, dead))) break;
+                stream(it);
             }
             if (!ok || *dead) {   // what is in flight ends (bounded) before the CTA does
                 volatile int none = 0;
@@ -258,8 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (BIAS && DKV && head != filled) {
                 filled = head;
                 asm volatile("bar.sync %0, 256;" ::"r"(3 + pair) : "memory");   // the last tile's reads are over
-                for (int i = tid & 255; i < lut_size(reach); i += 256)
-                    lut[i] = bias_log2<T>(a, bucket_of(a.edges, i - reach - kPad), hx * group + filled);
+                fill_lut<T>(lut, a, hx * group + filled, reach, warp & 7, 8);
                 asm volatile("bar.sync %0, 256;" ::"r"(3 + pair) : "memory");
             }
             // (after a wait that gave up a warp still meets its partners at the barriers above)

@@ -4,7 +4,7 @@
 // 128.  S = Q K^T (tcgen05, both operands in shared memory, K-major) lands in
 // 128 TMEM columns; a warpgroup reads it, one row a thread, adds the bias, and
 // takes the softmax in base 2 with a running reference m: p = 2^(s - m), l =
-// sum p.  P goes back to TMEM in 16 bits over S's own columns and is operand A
+// sum p.  P goes back to TMEM in 16 bits and is operand A
 // of O += P V (V from shared memory, contraction down its rows).  m is raised,
 // and O and l rescaled, only when a row's maximum passes it by more than
 // kSlack (2^kSlack stays in range of the 16-bit types), which after the first
@@ -35,9 +35,13 @@ template <int DP>
 struct Shape {
     static constexpr int kChunks = DP / 64;
     static constexpr int kTile = kChunks * kChunk;
-    // K and V tiles in flight: one of each for 128 elements (two CTAs an SM)
+    // K and V tiles in flight: one of each for 128 elements (two CTAs an SM); kApart needs two, since it asks for V
+    // tile j only after P j - 1
     static constexpr int kStages = DP == 64 ? 2 : 1;
-    static constexpr int kBars = 4 + 2 * kStages;
+    static constexpr int kBars = 5 + 2 * kStages;
+    // P has TMEM columns of its own, so that the next S is formed while this one's exponentials are taken; for 128
+    // elements there is no room and P overwrites S (that shape is bound by its products as it is)
+    static constexpr bool kApart = DP == 64;
     static constexpr size_t smem(int lut) { return 1024 + (size_t)kTile * (1 + 2 * kStages) + kBars * 8 + 16 + (size_t)lut * 4; }
 };
 
@@ -73,78 +77,89 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint8_t* const gbase = raw + (base - r0);
     const uint32_t sQ = base, sK = base + Sh::kTile, sV = sK + NST * Sh::kTile;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(gbase + (size_t)Sh::kTile * (1 + 2 * NST));
-    const uint32_t barQ = smem_addr(bars), barS = barQ + 8, barP = barQ + 16, barO = barQ + 24, barK = barQ + 32,
-                   barV = barK + 8 * NST;
+    const uint32_t barQ = smem_addr(bars), barS = barQ + 8, barP = barQ + 16, barO = barQ + 24, barR = barQ + 32,
+                   barK = barQ + 40, barV = barK + 8 * NST;
     volatile int* const dead = reinterpret_cast<volatile int*>(bars + Sh::kBars);
     uint32_t* const slot = reinterpret_cast<uint32_t*>(bars + Sh::kBars) + 1;
     float* const lut = reinterpret_cast<float*>(bars + Sh::kBars + 2);
     const int reach = BIAS ? reach_of(a.edges) : 0;
 
-    if (tid == 0) {
-        bar_init(barQ, 1), bar_init(barS, 1), bar_init(barP, 4), bar_init(barO, 1);
-        for (int s = 0; s < NST; ++s) bar_init(barK + 8 * s, 1), bar_init(barV + 8 * s, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        *dead = 0;
+    const int kh = h / (a.H / a.Hkv);
+    auto load = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, uint32_t bar) {
+        bar_expect(bar, Sh::kTile);
+#pragma unroll
+        for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * kChunk, tm, 64 * c, row, head, b, bar);
+    };
+    auto load_k = [&](int j) { load(sK + (j % NST) * Sh::kTile, &tmK, j * kRows, kh, barK + 8 * (j % NST)); };
+    auto load_v = [&](int j) { load(sV + (j % NST) * Sh::kTile, &tmV, j * kRows, kh, barV + 8 * (j % NST)); };
+    if (warp == 4) {   // barriers, and the first copies before the CTA meets
+        if (lane == 0) {
+            bar_init(barQ, 1), bar_init(barS, 1), bar_init(barP, 4), bar_init(barO, 1), bar_init(barR, 4);
+            for (int s = 0; s < NST; ++s) bar_init(barK + 8 * s, 1), bar_init(barV + 8 * s, 1);
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+            fence_async_smem();
+            *dead = 0;
+            load(sQ, &tmQ, q0, h, barQ);
+            for (int j = 0; j < NST && j < tiles; ++j) load_k(j), load_v(j);
+        }
+        __syncwarp();
+        tmem_alloc(smem_addr(slot), kColumns);
+    } else if (BIAS) {
+        fill_lut<T>(lut, a, h, reach, warp, 4);
     }
-    if (warp == 4) tmem_alloc(smem_addr(slot), kColumns);
-    if (BIAS)
-        for (int i = tid; i < lut_size(reach); i += kThreads) lut[i] = bias_log2<T>(a, bucket_of(a.edges, i - reach - kPad), h);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot, tO = tmem + 128;
+    const uint32_t tmem = *slot, tO = tmem + 128, tP = tmem + (Sh::kApart ? 192 : 0);
 
     if (warp == 4) {
-        if (lane == 0) {
-            const int kh = h / (a.H / a.Hkv);
-            auto load = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, uint32_t bar) {
-                bar_expect(bar, Sh::kTile);
+        // the whole warp runs this, so that the operands' words stay in uniform registers; one lane issues
+        const bool lead = elect_one();
+        const int nu = __shfl_sync(0xffffffffu, tiles, 0);
+        const uint32_t uS = __shfl_sync(0xffffffffu, tmem, 0), uO = uS + 128, uP = uS + (Sh::kApart ? 192 : 0);
+        constexpr uint32_t idS = mma_desc<T>(128, 128, false), idO = mma_desc<T>(128, DP, true);
+        auto scores = [&](int j) {
+            const int s = j % NST;
+            if (!bar_wait_warp(barK + 8 * s, (j / NST) & 1, dead)) return false;
+            tc_fence_after();
+            const uint32_t dQ = desc_along(sQ), dK = desc_along(sK + s * Sh::kTile);
 #pragma unroll
-                for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * kChunk, tm, 64 * c, row, head, b, bar);
-            };
-            load(sQ, &tmQ, q0, h, barQ);
-            for (int s = 0; s < NST && s < tiles; ++s) {
-                load(sK + s * Sh::kTile, &tmK, s * kRows, kh, barK + 8 * s);
-                load(sV + s * Sh::kTile, &tmV, s * kRows, kh, barV + 8 * s);
+            for (int k = 0; k < DP / 16; ++k) {
+                const uint32_t o = ((k / 4) * kChunk + (k % 4) * 32) / 16;
+                if (lead) mma_ss(uS, dQ + o, dK + o, idS, k != 0);
             }
-            constexpr uint32_t idS = mma_desc<T>(128, 128, false), idO = mma_desc<T>(128, DP, true);
-            bool ok = bar_wait(barQ, 0, dead);
-            int j = 0;
-            for (; ok && j < tiles; ++j) {
-                const int s = j % NST;
-                const uint32_t ph = (j / NST) & 1;
-                if (!(ok = bar_wait(barK + 8 * s, ph, dead))) break;
-                tc_fence_after();
-                const uint32_t dQ = desc_along(sQ), dK = desc_along(sK + s * Sh::kTile);
+            if (lead) tc_commit(barS);
+            return true;
+        };
+        bool ok = bar_wait_warp(barQ, 0, dead) && scores(0);
+        int j = 0;
+        for (; ok && j < nu; ++j) {
+            const int s = j % NST;
+            // S done, and read into registers where P has columns of its own: K's tile is free, and the next S can begin
+            if (!(ok = bar_wait_warp(Sh::kApart ? barR : barS, j & 1, dead))) break;
+            if (j + NST < nu && lead) load_k(j + NST);
+            // (S j was issued after the product before: that one is over too, and its V tile free)
+            if (!Sh::kApart && j > 0 && j - 1 + NST < nu && lead) load_v(j - 1 + NST);
+            if (Sh::kApart && j + 1 < nu && !(ok = scores(j + 1))) break;
+            if (!(ok = bar_wait_warp(barV + 8 * s, (j / NST) & 1, dead) && bar_wait_warp(barP, j & 1, dead))) break;
+            // (P j was written after the product before was over: its V tile is free)
+            if (Sh::kApart && j > 0 && j - 1 + NST < nu && lead) load_v(j - 1 + NST);
+            tc_fence_after();
+            const uint32_t dV = desc_down(sV + s * Sh::kTile, kChunk);
 #pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    const uint32_t o = ((k / 4) * kChunk + (k % 4) * 32) / 16;
-                    mma_ss(tmem, dQ + o, dK + o, idS, k != 0);
-                }
-                tc_commit(barS);
-                // S (and every product before it) done: its K tile is free, and V's of the tile before
-                if (!(ok = bar_wait(barS, j & 1, dead))) break;
-                if (j > 0 && j - 1 + NST < tiles) {
-                    const int t = j - 1 + NST;
-                    load(sV + (t % NST) * Sh::kTile, &tmV, t * kRows, kh, barV + 8 * (t % NST));
-                }
-                if (j + NST < tiles) load(sK + s * Sh::kTile, &tmK, (j + NST) * kRows, kh, barK + 8 * s);
-                if (!(ok = bar_wait(barV + 8 * s, ph, dead) && bar_wait(barP, j & 1, dead))) break;
-                tc_fence_after();
-                const uint32_t dV = desc_down(sV + s * Sh::kTile, kChunk);
-#pragma unroll
-                for (int k = 0; k < kRows / 16; ++k) mma_ts(tO, tmem + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
-                tc_commit(barO);
+            for (int k = 0; k < kRows / 16; ++k)
+                if (lead) mma_ts(uO, uP + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
+            if (lead) tc_commit(barO);
+            if (!Sh::kApart && j + 1 < nu) ok = scores(j + 1);
+        }
+        if (!ok) {   // a wait gave up: what is in flight ends (bounded) before the CTA does
+            volatile int none = 0;
+            for (int t = max(j - 1, 0); t < min(j + 1 + NST, nu); ++t) {
+                bar_wait(barK + 8 * (t % NST), (t / NST) & 1, &none);
+                bar_wait(barV + 8 * (t % NST), (t / NST) & 1, &none);
             }
-            if (!ok) {   // a wait gave up: what is in flight ends (bounded) before the CTA does
-                volatile int none = 0;
-                for (int t = max(j - 1, 0); t < min(j + NST, tiles); ++t) {
-                    bar_wait(barK + 8 * (t % NST), (t / NST) & 1, &none);
-                    bar_wait(barV + 8 * (t % NST), (t / NST) & 1, &none);
-                }
-                bar_wait(barQ, 0, &none);
-                atomicAdd(&g_gave_up, 1ull);
-            }
+            bar_wait(barQ, 0, &none);
+            if (lead) atomicAdd(&g_gave_up, 1ull);
         }
         __syncwarp();
     } else {
@@ -163,17 +178,24 @@ __global__ void __launch_bounds__(kThreads, 2)
             tmem_wait_ld();
 #pragma unroll
             for (int x = 0; x < 4; ++x) tmem_tie32(v + 32 * x);
+            if (Sh::kApart) {
+                tc_fence_before();
+                bar_arrive_warp(barR);
+            }
             float* const t = reinterpret_cast<float*>(v);
-            if (BIAS) {   // scores in base 2; tiles that lie past the last edge take one value
-                const int dmin = k0 - (q0 + kRows - 1 + off), dmax = k0 + kRows - 1 - (q0 + off);
-                if (dmin < reach && dmax > -reach) {
-                    const float* const lp = lut + (k0 - pos + reach + kPad);
+            if (BIAS) {   // scores in base 2; blocks of 32 x 32 that lie past the last edge take one value
+                const float* const lp = lut + (k0 - pos + reach + kPad);
+                const int dmin = k0 - (q0 + 32 * warp + 31 + off);
 #pragma unroll
-                    for (int x = 0; x < 128; ++x) t[x] = fmaf(t[x], c, lp[x]);
-                } else {
-                    const float far = dmin >= reach ? lut[lut_size(reach) - 1] : lut[0];
+                for (int x = 0; x < 128; x += 32) {
+                    if (dmin + x < reach && dmin + x + 62 > -reach) {
 #pragma unroll
-                    for (int x = 0; x < 128; ++x) t[x] = fmaf(t[x], c, far);
+                        for (int y = x; y < x + 32; ++y) t[y] = fmaf(t[y], c, lp[y]);
+                    } else {
+                        const float far = dmin + x >= reach ? lut[lut_size(reach) - 1] : lut[0];
+#pragma unroll
+                        for (int y = x; y < x + 32; ++y) t[y] = fmaf(t[y], c, far);
+                    }
                 }
             }
             if (k0 + kRows > lk || (a.causal && k0 + kRows - 1 > q0 + off)) {
@@ -195,9 +217,13 @@ __global__ void __launch_bounds__(kThreads, 2)
                 m = top;
                 l *= f;
             }
-            if (__any_sync(0xffffffffu, raise) && j > 0) {   // O's rows of this warp, once the product before is in
+            const bool rescale = __any_sync(0xffffffffu, raise) && j > 0;
+            // the product before reads P's columns and adds to O
+            if (j > 0 && (Sh::kApart || rescale)) {
                 if (!(ok = bar_wait_warp(barO, (j - 1) & 1, dead))) break;
                 tc_fence_after();
+            }
+            if (rescale) {   // O's rows of this warp
 #pragma unroll 1
                 for (int x = 0; x < DP; x += 32) {
                     uint32_t o[32];
@@ -223,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     sum[(y & 2) + 1] += e1;
                     p[y / 2] = pack2<T>(e0, e1);
                 }
-                tmem_st16(tmem + trow + x / 2, p);
+                tmem_st16(tP + trow + x / 2, p);
             }
             l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
             const int live = lk - k0;

@@ -180,6 +180,31 @@ constexpr int kPad = 256;
 __host__ __device__ inline int reach_of(const Edges& e) { return e.n ? e.e[e.n - 1] : 1; }
 __host__ __device__ inline int lut_size(int reach) { return 2 * (reach + kPad) + 1; }
 
+// positions d of bucket t, clipped to +-far
+__device__ __forceinline__ int2 bucket_range(const Edges& e, int t, int far) {
+    const int side = e.n + 1, u = t < side ? t : t - side;
+    const int lo = u ? e.e[u - 1] : 0, hi = u < e.n ? e.e[u] - 1 : far;
+    if (t >= side) return make_int2(max(lo, 1), min(hi, far));
+    return make_int2(-min(hi, far), !e.two && u == 0 ? far : -lo);
+}
+// fills lut for head h by `warps` warps, a bucket each in turn: its value is
+// fetched once, its positions are consecutive
+template <class T>
+__device__ __forceinline__ void fill_lut(float* lut, const AttnArgs& a, int h, int reach, int warp, int warps) {
+    const int lane = threadIdx.x & 31, nb = n_buckets(a.edges), far = reach + kPad;
+    float mine[(kMaxEdges + 1) / 16];
+#pragma unroll
+    for (int i = 0; i < (kMaxEdges + 1) / 16; ++i) mine[i] = lane + 32 * i < nb ? bias_log2<T>(a, lane + 32 * i, h) : 0.f;
+    for (int t = warp; t < nb; t += warps) {
+        float v = mine[0];
+#pragma unroll
+        for (int i = 1; i < (kMaxEdges + 1) / 16; ++i) v = t >> 5 == i ? mine[i] : v;
+        v = __shfl_sync(0xffffffffu, v, t & 31);
+        const int2 r = bucket_range(a.edges, t, far);
+        for (int d = r.x + lane; d <= r.y; d += 32) lut[d + far] = v;
+    }
+}
+
 // [B, L, heads, D] rows with element strides s (batch, position, head) as a 4-D
 // tensor (D, position, head, batch) in boxes of 64 elements x rows
 bool rows_map(CUtensorMap* tm, int dtype, const void* base, int B, int L, int heads, int D, const long long* s, int rows);
