@@ -1193,23 +1193,168 @@ Tensor dropout_add_cuda(const Tensor& x, const c10::optional<Tensor>& residual, 
     return y;
 }
 
+// ---- autograd: the user's operators, as nodes over the operators above (called through the dispatcher, so that
+// fake tensors meet their registered shapes) ----
+using OptTensor = c10::optional<Tensor>;
+OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+Tensor undef(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+
+std::tuple<Tensor, Tensor> call_attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
+                                                  const OptTensor& lengths, at::IntArrayRef edges, double scale, bool causal,
+                                                  bool want_lse) {
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("d2p_b200::attention_forward", "")
+                         .typed<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                                                           const OptTensor&, at::IntArrayRef, double, bool, bool)>();
+    return op.call(q, k, v, bias, lengths, edges, scale, causal, want_lse);
+}
+
+class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
+   public:
+    static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
+                          const OptTensor& lengths, at::IntArrayRef edges, double scale, bool causal) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto r = call_attention_forward(q, k, v, bias, lengths, edges, scale, causal, true);
+        ctx->save_for_backward({q, k, v, undef(bias), undef(lengths), std::get<0>(r), std::get<1>(r)});
+        ctx->saved_data["edges"] = edges.vec();
+        ctx->saved_data["scale"] = scale;
+        ctx->saved_data["causal"] = causal;
+        ctx->saved_data["want_bias"] = bias.has_value() && wants_grad(*bias);
+        return std::get<0>(r);
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        static auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("d2p_b200::attention_backward", "")
+                             .typed<std::tuple<Tensor, Tensor, Tensor, Tensor>(
+                                 const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                                 const OptTensor&, at::IntArrayRef, double, bool, const Tensor&, const Tensor&, bool)>();
+        auto s = ctx->get_saved_variables();
+        const std::vector<int64_t> edges = ctx->saved_data["edges"].toIntVector();
+        const bool want_bias = ctx->saved_data["want_bias"].toBool();
+        auto r = op.call(grads[0], s[0], s[1], s[2], opt(s[3]), opt(s[4]), edges, ctx->saved_data["scale"].toDouble(),
+                         ctx->saved_data["causal"].toBool(), s[5], s[6], want_bias);
+        return {std::get<0>(r), std::get<1>(r), std::get<2>(r), want_bias ? std::get<3>(r) : Tensor(),
+                Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias, const OptTensor& lengths,
+                          at::IntArrayRef edges, double scale, bool causal) {
+    if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(undef(bias))))
+        return AttentionFunction::apply(q, k, v, bias, lengths, edges, scale, causal);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return std::get<0>(call_attention_forward(q, k, v, bias, lengths, edges, scale, causal, false));
+}
+Tensor attention_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias, const OptTensor& lengths,
+                      at::IntArrayRef edges, double scale, bool causal) {
+    return std::get<0>(attention_forward_cuda(q, k, v, bias, lengths, edges, scale, causal, false));
+}
+
+std::tuple<Tensor, Tensor> call_norm_rope_forward(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
+                                                  const Tensor& cos, const Tensor& sin, const OptTensor& positions, double eps) {
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("d2p_b200::qk_norm_rope_forward", "")
+                         .typed<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                           const Tensor&, const Tensor&, const OptTensor&, double)>();
+    return op.call(q, k, qw, kw, cos, sin, positions, eps);
+}
+
+class NormRopeFunction : public torch::autograd::Function<NormRopeFunction> {
+   public:
+    static tensor_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
+                               const Tensor& cos, const Tensor& sin, const OptTensor& positions, double eps) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        auto r = call_norm_rope_forward(q, k, qw, kw, cos, sin, positions, eps);
+        ctx->save_for_backward({q, k, qw, kw, cos, sin, undef(positions)});
+        ctx->saved_data["eps"] = eps;
+        return {std::get<0>(r), std::get<1>(r)};
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        static auto op = c10::Dispatcher::singleton()
+                             .findSchemaOrThrow("d2p_b200::qk_norm_rope_backward", "")
+                             .typed<std::tuple<Tensor, Tensor, Tensor, Tensor>(
+                                 const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                 const Tensor&, const Tensor&, const OptTensor&, double)>();
+        auto s = ctx->get_saved_variables();
+        auto r = op.call(grads[0], grads[1], s[0], s[1], s[2], s[3], s[4], s[5], opt(s[6]), ctx->saved_data["eps"].toDouble());
+        return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+std::tuple<Tensor, Tensor> qk_norm_rope_autograd(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
+                                                 const Tensor& cos, const Tensor& sin, const OptTensor& positions, double eps) {
+    if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(qw) || wants_grad(kw))) {
+        auto r = NormRopeFunction::apply(q, k, qw, kw, cos, sin, positions, eps);
+        return {r[0], r[1]};
+    }
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_norm_rope_forward(q, k, qw, kw, cos, sin, positions, eps);
+}
+
+Tensor call_dropout(const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset) {
+    static auto op = c10::Dispatcher::singleton()
+                         .findSchemaOrThrow("d2p_b200::dropout_add_forward", "")
+                         .typed<Tensor(const Tensor&, const OptTensor&, double, int64_t, int64_t)>();
+    return op.call(x, residual, p, seed, offset);
+}
+
+class DropoutFunction : public torch::autograd::Function<DropoutFunction> {
+   public:
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset) {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        ctx->saved_data["p"] = p;
+        ctx->saved_data["seed"] = seed;
+        ctx->saved_data["offset"] = offset;
+        ctx->saved_data["dx"] = wants_grad(x);
+        ctx->saved_data["dr"] = residual.has_value() && wants_grad(*residual);
+        return call_dropout(x, residual, p, seed, offset);
+    }
+    static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
+        Tensor dx;
+        if (ctx->saved_data["dx"].toBool())
+            dx = call_dropout(grads[0], OptTensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
+                              ctx->saved_data["offset"].toInt());
+        return {dx, ctx->saved_data["dr"].toBool() ? grads[0] : Tensor(), Tensor(), Tensor(), Tensor()};
+    }
+};
+
+Tensor dropout_add_autograd(const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset) {
+    if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(undef(residual))))
+        return DropoutFunction::apply(x, residual, p, seed, offset);
+    at::AutoDispatchBelowADInplaceOrView guard;
+    return call_dropout(x, residual, p, seed, offset);
+}
+
 TORCH_LIBRARY_FRAGMENT(d2p_b200, m) {
     m.def("embed_scores(Tensor x, Tensor y, float scale) -> Tensor");
     m.def("embed_grad_scores(Tensor marginals, Tensor grad_value, float scale) -> Tensor");
+    // what a user calls (with gradients), and the parts they are made of
+    m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal) -> Tensor");
     m.def("attention_forward(Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal, bool want_lse) -> (Tensor, Tensor)");
     m.def("attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal, Tensor out, Tensor lse, bool want_bias) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("qk_norm_rope(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor)");
+    m.def("qk_norm_rope_forward(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor)");
     m.def("qk_norm_rope_backward(Tensor grad_q, Tensor grad_k, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("dropout_add(Tensor x, Tensor? residual, float p, int seed, int offset) -> Tensor");
+    m.def("dropout_add_forward(Tensor x, Tensor? residual, float p, int seed, int offset) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(d2p_b200, CUDA, m) {
     m.impl("embed_scores", embed_scores_cuda);
     m.impl("embed_grad_scores", embed_grad_scores_cuda);
+    m.impl("attention", attention_cuda);
     m.impl("attention_forward", attention_forward_cuda);
     m.impl("attention_backward", attention_backward_cuda);
     m.impl("qk_norm_rope", qk_norm_rope_cuda);
+    m.impl("qk_norm_rope_forward", qk_norm_rope_cuda);
     m.impl("qk_norm_rope_backward", qk_norm_rope_backward_cuda);
     m.impl("dropout_add", dropout_add_cuda);
+    m.impl("dropout_add_forward", dropout_add_cuda);
+}
+TORCH_LIBRARY_IMPL(d2p_b200, AutogradCUDA, m) {
+    m.impl("attention", attention_autograd);
+    m.impl("qk_norm_rope", qk_norm_rope_autograd);
+    m.impl("dropout_add", dropout_add_autograd);
 }
 
 TORCH_LIBRARY_FRAGMENT(d2p, m) {

@@ -16,6 +16,11 @@ import torch
 
 from . import _ops  # noqa: F401  the native extension (fails loudly if missing)
 
+# the operators with their gradients (autograd nodes in csrc/torch_bindings.cpp)
+_ops_attention = torch.ops.d2p_b200.attention.default
+_ops_qk_norm_rope = torch.ops.d2p_b200.qk_norm_rope.default
+_ops_dropout_add = torch.ops.d2p_b200.dropout_add.default
+
 _MAX_REACH = 1024
 _MAX_SIDE = 64
 
@@ -44,23 +49,6 @@ def relative_bucket_edges(num_buckets: int, max_distance: int = 128, two_sided: 
             n += 1
         edges.append(n)
     return tuple(edges)
-
-
-class _Attention(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, bias, lengths, edges, scale, causal):
-        out, lse = torch.ops.d2p_b200.attention_forward(q, k, v, bias, lengths, edges, scale, causal, True)
-        ctx.save_for_backward(q, k, v, bias, lengths, out, lse)
-        ctx.edges, ctx.scale, ctx.causal = edges, scale, causal
-        return out
-
-    @staticmethod
-    def backward(ctx, grad):
-        q, k, v, bias, lengths, out, lse = ctx.saved_tensors
-        want = bias is not None and ctx.needs_input_grad[3]
-        dq, dk, dv, db = torch.ops.d2p_b200.attention_backward(grad, q, k, v, bias, lengths, ctx.edges, ctx.scale,
-                                                               ctx.causal, out, lse, want)
-        return dq, dk, dv, db if want else None, None, None, None, None
 
 
 def attention(
@@ -103,25 +91,7 @@ def attention(
         edges = relative_bucket_edges(int(bias.shape[0]), int(max_distance), not causal)
     if lengths is not None and (lengths.dtype != torch.int32 or tuple(lengths.shape) != (q.shape[0], 2)):
         raise ValueError("attention: lengths must be int32 [B, 2]")
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, bias))
-    if grad:
-        return _Attention.apply(q, k, v, bias, lengths, edges, scale, bool(causal))
-    return torch.ops.d2p_b200.attention_forward(q, k, v, bias, lengths, edges, scale, bool(causal), False)[0]
-
-
-class _QKNormRope(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps):
-        ctx.save_for_backward(q, k, q_weight, k_weight, cos, sin, positions)
-        ctx.eps = eps
-        return torch.ops.d2p_b200.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps)
-
-    @staticmethod
-    def backward(ctx, gq, gk):
-        q, k, q_weight, k_weight, cos, sin, positions = ctx.saved_tensors
-        dq, dk, dqw, dkw = torch.ops.d2p_b200.qk_norm_rope_backward(gq, gk, q, k, q_weight, k_weight, cos, sin,
-                                                                    positions, ctx.eps)
-        return dq, dk, dqw, dkw, None, None, None, None
+    return _ops_attention(q, k, v, bias, lengths, edges, scale, bool(causal))
 
 
 def qk_norm_rope(
@@ -165,23 +135,7 @@ def qk_norm_rope(
         raise ValueError("qk_norm_rope: positions must be int32 or int64 [B, L] or [L]")
     if not eps >= 0.0:
         raise ValueError(f"qk_norm_rope: eps must not be negative, got {eps}")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, q_weight, k_weight)):
-        return _QKNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps))
-    return torch.ops.d2p_b200.qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, float(eps))
-
-
-class _DropoutAdd(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, residual, p, seed, offset):
-        ctx.p, ctx.seed, ctx.offset = p, seed, offset
-        return torch.ops.d2p_b200.dropout_add(x, residual, p, seed, offset)
-
-    @staticmethod
-    def backward(ctx, grad):
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = torch.ops.d2p_b200.dropout_add(grad, None, ctx.p, ctx.seed, ctx.offset)
-        return dx, grad if ctx.needs_input_grad[1] else None, None, None, None
+    return _ops_qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, float(eps))
 
 
 def dropout_add(
@@ -207,14 +161,16 @@ def dropout_add(
     for name, value in (("seed", seed), ("offset", offset)):
         if not 0 <= value < 2 ** 63:
             raise ValueError(f"dropout_add: {name} must be in [0, 2^63), got {value}")
-    if torch.is_grad_enabled() and (x.requires_grad or (residual is not None and residual.requires_grad)):
-        return _DropoutAdd.apply(x, residual, float(p), int(seed), int(offset))
-    return torch.ops.d2p_b200.dropout_add(x, residual, float(p), int(seed), int(offset))
+    return _ops_dropout_add(x, residual, float(p), int(seed), int(offset))
 
 
 def _attention_forward_fake(q, k, v, bias, lengths, bucket_edges, scale, causal, want_lse):
     lse = q.new_empty((q.shape[0] if want_lse else 0, q.shape[2], q.shape[1]), dtype=torch.float32)
     return q.new_empty(q.shape), lse
+
+
+def _attention_fake(q, k, v, bias, lengths, bucket_edges, scale, causal):
+    return q.new_empty(q.shape)
 
 
 def _attention_backward_fake(grad, q, k, v, bias, lengths, bucket_edges, scale, causal, out, lse, want_bias):
@@ -234,7 +190,7 @@ def _dropout_add_fake(x, residual, p, seed, offset):
     return x.new_empty(x.shape)
 
 
-for _name, _fake in (("attention_forward", _attention_forward_fake), ("attention_backward", _attention_backward_fake),
-                     ("qk_norm_rope", _qk_norm_rope_fake), ("qk_norm_rope_backward", _qk_norm_rope_backward_fake),
-                     ("dropout_add", _dropout_add_fake)):
+for _name, _fake in (("attention", _attention_fake), ("attention_forward", _attention_forward_fake), ("attention_backward", _attention_backward_fake),
+                     ("qk_norm_rope", _qk_norm_rope_fake), ("qk_norm_rope_forward", _qk_norm_rope_fake), ("qk_norm_rope_backward", _qk_norm_rope_backward_fake),
+                     ("dropout_add", _dropout_add_fake), ("dropout_add_forward", _dropout_add_fake)):
     torch.library.register_fake("d2p_b200::" + _name)(_fake)
