@@ -45,10 +45,23 @@ __device__ __forceinline__ void problem_lengths(const AttnArgs& a, int b, int* l
     }
 }
 
+// the softmax's running reference is raised when a row's maximum passes it by
+// more than kSlack (2^kSlack stays in range of the 16-bit types)
+template <class T>
+struct Softmax {   // fp16: probabilities start at 2^8, so that small ones stay above its subnormals
+    static constexpr float kShift = 0.f, kSlack = 8.f;
+};
+template <>
+struct Softmax<__half> {
+    static constexpr float kShift = 8.f, kSlack = 7.f;
+};
+
 // checks of the C entry points; fills *a
 int attn_args(const d2p_attention_args* p, AttnArgs* a);
 // out and lse (or null) by tiles of 128 query rows (enc_attn_fwd.cu)
 int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st);
+// the same for at most 16 query rows of a key head, split over the keys (enc_attn_token.cu)
+int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st);
 // the gradients (enc_attn_bwd.cu) and their workspace
 size_t attn_backward_bytes(const AttnArgs& a, bool dbias);
 int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const float* lse, const void* grad, void* dq,

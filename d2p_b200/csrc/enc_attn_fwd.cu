@@ -15,15 +15,6 @@
 namespace d2pb {
 namespace enc {
 
-template <class T>
-struct Softmax {   // fp16: probabilities start at 2^8, so that small ones stay above its subnormals
-    static constexpr float kShift = 0.f, kSlack = 8.f;
-};
-template <>
-struct Softmax<__half> {
-    static constexpr float kShift = 8.f, kSlack = 7.f;
-};
-
 namespace fwd {
 
 constexpr int kThreads = 160;   // a softmax warpgroup and the warp that copies and multiplies

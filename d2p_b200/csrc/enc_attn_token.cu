@@ -1,0 +1,292 @@
+// enc_attn_token.cu -- attention of a few query rows over a long cache: single
+// tokens when serving.
+//
+// The query rows of one key head (queries x the heads that share it, at most 16)
+// are one 16-row operand of the warp-level matrix instructions, so that each key
+// and value is read once for all of them: the cache's bytes are what bounds
+// this, and 16 rows are too few to gain from the larger tensor-core tiles.  The
+// keys are split over the CTAs of a cluster and over a CTA's warps; a warp takes
+// 16 keys at a time through its own ring of shared memory (cp.async, so no
+// barrier in the loop) with a running maximum and sum, and the partial results
+// join in shared memory, then through the cluster's: one launch, no workspace,
+// a fixed order.
+#include <cooperative_groups.h>
+
+#include "enc_attn.cuh"
+
+namespace d2pb {
+namespace enc {
+namespace tok {
+
+namespace cg = cooperative_groups;
+
+constexpr int kWarps = 4, kKeys = 16, kRowsM = 16;
+constexpr int kMinRounds = 2;   // of a CTA's warps: the least keys worth a CTA of their own
+
+template <int DP>
+struct Shape {
+    static constexpr int kStages = DP == 64 ? 4 : 3;
+    static constexpr int kTile = kKeys * DP * 2;                  // bytes of a warp's 16 keys (or values)
+    static constexpr int kRing = kWarps * kStages * 2 * kTile;    // 64 KB / 96 KB
+    static constexpr int kJoin = kWarps * kRowsM * (DP + 4) * 4 + 2 * kWarps * kRowsM * 4;   // in the ring's place
+};
+
+template <class T>
+__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t* r, uint32_t addr) {
+    if (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// one side's bucket of each position by search: only the few blocks near the queries come here
+__device__ __forceinline__ int bucket_of(const Edges& e, int d) {
+    const int n = e.two ? abs(d) : max(-d, 0);
+    int lo = 0, hi = e.n;         // the number of edges <= n
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (e.e[mid] <= n) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo + ((e.two && d > 0) ? e.n + 1 : 0);
+}
+
+template <class T, int DP>
+__global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_constant__ AttnArgs a, T* __restrict__ out,
+                                                                float* __restrict__ lse) {
+    using Sh = Shape<DP>;
+    constexpr int NST = Sh::kStages, CH = DP / 8;   // 16-byte units of a row
+    extern __shared__ __align__(128) uint8_t sm[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const int split = blockIdx.x, splits = gridDim.x, kh = blockIdx.y, b = blockIdx.z;
+    const int G = a.H / a.Hkv, rows = a.Lq * G;
+    int lq, lk;
+    problem_lengths(a, b, &lq, &lk);
+    const int off = a.causal ? lk - lq : 0;
+    // keys any row meets, and this CTA's share in whole rounds of its warps
+    const int most = lq > 0 ? (a.causal ? min(lk, lq + off) : lk) : 0;
+    const int round = kWarps * kKeys;
+    const int share = max(((most + splits - 1) / splits + round - 1) / round, kMinRounds) * round;
+    const int k0 = min(most, split * share), k1 = min(most, k0 + share);
+
+    // rows g and g + 8 of the operand: query i = row / G, head kh G + row % G
+    int qi[2], head[2], lim[2];
+    bool live[2];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const int r = g + 8 * w;
+        qi[w] = r / G, head[w] = kh * G + r % G;
+        live[w] = r < rows && qi[w] < lq;
+        lim[w] = live[w] ? (a.causal ? min(lk, qi[w] + off + 1) : lk) : 0;   // keys of the row: [0, lim)
+    }
+    uint32_t qa[DP / 16][4];
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int w = x & 1, d = 16 * k + 2 * t + 8 * (x >> 1);
+            qa[k][x] = 0;
+            if (live[w] && d < a.D)
+                qa[k][x] = *reinterpret_cast<const uint32_t*>((const T*)a.q + b * a.qs[0] + qi[w] * a.qs[1] + head[w] * a.qs[2] + d);
+        }
+    const int reach = a.edges.n ? a.edges.e[a.edges.n - 1] : 1;
+    float before[2] = {0.f, 0.f}, after[2] = {0.f, 0.f};   // the bias past the last edge, on either side
+    if (a.bias) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w)
+            if (live[w]) {
+                before[w] = bias_log2<T>(a, a.edges.n, head[w]);
+                if (a.edges.two) after[w] = bias_log2<T>(a, 2 * a.edges.n + 1, head[w]);
+            }
+    }
+
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * NST * 2 * Sh::kTile;
+    const T* const kb = (const T*)a.k + b * a.ks[0] + kh * a.ks[2];
+    const T* const vb = (const T*)a.v + b * a.vs[0] + kh * a.vs[2];
+    auto fetch = [&](int at, int stage) {   // 16 keys and values from position `at` (zeros past k1 and past the head's size)
+#pragma unroll
+        for (int e = lane; e < kKeys * CH; e += 32) {
+            const int r = e / CH, c = e % CH;
+            const bool in = at + r < k1 && 8 * c < a.D;
+            const long long row = in ? at + r : 0;
+            const int col = in ? 8 * c : 0;
+            const uint32_t dst = ring + stage * 2 * Sh::kTile + r * (DP * 2) + ((c ^ (r & 7)) << 4);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(kb + row * a.ks[1] + col), "r"(in ? 16 : 0) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + Sh::kTile), "l"(vb + row * a.vs[1] + col), "r"(in ? 16 : 0) : "memory");
+        }
+    };
+    const int first = k0 + warp * kKeys, n = first < k1 ? (k1 - first + round - 1) / round : 0;
+#pragma unroll
+    for (int s = 0; s < NST - 1; ++s) {
+        if (s < n) fetch(first + s * round, s);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+
+    float o[DP / 8][4];
+#pragma unroll
+    for (int x = 0; x < DP / 8; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    const float c2 = a.scale * kLog2e;
+    for (int it = 0; it < n; ++it) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
+        __syncwarp();
+        if (it + NST - 1 < n) fetch(first + (it + NST - 1) * round, (it + NST - 1) % NST);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        const uint32_t ks = ring + (it % NST) * 2 * Sh::kTile, vs = ks + Sh::kTile;
+        const int at = first + it * round;
+        float s[2][4] = {};
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {   // matrices: keys 0-7 / 8-15 (lane >> 4) by elements 0-7 / 8-15 (lane >> 3 & 1)
+            const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * k + ((lane >> 3) & 1);
+            uint32_t f[4];
+            ldmatrix4<false>(f, ks + r * (DP * 2) + ((c ^ (r & 7)) << 4));
+            mma16816<T>(s[0], qa[k], f[0], f[1]);
+            mma16816<T>(s[1], qa[k], f[2], f[3]);
+        }
+        // element (w, j): row g + 8 w, key at + 8 (j >> 1) + 2 t + (j & 1)
+        float p[2][4];
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+            const int pos = qi[w] + off;
+            float top = -INFINITY;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int key = at + 8 * (j >> 1) + 2 * t + (j & 1);
+                float v = s[j >> 1][2 * w + (j & 1)] * c2;
+                if (a.bias && live[w]) {
+                    const int d = key - pos;
+                    v += d <= -reach ? before[w] : (a.edges.two && d >= reach) ? after[w] : bias_log2<T>(a, bucket_of(a.edges, d), head[w]);
+                }
+                p[w][j] = key < lim[w] ? v : -INFINITY;
+                top = fmaxf(top, p[w][j]);
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const bool raise = top > m[w] + Softmax<T>::kSlack || (m[w] == -INFINITY && top > -INFINITY);
+            if (__any_sync(0xffffffffu, raise)) {
+                const float f = raise ? (m[w] == -INFINITY ? 0.f : exp2_fast(m[w] - top)) : 1.f;
+                m[w] = raise ? top : m[w];
+                l[w] *= f;
+#pragma unroll
+                for (int x = 0; x < DP / 8; ++x) o[x][2 * w] *= f, o[x][2 * w + 1] *= f;
+            }
+            const float ref = (m[w] == -INFINITY ? 0.f : m[w]) - Softmax<T>::kShift;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                p[w][j] = exp2_fast(p[w][j] - ref);
+                l[w] += p[w][j];
+            }
+        }
+        const uint32_t pa[4] = {pack2<T>(p[0][0], p[0][1]), pack2<T>(p[1][0], p[1][1]), pack2<T>(p[0][2], p[0][3]), pack2<T>(p[1][2], p[1][3])};
+#pragma unroll
+        for (int x = 0; x < DP / 16; ++x) {   // matrices: keys 0-7 / 8-15 (lane >> 3 & 1) by elements 0-7 / 8-15 (lane >> 4)
+            const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * x + (lane >> 4);
+            uint32_t f[4];
+            ldmatrix4<true>(f, vs + r * (DP * 2) + ((c ^ (r & 7)) << 4));
+            mma16816<T>(o[2 * x], pa, f[0], f[1]);
+            mma16816<T>(o[2 * x + 1], pa, f[2], f[3]);
+        }
+        __syncwarp();
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        l[w] += __shfl_xor_sync(0xffffffffu, l[w], 1);
+        l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
+    }
+
+    // the CTA's warps join in the ring's place: o [warp][16][DP + 4], m and l [warp][16]; then one set a CTA
+    constexpr int kPitch = DP + 4;
+    float* const jo = reinterpret_cast<float*>(sm);
+    float* const jm = jo + kWarps * kRowsM * kPitch;
+    float* const jl = jm + kWarps * kRowsM;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+        const int r = warp * kRowsM + g + 8 * w;
+#pragma unroll
+        for (int x = 0; x < DP / 8; ++x)
+            *reinterpret_cast<float2*>(jo + r * kPitch + 8 * x + 2 * t) = make_float2(o[x][2 * w], o[x][2 * w + 1]);
+        if (t == 0) jm[r] = m[w], jl[r] = l[w];
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    // every CTA of the cluster finishes its part of the rows from all partial results: splits x warps of them
+    const int units = a.D / 2, parts = splits * kWarps;
+    for (int e = split * 32 * kWarps + tid; e < rows * units; e += splits * 32 * kWarps) {
+        const int r = e / units, d = 2 * (e % units), i = r / G, h = kh * G + r % G;
+        float top = -INFINITY;
+        for (int p = 0; p < parts; ++p) top = fmaxf(top, cluster.map_shared_rank(jm, p / kWarps)[(p % kWarps) * kRowsM + r]);
+        float sum = 0.f, x = 0.f, y = 0.f;
+        for (int p = 0; p < parts; ++p) {
+            const int at = (p % kWarps) * kRowsM + r;
+            const float pm = cluster.map_shared_rank(jm, p / kWarps)[at];
+            const float f = pm == -INFINITY ? 0.f : exp2_fast(pm - top);
+            const float pl = cluster.map_shared_rank(jl, p / kWarps)[at];
+            sum = f == 0.f && pl == pl ? sum : sum + f * pl;
+            const float2 v = *reinterpret_cast<const float2*>(cluster.map_shared_rank(jo, p / kWarps) + at * kPitch + d);
+            x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
+        }
+        const bool some = (sum > 0.f || sum != sum) && i < lq;
+        const float w = some ? 1.f / sum : 0.f;
+        *reinterpret_cast<uint32_t*>(out + (((size_t)b * a.Lq + i) * a.H + h) * a.D + d) = some ? pack2<T>(x * w, y * w) : 0u;
+        if (lse && d == 0) lse[((size_t)b * a.H + h) * a.Lq + i] = some ? top - Softmax<T>::kShift + log2f(sum) : INFINITY;
+    }
+    cluster.sync();   // the partial results are read from other CTAs
+}
+
+template <class T, int DP>
+int launch(const AttnArgs& a, void* out, float* lse, cudaStream_t st) {
+    using Sh = Shape<DP>;
+    constexpr int smem = Sh::kRing > Sh::kJoin ? Sh::kRing : Sh::kJoin;
+    static DeviceSetup setup;
+    int dev = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    int rc = device_setup(setup, dev, [] {
+        return (int)cudaFuncSetAttribute(attn_token_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    }, &sms);
+    if (rc) return rc;
+    // CTAs for two a SM, as far as the keys go round
+    int splits = 1;
+    while (splits < 8 && (long long)a.B * a.Hkv * splits < 2 * sms && (long long)a.Lk > (long long)splits * kMinRounds * kWarps * kKeys)
+        splits *= 2;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(splits, a.Hkv, a.B), cfg.blockDim = dim3(32 * kWarps), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    return (int)cudaLaunchKernelEx(&cfg, attn_token_kernel<T, DP>, a, (T*)out, lse);
+}
+
+}  // namespace tok
+
+int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st) {
+    if (dtype == D2P_DTYPE_BF16)
+        return a.D <= 64 ? tok::launch<__nv_bfloat16, 64>(a, out, lse, st) : tok::launch<__nv_bfloat16, 128>(a, out, lse, st);
+    return a.D <= 64 ? tok::launch<__half, 64>(a, out, lse, st) : tok::launch<__half, 128>(a, out, lse, st);
+}
+
+}  // namespace enc
+}  // namespace d2pb
