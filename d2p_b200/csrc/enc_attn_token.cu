@@ -21,14 +21,18 @@ namespace tok {
 namespace cg = cooperative_groups;
 
 constexpr int kWarps = 4, kKeys = 16, kRowsM = 16;
+constexpr int kMaxSplits = 16;  // CTAs of a cluster: past 8 is allowed on this device on request
 constexpr int kMinRounds = 2;   // of a CTA's warps: the least keys worth a CTA of their own
 
 template <int DP>
 struct Shape {
-    static constexpr int kStages = DP == 64 ? 4 : 3;
-    static constexpr int kTile = kKeys * DP * 2;                  // bytes of a warp's 16 keys (or values)
-    static constexpr int kRing = kWarps * kStages * 2 * kTile;    // 64 KB / 96 KB
-    static constexpr int kJoin = kWarps * kRowsM * (DP + 4) * 4 + 2 * kWarps * kRowsM * 4;   // in the ring's place
+    static constexpr int kStages = 3;
+    static constexpr int kResident = DP == 64 ? 4 : 2;            // CTAs an SM holds
+    static constexpr int kTile = kKeys * DP * 2;                  // bytes of a warp's keys (or values)
+    static constexpr int kRing = kWarps * kStages * 2 * kTile;    // 48 KB / 96 KB
+    // in the ring's place: the warps' partial results, the CTA's, and the weights of the cluster's
+    static constexpr int kPitch = DP + 4;
+    static constexpr int kJoin = 4 * ((kWarps + 1) * kRowsM * (kPitch + 2) + kRowsM * kMaxSplits);
 };
 
 template <class T>
@@ -121,24 +125,28 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
     }
 
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(sm) + warp * NST * 2 * Sh::kTile;
-    const T* const kb = (const T*)a.k + b * a.ks[0] + kh * a.ks[2];
-    const T* const vb = (const T*)a.v + b * a.vs[0] + kh * a.vs[2];
-    auto fetch = [&](int at, int stage) {   // 16 keys and values from position `at` (zeros past k1 and past the head's size)
-#pragma unroll
-        for (int e = lane; e < kKeys * CH; e += 32) {
-            const int r = e / CH, c = e % CH;
-            const bool in = at + r < k1 && 8 * c < a.D;
-            const long long row = in ? at + r : 0;
-            const int col = in ? 8 * c : 0;
-            const uint32_t dst = ring + stage * 2 * Sh::kTile + r * (DP * 2) + ((c ^ (r & 7)) << 4);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(kb + row * a.ks[1] + col), "r"(in ? 16 : 0) : "memory");
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + Sh::kTile), "l"(vb + row * a.vs[1] + col), "r"(in ? 16 : 0) : "memory");
-        }
-    };
     const int first = k0 + warp * kKeys, n = first < k1 ? (k1 - first + round - 1) / round : 0;
+    // a lane copies unit fc of rows fr, fr + kStep, ..; zeros past k1 and past the head's size
+    constexpr int kStep = 32 / CH;
+    const int fr = lane / CH, fc = lane % CH;
+    const bool fin = 8 * fc < a.D;
+    const T* kp = (const T*)a.k + b * a.ks[0] + kh * a.ks[2] + (long long)(first + fr) * a.ks[1] + 8 * fc;
+    const T* vp = (const T*)a.v + b * a.vs[0] + kh * a.vs[2] + (long long)(first + fr) * a.vs[1] + 8 * fc;
+    int fat = first + fr;
+    auto fetch = [&](int stage) {
+        const uint32_t dst = ring + stage * 2 * Sh::kTile + fr * (DP * 2);
+#pragma unroll
+        for (int i = 0; i < kKeys / kStep; ++i) {
+            const bool in = fin && fat + i * kStep < k1;
+            const uint32_t d = dst + i * kStep * (DP * 2) + ((fc ^ ((fr + i * kStep) & 7)) << 4);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(in ? kp + i * kStep * a.ks[1] : (const T*)a.k), "r"(in ? 16 : 0) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + Sh::kTile), "l"(in ? vp + i * kStep * a.vs[1] : (const T*)a.v), "r"(in ? 16 : 0) : "memory");
+        }
+        kp += round * a.ks[1], vp += round * a.vs[1], fat += round;
+    };
 #pragma unroll
     for (int s = 0; s < NST - 1; ++s) {
-        if (s < n) fetch(first + s * round, s);
+        if (s < n) fetch(s);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
@@ -150,61 +158,71 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
     for (int it = 0; it < n; ++it) {
         asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
         __syncwarp();
-        if (it + NST - 1 < n) fetch(first + (it + NST - 1) * round, (it + NST - 1) % NST);
+        if (it + NST - 1 < n) fetch((it + NST - 1) % NST);
         asm volatile("cp.async.commit_group;" ::: "memory");
         const uint32_t ks = ring + (it % NST) * 2 * Sh::kTile, vs = ks + Sh::kTile;
         const int at = first + it * round;
-        float s[2][4] = {};
+        float s[kKeys / 8][4] = {};
 #pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {   // matrices: keys 0-7 / 8-15 (lane >> 4) by elements 0-7 / 8-15 (lane >> 3 & 1)
-            const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * k + ((lane >> 3) & 1);
-            uint32_t f[4];
-            ldmatrix4<false>(f, ks + r * (DP * 2) + ((c ^ (r & 7)) << 4));
-            mma16816<T>(s[0], qa[k], f[0], f[1]);
-            mma16816<T>(s[1], qa[k], f[2], f[3]);
-        }
+        for (int k = 0; k < DP / 16; ++k)   // matrices: keys 0-7 / 8-15 (lane >> 4) by elements 0-7 / 8-15 (lane >> 3 & 1)
+#pragma unroll
+            for (int y = 0; y < kKeys / 16; ++y) {
+                const int r = 16 * y + (lane & 7) + ((lane >> 4) << 3), c = 2 * k + ((lane >> 3) & 1);
+                uint32_t f[4];
+                ldmatrix4<false>(f, ks + r * (DP * 2) + ((c ^ (r & 7)) << 4));
+                mma16816<T>(s[2 * y], qa[k], f[0], f[1]);
+                mma16816<T>(s[2 * y + 1], qa[k], f[2], f[3]);
+            }
         // element (w, j): row g + 8 w, key at + 8 (j >> 1) + 2 t + (j & 1)
-        float p[2][4];
+        float p[2][kKeys / 4];
+        bool raised = false;
+        float f[2];
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
             const int pos = qi[w] + off;
             float top = -INFINITY;
+            // past the last edge on one side the bias is one value
+            const bool one = !a.bias || at + kKeys - 1 - pos <= -reach || (a.edges.two && at - pos >= reach);
+            const float flat = !a.bias ? 0.f : at + kKeys - 1 - pos <= -reach ? before[w] : after[w];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < kKeys / 4; ++j) {
                 const int key = at + 8 * (j >> 1) + 2 * t + (j & 1);
                 float v = s[j >> 1][2 * w + (j & 1)] * c2;
-                if (a.bias && live[w]) {
-                    const int d = key - pos;
-                    v += d <= -reach ? before[w] : (a.edges.two && d >= reach) ? after[w] : bias_log2<T>(a, bucket_of(a.edges, d), head[w]);
-                }
+                if (one) v += flat;
+                else if (live[w]) v += bias_log2<T>(a, bucket_of(a.edges, key - pos), head[w]);
                 p[w][j] = key < lim[w] ? v : -INFINITY;
                 top = fmaxf(top, p[w][j]);
             }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const bool raise = top > m[w] + Softmax<T>::kSlack || (m[w] == -INFINITY && top > -INFINITY);
-            if (__any_sync(0xffffffffu, raise)) {
-                const float f = raise ? (m[w] == -INFINITY ? 0.f : exp2_fast(m[w] - top)) : 1.f;
-                m[w] = raise ? top : m[w];
-                l[w] *= f;
-#pragma unroll
-                for (int x = 0; x < DP / 8; ++x) o[x][2 * w] *= f, o[x][2 * w + 1] *= f;
-            }
+            f[w] = raise ? (m[w] == -INFINITY ? 0.f : exp2_fast(m[w] - top)) : 1.f;
+            m[w] = raise ? top : m[w];
+            raised |= raise;
             const float ref = (m[w] == -INFINITY ? 0.f : m[w]) - Softmax<T>::kShift;
+            l[w] *= f[w];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < kKeys / 4; ++j) {
                 p[w][j] = exp2_fast(p[w][j] - ref);
                 l[w] += p[w][j];
             }
         }
-        const uint32_t pa[4] = {pack2<T>(p[0][0], p[0][1]), pack2<T>(p[1][0], p[1][1]), pack2<T>(p[0][2], p[0][3]), pack2<T>(p[1][2], p[1][3])};
+        if (__any_sync(0xffffffffu, raised)) {
 #pragma unroll
-        for (int x = 0; x < DP / 16; ++x) {   // matrices: keys 0-7 / 8-15 (lane >> 3 & 1) by elements 0-7 / 8-15 (lane >> 4)
-            const int r = (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * x + (lane >> 4);
-            uint32_t f[4];
-            ldmatrix4<true>(f, vs + r * (DP * 2) + ((c ^ (r & 7)) << 4));
-            mma16816<T>(o[2 * x], pa, f[0], f[1]);
-            mma16816<T>(o[2 * x + 1], pa, f[2], f[3]);
+            for (int x = 0; x < DP / 8; ++x) o[x][0] *= f[0], o[x][1] *= f[0], o[x][2] *= f[1], o[x][3] *= f[1];
+        }
+#pragma unroll
+        for (int y = 0; y < kKeys / 16; ++y) {
+            const uint32_t pa[4] = {pack2<T>(p[0][4 * y], p[0][4 * y + 1]), pack2<T>(p[1][4 * y], p[1][4 * y + 1]),
+                                    pack2<T>(p[0][4 * y + 2], p[0][4 * y + 3]), pack2<T>(p[1][4 * y + 2], p[1][4 * y + 3])};
+#pragma unroll
+            for (int x = 0; x < DP / 16; ++x) {   // matrices: keys 0-7 / 8-15 (lane >> 3 & 1) by elements 0-7 / 8-15 (lane >> 4)
+                const int r = 16 * y + (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * x + (lane >> 4);
+                uint32_t e[4];
+                ldmatrix4<true>(e, vs + r * (DP * 2) + ((c ^ (r & 7)) << 4));
+                mma16816<T>(o[2 * x], pa, e[0], e[1]);
+                mma16816<T>(o[2 * x + 1], pa, e[2], e[3]);
+            }
         }
         __syncwarp();
     }
@@ -215,44 +233,70 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
         l[w] += __shfl_xor_sync(0xffffffffu, l[w], 2);
     }
 
-    // the CTA's warps join in the ring's place: o [warp][16][DP + 4], m and l [warp][16]; then one set a CTA
-    constexpr int kPitch = DP + 4;
+    // join in the ring's place: o [set][16][pitch], m and l [set][16]; sets 0 .. kWarps - 1 the warps', set kWarps the CTA's
+    constexpr int kPitch = Sh::kPitch;
     float* const jo = reinterpret_cast<float*>(sm);
-    float* const jm = jo + kWarps * kRowsM * kPitch;
-    float* const jl = jm + kWarps * kRowsM;
+    float* const jm = jo + (kWarps + 1) * kRowsM * kPitch;
+    float* const jl = jm + (kWarps + 1) * kRowsM;
+    float* const jw = jl + (kWarps + 1) * kRowsM;   // [16][kMaxSplits] weights of the cluster's sets
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         const int r = warp * kRowsM + g + 8 * w;
+        if (g + 8 * w < rows) {
 #pragma unroll
-        for (int x = 0; x < DP / 8; ++x)
-            *reinterpret_cast<float2*>(jo + r * kPitch + 8 * x + 2 * t) = make_float2(o[x][2 * w], o[x][2 * w + 1]);
-        if (t == 0) jm[r] = m[w], jl[r] = l[w];
-    }
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    // every CTA of the cluster finishes its part of the rows from all partial results: splits x warps of them
-    const int units = a.D / 2, parts = splits * kWarps;
-    for (int e = split * 32 * kWarps + tid; e < rows * units; e += splits * 32 * kWarps) {
-        const int r = e / units, d = 2 * (e % units), i = r / G, h = kh * G + r % G;
-        float top = -INFINITY;
-        for (int p = 0; p < parts; ++p) top = fmaxf(top, cluster.map_shared_rank(jm, p / kWarps)[(p % kWarps) * kRowsM + r]);
-        float sum = 0.f, x = 0.f, y = 0.f;
-        for (int p = 0; p < parts; ++p) {
-            const int at = (p % kWarps) * kRowsM + r;
-            const float pm = cluster.map_shared_rank(jm, p / kWarps)[at];
-            const float f = pm == -INFINITY ? 0.f : exp2_fast(pm - top);
-            const float pl = cluster.map_shared_rank(jl, p / kWarps)[at];
-            sum = f == 0.f && pl == pl ? sum : sum + f * pl;
-            const float2 v = *reinterpret_cast<const float2*>(cluster.map_shared_rank(jo, p / kWarps) + at * kPitch + d);
-            x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
+            for (int x = 0; x < DP / 8; ++x)
+                *reinterpret_cast<float2*>(jo + r * kPitch + 8 * x + 2 * t) = make_float2(o[x][2 * w], o[x][2 * w + 1]);
+            if (t == 0) jm[r] = m[w], jl[r] = l[w];
         }
+    }
+    __syncthreads();
+    const int units = a.D / 2;
+    auto finish = [&](int r, int d, float x, float y, float top, float sum) {
+        const int i = r / G, h = kh * G + r % G;
         const bool some = (sum > 0.f || sum != sum) && i < lq;
         const float w = some ? 1.f / sum : 0.f;
         *reinterpret_cast<uint32_t*>(out + (((size_t)b * a.Lq + i) * a.H + h) * a.D + d) = some ? pack2<T>(x * w, y * w) : 0u;
         if (lse && d == 0) lse[((size_t)b * a.H + h) * a.Lq + i] = some ? top - Softmax<T>::kShift + log2f(sum) : INFINITY;
+    };
+    for (int e = tid; e < rows * units; e += 32 * kWarps) {
+        const int r = e / units, d = 2 * (e % units);
+        float top = jm[r], sum = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+        for (int p = 1; p < kWarps; ++p) top = fmaxf(top, jm[p * kRowsM + r]);
+#pragma unroll
+        for (int p = 0; p < kWarps; ++p) {
+            const float pm = jm[p * kRowsM + r], f = pm == -INFINITY ? 0.f : exp2_fast(pm - top);
+            const float2 v = *reinterpret_cast<const float2*>(jo + (p * kRowsM + r) * kPitch + d);
+            sum = fmaf(f, jl[p * kRowsM + r], sum), x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
+        }
+        if (splits == 1) {
+            finish(r, d, x, y, top, sum);
+        } else {
+            *reinterpret_cast<float2*>(jo + (kWarps * kRowsM + r) * kPitch + d) = make_float2(x, y);
+            if (d == 0) jm[kWarps * kRowsM + r] = top, jl[kWarps * kRowsM + r] = sum;
+        }
     }
-    cluster.sync();   // the partial results are read from other CTAs
+    if (splits == 1) return;
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    // every CTA finishes its part of the rows from all the cluster's sets: their weights first, then the sums
+    for (int e = tid; e < rows * splits; e += 32 * kWarps)
+        jw[(e / splits) * kMaxSplits + e % splits] = cluster.map_shared_rank(jm, e % splits)[kWarps * kRowsM + e / splits];
+    __syncthreads();
+    for (int e = split * 32 * kWarps + tid; e < rows * units; e += splits * 32 * kWarps) {
+        const int r = e / units, d = 2 * (e % units), at = kWarps * kRowsM + r;
+        float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
+        for (int p = 0; p < splits; ++p) top = fmaxf(top, jw[r * kMaxSplits + p]);
+#pragma unroll 8
+        for (int p = 0; p < splits; ++p) {
+            const float pm = jw[r * kMaxSplits + p], f = pm == -INFINITY ? 0.f : exp2_fast(pm - top);
+            const float2 v = *reinterpret_cast<const float2*>(cluster.map_shared_rank(jo, p) + at * kPitch + d);
+            sum = fmaf(f, cluster.map_shared_rank(jl, p)[at], sum), x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
+        }
+        finish(r, d, x, y, top, sum);
+    }
+    cluster.sync();   // the sets are read from other CTAs
 }
 
 template <class T, int DP>
@@ -264,12 +308,15 @@ int launch(const AttnArgs& a, void* out, float* lse, cudaStream_t st) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
     int rc = device_setup(setup, dev, [] {
-        return (int)cudaFuncSetAttribute(attn_token_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        cudaError_t e = cudaFuncSetAttribute(attn_token_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_token_kernel<T, DP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        return (int)e;
     }, &sms);
     if (rc) return rc;
-    // CTAs for two a SM, as far as the keys go round
+    // CTAs for every place there is, as far as the keys go round; 32 x 16 heads of 64, 4096 keys: 105 us (5.1 TB/s) with
+    // two CTAs a problem, 119 with one of larger steps; 8 x 8 heads of 128, 8192 keys: 63 us with places for all, 84 with twice as many
     int splits = 1;
-    while (splits < 8 && (long long)a.B * a.Hkv * splits < 2 * sms && (long long)a.Lk > (long long)splits * kMinRounds * kWarps * kKeys)
+    while (splits < kMaxSplits && (long long)a.B * a.Hkv * splits < (long long)Sh::kResident * sms && (long long)a.Lk > (long long)splits * kMinRounds * kWarps * kKeys)
         splits *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, a.Hkv, a.B), cfg.blockDim = dim3(32 * kWarps), cfg.dynamicSmemBytes = smem, cfg.stream = st;
