@@ -12,18 +12,37 @@
 namespace d2pb {
 namespace enc {
 
-__device__ __forceinline__ uint4 philox(uint64_t block, uint64_t seed, uint64_t offset) {
-    uint32_t a = (uint32_t)block, b = (uint32_t)(block >> 32), x = (uint32_t)offset, y = (uint32_t)(offset >> 32);
-    uint32_t k0 = (uint32_t)seed, k1 = (uint32_t)(seed >> 32);
+// a M in two words.  The widening multiply issues at an eighth of the plain rate
+// on this device, 16 a clock and SM, and is what bounds this kernel; the same
+// product from 16-bit halves on the plain multiply and the logic pipes costs
+// more (three of a block's products that way: 51 us against 46).
+template <uint32_t M>
+__device__ __forceinline__ uint2 wide(uint32_t a) {
+    const uint64_t p = (uint64_t)a * M;
+    return make_uint2((uint32_t)p, (uint32_t)(p >> 32));
+}
+constexpr uint32_t kM0 = 0xD2511F53u, kM1 = 0xCD9E8D57u, kW0 = 0x9E3779B9u, kW1 = 0xBB67AE85u;
+
+// what every block of a call shares: the key, and the first rounds' products of the offset (the block's high word is
+// zero below 2^34 elements, which leaves round 1's first word the same for all too)
+struct Stream {
+    uint32_t k0, k1, off1;      // key, offset's high word
+    uint2 q0;                   // round 0: offset's low word by M1
+    uint2 p1;                   // round 1: the word above by M0, where the block's high word is zero
+};
+// the block with counter (block, offset); p0 = block M0, which a caller steps by additions
+__device__ __forceinline__ uint4 philox(uint64_t block, uint64_t p0, const Stream& s) {
+    uint32_t k0 = s.k0, k1 = s.k1;
+    uint32_t a = s.q0.y ^ (uint32_t)(block >> 32) ^ k0, b = s.q0.x;
+    uint32_t x = (uint32_t)(p0 >> 32) ^ s.off1 ^ k1, y = (uint32_t)p0;
 #pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        const uint64_t p = (uint64_t)a * 0xD2511F53u, q = (uint64_t)x * 0xCD9E8D57u;
-        a = (uint32_t)(q >> 32) ^ b ^ k0;
-        b = (uint32_t)q;
-        x = (uint32_t)(p >> 32) ^ y ^ k1;
-        y = (uint32_t)p;
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
+    for (int r = 1; r < 10; ++r) {
+        k0 += kW0, k1 += kW1;
+        uint2 p = s.p1;
+        if (r > 1 || (block >> 32)) p = wide<kM0>(a);
+        const uint2 q = wide<kM1>(x);
+        a = q.y ^ b ^ k0, b = q.x;
+        x = p.y ^ y ^ k1, y = p.x;
     }
     return make_uint4(a, b, x, y);
 }
@@ -32,9 +51,12 @@ __device__ __forceinline__ uint4 philox(uint64_t block, uint64_t seed, uint64_t 
 template <class T, bool RES>
 __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, const T* __restrict__ res,
                                                       T* __restrict__ y, size_t n, uint32_t thr, float scale,
-                                                      uint64_t seed, uint64_t offset, int vec) {
+                                                      const Stream s, int vec) {
     const size_t step = (size_t)gridDim.x * blockDim.x * 8;
-    for (size_t e = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * 8; e < n; e += step) {
+    size_t e = ((size_t)blockIdx.x * blockDim.x + threadIdx.x) * 8;
+    // M0 times the low word of the block's counter, stepped with it (exact while the high word is zero; past that, anew)
+    uint64_t p0 = (uint64_t)(uint32_t)(e / 4) * kM0;
+    for (; e < n; e += step) {
         float v[8], r[8];
         const bool whole = vec && e + 8 <= n;
         if (whole) {
@@ -47,12 +69,15 @@ __global__ void __launch_bounds__(256) dropout_kernel(const T* __restrict__ x, c
                 if (RES) r[i] = e + i < n ? to_f<T>(res[e + i]) : 0.f;
             }
         }
-        const uint4 w0 = philox(e / 4, seed, offset), w1 = philox(e / 4 + 1, seed, offset);
+        const uint64_t block = e / 4;   // even, so that block + 1 has the same high word
+        if (block >> 32) p0 = (uint64_t)(uint32_t)block * kM0;
+        const uint4 w0 = philox(block, p0, s), w1 = philox(block + 1, p0 + kM0, s);
+        p0 += (uint64_t)(step / 4) * kM0;
         const uint32_t w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float d = w[i] >= thr ? v[i] * scale : 0.f;
-            v[i] = RES ? r[i] + d : d;
+            const float d = w[i] >= thr ? v[i] : 0.f;
+            v[i] = RES ? fmaf(d, scale, r[i]) : d * scale;
         }
         if (whole) {
             store8<T>(y + e, v);
@@ -70,10 +95,14 @@ int launch_dropout(const void* x, const void* res, void* y, size_t n, uint32_t t
     const int vec = ((((uintptr_t)x | (uintptr_t)res | (uintptr_t)y) & 15) == 0);
     const size_t want = (n + 8 * 256 - 1) / (8 * 256);
     const unsigned blocks = (unsigned)(want < (size_t)sms * 32 ? want : (size_t)sms * 32);
+    const uint64_t q0 = (uint64_t)(uint32_t)offset * kM1;
+    const uint64_t p1 = (uint64_t)((uint32_t)(q0 >> 32) ^ (uint32_t)seed) * kM0;
+    const Stream s = {(uint32_t)seed, (uint32_t)(seed >> 32), (uint32_t)(offset >> 32), {(uint32_t)q0, (uint32_t)(q0 >> 32)},
+                      {(uint32_t)p1, (uint32_t)(p1 >> 32)}};
     if (res)
-        dropout_kernel<T, true><<<blocks, 256, 0, st>>>((const T*)x, (const T*)res, (T*)y, n, thr, scale, seed, offset, vec);
+        dropout_kernel<T, true><<<blocks, 256, 0, st>>>((const T*)x, (const T*)res, (T*)y, n, thr, scale, s, vec);
     else
-        dropout_kernel<T, false><<<blocks, 256, 0, st>>>((const T*)x, nullptr, (T*)y, n, thr, scale, seed, offset, vec);
+        dropout_kernel<T, false><<<blocks, 256, 0, st>>>((const T*)x, nullptr, (T*)y, n, thr, scale, s, vec);
     return (int)cudaGetLastError();
 }
 

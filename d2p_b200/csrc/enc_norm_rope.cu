@@ -28,6 +28,7 @@ struct NormRopeArgs {
     long long pos_bs;            // batch stride of pos (0: shared)
     int P, B, L, heads[2], D, R;
     float eps;
+    int span;                    // backward: heads of a token that a group takes together
     float* part;                 // backward: [2][gridDim.x][D] partial sums of dw
 };
 
@@ -47,8 +48,9 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
-template <class T, class W, int G, bool BWD>
-__global__ void __launch_bounds__(kThreadsNR) norm_rope_kernel(const NormRopeArgs a) {
+// a row a group of G threads and step
+template <class T, class W, int G>
+__global__ void __launch_bounds__(kThreadsNR) norm_rope_fwd_kernel(const NormRopeArgs a) {
     constexpr int kRows = kThreadsNR / G;                 // rows a block takes per step
     const int lane = threadIdx.x & (G - 1), grp = threadIdx.x / G;
     const int pairs = a.D >> 4;
@@ -58,7 +60,6 @@ __global__ void __launch_bounds__(kThreadsNR) norm_rope_kernel(const NormRopeArg
     const bool turn = on && lane < (a.R >> 4);
     const float invD = 1.f / (float)a.D;
     const long long tokens = (long long)a.B * a.L;
-    __shared__ float red[BWD ? (kThreadsNR / 32) * 256 : 1];
 
 #pragma unroll 1
     for (int part = 0; part < 2; ++part) {
@@ -72,19 +73,16 @@ __global__ void __launch_bounds__(kThreadsNR) norm_rope_kernel(const NormRopeArg
 #pragma unroll
             for (int i = 0; i < 16; ++i) w[i] = 0.f;
         }
-        float dw[16];
-        if (BWD) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) dw[i] = 0.f;
-        }
         const long long rows = tokens * H;
         // the loop's bound is the same for a warp's groups: shuffles stay converged
         for (long long r0 = (long long)blockIdx.x * kRows; r0 < rows; r0 += (long long)gridDim.x * kRows) {
             const long long row = r0 + grp;
             const bool live = on && row < rows;
             const long long rr = row < rows ? row : rows - 1;
-            const long long tok = rr / H;
-            const int h = (int)(rr - tok * H), b = (int)(tok / a.L), l = (int)(tok - (long long)b * a.L);
+            long long tok, b;
+            if (rows < (1ll << 31)) tok = (unsigned)rr / (unsigned)H, b = (unsigned)tok / (unsigned)a.L;   // (64-bit division is several times as long)
+            else tok = rr / H, b = tok / a.L;
+            const int h = (int)(rr - tok * H), l = (int)(tok - b * a.L);
             float x[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) x[i] = 0.f;
@@ -111,38 +109,11 @@ __global__ void __launch_bounds__(kThreadsNR) norm_rope_kernel(const NormRopeArg
             for (int i = 0; i < 16; ++i) q = fmaf(x[i], x[i], q);
             const float r = rsqrtf(group_sum<G>(q) * invD + a.eps);
             float o[16];
-            if (!BWD) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float u = x[i] * r * w[i], v = x[8 + i] * r * w[8 + i];
-                    o[i] = u * c[i] - v * s[i];
-                    o[8 + i] = v * c[i] + u * s[i];
-                }
-            } else {
-                float g[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) g[i] = 0.f;
-                if (live) {
-                    const T* pg = (const T*)a.g[part] + rr * a.D;
-                    load8<T>(pg + ea, g);
-                    load8<T>(pg + eb, g + 8);
-                }
-                float dot = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float u = g[i] * c[i] + g[8 + i] * s[i], v = g[8 + i] * c[i] - g[i] * s[i];
-                    x[i] *= r;
-                    x[8 + i] *= r;
-                    dw[i] = fmaf(u, x[i], dw[i]);
-                    dw[8 + i] = fmaf(v, x[8 + i], dw[8 + i]);
-                    o[i] = u * w[i];
-                    o[8 + i] = v * w[8 + i];
-                    dot = fmaf(o[i], x[i], dot);
-                    dot = fmaf(o[8 + i], x[8 + i], dot);
-                }
-                dot = group_sum<G>(dot) * invD;
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[i] = r * (o[i] - x[i] * dot);
+            for (int i = 0; i < 8; ++i) {
+                const float u = x[i] * r * w[i], v = x[8 + i] * r * w[8 + i];
+                o[i] = u * c[i] - v * s[i];
+                o[8 + i] = v * c[i] + u * s[i];
             }
             if (live) {
                 T* py = (T*)a.y[part] + rr * a.D;
@@ -150,7 +121,158 @@ __global__ void __launch_bounds__(kThreadsNR) norm_rope_kernel(const NormRopeArg
                 store8<T>(py + eb, o + 8);
             }
         }
-        if (BWD) {   // the block's dw: groups of a warp by shuffles, warps in order
+    }
+}
+
+// a row's two units as they lie in memory
+template <class T>
+struct Units {
+    uint4 v[sizeof(T)];
+    __device__ __forceinline__ void load(const T* p, int ea, int eb) {
+        constexpr int n = sizeof(T) / 2;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            v[i] = reinterpret_cast<const uint4*>(p + ea)[i];
+            v[n + i] = reinterpret_cast<const uint4*>(p + eb)[i];
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T); ++i) v[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void get(float* f) const {
+        const T* h = reinterpret_cast<const T*>(v);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) f[i] = to_f<T>(h[i]);
+    }
+};
+
+// A group of G threads takes `span` heads of one token at a time, which share the
+// token's cosines and sines (as many bytes as a row of 16 bits itself).  The next
+// row is asked for before this one is used, across tokens too.
+template <class T, class W, int G>
+__global__ void __launch_bounds__(kThreadsNR, sizeof(T) == 4 ? 1 : 2) norm_rope_bwd_kernel(const NormRopeArgs a) {
+    constexpr int kGroups = kThreadsNR / G;
+    const int lane = threadIdx.x & (G - 1), grp = threadIdx.x / G;
+    const int pairs = a.D >> 4;
+    const bool on = lane < pairs;
+    int ea, eb;
+    units(on ? lane : 0, a.R, &ea, &eb);
+    const bool turn = on && lane < (a.R >> 4);
+    const float invD = 1.f / (float)a.D;
+    const long long tokens = (long long)a.B * a.L;
+    __shared__ float red[(kThreadsNR / 32) * 256];
+
+#pragma unroll 1
+    for (int part = 0; part < 2; ++part) {
+        const int H = a.heads[part], span = min(a.span, H), sets = span ? (H + span - 1) / span : 0;
+        const long long work = tokens * sets, step = (long long)gridDim.x * kGroups;
+        float w[16];
+        if (on) {
+            load8<W>((const W*)a.w[part] + ea, w);
+            load8<W>((const W*)a.w[part] + eb, w + 8);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) w[i] = 0.f;
+        }
+        float dw[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) dw[i] = 0.f;
+        if (work > 0) {
+            // a unit (set of heads, position, batch) is stepped with carries rather than divided out
+            const long long u0 = (long long)blockIdx.x * kGroups + grp, t0 = u0 / sets, dtok = step / sets;
+            int set = (int)(u0 - t0 * sets), l = (int)(t0 % a.L);
+            long long b = t0 / a.L;
+            const int dset = (int)(step - dtok * sets), dl = (int)(dtok % a.L);
+            const long long db = dtok / a.L;
+            const long long hs = a.xs[part][2];
+            const T *px, *pg;   // the row asked for next
+            bool live, ahead;   // whether this unit, and the one asked for, is one there is
+            auto seek = [&]() {
+                ahead = on && b < a.B;
+                const long long tok = b * a.L + l;
+                px = (const T*)a.x[part] + b * a.xs[part][0] + l * a.xs[part][1] + set * span * hs;
+                pg = (const T*)a.g[part] + (tok * H + set * span) * a.D;
+            };
+            auto ask = [&](Units<T>& x, Units<T>& g, int h) {   // row h of the token
+                if (ahead && h < H) {
+                    x.load(px, ea, eb);
+                    g.load(pg, ea, eb);
+                } else {
+                    x.zero();
+                    g.zero();
+                }
+                px += hs;
+                pg += a.D;
+            };
+            auto place = [&]() -> long long {   // the unit's position in the tables
+                if (!turn || b >= a.B) return 0;
+                if (!a.pos) return l;
+                const long long at = b * a.pos_bs + l;
+                return a.pos64 ? ((const long long*)a.pos)[at] : (long long)((const int*)a.pos)[at];
+            };
+            Units<T> xs, gs, nx, ng;
+            seek();
+            ask(nx, ng, set * span);
+            long long at = place();
+            // the loops' bounds are the same for a warp's groups: shuffles stay converged
+            for (long long base = (long long)blockIdx.x * kGroups; base < work; base += step) {
+                float c[8], s[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) c[i] = 1.f, s[i] = 0.f;
+                if (turn) {
+                    const long long p = at < 0 ? 0 : (at >= a.P ? a.P - 1 : at);   // past the table: its last row
+                    load8<float>(a.cosv + p * (a.R >> 1) + ea, c);
+                    load8<float>(a.sinv + p * (a.R >> 1) + ea, s);
+                }
+                const int h0 = set * span;
+                T* py = (T*)a.y[part] + ((b * a.L + l) * H + h0) * a.D;
+                live = ahead;
+                for (int k = 0; k < span; ++k, py += a.D) {
+                    xs = nx;
+                    gs = ng;
+                    if (k + 1 < span) {
+                        ask(nx, ng, h0 + k + 1);
+                    } else {
+                        set += dset, l += dl, b += db;
+                        if (set >= sets) set -= sets, ++l;
+                        if (l >= a.L) l -= a.L, ++b;
+                        seek();
+                        ask(nx, ng, set * span);
+                        at = place();
+                    }
+                    float x[16], o[16];
+                    xs.get(x);
+                    float q = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) q = fmaf(x[i], x[i], q);
+                    const float r = rsqrtf(group_sum<G>(q) * invD + a.eps);
+                    float g[16];
+                    gs.get(g);
+                    float dot = 0.f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float u = g[i] * c[i] + g[8 + i] * s[i], v = g[8 + i] * c[i] - g[i] * s[i];
+                        x[i] *= r;
+                        x[8 + i] *= r;
+                        dw[i] = fmaf(u, x[i], dw[i]);
+                        dw[8 + i] = fmaf(v, x[8 + i], dw[8 + i]);
+                        o[i] = u * w[i];
+                        o[8 + i] = v * w[8 + i];
+                        dot = fmaf(o[i], x[i], dot);
+                        dot = fmaf(o[8 + i], x[8 + i], dot);
+                    }
+                    dot = group_sum<G>(dot) * invD;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] = r * (o[i] - x[i] * dot);
+                    if (live && h0 + k < H) {
+                        store8<T>(py + ea, o);
+                        store8<T>(py + eb, o + 8);
+                    }
+                }
+            }
+        }
+        {   // the block's dw: groups of a warp by shuffles, warps in order
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
 #pragma unroll
@@ -177,18 +299,20 @@ __global__ void __launch_bounds__(kThreadsNR) norm_rope_kernel(const NormRopeArg
 
 // dw[part][d] = sum of the blocks' partial sums, in a fixed order
 template <class W>
-__global__ void __launch_bounds__(256) norm_rope_dw_kernel(const float* __restrict__ part, int blocks, int D, W* dq,
-                                                           W* dk) {
-    __shared__ float red[8][32];
+__global__ void __launch_bounds__(1024) norm_rope_dw_kernel(const float* __restrict__ part, int blocks, int D, W* dq,
+                                                            W* dk) {
+    __shared__ float red[32][32];
     const int d = blockIdx.x * 32 + (threadIdx.x & 31), k = threadIdx.x >> 5, which = blockIdx.y;
     float t = 0.f;
-    if (d < D)
-        for (int i = k; i < blocks; i += 8) t += part[((size_t)which * blocks + i) * D + d];
+    if (d < D) {
+#pragma unroll 8
+        for (int i = k; i < blocks; i += 32) t += part[((size_t)which * blocks + i) * D + d];
+    }
     red[k][threadIdx.x & 31] = t;
     __syncthreads();
     if (k == 0 && d < D) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) t += red[i][threadIdx.x & 31];
+        for (int i = 1; i < 32; ++i) t += red[i][threadIdx.x & 31];
         (which ? dk : dq)[d] = from_f<W>(t);
     }
 }
@@ -198,30 +322,39 @@ int norm_rope_group(int D) {
     while (g < D / 16) g *= 2;
     return g;
 }
+// backward: two blocks a SM (each leaves a row of partial sums), and as many heads of a token at a time as leave every
+// group eight units
 int norm_rope_blocks(const NormRopeArgs& a, int sms, bool bwd) {
     const long long heads = a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1];
     const long long rows = (long long)a.B * a.L * heads, per = kThreadsNR / norm_rope_group(a.D);
-    const long long want = (rows + per - 1) / per, most = (long long)sms * (bwd ? 4 : 16);
+    const long long want = (rows + per - 1) / per, most = (long long)sms * (bwd ? 2 : 16);
     return (int)(want < most ? (want > 0 ? want : 1) : most);
 }
+int norm_rope_span(const NormRopeArgs& a, int blocks) {
+    const int heads = a.heads[0] > a.heads[1] ? a.heads[0] : a.heads[1];
+    const long long groups = (long long)blocks * (kThreadsNR / norm_rope_group(a.D)), tokens = (long long)a.B * a.L;
+    int span = 1;
+    while (2 * span <= heads && tokens * (heads / (2 * span)) >= 8 * groups) span *= 2;
+    return span;
+}
 
-template <class T, class W, bool BWD>
-int launch_norm_rope(const NormRopeArgs& a, int blocks, cudaStream_t st) {
-    switch (norm_rope_group(a.D)) {
-        case 1: norm_rope_kernel<T, W, 1, BWD><<<blocks, kThreadsNR, 0, st>>>(a); break;
-        case 2: norm_rope_kernel<T, W, 2, BWD><<<blocks, kThreadsNR, 0, st>>>(a); break;
-        case 4: norm_rope_kernel<T, W, 4, BWD><<<blocks, kThreadsNR, 0, st>>>(a); break;
-        case 8: norm_rope_kernel<T, W, 8, BWD><<<blocks, kThreadsNR, 0, st>>>(a); break;
-        default: norm_rope_kernel<T, W, 16, BWD><<<blocks, kThreadsNR, 0, st>>>(a); break;
-    }
-    return (int)cudaGetLastError();
+template <class T, class W, int G>
+void launch_group(const NormRopeArgs& a, int blocks, cudaStream_t st) {
+    if (a.part) norm_rope_bwd_kernel<T, W, G><<<blocks, kThreadsNR, 0, st>>>(a);
+    else norm_rope_fwd_kernel<T, W, G><<<blocks, kThreadsNR, 0, st>>>(a);
 }
 template <class T, class W>
 int launch_norm_rope(const NormRopeArgs& a, int blocks, void* dqw, void* dkw, cudaStream_t st) {
-    if (!a.part) return launch_norm_rope<T, W, false>(a, blocks, st);
-    int rc = launch_norm_rope<T, W, true>(a, blocks, st);
-    if (rc) return rc;
-    norm_rope_dw_kernel<W><<<dim3((a.D + 31) / 32, 2), 256, 0, st>>>(a.part, blocks, a.D, (W*)dqw, (W*)dkw);
+    switch (norm_rope_group(a.D)) {
+        case 1: launch_group<T, W, 1>(a, blocks, st); break;
+        case 2: launch_group<T, W, 2>(a, blocks, st); break;
+        case 4: launch_group<T, W, 4>(a, blocks, st); break;
+        case 8: launch_group<T, W, 8>(a, blocks, st); break;
+        default: launch_group<T, W, 16>(a, blocks, st); break;
+    }
+    const int rc = (int)cudaGetLastError();
+    if (rc || !a.part) return rc;
+    norm_rope_dw_kernel<W><<<dim3((a.D + 31) / 32, 2), 1024, 0, st>>>(a.part, blocks, a.D, (W*)dqw, (W*)dkw);
     return (int)cudaGetLastError();
 }
 template <class T>
@@ -301,6 +434,7 @@ int d2p_norm_rope_backward(const d2p_norm_rope_args* p, const void* dq_out, cons
     if ((rc = norm_rope_sms(&sms))) return rc;
     enc::NormRopeArgs a = norm_rope_args(p);
     const int blocks = enc::norm_rope_blocks(a, sms, true);
+    a.span = enc::norm_rope_span(a, blocks);
     if (workspace_bytes < (size_t)2 * blocks * p->D * sizeof(float)) return D2P_ERR_WORKSPACE_TOO_SMALL;
     a.y[0] = dq, a.y[1] = dk, a.g[0] = dq_out, a.g[1] = dk_out, a.part = (float*)workspace;
     return norm_rope_run(a, p, blocks, dq_weight, dk_weight, (cudaStream_t)stream);
