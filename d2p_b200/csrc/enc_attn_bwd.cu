@@ -43,26 +43,25 @@ constexpr int kBuckets = 2 * (kMaxEdges + 1);
 template <int DP, bool DKV>
 __host__ __device__ constexpr int buffers() { return DKV && DP == 128 ? 2 : 3; }
 
-template <int DP>
+template <int DP, bool BIAS>
 struct Shape {
     static constexpr int kChunks = DP / 64;
     static constexpr int kX = kChunks * kChunkX, kY = kChunks * kChunkY;
     static constexpr int kRowStats = 2 * kStep * 4;               // lse and delta of a streamed tile's queries
     static constexpr int kStage = 2 * kY + 1024;                  // keeps the tiles at 1024-byte boundaries
-    static constexpr int kStages = DP == 64 ? 8 : 4;
+    static constexpr int kStages = DP == 64 ? 8 : BIAS ? 3 : 4;   // (the bias by position takes up to 35 KB)
     static constexpr int kBars = 2 + 2 * kStages + 6;
     static constexpr size_t fixed() { return 1024 + 2 * (size_t)kX + (size_t)kStages * kStage + kBars * 8 + 16; }
 };
-// after the tiles: the bias by position (keys pass: one for each pair of warpgroups, whose tiles may be of two heads), then
-// (query pass) the diagonals' stage of each warp and the buckets' ranges
+// after the tiles: the bias by position, then (query pass) the diagonals' stage of each warp and the buckets' ranges
 __host__ __device__ inline size_t extra(bool bias, bool dkv, int reach) {
     if (!bias) return 0;
-    return 4 * (size_t)lut_size(reach) * (dkv ? 2 : 1) + (dkv ? 0 : 4 * (size_t)(16 * 72 + 16 * kBuckets + 2 * kBuckets));
+    return 4 * (size_t)lut_size(reach) + (dkv ? 0 : 4 * (size_t)(16 * 72 + 16 * kBuckets + 2 * kBuckets));
 }
 // at least 116 KB: one CTA an SM, since it takes the whole TMEM (no allocation waits)
-template <int DP>
-size_t smem_bytes(bool bias, bool dkv, int reach) {
-    const size_t n = Shape<DP>::fixed() + extra(bias, dkv, reach);
+template <int DP, bool BIAS>
+size_t smem_bytes(bool dkv, int reach) {
+    const size_t n = Shape<DP, BIAS>::fixed() + extra(BIAS, dkv, reach);
     return n < 116 * 1024 ? 116 * 1024 : n;
 }
 
@@ -83,7 +82,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ CUtensorMap tmY1, const __grid_constant__ CUtensorMap tmY2,
                     const __grid_constant__ CUtensorMap tmD1, const __grid_constant__ CUtensorMap tmD2,
                     const __grid_constant__ Args g) {
-    using Sh = Shape<DP>;
+    using Sh = Shape<DP, BIAS>;
     constexpr int NST = Sh::kStages, NB = buffers<DP, DKV>();
     const AttnArgs& a = g.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -125,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                    barP = barS + 24;
     volatile int* const dead = reinterpret_cast<volatile int*>(bars + Sh::kBars);
     uint32_t* const slot = reinterpret_cast<uint32_t*>(bars + Sh::kBars) + 1;
-    float* lut = reinterpret_cast<float*>(bars + Sh::kBars + 2);
+    float* const lut = reinterpret_cast<float*>(bars + Sh::kBars + 2);
     const int reach = BIAS ? reach_of(a.edges) : 0;
     float* const diag = lut + lut_size(reach);                        // [16][72] a warp's diagonals, scanned in place
     float* const red = diag + 16 * 72;                                // [16][kBuckets]
@@ -253,19 +252,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int i = 0; i < kBuckets / 32; ++i) bsum[i] = 0.f;
         bool ok = true;
-        int filled = -1;   // keys pass: the head of the group whose bias is in the pair's lut
-        if (BIAS && DKV && pair) lut += lut_size(reach);
         float* const dw = diag + warp * 72;
-        int head = 0, step = pair;   // of tile it: the head of the group and the tile of its rows
-        for (int it = pair; it < n; it += 2, step += 2) {
-            while (step >= per) step -= per, ++head;
-            const int s = it % NST, buf = it % NB, yb = y0 + step * kStep;
-            if (BIAS && DKV && head != filled) {
-                filled = head;
-                asm volatile("bar.sync %0, 256;" ::"r"(3 + pair) : "memory");   // the last tile's reads are over
-                fill_lut<T>(lut, a, hx * group + filled, reach, warp & 7, 8);
-                asm volatile("bar.sync %0, 256;" ::"r"(3 + pair) : "memory");
-            }
+        for (int head = 0; head < (DKV ? group : 1); ++head) {
+        if (BIAS && DKV) {   // keys pass: the bias of the group's next head, once every warp is past the one before
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            fill_lut<T>(lut, a, hx * group + head, reach, warp, kWork / 32);
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+        }
+        for (int step = (pair ^ (head * per)) & 1; step < per; step += 2) {   // this pair's tiles of the head
+            const int it = head * per + step, s = it % NST, buf = it % NB, yb = y0 + step * kStep;
             // (after a wait that gave up a warp still meets its partners at the barriers above)
             // (the streamed tile's own barrier: the keys pass reads the row statistics that came with it)
             ok = ok && (!DKV || bar_wait_warp(barY + 8 * s, (it / NST) & 1, dead)) &&
@@ -291,8 +286,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             // (forms without the masks and without the bias by position: a block needs them rarely)
             auto block = [&](auto edge_c, auto near_c) {
                 constexpr bool EDGE = decltype(edge_c)::value, NEAR = decltype(near_c)::value;
-                const float* const lp = lut + (d0 + reach + kPad);
-                const float flat = BIAS && !NEAR ? (lo >= reach ? lut[lut_size(reach) - 1] : lut[0]) : 0.f;
+                // four columns' entries at lp +- y: the keys pass meets them in falling order
+                const float* const lp = lut_row(lut, reach, d0 + reach + kPad - (DKV ? 3 : 0));
+                const float flat = BIAS && !NEAR ? (lo >= reach ? lut[lut_entries(reach) - 1] : lut[0]) : 0.f;
                 uint32_t sv[32], dv[32];
                 tmem_ld32(tS + col0, sv);
                 tmem_ld32(tD + col0, dv);
@@ -308,12 +304,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         L = make_float4(rl, rl, rl, rl), E = make_float4(rd, rd, rd, rd);
                     }
                     const float Lv[4] = {L.x, L.y, L.z, L.w}, Ev[4] = {E.x, E.y, E.z, E.w};
+                    float4 e = make_float4(flat, flat, flat, flat);
+                    if (BIAS && NEAR) e = *reinterpret_cast<const float4*>(DKV ? lp - y : lp + y);
+                    const float Bv[4] = {DKV ? e.w : e.x, DKV ? e.z : e.y, DKV ? e.y : e.z, DKV ? e.x : e.w};
                     float pv[4], gv[4];
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
                         const int col = y + z;
                         const float raw_s = __uint_as_float(sv[col]);
-                        const float t = BIAS ? fmaf(raw_s, c, NEAR ? (DKV ? lp[-col] : lp[col]) : flat) - Lv[z] : fmaf(raw_s, c, -Lv[z]);
+                        const float t = BIAS ? fmaf(raw_s, c, Bv[z]) - Lv[z] : fmaf(raw_s, c, -Lv[z]);
                         pv[z] = ex2(t);
                         gv[z] = pv[z] * (__uint_as_float(dv[col]) - Ev[z]);
                         if (EDGE) {
@@ -390,6 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     far0 += all;
                 }
             }
+        }
         }
         ok = ok && bar_wait_warp(barF, 0, dead);
         tc_fence_after();
@@ -507,11 +507,11 @@ int launch_pass(const Args& g, const CUtensorMap* tm, cudaStream_t st) {
     if (e != cudaSuccess) return (int)e;
     int rc = device_setup(setup, dev, [] {
         return (int)cudaFuncSetAttribute(attn_bwd_kernel<T, DP, BIAS, DKV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem_bytes<DP>(BIAS, DKV, kMaxReach));
+                                         (int)smem_bytes<DP, BIAS>(DKV, kMaxReach));
     }, &sms);
     if (rc) return rc;
     const int reach = BIAS ? reach_of(g.a.edges) : 0;
-    const size_t smem = smem_bytes<DP>(BIAS, DKV, reach);
+    const size_t smem = smem_bytes<DP, BIAS>(DKV, reach);
     const dim3 grid(tiles_of(DKV ? g.a.Lk : g.a.Lq), DKV ? g.a.Hkv : g.a.H, g.a.B);
     attn_bwd_kernel<T, DP, BIAS, DKV><<<grid, kThreads, smem, st>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], g);
     return (int)cudaGetLastError();

@@ -212,6 +212,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float c = a.scale * kLog2e;
         bool ok = true;
         int tt = 0;   // tiles so far
+        // the bias past the last edge on either side; as it is added last it must not be so large that it would swallow
+        // the scores near the diagonal, where it is added first
+        float before = 0.f, after = 0.f;
+        if (BIAS) before = lut[0], after = lut[lut_entries(reach) - 1];
+        const bool late = __all_sync(0xffffffffu, fabsf(before) < 65536.f && fabsf(after) < 65536.f);
         for (int e = 0; e < count; ++e) {
             const int4 en = entry[e];
             const Item w = {en.x, en.y, en.z, en.w, a.causal ? en.w - en.z : 0, tiles[e]};
@@ -239,24 +244,25 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) mul[x] = c, add[x] = 0.f;
                 if (BIAS) {
-                    const float* const lp = lut + (k0 - pos + reach + kPad);
-                    const int dmin = k0 - (w.q0 + 32 * warp + 31 + w.off);   // of the warp's 32 rows and the first 32 keys
+                    const float* const lp = lut_row(lut, reach, k0 - pos + reach + kPad);
+                    // (from one lane for all, so that the branches are known to be the warp's)
+                    const int dmin = __shfl_sync(0xffffffffu, k0 - (w.q0 + 32 * warp + 31 + w.off), 0);   // of the warp's 32 rows and the first 32 keys
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const int lo = dmin + 32 * x;
+                        add[x] = lo >= reach ? after : before;
                         if (lo < reach && lo + 62 > -reach) {
 #pragma unroll
-                            for (int y = 32 * x; y < 32 * x + 32; ++y) t[y] = fmaf(t[y], c, lp[y]);
-                            mul[x] = 1.f;
-                        } else {
-                            const float flat = lo >= reach ? lut[lut_size(reach) - 1] : lut[0];
-                            if (fabsf(flat) < 65536.f) {
-                                add[x] = flat;
-                            } else {   // a value that swallows the scores has to do so here as it does near the diagonal
-#pragma unroll
-                                for (int y = 32 * x; y < 32 * x + 32; ++y) t[y] = fmaf(t[y], c, flat);
-                                mul[x] = 1.f;
+                            for (int y = 32 * x; y < 32 * x + 32; y += 4) {
+                                const float4 e = *reinterpret_cast<const float4*>(lp + y);
+                                t[y] = fmaf(t[y], c, e.x), t[y + 1] = fmaf(t[y + 1], c, e.y);
+                                t[y + 2] = fmaf(t[y + 2], c, e.z), t[y + 3] = fmaf(t[y + 3], c, e.w);
                             }
+                            mul[x] = 1.f, add[x] = 0.f;
+                        } else if (!late) {
+#pragma unroll
+                            for (int y = 32 * x; y < 32 * x + 32; ++y) t[y] = fmaf(t[y], c, add[x]);
+                            mul[x] = 1.f, add[x] = 0.f;
                         }
                     }
                 }

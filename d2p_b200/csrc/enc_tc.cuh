@@ -173,12 +173,22 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// The bias by relative position of one head, in shared memory: lut[d + E + kPad]
-// for d in [-(E + kPad), E + kPad], E the largest edge, so that a tile that
-// touches |d| < E reads it without clamping (a tile's positions span < kPad)
-constexpr int kPad = 256;
+// The bias by relative position of one head, in shared memory: entry d + reach +
+// kPad for d in [-(reach + kPad), reach + kPad], reach the largest edge, so that a
+// 32 x 32 block that touches |d| < reach reads it without clamping.  Four copies,
+// copy k shifted by k entries, give a thread the entries of four columns in one
+// aligned load whatever its row (one load a column made the biased kernel half as
+// slow again); copies are 8 words apart modulo the 32 banks, so that the rows of a
+// load meet no bank twice.
+constexpr int kPad = 64;
 __host__ __device__ inline int reach_of(const Edges& e) { return e.n ? e.e[e.n - 1] : 1; }
-__host__ __device__ inline int lut_size(int reach) { return 2 * (reach + kPad) + 1; }
+__host__ __device__ inline int lut_entries(int reach) { return 2 * (reach + kPad) + 1; }
+__host__ __device__ inline int lut_pitch(int reach) { return ((lut_entries(reach) + 3 - 8 + 31) & ~31) + 8; }   // of a copy
+__host__ __device__ inline int lut_size(int reach) { return 4 * lut_pitch(reach); }
+// the four entries from `at` on are at lut_row(..)[0 .. 3]
+__device__ __forceinline__ const float* lut_row(const float* lut, int reach, int at) {
+    return lut + (at & 3) * lut_pitch(reach) + (at & ~3);
+}
 
 // positions d of bucket t, clipped to +-far
 __device__ __forceinline__ int2 bucket_range(const Edges& e, int t, int far) {
@@ -201,7 +211,10 @@ __device__ __forceinline__ void fill_lut(float* lut, const AttnArgs& a, int h, i
         for (int i = 1; i < (kMaxEdges + 1) / 16; ++i) v = t >> 5 == i ? mine[i] : v;
         v = __shfl_sync(0xffffffffu, v, t & 31);
         const int2 r = bucket_range(a.edges, t, far);
-        for (int d = r.x + lane; d <= r.y; d += 32) lut[d + far] = v;
+        for (int d = r.x + lane; d <= r.y; d += 32)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (d + far >= k) lut[k * lut_pitch(reach) + d + far - k] = v;
     }
 }
 
