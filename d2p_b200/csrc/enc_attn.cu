@@ -44,17 +44,27 @@ using namespace d2pb;
 
 extern "C" {
 
-int d2p_attention_forward(const d2p_attention_args* p, void* out, float* lse, void* stream) {
+// few query rows of a key head: tiles of 128 rows would be mostly empty, and the keys of one problem stay with one CTA;
+// 32 x 16 heads over ragged caches of up to 4096: 119 us by tiles against 72
+static bool few_rows(const enc::AttnArgs& a) { return (long long)a.Lq * (a.H / a.Hkv) <= 16; }
+
+size_t d2p_attention_forward_workspace_bytes(const d2p_attention_args* p) {
+    enc::AttnArgs a;
+    if (enc::attn_args(p, &a)) return (size_t)-1;
+    return a.B == 0 || a.Lq == 0 || few_rows(a) ? 0 : enc::attn_forward_bytes(a);
+}
+
+int d2p_attention_forward(const d2p_attention_args* p, void* out, float* lse, void* workspace, size_t workspace_bytes,
+                          void* stream) {
     enc::AttnArgs a;
     const int rc = enc::attn_args(p, &a);
     if (rc) return rc;
     if (a.B == 0 || a.Lq == 0) return D2P_OK;
-    if (!out) return D2P_ERR_INVALID_ARGUMENT;
-    if ((uintptr_t)out & 15) return D2P_ERR_INVALID_ARGUMENT;
-    // few query rows of a key head: tiles of 128 rows would be mostly empty, and the keys of one problem stay with
-    // one CTA; 32 x 16 heads over ragged caches of up to 4096: 119 us by tiles
-    if ((long long)a.Lq * (a.H / a.Hkv) <= 16) return enc::attn_forward_tokens(a, p->dtype, out, lse, (cudaStream_t)stream);
-    return enc::attn_forward_tiles(a, p->dtype, out, lse, (cudaStream_t)stream);
+    if (!out || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 15)) return D2P_ERR_INVALID_ARGUMENT;
+    if (few_rows(a)) return enc::attn_forward_tokens(a, p->dtype, out, lse, (cudaStream_t)stream);
+    const size_t need = enc::attn_forward_bytes(a);
+    if (need && (!workspace || workspace_bytes < need)) return D2P_ERR_WORKSPACE_TOO_SMALL;
+    return enc::attn_forward_tiles(a, p->dtype, out, lse, workspace, (cudaStream_t)stream);
 }
 
 size_t d2p_attention_backward_workspace_bytes(const d2p_attention_args* p, int want_dbias) {

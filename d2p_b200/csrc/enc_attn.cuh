@@ -59,7 +59,8 @@ struct Softmax<__half> {
 // checks of the C entry points; fills *a
 int attn_args(const d2p_attention_args* p, AttnArgs* a);
 // out and lse (or null) by tiles of 128 query rows (enc_attn_fwd.cu)
-int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st);
+int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaStream_t st);
+size_t attn_forward_bytes(const AttnArgs& a);
 // the same for at most 16 query rows of a key head, split over the keys (enc_attn_token.cu)
 int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st);
 // the gradients (enc_attn_bwd.cu) and their workspace

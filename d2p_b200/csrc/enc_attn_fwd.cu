@@ -48,8 +48,9 @@ struct Shape {
 struct Item {
     int b, q0, lq, lk, off, tiles;
 };
-__device__ __forceinline__ Item item_at(const AttnArgs& a, int index, int row_tiles) {
+__device__ __forceinline__ Item item_at(const AttnArgs& a, const int* order, int index, int row_tiles) {
     Item w;
+    if (order) index = order[index];
     // causal: the rows with the most keys first, over all problems
     const int t = a.causal ? row_tiles - 1 - index / a.B : index % row_tiles;
     w.b = a.causal ? index % a.B : index / row_tiles;
@@ -77,7 +78,7 @@ template <class T, int DP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs a, T* __restrict__ out,
-                    float* __restrict__ lse) {
+                    float* __restrict__ lse, const int* __restrict__ order) {
     using Sh = Shape<DP>;
     constexpr int NST = Sh::kStages;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -98,11 +99,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     float* const lut = reinterpret_cast<float*>(tiles + kMaxItems);
     const int reach = BIAS ? reach_of(a.edges) : 0;
 
-    for (int e = tid; e < count; e += kThreads) {
-        const Item w = item_at(a, blockIdx.y + e * gridDim.y, row_tiles);
-        entry[e] = make_int4(w.b, w.q0, w.lq, w.lk);
-        tiles[e] = w.tiles;
-    }
+    const int kh = h / (a.H / a.Hkv);
+    auto load = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, int b, uint32_t bar) {
+        bar_expect(bar, Sh::kTile);
+#pragma unroll
+        for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * kChunk, tm, 64 * c, row, head, b, bar);
+    };
     if (warp == 5) {
         if (lane == 0) {
             bar_init(barQ, 1), bar_init(barS, 1), bar_init(barP, 4), bar_init(barO, 1), bar_init(barR, 4), bar_init(barQE, 1);
@@ -111,12 +113,24 @@ __global__ void __launch_bounds__(kThreads, 2)
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
             *dead = 0;
+            const Item w = item_at(a, order, blockIdx.y, row_tiles);   // the first item's Q and first tile before the CTA meets
+            if (w.tiles) {
+                load(sQ, &tmQ, w.q0, h, w.b, barQ);
+                load(sK, &tmK, 0, kh, w.b, barK);
+                load(sV, &tmV, 0, kh, w.b, barV);
+            }
         }
         __syncwarp();
     } else if (warp == 4) {
         tmem_alloc(smem_addr(slot), kColumns);
-    } else if (BIAS) {
-        fill_lut<T>(lut, a, h, reach, warp < 4 ? warp : warp - 2, 6);
+    } else {
+        for (int e = warp < 4 ? tid : tid - 64; e < count; e += 192) {
+            const Item w = item_at(a, order, blockIdx.y + e * gridDim.y, row_tiles);
+            entry[e] = make_int4(w.b, w.q0, w.lq, w.lk);
+            tiles[e] = w.tiles;
+        }
+        __syncwarp();
+        if (BIAS) fill_lut<T>(lut, a, h, reach, warp < 4 ? warp : warp - 2, 6);
     }
     tc_fence_before();
     __syncthreads();
@@ -125,14 +139,19 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     if (warp >= 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp == 5) {   // copies
+    if (warp > 5) {   // items no row of which has a key
+        for (int e = warp - 6; e < count; e += 2) {
+            if (tiles[e]) continue;
+            const int4 w = entry[e];
+            const int rows = min(kRows, a.Lq - w.y), units = a.D / 8;
+            for (int x = lane; x < rows * units; x += 32)
+                *reinterpret_cast<uint4*>(out + (((size_t)w.x * a.Lq + w.y + x / units) * a.H + h) * a.D + (x % units) * 8) =
+                    make_uint4(0, 0, 0, 0);
+            if (lse)
+                for (int x = lane; x < rows; x += 32) lse[((size_t)w.x * a.H + h) * a.Lq + w.y + x] = INFINITY;
+        }
+    } else if (warp == 5) {   // copies
         if (lane == 0) {
-            const int kh = h / (a.H / a.Hkv);
-            auto load = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, int b, uint32_t bar) {
-                bar_expect(bar, Sh::kTile);
-#pragma unroll
-                for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * kChunk, tm, 64 * c, row, head, b, bar);
-            };
             bool ok = true;
             int t = 0, q = 0;   // tiles and items asked for
             for (int i = 0; ok && i < count; ++i) {
@@ -140,14 +159,14 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (n == 0) continue;
                 const int4 e = entry[i];
                 if (q > 0 && !(ok = bar_wait(barQE, (q - 1) & 1, dead))) break;
-                load(sQ, &tmQ, e.y, h, e.x, barQ);
+                if (i > 0) load(sQ, &tmQ, e.y, h, e.x, barQ);   // (the first one's is under way)
                 ++q;
                 for (int j = 0; j < n; ++j, ++t) {
                     const int s = t % NST;
                     if (t >= NST && !(ok = bar_wait(barKE + 8 * s, (t / NST - 1) & 1, dead))) break;
-                    load(sK + s * Sh::kTile, &tmK, j * kRows, kh, e.x, barK + 8 * s);
+                    if (i + j > 0) load(sK + s * Sh::kTile, &tmK, j * kRows, kh, e.x, barK + 8 * s);
                     if (t >= NST && !(ok = bar_wait(barVE + 8 * s, (t / NST - 1) & 1, dead))) break;
-                    load(sV + s * Sh::kTile, &tmV, j * kRows, kh, e.x, barV + 8 * s);
+                    if (i + j > 0) load(sV + s * Sh::kTile, &tmV, j * kRows, kh, e.x, barV + 8 * s);
                 }
             }
             if (!ok || *dead) {   // a wait gave up: what is in flight ends (bounded) before the CTA does
@@ -190,8 +209,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         bool ok = cs.i >= count || scores();
         for (int t = 0; ok && cp.i < count; ++t) {
             const int s = t % NST;
-            // S read into registers, where P has columns of its own: the next S can begin
-            if (Sh::kApart && !(ok = bar_wait_warp(barR, t & 1, dead) && (cs.i >= count || scores()))) break;
+            const bool last = cp.j + 1 == cp.n;
+            // S read into registers, where P has columns of its own: the next S can begin (an item's first after the last
+            // product of the one before, which waits for nothing else)
+            if (Sh::kApart && !(ok = bar_wait_warp(barR, t & 1, dead) && (last || scores()))) break;
             if (!(ok = bar_wait_warp(barV + 8 * s, (t / NST) & 1, dead) && bar_wait_warp(barP, t & 1, dead))) break;
             tc_fence_after();
             const uint32_t su = __shfl_sync(0xffffffffu, (uint32_t)s, 0), jj = __shfl_sync(0xffffffffu, (uint32_t)cp.j, 0);
@@ -201,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (lead) mma_ts(uO, uP + 8 * k, dV + k * (2048 / 16), idO, (jj | k) != 0);
             if (lead) tc_commit(barO), tc_commit(barVE + 8 * su);
             cp.next(tiles, count);
-            if (!Sh::kApart && cs.i < count) ok = scores();
+            if ((last || !Sh::kApart) && cs.i < count) ok = scores();
         }
         if (!ok && lead) atomicAdd(&g_gave_up, 1ull);
         __syncwarp();
@@ -212,14 +233,20 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float c = a.scale * kLog2e;
         bool ok = true;
         int tt = 0;   // tiles so far
-        // the bias past the last edge on either side; as it is added last it must not be so large that it would swallow
-        // the scores near the diagonal, where it is added first
-        float before = 0.f, after = 0.f;
-        if (BIAS) before = lut[0], after = lut[lut_entries(reach) - 1];
-        const bool late = __all_sync(0xffffffffu, fabsf(before) < 65536.f && fabsf(after) < 65536.f);
+        // the bias past the last edge on either side, and what multiplies the scores there: it is added last, and one so
+        // large that it swallows the scores near the diagonal, where it is added first, has to do so there too (the
+        // factor leaves a masked -inf what it is)
+        float before = 0.f, after = 0.f, mul_before = c, mul_after = c;
+        if (BIAS) {
+            before = lut[0], after = lut[lut_entries(reach) - 1];
+            mul_before = fabsf(before) < 2147483648.f ? c : 1e-30f, mul_after = fabsf(after) < 2147483648.f ? c : 1e-30f;
+        }
         for (int e = 0; e < count; ++e) {
             const int4 en = entry[e];
-            const Item w = {en.x, en.y, en.z, en.w, a.causal ? en.w - en.z : 0, tiles[e]};
+            // (from one lane for all, so that the branches on them are known to be the warp's)
+            const int lku = __shfl_sync(0xffffffffu, en.w, 0), offu = __shfl_sync(0xffffffffu, a.causal ? en.w - en.z : 0, 0);
+            const Item w = {en.x, __shfl_sync(0xffffffffu, en.y, 0), en.z, lku, offu, __shfl_sync(0xffffffffu, tiles[e], 0)};
+            if (w.tiles == 0) continue;
             const int i = w.q0 + tid, pos = i + w.off, lk = w.lk;
             T* const orow = out + (((size_t)w.b * a.Lq + i) * a.H + h) * a.D;
             float m = -INFINITY, l = 0.f;
@@ -250,7 +277,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         const int lo = dmin + 32 * x;
-                        add[x] = lo >= reach ? after : before;
+                        add[x] = lo >= reach ? after : before, mul[x] = lo >= reach ? mul_after : mul_before;
                         if (lo < reach && lo + 62 > -reach) {
 #pragma unroll
                             for (int y = 32 * x; y < 32 * x + 32; y += 4) {
@@ -258,10 +285,6 @@ __global__ void __launch_bounds__(kThreads, 2)
                                 t[y] = fmaf(t[y], c, e.x), t[y + 1] = fmaf(t[y + 1], c, e.y);
                                 t[y + 2] = fmaf(t[y + 2], c, e.z), t[y + 3] = fmaf(t[y + 3], c, e.w);
                             }
-                            mul[x] = 1.f, add[x] = 0.f;
-                        } else if (!late) {
-#pragma unroll
-                            for (int y = 32 * x; y < 32 * x + 32; ++y) t[y] = fmaf(t[y], c, add[x]);
                             mul[x] = 1.f, add[x] = 0.f;
                         }
                     }
@@ -337,15 +360,15 @@ __global__ void __launch_bounds__(kThreads, 2)
                 tc_fence_before();
                 bar_arrive_warp(barP);
             }
-            const bool some = w.tiles > 0 && i < w.lq && (l > 0.f || l != l);
-            if (w.tiles > 0) ok = ok && bar_wait_warp(barO, (tt - 1) & 1, dead);
+            const bool some = i < w.lq && (l > 0.f || l != l);
+            ok = ok && bar_wait_warp(barO, (tt - 1) & 1, dead);
             tc_fence_after();
             const float s = !ok ? NAN : (some ? 1.f / l : 0.f);
             // O / l, a row a thread: whole 32-byte sectors
 #pragma unroll 1
             for (int x = 0; x < DP; x += 32) {
                 uint32_t o[32];
-                if (ok && w.tiles > 0) {
+                if (ok) {
                     tmem_ld32(tO + trow + x, o);
                     tmem_wait_ld();
                     tmem_tie32(o);
@@ -373,8 +396,44 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (warp == 4) tmem_free(tmem, kColumns);
 }
 
+// items by falling number of key tiles (any order among equals), for batches of uneven lengths
+constexpr int kBins = 1024, kMaxOrder = 1 << 16;
+__global__ void __launch_bounds__(1024) attn_order_kernel(const __grid_constant__ AttnArgs a, int* __restrict__ order) {
+    __shared__ int first[kBins], warp_sum[32];
+    const int row_tiles = (a.Lq + kRows - 1) / kRows, items = a.B * row_tiles, t = threadIdx.x;
+    first[t] = 0;
+    __syncthreads();
+    for (int i = t; i < items; i += 1024) atomicAdd(&first[kBins - 1 - min(item_at(a, nullptr, i, row_tiles).tiles, kBins - 1)], 1);
+    __syncthreads();
+    const int n = first[t];
+    int sum = n;   // inclusive scan over the bins
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if ((t & 31) >= o) sum += v;
+    }
+    if ((t & 31) == 31) warp_sum[t >> 5] = sum;
+    __syncthreads();
+    for (int w = 0; w < (t >> 5); ++w) sum += warp_sum[w];
+    first[t] = sum - n;
+    __syncthreads();
+    for (int i = t; i < items; i += 1024) order[atomicAdd(&first[kBins - 1 - min(item_at(a, nullptr, i, row_tiles).tiles, kBins - 1)], 1)] = i;
+}
+
+// a CTA for each item, or, where each place on the device (two CTAs an SM) would see four or more of them, a CTA for
+// each place, which takes its share: 256 x 512, 8 heads of 64: 243 us against 277
+long long stays(const AttnArgs& a, int sms) {
+    const long long items = (long long)a.B * ((a.Lq + kRows - 1) / kRows), places = 2LL * sms;
+    if (items * a.H < 4 * places) return 0;
+    return std::max<long long>(places > a.H ? places / a.H : 1, (items + kMaxItems - 1) / kMaxItems);
+}
+// whether its items are put in order first: lengths differ, and the shares with them (ragged, 180 us unordered)
+bool ordered(const AttnArgs& a, int sms) {
+    return (a.lengths || a.causal) && stays(a, sms) && (long long)a.B * ((a.Lq + kRows - 1) / kRows) <= kMaxOrder;
+}
+
 template <class T, int DP, bool BIAS>
-int launch(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st) {
+int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaStream_t st) {
     using Sh = Shape<DP>;
     static DeviceSetup setup;
     int dev = 0, sms = 0;
@@ -400,21 +459,21 @@ int launch(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st)
     // at least a third of the SM's shared memory: no more than two CTAs (2 x 256 TMEM columns), so no allocation waits
     size_t smem = Sh::smem(lut);
     if (smem < 80 * 1024) smem = 80 * 1024;
-    // a CTA for each row tile, or, where each place on the device would see eight or more of them, a CTA for each place
-    const long long items = (long long)a.B * ((a.Lq + kRows - 1) / kRows);
-    if (items > (1 << 30)) return D2P_ERR_TOO_LARGE;
-    const int places = 2 * sms;
-    long long per_head = items;
-    if (items * a.H >= 8LL * places) per_head = std::max<long long>(places > a.H ? places / a.H : 1, (items + kMaxItems - 1) / kMaxItems);
-    if (per_head > 65535) return D2P_ERR_TOO_LARGE;
-    attn_fwd_kernel<T, DP, BIAS><<<dim3(a.H, (unsigned)per_head), kThreads, smem, st>>>(q, k, v, a, (T*)out, lse);
+    const long long stay = stays(a, sms), ctas = stay ? stay : (long long)a.B * ((a.Lq + kRows - 1) / kRows);
+    if (ctas > 65535) return D2P_ERR_TOO_LARGE;
+    int* order = nullptr;
+    if (ordered(a, sms)) {
+        order = (int*)ws;
+        attn_order_kernel<<<1, 1024, 0, st>>>(a, order);
+    }
+    attn_fwd_kernel<T, DP, BIAS><<<dim3(a.H, (unsigned)ctas), kThreads, smem, st>>>(q, k, v, a, (T*)out, lse, order);
     return (int)cudaGetLastError();
 }
 
 template <class T>
-int pick(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st) {
-    if (a.D <= 64) return a.bias ? launch<T, 64, true>(a, dtype, out, lse, st) : launch<T, 64, false>(a, dtype, out, lse, st);
-    return a.bias ? launch<T, 128, true>(a, dtype, out, lse, st) : launch<T, 128, false>(a, dtype, out, lse, st);
+int pick(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaStream_t st) {
+    if (a.D <= 64) return a.bias ? launch<T, 64, true>(a, dtype, out, lse, ws, st) : launch<T, 64, false>(a, dtype, out, lse, ws, st);
+    return a.bias ? launch<T, 128, true>(a, dtype, out, lse, ws, st) : launch<T, 128, false>(a, dtype, out, lse, ws, st);
 }
 
 }  // namespace fwd
@@ -447,8 +506,14 @@ bool rows_map(CUtensorMap* tm, int dtype, const void* base, int B, int L, int he
 
 int attn_forward_gave_up(unsigned long long* n) { return (int)cudaMemcpyFromSymbol(n, g_gave_up, sizeof(*n)); }
 
-int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st) {
-    return dtype == D2P_DTYPE_BF16 ? fwd::pick<__nv_bfloat16>(a, dtype, out, lse, st) : fwd::pick<__half>(a, dtype, out, lse, st);
+size_t attn_forward_bytes(const AttnArgs& a) {
+    static DeviceSetup setup;
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || device_setup(setup, dev, [] { return 0; }, &sms)) return (size_t)-1;
+    return fwd::ordered(a, sms) ? (size_t)a.B * ((a.Lq + fwd::kRows - 1) / fwd::kRows) * sizeof(int) : 0;
+}
+int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaStream_t st) {
+    return dtype == D2P_DTYPE_BF16 ? fwd::pick<__nv_bfloat16>(a, dtype, out, lse, ws, st) : fwd::pick<__half>(a, dtype, out, lse, ws, st);
 }
 
 }  // namespace enc

@@ -1061,7 +1061,11 @@ std::tuple<Tensor, Tensor> attention_forward_cuda(const Tensor& q, const Tensor&
     attn_fill(f, q, k, v, bias, lengths, edges, scale, causal);
     Tensor out = torch::empty({q.size(0), q.size(1), q.size(2), q.size(3)}, q.options());
     Tensor lse = torch::empty({want_lse ? q.size(0) : 0, q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
-    check_rc(d2p_attention_forward(&f.a, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr, cur_stream()),
+    const size_t n = d2p_attention_forward_workspace_bytes(&f.a);
+    TORCH_CHECK(n != static_cast<size_t>(-1), "attention: problem not supported");
+    Tensor ws = n ? torch::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte)) : Tensor();
+    check_rc(d2p_attention_forward(&f.a, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
+                                   n ? ws.data_ptr() : nullptr, n, cur_stream()),
              "d2p_attention_forward");
     return {out, lse};
 }

@@ -339,7 +339,9 @@ typedef struct {
 /* out [B, Lq, H, D] contiguous, the inputs' type; lse [B, H, Lq] fp32 or NULL:
  * what the backward pass takes (log2 of the sum of exponentials, +inf in rows
  * with no allowed key). */
-D2P_API int d2p_attention_forward(const d2p_attention_args* args, void* out, float* lse, void* stream);
+D2P_API size_t d2p_attention_forward_workspace_bytes(const d2p_attention_args* args);
+D2P_API int d2p_attention_forward(const d2p_attention_args* args, void* out, float* lse, void* workspace,
+                                  size_t workspace_bytes, void* stream);
 /* Gradients of the above with the probabilities recomputed: grad, out [B, Lq, H,
  * D] contiguous, lse from the forward call; dq, dk, dv contiguous in the inputs'
  * type (zero outside the lengths); dbias [num_buckets, H] in bias_dtype, or NULL.
