@@ -3,8 +3,8 @@
 //   P = 2^(s - lse),  dP = dO V^T,  dS = P (dP - delta),  delta = rowsum(dO O),
 //   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K,  dbias = buckets' sums of dS.
 //
-// Two passes of one kernel, each a CTA per 128 rows that it owns, so that every
-// sum stays in the CTA's accumulators and no atomics are needed: the key pass
+// Two passes of one kernel, a CTA taking 128 rows that it owns at a time, so that
+// every sum stays in the CTA's accumulators and no atomics are needed: the key pass
 // (DKV) owns 128 keys and streams 64 queries at a time of every head that shares
 // them, the query pass owns 128 queries and streams 64 keys.  With X1, X2 the
 // owned and Y1, Y2 the streamed rows (keys pass: K, V / Q, dO; query pass: Q, dO
@@ -20,10 +20,16 @@
 // twice (7 products a tile pair rather than 5); in exchange dQ needs no
 // cross-CTA sums, whose order would change results from run to run.
 //
+// Setting up a CTA, its first copies and its last products cost 5 to 7 us, as much
+// as 512 streamed rows: where there are many owned tiles a CTA stays and takes one
+// after the other, in order of their work, and the next one's copies and scores
+// begin while this one's results leave.
+//
 // The query pass also sums dS by relative position.  Along a diagonal of a
 // warp's 32 x 32 block the sum moves one lane per column (one shuffle each), the
 // 63 sums are scanned, and each lane takes its buckets as differences of the
 // scan: registers only, in a fixed order.
+#include <algorithm>
 #include <type_traits>
 
 #include "enc_tc.cuh"
@@ -34,11 +40,12 @@ namespace enc {
 namespace bwd {
 
 constexpr int kWork = 512;              // four warpgroups: two for a tile, half of its columns each
-constexpr int kThreads = kWork + 64;    // and the products' warp and the copies' warp
+constexpr int kThreads = kWork + 96;    // and the warps of the scores, of the sums' products and of the copies
 constexpr int kOwn = 128, kStep = 64;
 constexpr int kColumns = 512;   // TMEM: buffers of 64 columns of S and 64 of dP, then the accumulators
 constexpr int kChunkX = kOwn * 128, kChunkY = kStep * 128;
 constexpr int kBuckets = 2 * (kMaxEdges + 1);
+constexpr int kMaxItems = 64;   // owned tiles a CTA takes at most
 
 template <int DP, bool DKV>
 __host__ __device__ constexpr int buffers() { return DKV && DP == 128 ? 2 : 3; }
@@ -49,9 +56,11 @@ struct Shape {
     static constexpr int kX = kChunks * kChunkX, kY = kChunks * kChunkY;
     static constexpr int kRowStats = 2 * kStep * 4;               // lse and delta of a streamed tile's queries
     static constexpr int kStage = 2 * kY + 1024;                  // keeps the tiles at 1024-byte boundaries
-    static constexpr int kStages = DP == 64 ? 8 : BIAS ? 3 : 4;   // (the bias by position takes up to 35 KB)
-    static constexpr int kBars = 2 + 2 * kStages + 6;
-    static constexpr size_t fixed() { return 1024 + 2 * (size_t)kX + (size_t)kStages * kStage + kBars * 8 + 16; }
+    static constexpr int kOwned = DP == 64 ? 2 : 1;                          // owned tiles in shared memory: the next one's copies early
+    static constexpr int kStages = DP == 64 ? 6 : BIAS ? 3 : 4;              // (the bias by position takes up to 35 KB)
+    static constexpr int kBars = 2 * kOwned + 2 + 2 * kStages + 9;
+    static constexpr size_t kTiles = 2 * (size_t)kOwned * kX + (size_t)kStages * kStage;
+    static constexpr size_t fixed() { return 1024 + kTiles + kBars * 8 + 32 + kMaxItems * 24; }
 };
 // after the tiles: the bias by position, then (query pass) the diagonals' stage of each warp and the buckets' ranges
 __host__ __device__ inline size_t extra(bool bias, bool dkv, int reach) {
@@ -72,75 +81,84 @@ struct Args {
     int Lp;
     void* dx1;             // keys pass: dv; query pass: unused
     void* dx2;             // dk or dq
-    float* part;           // query pass: [H][buckets][B][gridDim.x] sums of dS, or null
+    float* part;           // query pass: [H][buckets][B][row tiles] sums of dS, or null
+    const int* order;      // items in order of their work, or null
 };
+
+// one owned tile: its rows [x0, x0 + 128) of problem b, and the streamed rows [y0, ..) in `per` tiles that any of them meets
+struct Item {
+    int b, x0, lq, lk, y0, per;
+};
+template <bool DKV>
+__device__ __forceinline__ Item item_at(const AttnArgs& a, const int* order, int index) {
+    Item w;
+    const int row_tiles = ((DKV ? a.Lk : a.Lq) + kOwn - 1) / kOwn;
+    if (order) index = order[index];
+    // causal: the first keys and the last queries have the most to do, over all problems
+    w.b = a.causal ? index % a.B : index / row_tiles;
+    int t = a.causal ? index / a.B : index % row_tiles;
+    if (a.causal && !DKV) t = row_tiles - 1 - t;
+    w.x0 = t * kOwn;
+    problem_lengths(a, w.b, &w.lq, &w.lk);
+    const int off = a.causal ? w.lk - w.lq : 0;
+    w.y0 = 0;
+    int y1 = w.x0 < (DKV ? w.lk : w.lq) ? (DKV ? w.lq : w.lk) : 0;
+    if (a.causal) {
+        if (DKV) w.y0 = max(0, w.x0 - off) / kStep * kStep;
+        else y1 = min(y1, min(w.x0 + kOwn, w.lq) + off);
+    }
+    w.per = y1 > w.y0 ? (y1 - w.y0 + kStep - 1) / kStep : 0;
+    return w;
+}
 
 // rows of X past the lengths never reach a sum of another row; rows of Y do (0 x NaN), and are zeroed in shared memory
 template <class T, int DP, bool BIAS, bool DKV>
 __global__ void __launch_bounds__(kThreads, 1)
     attn_bwd_kernel(const __grid_constant__ CUtensorMap tmX1, const __grid_constant__ CUtensorMap tmX2,
                     const __grid_constant__ CUtensorMap tmY1, const __grid_constant__ CUtensorMap tmY2,
-                    const __grid_constant__ CUtensorMap tmD1, const __grid_constant__ CUtensorMap tmD2,
                     const __grid_constant__ Args g) {
     using Sh = Shape<DP, BIAS>;
-    constexpr int NST = Sh::kStages, NB = buffers<DP, DKV>();
+    constexpr int NST = Sh::kStages, NB = buffers<DP, DKV>(), NX = Sh::kOwned;
     const AttnArgs& a = g.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    // causal: the first keys and the last queries have the most to do
-    const int x0 = (a.causal && !DKV ? gridDim.x - 1 - blockIdx.x : blockIdx.x) * kOwn, hx = blockIdx.y, b = blockIdx.z;
-    int lq, lk;
-    problem_lengths(a, b, &lq, &lk);
-    const int off = a.causal ? lk - lq : 0, group = a.H / a.Hkv;
-    const int lx = DKV ? lk : lq, ly = DKV ? lq : lk, Lx = DKV ? a.Lk : a.Lq, heads = DKV ? a.Hkv : a.H;
-    // the streamed rows [y0, y1) that any owned row meets, in tiles of kStep
-    int y0 = 0, y1 = x0 < lx ? ly : 0;
-    if (a.causal) {
-        if (DKV) y0 = max(0, x0 - off) / kStep * kStep;
-        else y1 = min(y1, min(x0 + kOwn, lq) + off);
-    }
-    const int per = y1 > y0 ? (y1 - y0 + kStep - 1) / kStep : 0, n = DKV ? per * group : per;
-    if (n == 0) {   // nothing meets these rows
-        const int rows = min(kOwn, Lx - x0), units = a.D / 8;
-        for (int e = tid; e < rows * units; e += kThreads) {
-            const size_t at = (((size_t)b * Lx + x0 + e / units) * heads + hx) * a.D + (e % units) * 8;
-            *reinterpret_cast<uint4*>((T*)g.dx2 + at) = make_uint4(0, 0, 0, 0);
-            if (DKV) *reinterpret_cast<uint4*>((T*)g.dx1 + at) = make_uint4(0, 0, 0, 0);
-        }
-        if (!DKV && BIAS && g.part) {
-            const int nb = n_buckets(a.edges);
-            for (int t = tid; t < nb; t += kThreads)
-                g.part[(((size_t)hx * nb + t) * a.B + b) * gridDim.x + blockIdx.x] = 0.f;
-        }
-        return;
-    }
+    const int hx = blockIdx.x, group = a.H / a.Hkv;
+    const int Lx = DKV ? a.Lk : a.Lq, heads = DKV ? a.Hkv : a.H, row_tiles = (Lx + kOwn - 1) / kOwn, items = a.B * row_tiles;
+    const int count = (items - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;   // of this CTA: blockIdx.y, + gridDim.y, ..
 
     extern __shared__ uint8_t raw[];
     const uint32_t r0 = smem_addr(raw), base = (r0 + 1023u) & ~1023u;
     uint8_t* const gb = raw + (base - r0);
-    const uint32_t sX1 = base, sX2 = base + Sh::kX, sY = base + 2 * Sh::kX;
-    constexpr size_t kTiles = 2 * (size_t)Sh::kX + (size_t)NST * Sh::kStage;
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(gb + kTiles);
-    const uint32_t barX = smem_addr(bars), barF = barX + 8, barY = barX + 16, barE = barY + 8 * NST, barS = barE + 8 * NST,
-                   barP = barS + 24;
-    volatile int* const dead = reinterpret_cast<volatile int*>(bars + Sh::kBars);
-    uint32_t* const slot = reinterpret_cast<uint32_t*>(bars + Sh::kBars) + 1;
-    float* const lut = reinterpret_cast<float*>(bars + Sh::kBars + 2);
+    const uint32_t sY = base + 2 * NX * Sh::kX;
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(gb + Sh::kTiles);
+    const uint32_t barX = smem_addr(bars), barXE = barX + 8 * NX, barF = barXE + 8 * NX, barA = barF + 8, barY = barA + 8,
+                   barE = barY + 8 * NST, barS = barE + 8 * NST, barP = barS + 24, barPE = barP + 24;
+    uint8_t* const after = gb + (Sh::kTiles + Sh::kBars * 8 + 15) / 16 * 16;
+    volatile int* const dead = reinterpret_cast<volatile int*>(after);
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(after) + 1;
+    int4* const entry = reinterpret_cast<int4*>(after + 16);                 // b, x0, lq, lk of an item
+    int2* const span = reinterpret_cast<int2*>(entry + kMaxItems);           // and y0, per
+    float* const lut = reinterpret_cast<float*>(span + kMaxItems);
     const int reach = BIAS ? reach_of(a.edges) : 0;
     float* const diag = lut + lut_size(reach);                        // [16][72] a warp's diagonals, scanned in place
     float* const red = diag + 16 * 72;                                // [16][kBuckets]
     int* const range = reinterpret_cast<int*>(red + 16 * kBuckets);   // [kBuckets][2] positions of a bucket
     const bool sums = !DKV && BIAS && g.part;
 
-    auto copy = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, uint32_t bar, int chunk) {
+    auto copy = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, int b, uint32_t bar, int chunk) {
 #pragma unroll
         for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * chunk, tm, 64 * c, row, head, b, bar);
     };
-    auto stream = [&](int it) {
-        const int s = it % NST, head = DKV ? hx * group + it / per : hx / group, row = y0 + (it % per) * kStep;
-        const uint32_t dst = sY + s * Sh::kStage, bar = barY + 8 * s;
+    auto own = [&](int i, int b, int x0) {   // item i (of those with work): its X1 and X2
+        const uint32_t dst = base + (i % NX) * 2 * Sh::kX, bar = barX + 8 * (i % NX);
+        bar_expect(bar, 2 * Sh::kX);
+        copy(dst, &tmX1, x0, hx, b, bar, kChunkX);
+        copy(dst + Sh::kX, &tmX2, x0, hx, b, bar, kChunkX);
+    };
+    auto stream = [&](int t, int b, int row, int head) {   // streamed tile t: its Y1, Y2 and row statistics
+        const uint32_t dst = sY + (t % NST) * Sh::kStage, bar = barY + 8 * (t % NST);
         bar_expect(bar, 2 * Sh::kY + (DKV ? Sh::kRowStats : 0));
-        copy(dst, &tmY1, row, head, bar, kChunkY);
-        copy(dst + Sh::kY, &tmY2, row, head, bar, kChunkY);
+        copy(dst, &tmY1, row, head, b, bar, kChunkY);
+        copy(dst + Sh::kY, &tmY2, row, head, b, bar, kChunkY);
         if (DKV) {
             const size_t at = ((size_t)b * a.H + head) * g.Lp + row;
 #pragma unroll
@@ -152,24 +170,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                     : "memory");
         }
     };
-    if (warp == kWork / 32 + 1) {   // barriers, and the first copies before the CTA meets
+    if (warp == kWork / 32 + 2) {   // barriers, and the first item's copies before the CTA meets
         if (lane == 0) {
-            bar_init(barX, 1), bar_init(barF, 1);
+            for (int s = 0; s < NX; ++s) bar_init(barX + 8 * s, 1), bar_init(barXE + 8 * s, 1);
+            bar_init(barF, 1), bar_init(barA, kWork / 32);
             for (int s = 0; s < NST; ++s) bar_init(barY + 8 * s, 1), bar_init(barE + 8 * s, 1);
-            for (int s = 0; s < NB; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 8);
+            for (int s = 0; s < NB; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 8), bar_init(barPE + 8 * s, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
             *dead = 0;
-            bar_expect(barX, 2 * Sh::kX);
-            copy(sX1, &tmX1, x0, hx, barX, kChunkX);
-            copy(sX2, &tmX2, x0, hx, barX, kChunkX);
-            for (int it = 0; it < NST && it < n; ++it) stream(it);
+            const Item w = item_at<DKV>(a, g.order, blockIdx.y);
+            if (w.per) {
+                own(0, w.b, w.x0);
+                stream(0, w.b, w.y0, DKV ? hx * group : hx / group);
+            }
         }
         __syncwarp();
     } else if (warp == kWork / 32) {
         tmem_alloc(smem_addr(slot), kColumns);
-    } else if (BIAS && !DKV) {
-        fill_lut<T>(lut, a, hx, reach, warp, kWork / 32);
+    } else if (warp < kWork / 32) {
+        for (int e = tid; e < count; e += kWork) {
+            const Item w = item_at<DKV>(a, g.order, blockIdx.y + e * gridDim.y);
+            entry[e] = make_int4(w.b, w.x0, w.lq, w.lk);
+            span[e] = make_int2(w.y0, w.per);
+        }
+        __syncwarp();
+        if (BIAS && (!DKV || group == 1)) fill_lut<T>(lut, a, hx, reach, warp, kWork / 32);
         if (sums)
             for (int t = tid; t < n_buckets(a.edges); t += kWork) {
                 const int2 v = bucket_range(a.edges, t, 1 << 29);
@@ -181,274 +207,330 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     const uint32_t tmem = *slot, tA1 = tmem + 128 * NB, tA2 = DKV ? tA1 + DP : tA1;
 
-    if (warp == kWork / 32 + 1) {   // copies
+    if (warp == kWork / 32 + 2) {   // copies
         if (lane == 0) {
             bool ok = true;
-            int it = min(n, NST);
-            for (; it < n; ++it) {
-                if (!(ok = bar_wait(barE + 8 * (it % NST), (it / NST - 1) & 1, dead))) break;
-                stream(it);
+            int t = 0, i = 0;   // streamed tiles and items (with work) asked for
+            for (int e = 0; ok && e < count; ++e) {
+                const int per = span[e].y, y0 = span[e].x;
+                if (per == 0) continue;
+                const int b = entry[e].x;
+                if (i >= NX && !(ok = bar_wait(barXE + 8 * (i % NX), (i / NX - 1) & 1, dead))) break;
+                if (e > 0) own(i, b, entry[e].y);   // (the first item's are under way)
+                ++i;
+                for (int k = 0; ok && k < (DKV ? group : 1); ++k)
+                    for (int step = 0; step < per; ++step, ++t) {
+                        if (t >= NST && !(ok = bar_wait(barE + 8 * (t % NST), (t / NST - 1) & 1, dead))) break;
+                        if (e + t > 0) stream(t, b, y0 + step * kStep, DKV ? hx * group + k : hx / group);
+                    }
             }
             if (!ok || *dead) {   // what is in flight ends (bounded) before the CTA does
                 volatile int none = 0;
-                bar_wait(barX, 0, &none);
-                for (int t = max(0, it - NST); t < it; ++t) bar_wait(barY + 8 * (t % NST), (t / NST) & 1, &none);
+                for (int x = max(0, i - NX); x < i; ++x) bar_wait(barX + 8 * (x % NX), (x / NX) & 1, &none);
+                for (int x = max(0, t - NST); x < t; ++x) bar_wait(barY + 8 * (x % NST), (x / NST) & 1, &none);
             }
         }
         __syncwarp();
-    } else if (warp == kWork / 32) {   // products
-        {
-            // the whole warp runs this, so that the operands' words stay in uniform registers; one lane issues
-            const bool lead = elect_one();
-            const int nu = __shfl_sync(0xffffffffu, n, 0);
-            const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0), uA1 = tm + 128 * NB, uA2 = DKV ? uA1 + DP : uA1;
-            constexpr uint32_t idS = mma_desc<T>(128, kStep, false), idA = mma_desc<T>(128, DP, true);
-            auto scores = [&](int it) {
-                const int s = it % NST;
-                if (!bar_wait_warp(barY + 8 * s, (it / NST) & 1, dead)) return false;
-                tc_fence_after();
-                const uint32_t d = tm + (it % NB) * 128, dX = desc_along(sX1), dY = desc_along(sY + s * Sh::kStage);
+    } else if (warp >= kWork / 32) {
+        // Products: one warp forms the scores, one the sums, so that neither's waits and issues stand before the other's;
+        // with two buffers only, one warp does both, since there the scores should follow the sums' products at once (keys
+        // pass, heads of 128: 1830 clocks a tile together, 2325 apart; query pass: 1677 together, 1428 apart).
+        // A whole warp runs this, its operands' words in uniform registers; one lane issues
+        constexpr bool kApart = NB > 2;
+        const bool lead = elect_one();
+        const uint32_t tm = uniform(tmem), uA1 = tm + 128 * NB, uA2 = DKV ? uA1 + DP : uA1;
+        bool ok = true;
+        int t = 0, i = 0;   // tiles and items (with work) so far
+        constexpr uint32_t idS = mma_desc<T>(128, kStep, false), idA = mma_desc<T>(128, DP, true);
+        auto scores = [&](int t, uint32_t dX) {
+            const int s = t % NST, buf = t % NB;
+            if (!bar_wait_warp(barY + 8 * s, (t / NST) & 1, dead)) return false;
+            if (kApart && t >= NB && !bar_wait_warp(barPE + 8 * buf, (t / NB - 1) & 1, dead)) return false;
+            tc_fence_after();
+            const uint32_t d = tm + buf * 128, dY = desc_along(sY + s * Sh::kStage);
 #pragma unroll
-                for (int w = 0; w < 2; ++w)
+            for (int w = 0; w < 2; ++w)
 #pragma unroll
-                    for (int k = 0; k < DP / 16; ++k)
-                        if (lead) mma_ss(d + 64 * w, dX + (w * Sh::kX + (k / 4) * kChunkX + (k % 4) * 32) / 16,
-                               dY + (w * Sh::kY + (k / 4) * kChunkY + (k % 4) * 32) / 16, idS, k != 0);
-                if (lead) tc_commit(barS + 8 * (it % NB));
-                return true;
-            };
-            bool ok = bar_wait_warp(barX, 0, dead);
-            for (int it = 0; ok && it < NB && it < nu; ++it) ok = scores(it);
-            for (int it = 0; ok && it < nu; ++it) {
-                const int s = it % NST;
-                if (!(ok = bar_wait_warp(barP + 8 * (it % NB), (it / NB) & 1, dead))) break;
-                tc_fence_after();
-                const uint32_t p = tm + (it % NB) * 128, dY = desc_down(sY + s * Sh::kStage, kChunkY);
-                if (DKV) {
+                for (int k = 0; k < DP / 16; ++k)
+                    if (lead) mma_ss(d + 64 * w, dX + (w * Sh::kX + (k / 4) * kChunkX + (k % 4) * 32) / 16,
+                                     dY + (w * Sh::kY + (k / 4) * kChunkY + (k % 4) * 32) / 16, idS, k != 0);
+            if (lead) tc_commit(barS + 8 * buf);
+            return true;
+        };
+        if (kApart && warp == kWork / 32) {
+            for (int e = 0; ok && e < count; ++e) {
+                const int n = (int)uniform(span[e].y * (DKV ? group : 1));
+                if (n == 0) continue;
+                const int xs = i % NX;
+                if (!(ok = bar_wait_warp(barX + 8 * xs, (i / NX) & 1, dead))) break;
+                const uint32_t dX = desc_along(base + xs * 2 * Sh::kX);
+                for (int it = 0; it < n; ++it, ++t)
+                    if (!(ok = scores(t, dX))) break;
+                if (lead) tc_commit(barXE + 8 * xs);   // the owned tile's last use
+                ++i;
+            }
+        } else if (warp == kWork / 32 + 1) {
+            for (int e = 0; ok && e < count; ++e) {
+                const int n = (int)uniform(span[e].y * (DKV ? group : 1));
+                if (n == 0) continue;
+                const int xs = i % NX;
+                const uint32_t dX = desc_along(base + xs * 2 * Sh::kX);
+                if (!kApart) {
+                    ok = bar_wait_warp(barX + 8 * xs, (i / NX) & 1, dead);
+                    for (int it = 0; ok && it < NB && it < n; ++it) ok = scores(t + it, dX);
+                    if (!ok) break;
+                }
+                for (int it = 0; it < n; ++it, ++t) {
+                    const int s = t % NST, buf = t % NB;
+                    if (!(ok = bar_wait_warp(barP + 8 * buf, (t / NB) & 1, dead))) break;
+                    if (it == 0 && i > 0 && !(ok = bar_wait_warp(barA, (i - 1) & 1, dead))) break;   // the results before are read
+                    tc_fence_after();
+                    const uint32_t p = tm + buf * 128, dY = desc_down(sY + s * Sh::kStage, kChunkY);
+                    if (DKV) {
+#pragma unroll
+                        for (int k = 0; k < kStep / 16; ++k)
+                            if (lead) mma_ts(uA1, p + 32 * (k / 2) + 8 * (k % 2), dY + (Sh::kY + k * 2048) / 16, idA, (it | k) != 0);
+                    }
 #pragma unroll
                     for (int k = 0; k < kStep / 16; ++k)
-                        if (lead) mma_ts(uA1, p + 32 * (k / 2) + 8 * (k % 2), dY + (Sh::kY + k * 2048) / 16, idA, (it | k) != 0);
+                        if (lead) mma_ts(uA2, p + 64 + 32 * (k / 2) + 8 * (k % 2), dY + k * (2048 / 16), idA, (it | k) != 0);
+                    if (lead) tc_commit(barE + 8 * s);
+                    if (kApart) {
+                        if (lead) tc_commit(barPE + 8 * buf);
+                    } else {
+                        if (it + NB < n && !(ok = scores(t + NB, dX))) break;
+                        if (it + NB == max(n, NB) && lead) tc_commit(barXE + 8 * xs);   // the owned tile's last use
+                    }
                 }
-#pragma unroll
-                for (int k = 0; k < kStep / 16; ++k)
-                    if (lead) mma_ts(uA2, p + 64 + 32 * (k / 2) + 8 * (k % 2), dY + k * (2048 / 16), idA, (it | k) != 0);
-                if (lead) tc_commit(barE + 8 * s);
-                if (it + NB < nu) ok = scores(it + NB);
+                if (lead) tc_commit(barF);
+                ++i;
             }
-            if (lead) tc_commit(barF);
             if (!ok && lead) atomicAdd(&g_gave_up, 1ull);
         }
         __syncwarp();
     } else {   // P and dS of a tile
-        const int pair = warp >> 3, half = (warp >> 2) & 1, w4 = warp & 3, r = tid & 127, x = x0 + r;
+        const int pair = warp >> 3, half = (warp >> 2) & 1, w4 = warp & 3, r = tid & 127;
         const uint32_t trow = (uint32_t)(32 * w4) << 16;
         const float c = a.scale * kLog2e;
-        float rl = 0.f, rd = 0.f;
-        if (!DKV) {
-            const size_t at = ((size_t)b * a.H + hx) * g.Lp + x;   // Lp covers the tile
-            rl = g.lse[at], rd = g.delta[at];
-        }
-        float far0 = 0.f, far1 = 0.f, bsum[kBuckets / 32];
-#pragma unroll
-        for (int i = 0; i < kBuckets / 32; ++i) bsum[i] = 0.f;
         bool ok = true;
         float* const dw = diag + warp * 72;
-        for (int head = 0; head < (DKV ? group : 1); ++head) {
-        if (BIAS && DKV) {   // keys pass: the bias of the group's next head, once every warp is past the one before
-            asm volatile("bar.sync 1, 512;" ::: "memory");
-            fill_lut<T>(lut, a, hx * group + head, reach, warp, kWork / 32);
-            asm volatile("bar.sync 1, 512;" ::: "memory");
-        }
-        for (int step = (pair ^ (head * per)) & 1; step < per; step += 2) {   // this pair's tiles of the head
-            const int it = head * per + step, s = it % NST, buf = it % NB, yb = y0 + step * kStep;
-            // (after a wait that gave up a warp still meets its partners at the barriers above)
-            // (the streamed tile's own barrier: the keys pass reads the row statistics that came with it)
-            ok = ok && (!DKV || bar_wait_warp(barY + 8 * s, (it / NST) & 1, dead)) &&
-                 bar_wait_warp(barS + 8 * buf, (it / NB) & 1, dead);
-            if (!ok) continue;
-            tc_fence_after();
-            const int col0 = 32 * half, yc = yb + col0;
-            const uint32_t tS = tmem + trow + buf * 128, tD = tS + 64;
-            const float* const st = reinterpret_cast<const float*>(gb + 2 * Sh::kX + s * Sh::kStage + 2 * Sh::kY) + col0;
-            // d = key position - query position of this row and the block's first column; a column is one less or one more
-            const int d0 = DKV ? x - (yc + off) : yc - (x + off);
-            // the range of d in the warp's block of 32 x 32
-            const int lo = DKV ? x0 + 32 * w4 - (yc + 31 + off) : yc - (x0 + 32 * w4 + 31 + off), hi = lo + 62;
-            const bool near = BIAS && lo < reach && hi > -reach;
-            // columns this row meets: [c0, c1)
-            int c0 = 0, c1 = x < lx ? min(32, ly - yc) : 0;
-            if (a.causal) {
-                if (DKV) c0 = max(0, d0);
-                else c1 = min(c1, 1 - d0);
+        int t0 = 0, done = 0;   // tiles and items (with work) so far
+        for (int e = 0; e < count; ++e) {
+            const int4 en = entry[e];
+            // (from one lane for all, so that the branches on them are known to be the warp's)
+            const int x0 = __shfl_sync(0xffffffffu, en.y, 0), lq = __shfl_sync(0xffffffffu, en.z, 0), lk = __shfl_sync(0xffffffffu, en.w, 0);
+            const int y0 = __shfl_sync(0xffffffffu, span[e].x, 0), per = __shfl_sync(0xffffffffu, span[e].y, 0);
+            const int b = en.x, off = a.causal ? lk - lq : 0, lx = DKV ? lk : lq, ly = DKV ? lq : lk, x = x0 + r;
+            float* const part = sums ? g.part + ((size_t)hx * n_buckets(a.edges) * a.B + b) * row_tiles + x0 / kOwn : nullptr;
+            if (per == 0) {   // nothing meets these rows
+                const int rows = min(kOwn, Lx - x0), units = a.D / 8;
+                for (int v = tid; v < rows * units; v += kWork) {
+                    const size_t at = (((size_t)b * Lx + x0 + v / units) * heads + hx) * a.D + (v % units) * 8;
+                    *reinterpret_cast<uint4*>((T*)g.dx2 + at) = make_uint4(0, 0, 0, 0);
+                    if (DKV) *reinterpret_cast<uint4*>((T*)g.dx1 + at) = make_uint4(0, 0, 0, 0);
+                }
+                if (sums)
+                    for (int t = tid; t < n_buckets(a.edges); t += kWork) part[(size_t)t * a.B * row_tiles] = 0.f;
+                continue;
             }
-            const bool edge = __any_sync(0xffffffffu, c0 > 0 || c1 < 32);
-            float run = 0.f, all = 0.f;   // the diagonals under way; the sum of a block in one bucket
-            // (forms without the masks and without the bias by position: a block needs them rarely)
-            auto block = [&](auto edge_c, auto near_c) {
-                constexpr bool EDGE = decltype(edge_c)::value, NEAR = decltype(near_c)::value;
-                // four columns' entries at lp +- y: the keys pass meets them in falling order
-                const float* const lp = lut_row(lut, reach, d0 + reach + kPad - (DKV ? 3 : 0));
-                const float flat = BIAS && !NEAR ? (lo >= reach ? lut[lut_entries(reach) - 1] : lut[0]) : 0.f;
-                uint32_t sv[32], dv[32];
-                tmem_ld32(tS + col0, sv);
-                tmem_ld32(tD + col0, dv);
-                tmem_wait_ld();
-                tmem_tie32(sv), tmem_tie32(dv);
+            float rl = 0.f, rd = 0.f;
+            if (!DKV) {
+                const size_t at = ((size_t)b * a.H + hx) * g.Lp + x;   // Lp covers the tile
+                rl = g.lse[at], rd = g.delta[at];
+            }
+            float far0 = 0.f, far1 = 0.f, bsum[kBuckets / 32];
 #pragma unroll
-                for (int y = 0; y < 32; y += 4) {
-                    float4 L, E;
-                    if (DKV) {
-                        L = *reinterpret_cast<const float4*>(st + y);
-                        E = *reinterpret_cast<const float4*>(st + kStep + y);
-                    } else {
-                        L = make_float4(rl, rl, rl, rl), E = make_float4(rd, rd, rd, rd);
+            for (int i = 0; i < kBuckets / 32; ++i) bsum[i] = 0.f;
+            for (int head = 0; head < (DKV ? group : 1); ++head) {
+                if (BIAS && DKV && group > 1) {   // keys pass: the bias of the group's next head, once every warp is past the one before
+                    asm volatile("bar.sync 1, 512;" ::: "memory");
+                    fill_lut<T>(lut, a, hx * group + head, reach, warp, kWork / 32);
+                    asm volatile("bar.sync 1, 512;" ::: "memory");
+                }
+                for (int step = (pair ^ (t0 + head * per)) & 1; step < per; step += 2) {   // this pair's tiles of the head
+                    const int t = t0 + head * per + step, s = t % NST, buf = t % NB, yb = y0 + step * kStep;
+                    // (after a wait that gave up a warp still meets its partners at the barriers above)
+                    // (the streamed tile's own barrier: the keys pass reads the row statistics that came with it)
+                    ok = ok && (!DKV || bar_wait_warp(barY + 8 * s, (t / NST) & 1, dead)) &&
+                         bar_wait_warp(barS + 8 * buf, (t / NB) & 1, dead);
+                    if (!ok) continue;
+                    tc_fence_after();
+                    const int col0 = 32 * half, yc = yb + col0;
+                    const uint32_t tS = tmem + trow + buf * 128, tD = tS + 64;
+                    const float* const st = reinterpret_cast<const float*>(gb + 2 * NX * Sh::kX + s * Sh::kStage + 2 * Sh::kY) + col0;
+                    // d = key position - query position of this row and the block's first column; a column is one less or one more
+                    const int d0 = DKV ? x - (yc + off) : yc - (x + off);
+                    // the range of d in the warp's block of 32 x 32
+                    const int lo = DKV ? x0 + 32 * w4 - (yc + 31 + off) : yc - (x0 + 32 * w4 + 31 + off), hi = lo + 62;
+                    const bool near = BIAS && lo < reach && hi > -reach;
+                    // columns this row meets: [c0, c1)
+                    int c0 = 0, c1 = x < lx ? min(32, ly - yc) : 0;
+                    if (a.causal) {
+                        if (DKV) c0 = max(0, d0);
+                        else c1 = min(c1, 1 - d0);
                     }
-                    const float Lv[4] = {L.x, L.y, L.z, L.w}, Ev[4] = {E.x, E.y, E.z, E.w};
-                    float4 e = make_float4(flat, flat, flat, flat);
-                    if (BIAS && NEAR) e = *reinterpret_cast<const float4*>(DKV ? lp - y : lp + y);
-                    const float Bv[4] = {DKV ? e.w : e.x, DKV ? e.z : e.y, DKV ? e.y : e.z, DKV ? e.x : e.w};
-                    float pv[4], gv[4];
+                    const bool edge = __any_sync(0xffffffffu, c0 > 0 || c1 < 32);
+                    float run = 0.f, all = 0.f;   // the diagonals under way; the sum of a block in one bucket
+                    // (forms without the masks and without the bias by position: a block needs them rarely)
+                    auto block = [&](auto edge_c, auto near_c) {
+                        constexpr bool EDGE = decltype(edge_c)::value, NEAR = decltype(near_c)::value;
+                        // four columns' entries at lp +- y: the keys pass meets them in falling order
+                        const float* const lp = lut_row(lut, reach, d0 + reach + kPad - (DKV ? 3 : 0));
+                        const float flat = BIAS && !NEAR ? (lo >= reach ? lut[lut_entries(reach) - 1] : lut[0]) : 0.f;
+                        uint32_t sv[32], dv[32];
+                        tmem_ld32(tS + col0, sv);
+                        tmem_ld32(tD + col0, dv);
+                        tmem_wait_ld();
+                        tmem_tie32(sv), tmem_tie32(dv);
+#pragma unroll
+                        for (int y = 0; y < 32; y += 4) {
+                            float4 L, E;
+                            if (DKV) {
+                                L = *reinterpret_cast<const float4*>(st + y);
+                                E = *reinterpret_cast<const float4*>(st + kStep + y);
+                            } else {
+                                L = make_float4(rl, rl, rl, rl), E = make_float4(rd, rd, rd, rd);
+                            }
+                            const float Lv[4] = {L.x, L.y, L.z, L.w}, Ev[4] = {E.x, E.y, E.z, E.w};
+                            float4 e = make_float4(flat, flat, flat, flat);
+                            if (BIAS && NEAR) e = *reinterpret_cast<const float4*>(DKV ? lp - y : lp + y);
+                            const float Bv[4] = {DKV ? e.w : e.x, DKV ? e.z : e.y, DKV ? e.y : e.z, DKV ? e.x : e.w};
+                            float pv[4], gv[4];
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) {
+                                const int col = y + z;
+                                const float raw_s = __uint_as_float(sv[col]);
+                                const float t = BIAS ? fmaf(raw_s, c, Bv[z]) - Lv[z] : fmaf(raw_s, c, -Lv[z]);
+                                pv[z] = ex2(t);
+                                gv[z] = pv[z] * (__uint_as_float(dv[col]) - Ev[z]);
+                                if (EDGE) {
+                                    const bool in = col >= c0 && col < c1;
+                                    pv[z] = in ? pv[z] : 0.f;
+                                    gv[z] = in ? gv[z] : 0.f;
+                                }
+                                if (BIAS && !DKV) {
+                                    if (NEAR) {
+                                        run = __shfl_up_sync(0xffffffffu, run, 1);
+                                        run = (lane ? run : 0.f) + gv[z];
+                                        if (lane == 31) dw[col] = run;
+                                    } else {
+                                        all += gv[z];
+                                    }
+                                }
+                            }
+                            sv[y / 2] = pack2<T>(pv[0], pv[1]), sv[y / 2 + 1] = pack2<T>(pv[2], pv[3]);
+                            dv[y / 2] = pack2<T>(gv[0], gv[1]), dv[y / 2 + 1] = pack2<T>(gv[2], gv[3]);
+                        }
+                        if (DKV) tmem_st16(tS + col0, sv);
+                        tmem_st16(tD + col0, dv);
+                    };
+                    if (BIAS && near) {
+                        if (edge) block(std::true_type{}, std::true_type{});
+                        else block(std::false_type{}, std::true_type{});
+                    } else {
+                        if (edge) block(std::true_type{}, std::false_type{});
+                        else block(std::false_type{}, std::false_type{});
+                    }
+                    const int live = ly - yb;
+                    if (live < kStep) {   // rows of Y past the length to zero, for the products that sum over them
+                        uint8_t* const y = gb + 2 * NX * Sh::kX + s * Sh::kStage;
+                        const int dead_units = (kStep - live) * 8;
+                        for (int e = tid & 255; e < dead_units * Sh::kChunks * (DKV ? 2 : 1); e += 256) {
+                            const int ch = e / dead_units, o = e % dead_units;
+                            *reinterpret_cast<uint4*>(y + ch * kChunkY + live * 128 + o * 16) = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_async_smem();
+                    }
+                    tmem_wait_st();
+                    tc_fence_before();
+                    bar_arrive_warp(barP + 8 * buf);
+                    if (sums) {
+                        if (near) {
+                            dw[62 - lane] = run;   // the diagonals still under way; lane 31's is in place
+                            __syncwarp();
+                            // the 63 sums (and a zero) scanned: lane l takes 2 l and 2 l + 1
+                            const float s0 = dw[2 * lane], s1 = s0 + (lane < 31 ? dw[2 * lane + 1] : 0.f);
+                            float t = s1;
+#pragma unroll
+                            for (int o = 1; o < 32; o <<= 1) {
+                                const float u = __shfl_up_sync(0xffffffffu, t, o);
+                                if (lane >= o) t += u;
+                            }
+                            __syncwarp();
+                            dw[2 * lane + 1] = t - s1 + s0, dw[2 * lane + 2] = t;
+                            if (lane == 0) dw[0] = 0.f;
+                            __syncwarp();
+                            // entry e now holds the sum of the diagonals d in [lo, lo + e)
+                            const int nb = n_buckets(a.edges);
+#pragma unroll
+                            for (int i = 0; i < kBuckets / 32; ++i) {
+                                const int t2 = lane + 32 * i;
+                                if (t2 < nb) {
+                                    const int e0 = max(range[2 * t2] - lo, 0), e1 = min(range[2 * t2 + 1] - lo + 1, 63);
+                                    if (e0 < e1) bsum[i] += dw[e1] - dw[e0];
+                                }
+                            }
+                            __syncwarp();
+                        } else if (lo >= reach) {
+                            far1 += all;
+                        } else {
+                            far0 += all;
+                        }
+                    }
+                }
+            }
+            if (sums) {   // the tile's sums, warp by warp in order
+                const int nb = n_buckets(a.edges);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) {
+                    far0 += __shfl_xor_sync(0xffffffffu, far0, o);
+                    far1 += __shfl_xor_sync(0xffffffffu, far1, o);
+                }
+#pragma unroll
+                for (int i = 0; i < kBuckets / 32; ++i) {
+                    const int t = lane + 32 * i;
+                    if (t < nb) red[warp * kBuckets + t] = bsum[i] + (t == a.edges.n ? far0 : 0.f) + (a.edges.two && t == nb - 1 ? far1 : 0.f);
+                }
+                asm volatile("bar.sync 1, 512;" ::: "memory");
+                for (int t = tid; t < nb; t += kWork) {
+                    float v = 0.f;
+#pragma unroll
+                    for (int k = 0; k < kWork / 32; ++k) v += red[k * kBuckets + t];
+                    part[(size_t)t * a.B * row_tiles] = v;
+                }
+                asm volatile("bar.sync 1, 512;" ::: "memory");   // read before the next tile's
+            }
+            ok = ok && bar_wait_warp(barF, done & 1, dead);
+            tc_fence_after();
+            // keys pass: half of dV's or dK's columns a warpgroup; query pass: a quarter of dQ's.  A row a thread, whole
+            // 32-byte sectors
+            const bool row = x < lx, first = DKV && pair == 0;
+            const float w = first ? 1.f : a.scale;
+            const int f0 = DKV ? half * (DP / 2) : (warp >> 2) * (DP / 4);
+            constexpr int kCols = DKV ? DP / 2 : DP / 4;
+            const uint32_t acc = (first ? tA1 : tA2) + trow;
+            uint32_t o[kCols];
+#pragma unroll
+            for (int f = 0; f < kCols; f += 16) tmem_ld16(acc + f0 + f, o + f);
+            tmem_wait_ld();
+#pragma unroll
+            for (int f = 0; f < kCols; f += 16) tmem_tie16(o + f);
+            tc_fence_before();
+            bar_arrive_warp(barA);   // the next item's products may overwrite them
+            if (x < Lx) {
+                T* const rp = (T*)(first ? g.dx1 : g.dx2) + (((size_t)b * Lx + x) * heads + hx) * a.D + f0;
+#pragma unroll
+                for (int y = 0; y < kCols; y += 8) {
+                    uint32_t p[4];
 #pragma unroll
                     for (int z = 0; z < 4; ++z) {
-                        const int col = y + z;
-                        const float raw_s = __uint_as_float(sv[col]);
-                        const float t = BIAS ? fmaf(raw_s, c, Bv[z]) - Lv[z] : fmaf(raw_s, c, -Lv[z]);
-                        pv[z] = ex2(t);
-                        gv[z] = pv[z] * (__uint_as_float(dv[col]) - Ev[z]);
-                        if (EDGE) {
-                            const bool in = col >= c0 && col < c1;
-                            pv[z] = in ? pv[z] : 0.f;
-                            gv[z] = in ? gv[z] : 0.f;
-                        }
-                        if (BIAS && !DKV) {
-                            if (NEAR) {
-                                run = __shfl_up_sync(0xffffffffu, run, 1);
-                                run = (lane ? run : 0.f) + gv[z];
-                                if (lane == 31) dw[col] = run;
-                            } else {
-                                all += gv[z];
-                            }
-                        }
+                        const float u0 = __uint_as_float(o[y + 2 * z]) * w, u1 = __uint_as_float(o[y + 2 * z + 1]) * w;
+                        p[z] = !row ? 0u : ok ? pack2<T>(u0, u1) : pack2<T>(NAN, NAN);
                     }
-                    sv[y / 2] = pack2<T>(pv[0], pv[1]), sv[y / 2 + 1] = pack2<T>(pv[2], pv[3]);
-                    dv[y / 2] = pack2<T>(gv[0], gv[1]), dv[y / 2 + 1] = pack2<T>(gv[2], gv[3]);
-                }
-                if (DKV) tmem_st16(tS + col0, sv);
-                tmem_st16(tD + col0, dv);
-            };
-            if (BIAS && near) {
-                if (edge) block(std::true_type{}, std::true_type{});
-                else block(std::false_type{}, std::true_type{});
-            } else {
-                if (edge) block(std::true_type{}, std::false_type{});
-                else block(std::false_type{}, std::false_type{});
-            }
-            const int live = ly - yb;
-            if (live < kStep) {   // rows of Y past the length to zero, for the products that sum over them
-                uint8_t* const y = gb + 2 * Sh::kX + s * Sh::kStage;
-                const int dead_units = (kStep - live) * 8;
-                for (int e = tid & 255; e < dead_units * Sh::kChunks * (DKV ? 2 : 1); e += 256) {
-                    const int ch = e / dead_units, o = e % dead_units;
-                    *reinterpret_cast<uint4*>(y + ch * kChunkY + live * 128 + o * 16) = make_uint4(0, 0, 0, 0);
-                }
-                fence_async_smem();
-            }
-            tmem_wait_st();
-            tc_fence_before();
-            bar_arrive_warp(barP + 8 * buf);
-            if (sums) {
-                if (near) {
-                    dw[62 - lane] = run;   // the diagonals still under way; lane 31's is in place
-                    __syncwarp();
-                    // the 63 sums (and a zero) scanned: lane l takes 2 l and 2 l + 1
-                    const float s0 = dw[2 * lane], s1 = s0 + (lane < 31 ? dw[2 * lane + 1] : 0.f);
-                    float t = s1;
-#pragma unroll
-                    for (int o = 1; o < 32; o <<= 1) {
-                        const float u = __shfl_up_sync(0xffffffffu, t, o);
-                        if (lane >= o) t += u;
-                    }
-                    __syncwarp();
-                    dw[2 * lane + 1] = t - s1 + s0, dw[2 * lane + 2] = t;
-                    if (lane == 0) dw[0] = 0.f;
-                    __syncwarp();
-                    // entry e now holds the sum of the diagonals d in [lo, lo + e)
-                    const int nb = n_buckets(a.edges);
-#pragma unroll
-                    for (int i = 0; i < kBuckets / 32; ++i) {
-                        const int t2 = lane + 32 * i;
-                        if (t2 < nb) {
-                            const int e0 = max(range[2 * t2] - lo, 0), e1 = min(range[2 * t2 + 1] - lo + 1, 63);
-                            if (e0 < e1) bsum[i] += dw[e1] - dw[e0];
-                        }
-                    }
-                    __syncwarp();
-                } else if (lo >= reach) {
-                    far1 += all;
-                } else {
-                    far0 += all;
+                    if (f0 + y < a.D) *reinterpret_cast<uint4*>(rp + y) = make_uint4(p[0], p[1], p[2], p[3]);
                 }
             }
-        }
-        }
-        ok = ok && bar_wait_warp(barF, 0, dead);
-        tc_fence_after();
-        // accumulators to the owned tiles' shared memory (their last use is over), swizzled as the copy out reads them:
-        // keys pass: half of dV's or dK's columns a warpgroup; query pass: a quarter of dQ's
-        const bool row = x < lx;
-        const bool first = DKV && pair == 0;
-        const float w = !ok ? NAN : (first ? 1.f : a.scale);
-        const int f0 = DKV ? half * (DP / 2) : (warp >> 2) * (DP / 4), f1 = f0 + (DKV ? DP / 2 : DP / 4);
-        const uint32_t acc = (first ? tA1 : tA2) + trow;
-        uint8_t* const stage = gb + (first ? 0 : Sh::kX);
-#pragma unroll 1
-        for (int f = f0; f < f1; f += 16) {
-            uint32_t o[16];
-            tmem_ld16(acc + f, o);
-            tmem_wait_ld();
-            tmem_tie16(o);
-            uint8_t* const rp = stage + (f / 64) * kChunkX + r * 128;
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                uint32_t p[4];
-#pragma unroll
-                for (int z = 0; z < 4; ++z)
-                    p[z] = row ? pack2<T>(__uint_as_float(o[8 * y + 2 * z]) * w, __uint_as_float(o[8 * y + 2 * z + 1]) * w) : 0u;
-                *reinterpret_cast<uint4*>(rp + ((((f % 64) / 8 + y) ^ (r & 7)) << 4)) = make_uint4(p[0], p[1], p[2], p[3]);
-            }
-        }
-        if (sums) {
-            const int nb = n_buckets(a.edges);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) {
-                far0 += __shfl_xor_sync(0xffffffffu, far0, o);
-                far1 += __shfl_xor_sync(0xffffffffu, far1, o);
-            }
-#pragma unroll
-            for (int i = 0; i < kBuckets / 32; ++i) {
-                const int t = lane + 32 * i;
-                if (t < nb) red[warp * kBuckets + t] = bsum[i] + (t == a.edges.n ? far0 : 0.f) + (a.edges.two && t == nb - 1 ? far1 : 0.f);
-            }
-        }
-        fence_async_smem();
-        asm volatile("bar.sync 1, 512;" ::: "memory");
-        if (tid == 0) {
-#pragma unroll
-            for (int ch = 0; ch < Sh::kChunks; ++ch) {
-                if (DKV) tma_store(&tmD1, 64 * ch, x0, hx, b, sX1 + ch * kChunkX);
-                tma_store(&tmD2, 64 * ch, x0, hx, b, sX2 + ch * kChunkX);
-            }
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-        }
-        if (sums) {
-            const int nb = n_buckets(a.edges);
-            for (int t = tid; t < nb; t += kWork) {
-                float v = 0.f;
-#pragma unroll
-                for (int k = 0; k < kWork / 32; ++k) v += red[k * kBuckets + t];
-                g.part[(((size_t)hx * nb + t) * a.B + b) * gridDim.x + blockIdx.x] = v;
-            }
+            t0 += per * (DKV ? group : 1), ++done;
         }
     }
     tc_fence_before();
@@ -495,12 +577,55 @@ __global__ void __launch_bounds__(128) attn_dbias_kernel(const float* part, int 
     if (lane == 0) dbias[(size_t)t * H + h] = from_f<T>(s);
 }
 
+// items by falling number of streamed tiles (any order among equals)
+constexpr int kBins = 1024, kMaxOrder = 1 << 16;
+template <bool DKV>
+__device__ void order_items(const AttnArgs& a, int* order) {
+    __shared__ int first[kBins], warp_sum[32];
+    const int items = a.B * (((DKV ? a.Lk : a.Lq) + kOwn - 1) / kOwn), t = threadIdx.x;
+    auto bin = [&](int i) { return kBins - 1 - min(item_at<DKV>(a, nullptr, i).per, kBins - 1); };
+    first[t] = 0;
+    __syncthreads();
+    for (int i = t; i < items; i += 1024) atomicAdd(&first[bin(i)], 1);
+    __syncthreads();
+    const int n = first[t];
+    int sum = n;   // inclusive scan over the bins
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if ((t & 31) >= o) sum += v;
+    }
+    if ((t & 31) == 31) warp_sum[t >> 5] = sum;
+    __syncthreads();
+    for (int w = 0; w < (t >> 5); ++w) sum += warp_sum[w];
+    first[t] = sum - n;
+    __syncthreads();
+    for (int i = t; i < items; i += 1024) order[atomicAdd(&first[bin(i)], 1)] = i;
+}
+__global__ void __launch_bounds__(1024) attn_order_kernel(const __grid_constant__ AttnArgs a, int* keys, int* queries) {
+    if (blockIdx.x == 0 && keys) order_items<true>(a, keys);
+    if (blockIdx.x == 1 && queries) order_items<false>(a, queries);
+}
+
 int tiles_of(int L) { return (L + kOwn - 1) / kOwn; }
 size_t stats_floats(const AttnArgs& a) { return (size_t)a.B * a.H * tiles_of(a.Lq) * kOwn; }
-size_t part_floats(const AttnArgs& a) { return (size_t)((a.edges.n + 1) << a.edges.two) * a.H * a.B * tiles_of(a.Lq); }
+size_t part_floats(const AttnArgs& a) {
+    return ((size_t)((a.edges.n + 1) << a.edges.two) * a.H * a.B * tiles_of(a.Lq) + 3) & ~(size_t)3;
+}
+// CTAs of a head: one for each owned tile, or, where each SM would see four or more of them, its share of the SMs
+long long ctas_of(const AttnArgs& a, bool dkv, int sms) {
+    const long long items = (long long)a.B * tiles_of(dkv ? a.Lk : a.Lq), heads = dkv ? a.Hkv : a.H;
+    if (items * heads < 4LL * sms) return items;
+    return std::max<long long>(sms > heads ? sms / heads : 1, (items + kMaxItems - 1) / kMaxItems);
+}
+// ints of its items' order, where lengths differ and CTAs take several
+size_t order_ints(const AttnArgs& a, bool dkv, int sms) {
+    const long long items = (long long)a.B * tiles_of(dkv ? a.Lk : a.Lq);
+    return (a.lengths || a.causal) && ctas_of(a, dkv, sms) < items && items <= kMaxOrder ? (size_t)(items + 3) & ~(size_t)3 : 0;
+}
 
 template <class T, int DP, bool BIAS, bool DKV>
-int launch_pass(const Args& g, const CUtensorMap* tm, cudaStream_t st) {
+int launch_pass(const Args& g, const CUtensorMap* tm, long long ctas, cudaStream_t st) {
     static DeviceSetup setup;
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
@@ -512,24 +637,32 @@ int launch_pass(const Args& g, const CUtensorMap* tm, cudaStream_t st) {
     if (rc) return rc;
     const int reach = BIAS ? reach_of(g.a.edges) : 0;
     const size_t smem = smem_bytes<DP, BIAS>(DKV, reach);
-    const dim3 grid(tiles_of(DKV ? g.a.Lk : g.a.Lq), DKV ? g.a.Hkv : g.a.H, g.a.B);
-    attn_bwd_kernel<T, DP, BIAS, DKV><<<grid, kThreads, smem, st>>>(tm[0], tm[1], tm[2], tm[3], tm[4], tm[5], g);
+    attn_bwd_kernel<T, DP, BIAS, DKV><<<dim3(DKV ? g.a.Hkv : g.a.H, (unsigned)ctas), kThreads, smem, st>>>(tm[0], tm[1], tm[2], tm[3], g);
     return (int)cudaGetLastError();
 }
 template <class T, int DP>
-int launch_pass(const Args& g, bool dkv, const CUtensorMap* tm, cudaStream_t st) {
-    if (g.a.bias) return dkv ? launch_pass<T, DP, true, true>(g, tm, st) : launch_pass<T, DP, true, false>(g, tm, st);
-    return dkv ? launch_pass<T, DP, false, true>(g, tm, st) : launch_pass<T, DP, false, false>(g, tm, st);
+int launch_pass(const Args& g, bool dkv, const CUtensorMap* tm, long long ctas, cudaStream_t st) {
+    if (ctas > 65535) return D2P_ERR_TOO_LARGE;
+    if (g.a.bias) return dkv ? launch_pass<T, DP, true, true>(g, tm, ctas, st) : launch_pass<T, DP, true, false>(g, tm, ctas, st);
+    return dkv ? launch_pass<T, DP, false, true>(g, tm, ctas, st) : launch_pass<T, DP, false, false>(g, tm, ctas, st);
 }
 
 template <class T>
 int run(const AttnArgs& a, int dtype, const void* out, const float* lse, const void* grad, void* dq, void* dk, void* dv,
-        void* dbias, void* ws, cudaStream_t st) {
+        void* dbias, void* ws, int sms, cudaStream_t st) {
     const int Lp = tiles_of(a.Lq) * kOwn;
     float* const lp = (float*)ws;
     float* const dp = lp + stats_floats(a);
     float* const part = dp + stats_floats(a);
+    int* const order = (int*)(part + (dbias ? part_floats(a) : 0));
+    const size_t ok = order_ints(a, true, sms), oq = order_ints(a, false, sms);
+    int* const order_k = ok ? order : nullptr;
+    int* const order_q = oq ? order + ok : nullptr;
     int rc = 0;
+    if (ok || oq) {
+        attn_order_kernel<<<2, 1024, 0, st>>>(a, order_k, order_q);
+        if ((rc = (int)cudaGetLastError())) return rc;
+    }
     if (a.B && a.Lq) {
         attn_stats_kernel<T><<<dim3(Lp / 16, a.H, a.B), 256, 0, st>>>(a, (const T*)out, lse, (const T*)grad, Lp, lp, dp);
         if ((rc = (int)cudaGetLastError())) return rc;
@@ -537,38 +670,36 @@ int run(const AttnArgs& a, int dtype, const void* out, const float* lse, const v
     if (a.B && (a.Lq || a.Lk)) {
         // maps of the rows there are; an axis without rows is never read
         const long long gs[3] = {(long long)a.Lq * a.H * a.D, (long long)a.H * a.D, a.D};
-        const long long os[3] = {(long long)a.Lk * a.Hkv * a.D, (long long)a.Hkv * a.D, a.D};
-        CUtensorMap own[4] = {}, str[4] = {}, res[3] = {};   // q, dO, k, v; dq, dk, dv
-        bool ok = true;
+        CUtensorMap own[4] = {}, str[4] = {};   // q, dO, k, v
+        bool fine = true;
         if (a.Lq) {
             for (int w = 0; w < 2; ++w) {
                 CUtensorMap* const m = w ? str : own;
-                ok = ok && rows_map(m, dtype, a.q, a.B, a.Lq, a.H, a.D, a.qs, w ? kStep : kOwn) &&
+                fine = fine && rows_map(m, dtype, a.q, a.B, a.Lq, a.H, a.D, a.qs, w ? kStep : kOwn) &&
                      rows_map(m + 1, dtype, grad, a.B, a.Lq, a.H, a.D, gs, w ? kStep : kOwn);
             }
-            ok = ok && rows_map(res, dtype, dq, a.B, a.Lq, a.H, a.D, gs, kOwn);
         }
         if (a.Lk) {
             for (int w = 0; w < 2; ++w) {
                 CUtensorMap* const m = w ? str : own;
-                ok = ok && rows_map(m + 2, dtype, a.k, a.B, a.Lk, a.Hkv, a.D, a.ks, w ? kStep : kOwn) &&
+                fine = fine && rows_map(m + 2, dtype, a.k, a.B, a.Lk, a.Hkv, a.D, a.ks, w ? kStep : kOwn) &&
                      rows_map(m + 3, dtype, a.v, a.B, a.Lk, a.Hkv, a.D, a.vs, w ? kStep : kOwn);
             }
-            ok = ok && rows_map(res + 1, dtype, dk, a.B, a.Lk, a.Hkv, a.D, os, kOwn) &&
-                 rows_map(res + 2, dtype, dv, a.B, a.Lk, a.Hkv, a.D, os, kOwn);
         }
-        if (!ok) return D2P_ERR_INVALID_ARGUMENT;
-        Args g = {a, lp, dp, Lp, nullptr, nullptr, nullptr};
+        if (!fine) return D2P_ERR_INVALID_ARGUMENT;
+        Args g = {a, lp, dp, Lp, nullptr, nullptr, nullptr, nullptr};
         if (a.Lk) {
-            g.dx1 = dv, g.dx2 = dk;
-            const CUtensorMap tm[6] = {own[2], own[3], str[0], str[1], res[2], res[1]};
-            rc = a.D <= 64 ? launch_pass<T, 64>(g, true, tm, st) : launch_pass<T, 128>(g, true, tm, st);
+            g.dx1 = dv, g.dx2 = dk, g.order = order_k;
+            const CUtensorMap tm[4] = {own[2], own[3], str[0], str[1]};
+            const long long n = ctas_of(a, true, sms);
+            rc = a.D <= 64 ? launch_pass<T, 64>(g, true, tm, n, st) : launch_pass<T, 128>(g, true, tm, n, st);
             if (rc) return rc;
         }
         if (a.Lq) {
-            g.dx1 = nullptr, g.dx2 = dq, g.part = dbias ? part : nullptr;
-            const CUtensorMap tm[6] = {own[0], own[1], str[2], str[3], res[0], res[0]};
-            rc = a.D <= 64 ? launch_pass<T, 64>(g, false, tm, st) : launch_pass<T, 128>(g, false, tm, st);
+            g.dx1 = nullptr, g.dx2 = dq, g.part = dbias ? part : nullptr, g.order = order_q;
+            const CUtensorMap tm[4] = {own[0], own[1], str[2], str[3]};
+            const long long n = ctas_of(a, false, sms);
+            rc = a.D <= 64 ? launch_pass<T, 64>(g, false, tm, n, st) : launch_pass<T, 128>(g, false, tm, n, st);
             if (rc) return rc;
         }
     }
@@ -587,13 +718,26 @@ int run(const AttnArgs& a, int dtype, const void* out, const float* lse, const v
 
 int attn_backward_gave_up(unsigned long long* n) { return (int)cudaMemcpyFromSymbol(n, g_gave_up, sizeof(*n)); }
 
+static int sms_of(int* sms) {
+    static DeviceSetup setup;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return (int)e;
+    return device_setup(setup, dev, [] { return 0; }, sms);
+}
 size_t attn_backward_bytes(const AttnArgs& a, bool dbias) {
-    return (2 * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a) : 0)) * sizeof(float);
+    int sms = 0;
+    if (sms_of(&sms)) return (size_t)-1;
+    return (2 * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a) : 0) + bwd::order_ints(a, true, sms) +
+            bwd::order_ints(a, false, sms)) * sizeof(float);
 }
 int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const float* lse, const void* grad, void* dq,
                         void* dk, void* dv, void* dbias, void* ws, cudaStream_t st) {
-    return dtype == D2P_DTYPE_BF16 ? bwd::run<__nv_bfloat16>(a, dtype, out, lse, grad, dq, dk, dv, dbias, ws, st)
-                                   : bwd::run<__half>(a, dtype, out, lse, grad, dq, dk, dv, dbias, ws, st);
+    int sms = 0;
+    const int rc = sms_of(&sms);
+    if (rc) return rc;
+    return dtype == D2P_DTYPE_BF16 ? bwd::run<__nv_bfloat16>(a, dtype, out, lse, grad, dq, dk, dv, dbias, ws, sms, st)
+                                   : bwd::run<__half>(a, dtype, out, lse, grad, dq, dk, dv, dbias, ws, sms, st);
 }
 
 }  // namespace enc

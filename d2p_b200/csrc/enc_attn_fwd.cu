@@ -23,7 +23,7 @@ namespace enc {
 
 namespace fwd {
 
-constexpr int kThreads = 256;   // a softmax warpgroup; the products' warp, the copies' warp and two that only set up
+constexpr int kThreads = 256;   // a softmax warpgroup; the warps of S, of O, of the copies and of the empty row tiles
 constexpr int kRows = 128;
 constexpr int kColumns = 256;   // TMEM: S 128, O up to 128; two CTAs a SM
 constexpr int kChunk = kRows * 128;
@@ -62,18 +62,6 @@ __device__ __forceinline__ Item item_at(const AttnArgs& a, const int* order, int
     w.tiles = keys > 0 ? (keys + kRows - 1) / kRows : 0;
     return w;
 }
-// the key tiles of a CTA's items, one after the other
-struct Cursor {
-    int i, j, n;   // item, its tile, how many it has
-    __device__ __forceinline__ void seek(const int* tiles, int count) {
-        while (i < count && (n = tiles[i]) == 0) ++i;
-        j = 0;
-    }
-    __device__ __forceinline__ void next(const int* tiles, int count) {
-        if (++j == n) ++i, seek(tiles, count);
-    }
-};
-
 template <class T, int DP, bool BIAS>
 __global__ void __launch_bounds__(kThreads, 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -139,8 +127,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     if (warp >= 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
-    if (warp > 5) {   // items no row of which has a key
-        for (int e = warp - 6; e < count; e += 2) {
+    if (warp == 6) {   // items no row of which has a key
+        for (int e = 0; e < count; ++e) {
             if (tiles[e]) continue;
             const int4 w = entry[e];
             const int rows = min(kRows, a.Lq - w.y), units = a.D / 8;
@@ -179,52 +167,60 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
         }
         __syncwarp();
-    } else if (warp == 4) {   // products
-        // the whole warp runs this, so that the operands' words stay in uniform registers; one lane issues
+    } else {
+        // Products.  Where P has columns of its own one warp forms S and one O, so that neither's waits and issues stand
+        // before the other's; else one does both in turn.  A whole warp runs this, its operands' words in uniform
+        // registers; one lane issues
         const bool lead = elect_one();
-        const uint32_t uS = __shfl_sync(0xffffffffu, tmem, 0), uO = uS + 128, uP = uS + (Sh::kApart ? 192 : 0);
+        const uint32_t uS = uniform(tmem), uO = uS + 128, uP = uS + (Sh::kApart ? 192 : 0);
         constexpr uint32_t idS = mma_desc<T>(128, 128, false), idO = mma_desc<T>(128, DP, true);
-        Cursor cs = {0, 0, 0}, cp;   // the tile whose scores come next, and the one whose product does
-        cs.seek(tiles, count);
-        cp = cs;
-        int ts = 0, qs = 0;          // scores formed, items begun
-        auto scores = [&]() {
-            if (cs.j == 0 && !bar_wait_warp(barQ, qs++ & 1, dead)) return false;
-            const int s = ts % NST;
-            if (!bar_wait_warp(barK + 8 * s, (ts / NST) & 1, dead)) return false;
+        bool ok = true;
+        int t = 0, q = 0;   // tiles and items begun
+        auto scores = [&](int t) {
+            const int s = t % NST;
+            if (!bar_wait_warp(barK + 8 * s, (t / NST) & 1, dead)) return false;
             tc_fence_after();
-            const uint32_t su = __shfl_sync(0xffffffffu, (uint32_t)s, 0);
-            const uint32_t dQ = desc_along(sQ), dK = desc_along(sK + su * Sh::kTile);
+            const uint32_t dQ = desc_along(sQ), dK = desc_along(sK + s * Sh::kTile);
 #pragma unroll
             for (int k = 0; k < DP / 16; ++k) {
                 const uint32_t o = ((k / 4) * kChunk + (k % 4) * 32) / 16;
                 if (lead) mma_ss(uS, dQ + o, dK + o, idS, k != 0);
             }
-            if (lead) tc_commit(barS), tc_commit(barKE + 8 * su);
-            if (cs.j + 1 == cs.n && lead) tc_commit(barQE);
-            ++ts;
-            cs.next(tiles, count);
+            if (lead) tc_commit(barS), tc_commit(barKE + 8 * s);
             return true;
         };
-        bool ok = cs.i >= count || scores();
-        for (int t = 0; ok && cp.i < count; ++t) {
-            const int s = t % NST;
-            const bool last = cp.j + 1 == cp.n;
-            // S read into registers, where P has columns of its own: the next S can begin (an item's first after the last
-            // product of the one before, which waits for nothing else)
-            if (Sh::kApart && !(ok = bar_wait_warp(barR, t & 1, dead) && (last || scores()))) break;
-            if (!(ok = bar_wait_warp(barV + 8 * s, (t / NST) & 1, dead) && bar_wait_warp(barP, t & 1, dead))) break;
-            tc_fence_after();
-            const uint32_t su = __shfl_sync(0xffffffffu, (uint32_t)s, 0), jj = __shfl_sync(0xffffffffu, (uint32_t)cp.j, 0);
-            const uint32_t dV = desc_down(sV + su * Sh::kTile, kChunk);
+        if (Sh::kApart && warp == 4) {
+            for (int e = 0; ok && e < count; ++e) {
+                const int n = (int)uniform(tiles[e]);
+                if (n == 0) continue;
+                if (!(ok = bar_wait_warp(barQ, q++ & 1, dead))) break;
+                for (int j = 0; j < n; ++j, ++t)   // S's columns are free once the one before is in registers
+                    if (!(ok = (t == 0 || bar_wait_warp(barR, (t - 1) & 1, dead)) && scores(t))) break;
+                if (lead) tc_commit(barQE);
+            }
+        } else if (warp == (Sh::kApart ? 7 : 4)) {
+            for (int e = 0; ok && e < count; ++e) {
+                const int n = (int)uniform(tiles[e]);
+                if (n == 0) continue;
+                if (!Sh::kApart && !(ok = bar_wait_warp(barQ, q++ & 1, dead) && scores(t))) break;
+                if (!Sh::kApart && n == 1 && lead) tc_commit(barQE);
+                for (int j = 0; j < n; ++j, ++t) {
+                    const int s = t % NST;
+                    if (!(ok = bar_wait_warp(barV + 8 * s, (t / NST) & 1, dead) && bar_wait_warp(barP, t & 1, dead))) break;
+                    tc_fence_after();
+                    const uint32_t dV = desc_down(sV + s * Sh::kTile, kChunk);
 #pragma unroll
-            for (int k = 0; k < kRows / 16; ++k)
-                if (lead) mma_ts(uO, uP + 8 * k, dV + k * (2048 / 16), idO, (jj | k) != 0);
-            if (lead) tc_commit(barO), tc_commit(barVE + 8 * su);
-            cp.next(tiles, count);
-            if ((last || !Sh::kApart) && cs.i < count) ok = scores();
+                    for (int k = 0; k < kRows / 16; ++k)
+                        if (lead) mma_ts(uO, uP + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
+                    if (lead) tc_commit(barO), tc_commit(barVE + 8 * s);
+                    if (!Sh::kApart && j + 1 < n) {
+                        if (!(ok = scores(t + 1))) break;
+                        if (j + 2 == n && lead) tc_commit(barQE);
+                    }
+                }
+            }
+            if (!ok && lead) atomicAdd(&g_gave_up, 1ull);
         }
-        if (!ok && lead) atomicAdd(&g_gave_up, 1ull);
         __syncwarp();
     }
     } else {

@@ -56,6 +56,9 @@ __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, vol
     return __all_sync(0xffffffffu, bar_wait(bar, parity, dead));
 }
 
+// a value that all lanes of the warp share, by a reduction, whose result lives in a uniform register
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __reduce_or_sync(0xffffffffu, v); }
+
 // true in one lane of a converged warp
 __device__ __forceinline__ bool elect_one() {
     uint32_t p;
