@@ -76,7 +76,7 @@ size_t smem_bytes(bool dkv, int reach) {
 
 struct Args {
     AttnArgs a;
-    const float* lse;      // [B, H, Lp] padded copies: +inf and 0 in dead rows
+    const float* lse;      // [B, H, Lp] padded copies, negated: -inf and 0 in dead rows
     const float* delta;
     int Lp;
     void* dx1;             // keys pass: dv; query pass: unused
@@ -377,6 +377,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                         // four columns' entries at lp +- y: the keys pass meets them in falling order
                         const float* const lp = lut_row(lut, reach, d0 + reach + kPad - (DKV ? 3 : 0));
                         const float flat = BIAS && !NEAR ? (lo >= reach ? lut[lut_entries(reach) - 1] : lut[0]) : 0.f;
+                        // (a value that swallows the scores near the diagonal has to do so here, where it is added last)
+                        const float mul = fabsf(flat) < 2147483648.f ? c : 1e-30f;
                         uint32_t sv[32], dv[32];
                         tmem_ld32(tS + col0, sv);
                         tmem_ld32(tD + col0, dv);
@@ -384,25 +386,31 @@ __global__ void __launch_bounds__(kThreads, 1)
                         tmem_tie32(sv), tmem_tie32(dv);
 #pragma unroll
                         for (int y = 0; y < 32; y += 4) {
-                            float4 L, E;
+                            float4 L = make_float4(rl, rl, rl, rl), E = make_float4(rd, rd, rd, rd);   // -lse and -delta
                             if (DKV) {
                                 L = *reinterpret_cast<const float4*>(st + y);
                                 E = *reinterpret_cast<const float4*>(st + kStep + y);
-                            } else {
-                                L = make_float4(rl, rl, rl, rl), E = make_float4(rd, rd, rd, rd);
                             }
-                            const float Lv[4] = {L.x, L.y, L.z, L.w}, Ev[4] = {E.x, E.y, E.z, E.w};
-                            float4 e = make_float4(flat, flat, flat, flat);
-                            if (BIAS && NEAR) e = *reinterpret_cast<const float4*>(DKV ? lp - y : lp + y);
-                            const float Bv[4] = {DKV ? e.w : e.x, DKV ? e.z : e.y, DKV ? e.y : e.z, DKV ? e.x : e.w};
                             float pv[4], gv[4];
+                            Two t0(__uint_as_float(sv[y]), __uint_as_float(sv[y + 1])), t1(__uint_as_float(sv[y + 2]), __uint_as_float(sv[y + 3]));
+                            const Two L0(L.x, L.y), L1(L.z, L.w);
+                            if (BIAS && NEAR) {
+                                const float4 e = *reinterpret_cast<const float4*>(DKV ? lp - y : lp + y);
+                                t0 = add2(fma2(t0, Two(c, c), DKV ? Two(e.w, e.z) : Two(e.x, e.y)), L0);
+                                t1 = add2(fma2(t1, Two(c, c), DKV ? Two(e.y, e.x) : Two(e.z, e.w)), L1);
+                            } else {
+                                const Two m(mul, mul), f(flat, flat);
+                                t0 = fma2(t0, m, BIAS ? add2(f, L0) : L0), t1 = fma2(t1, m, BIAS ? add2(f, L1) : L1);
+                            }
+                            t0.get(pv, pv + 1), t1.get(pv + 2, pv + 3);
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) pv[z] = ex2(pv[z]);
+                            const Two d0(__uint_as_float(dv[y]), __uint_as_float(dv[y + 1])), d1(__uint_as_float(dv[y + 2]), __uint_as_float(dv[y + 3]));
+                            mul2(Two(pv[0], pv[1]), add2(d0, Two(E.x, E.y))).get(gv, gv + 1);
+                            mul2(Two(pv[2], pv[3]), add2(d1, Two(E.z, E.w))).get(gv + 2, gv + 3);
 #pragma unroll
                             for (int z = 0; z < 4; ++z) {
                                 const int col = y + z;
-                                const float raw_s = __uint_as_float(sv[col]);
-                                const float t = BIAS ? fmaf(raw_s, c, Bv[z]) - Lv[z] : fmaf(raw_s, c, -Lv[z]);
-                                pv[z] = ex2(t);
-                                gv[z] = pv[z] * (__uint_as_float(dv[col]) - Ev[z]);
                                 if (EDGE) {
                                     const bool in = col >= c0 && col < c1;
                                     pv[z] = in ? pv[z] : 0.f;
@@ -538,29 +546,42 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kWork / 32) tmem_free(tmem, kColumns);
 }
 
-// delta = rowsum(dO O) and lse in rows padded to whole tiles: +inf and 0 where no key is met.  16 lanes a row
-template <class T>
+// -delta = -rowsum(dO O) and -lse in rows padded to whole tiles: 0 and -inf where no key is met.  A block takes 32
+// positions of up to 8 heads: rows are read as they lie, heads of a position together, and the sums leave by head, 32
+// positions together.  LANES threads a row
+constexpr int kStatRows = 32, kStatHeads = 8;
+template <class T, int LANES>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ AttnArgs a, const T* __restrict__ out,
                                                          const float* __restrict__ lse, const T* __restrict__ grad, int Lp,
                                                          float* __restrict__ lp, float* __restrict__ dp) {
-    const int lane = threadIdx.x & 15, h = blockIdx.y, b = blockIdx.z, i = blockIdx.x * 16 + (threadIdx.x >> 4);
+    __shared__ float sum[kStatHeads][kStatRows + 1];
+    const int lane = threadIdx.x % LANES, i0 = blockIdx.x * kStatRows, h0 = blockIdx.y * kStatHeads, b = blockIdx.z;
+    const int heads = min(kStatHeads, a.H - h0);
     int lq, lk;
     problem_lengths(a, b, &lq, &lk);
-    float d = 0.f;
-    if (i < lq && 8 * lane < a.D) {
-        const size_t at = (((size_t)b * a.Lq + i) * a.H + h) * a.D + 8 * lane;
-        float o[8], g[8];
-        load8<T>(out + at, o);
-        load8<T>(grad + at, g);
+    constexpr int kStride = 256 / LANES;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) d = fmaf(o[x], g[x], d);
+    for (int k = 0; k < kStatRows * kStatHeads / kStride; ++k) {
+        const int row = k * kStride + threadIdx.x / LANES, i = i0 + row / kStatHeads, h = row % kStatHeads;
+        float d = 0.f;
+        if (i < lq && h < heads && 8 * lane < a.D) {
+            const size_t at = (((size_t)b * a.Lq + i) * a.H + h0 + h) * a.D + 8 * lane;
+            float o[8], g[8];
+            load8<T>(out + at, o);
+            load8<T>(grad + at, g);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) d = fmaf(o[x], g[x], d);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        if (lane == 0) sum[h][row / kStatHeads] = d;
     }
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-    if (lane == 0) {
-        const size_t at = ((size_t)b * a.H + h) * Lp + i;
-        dp[at] = d;
-        lp[at] = i < lq ? lse[((size_t)b * a.H + h) * a.Lq + i] : INFINITY;
+    __syncthreads();
+    const int h = threadIdx.x / kStatRows, i = i0 + threadIdx.x % kStatRows;
+    if (h < heads) {
+        const size_t at = ((size_t)b * a.H + h0 + h) * Lp + i;
+        dp[at] = -sum[h][threadIdx.x % kStatRows];
+        lp[at] = i < lq ? -lse[((size_t)b * a.H + h0 + h) * a.Lq + i] : -INFINITY;
     }
 }
 
@@ -664,7 +685,9 @@ int run(const AttnArgs& a, int dtype, const void* out, const float* lse, const v
         if ((rc = (int)cudaGetLastError())) return rc;
     }
     if (a.B && a.Lq) {
-        attn_stats_kernel<T><<<dim3(Lp / 16, a.H, a.B), 256, 0, st>>>(a, (const T*)out, lse, (const T*)grad, Lp, lp, dp);
+        const dim3 grid(Lp / kStatRows, (a.H + kStatHeads - 1) / kStatHeads, a.B);
+        if (a.D <= 64) attn_stats_kernel<T, 8><<<grid, 256, 0, st>>>(a, (const T*)out, lse, (const T*)grad, Lp, lp, dp);
+        else attn_stats_kernel<T, 16><<<grid, 256, 0, st>>>(a, (const T*)out, lse, (const T*)grad, Lp, lp, dp);
         if ((rc = (int)cudaGetLastError())) return rc;
     }
     if (a.B && (a.Lq || a.Lk)) {

@@ -278,8 +278,8 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                             for (int y = 32 * x; y < 32 * x + 32; y += 4) {
                                 const float4 e = *reinterpret_cast<const float4*>(lp + y);
-                                t[y] = fmaf(t[y], c, e.x), t[y + 1] = fmaf(t[y + 1], c, e.y);
-                                t[y + 2] = fmaf(t[y + 2], c, e.z), t[y + 3] = fmaf(t[y + 3], c, e.w);
+                                fma2(Two(t[y], t[y + 1]), Two(c, c), Two(e.x, e.y)).get(t + y, t + y + 1);
+                                fma2(Two(t[y + 2], t[y + 3]), Two(c, c), Two(e.z, e.w)).get(t + y + 2, t + y + 3);
                             }
                             mul[x] = 1.f, add[x] = 0.f;
                         }
@@ -327,21 +327,26 @@ __global__ void __launch_bounds__(kThreads, 2)
                     tmem_wait_st();
                 }
                 const float ref = (m == -INFINITY ? 0.f : m) - Softmax<T>::kShift;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                Two sum[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
 #pragma unroll
                 for (int x = 0; x < 128; x += 32) {
                     uint32_t p[16];
-                    const float u = mul[x / 32], v0 = add[x / 32] - ref;
+                    const Two u(mul[x / 32], mul[x / 32]), v0(add[x / 32] - ref, add[x / 32] - ref);
 #pragma unroll
                     for (int y = 0; y < 32; y += 2) {
-                        const float e0 = ex2(fmaf(t[x + y], u, v0)), e1 = ex2(fmaf(t[x + y + 1], u, v0));
-                        sum[y & 2] += e0;
-                        sum[(y & 2) + 1] += e1;
+                        float e0, e1;
+                        fma2(Two(t[x + y], t[x + y + 1]), u, v0).get(&e0, &e1);
+                        e0 = ex2(e0), e1 = ex2(e1);
+                        sum[(y / 2) & 1] = add2(sum[(y / 2) & 1], Two(e0, e1));
                         p[y / 2] = pack2<T>(e0, e1);
                     }
                     tmem_st16(tP + trow + x / 2, p);
                 }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                {
+                    float s0, s1;
+                    add2(sum[0], sum[1]).get(&s0, &s1);
+                    l += s0 + s1;
+                }
                 const int live = lk - k0;
                 if (live < kRows) {   // the keys' last tile: rows of V past them to zero
                     if (!(ok = bar_wait_warp(barV + 8 * (tt % NST), (tt / NST) & 1, dead))) break;
