@@ -81,7 +81,7 @@ struct Args {
     int Lp;
     void* dx1;             // keys pass: dv; query pass: unused
     void* dx2;             // dk or dq
-    float* part;           // query pass: [H][buckets][B][row tiles] sums of dS, or null
+    float* part;           // query pass: [H][buckets][CTAs of a head] sums of dS, or null
     const int* order;      // items in order of their work, or null
 };
 
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int hx = blockIdx.x, group = a.H / a.Hkv;
     const int Lx = DKV ? a.Lk : a.Lq, heads = DKV ? a.Hkv : a.H, row_tiles = (Lx + kOwn - 1) / kOwn, items = a.B * row_tiles;
-    const int count = (items - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;   // of this CTA: blockIdx.y, + gridDim.y, ..
+    const int count = item_count(items, blockIdx.y, gridDim.y);   // of this CTA
 
     extern __shared__ uint8_t raw[];
     const uint32_t r0 = smem_addr(raw), base = (r0 + 1023u) & ~1023u;
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
             *dead = 0;
-            const Item w = item_at<DKV>(a, g.order, blockIdx.y);
+            const Item w = item_at<DKV>(a, g.order, item_index(0, blockIdx.y, gridDim.y));
             if (w.per) {
                 own(0, w.b, w.x0);
                 stream(0, w.b, w.y0, DKV ? hx * group : hx / group);
@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_alloc(smem_addr(slot), kColumns);
     } else if (warp < kWork / 32) {
         for (int e = tid; e < count; e += kWork) {
-            const Item w = item_at<DKV>(a, g.order, blockIdx.y + e * gridDim.y);
+            const Item w = item_at<DKV>(a, g.order, item_index(e, blockIdx.y, gridDim.y));
             entry[e] = make_int4(w.b, w.x0, w.lq, w.lk);
             span[e] = make_int2(w.y0, w.per);
         }
@@ -315,13 +315,63 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool ok = true;
         float* const dw = diag + warp * 72;
         int t0 = 0, done = 0;   // tiles and items (with work) so far
+        float far0 = 0.f, far1 = 0.f, bsum[kBuckets / 32];   // dS by position, over all the CTA's items
+#pragma unroll
+        for (int i = 0; i < kBuckets / 32; ++i) bsum[i] = 0.f;
+
+        // An item's results are stored after this warp's first tile of the next one, whose work covers the wait for the
+        // last products.  keys pass: half of dV's or dK's columns a warpgroup; query pass: a quarter of dQ's.  A row a
+        // thread, whole 32-byte sectors
+        int kept_b = -1, kept_x = 0, kept_l = 0;   // problem, this thread's row, rows there are
+        auto store = [&]() {
+            ok = ok && bar_wait_warp(barF, (done - 1) & 1, dead);
+            tc_fence_after();
+            const bool row = kept_x < kept_l, first = DKV && pair == 0;
+            const float w = first ? 1.f : a.scale;
+            const int f0 = DKV ? half * (DP / 2) : (warp >> 2) * (DP / 4);
+            constexpr int kCols = DKV ? DP / 2 : DP / 4;
+            const uint32_t acc = (first ? tA1 : tA2) + trow;
+            uint32_t o[kCols];
+#pragma unroll
+            for (int f = 0; f < kCols; f += 16) tmem_ld16(acc + f0 + f, o + f);
+            tmem_wait_ld();
+#pragma unroll
+            for (int f = 0; f < kCols; f += 16) tmem_tie16(o + f);
+            tc_fence_before();
+            bar_arrive_warp(barA);   // the next item's products may overwrite them
+            if (kept_x < Lx) {
+                T* const rp = (T*)(first ? g.dx1 : g.dx2) + (((size_t)kept_b * Lx + kept_x) * heads + hx) * a.D + f0;
+#pragma unroll
+                for (int y = 0; y < kCols; y += 8) {
+                    uint32_t p[4];
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const float u0 = __uint_as_float(o[y + 2 * z]) * w, u1 = __uint_as_float(o[y + 2 * z + 1]) * w;
+                        p[z] = !row ? 0u : ok ? pack2<T>(u0, u1) : pack2<T>(NAN, NAN);
+                    }
+                    if (f0 + y < a.D) *reinterpret_cast<uint4*>(rp + y) = make_uint4(p[0], p[1], p[2], p[3]);
+                }
+            }
+            kept_b = -1;
+        };
+        // the row statistics of the next item, asked for one ahead (query pass)
+        float nl = 0.f, nd = 0.f;
+        auto ask = [&](int e) {
+            if (!DKV && e < count) {
+                const int4 en = entry[e];
+                const size_t at = ((size_t)en.x * a.H + hx) * g.Lp + en.y + r;   // Lp covers the tile
+                nl = g.lse[at], nd = g.delta[at];
+            }
+        };
+        ask(0);
         for (int e = 0; e < count; ++e) {
             const int4 en = entry[e];
+            const float rl = nl, rd = nd;
+            ask(e + 1);
             // (from one lane for all, so that the branches on them are known to be the warp's)
             const int x0 = __shfl_sync(0xffffffffu, en.y, 0), lq = __shfl_sync(0xffffffffu, en.z, 0), lk = __shfl_sync(0xffffffffu, en.w, 0);
             const int y0 = __shfl_sync(0xffffffffu, span[e].x, 0), per = __shfl_sync(0xffffffffu, span[e].y, 0);
             const int b = en.x, off = a.causal ? lk - lq : 0, lx = DKV ? lk : lq, ly = DKV ? lq : lk, x = x0 + r;
-            float* const part = sums ? g.part + ((size_t)hx * n_buckets(a.edges) * a.B + b) * row_tiles + x0 / kOwn : nullptr;
             if (per == 0) {   // nothing meets these rows
                 const int rows = min(kOwn, Lx - x0), units = a.D / 8;
                 for (int v = tid; v < rows * units; v += kWork) {
@@ -329,18 +379,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     *reinterpret_cast<uint4*>((T*)g.dx2 + at) = make_uint4(0, 0, 0, 0);
                     if (DKV) *reinterpret_cast<uint4*>((T*)g.dx1 + at) = make_uint4(0, 0, 0, 0);
                 }
-                if (sums)
-                    for (int t = tid; t < n_buckets(a.edges); t += kWork) part[(size_t)t * a.B * row_tiles] = 0.f;
                 continue;
             }
-            float rl = 0.f, rd = 0.f;
-            if (!DKV) {
-                const size_t at = ((size_t)b * a.H + hx) * g.Lp + x;   // Lp covers the tile
-                rl = g.lse[at], rd = g.delta[at];
-            }
-            float far0 = 0.f, far1 = 0.f, bsum[kBuckets / 32];
-#pragma unroll
-            for (int i = 0; i < kBuckets / 32; ++i) bsum[i] = 0.f;
             for (int head = 0; head < (DKV ? group : 1); ++head) {
                 if (BIAS && DKV && group > 1) {   // keys pass: the bias of the group's next head, once every warp is past the one before
                     asm volatile("bar.sync 1, 512;" ::: "memory");
@@ -452,6 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tmem_wait_st();
                     tc_fence_before();
                     bar_arrive_warp(barP + 8 * buf);
+                    if (kept_b >= 0) store();   // the item before
                     if (sums) {
                         if (near) {
                             dw[62 - lane] = run;   // the diagonals still under way; lane 31's is in place
@@ -487,58 +528,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            if (sums) {   // the tile's sums, warp by warp in order
-                const int nb = n_buckets(a.edges);
-#pragma unroll
-                for (int o = 16; o > 0; o >>= 1) {
-                    far0 += __shfl_xor_sync(0xffffffffu, far0, o);
-                    far1 += __shfl_xor_sync(0xffffffffu, far1, o);
-                }
-#pragma unroll
-                for (int i = 0; i < kBuckets / 32; ++i) {
-                    const int t = lane + 32 * i;
-                    if (t < nb) red[warp * kBuckets + t] = bsum[i] + (t == a.edges.n ? far0 : 0.f) + (a.edges.two && t == nb - 1 ? far1 : 0.f);
-                }
-                asm volatile("bar.sync 1, 512;" ::: "memory");
-                for (int t = tid; t < nb; t += kWork) {
-                    float v = 0.f;
-#pragma unroll
-                    for (int k = 0; k < kWork / 32; ++k) v += red[k * kBuckets + t];
-                    part[(size_t)t * a.B * row_tiles] = v;
-                }
-                asm volatile("bar.sync 1, 512;" ::: "memory");   // read before the next tile's
-            }
-            ok = ok && bar_wait_warp(barF, done & 1, dead);
-            tc_fence_after();
-            // keys pass: half of dV's or dK's columns a warpgroup; query pass: a quarter of dQ's.  A row a thread, whole
-            // 32-byte sectors
-            const bool row = x < lx, first = DKV && pair == 0;
-            const float w = first ? 1.f : a.scale;
-            const int f0 = DKV ? half * (DP / 2) : (warp >> 2) * (DP / 4);
-            constexpr int kCols = DKV ? DP / 2 : DP / 4;
-            const uint32_t acc = (first ? tA1 : tA2) + trow;
-            uint32_t o[kCols];
-#pragma unroll
-            for (int f = 0; f < kCols; f += 16) tmem_ld16(acc + f0 + f, o + f);
-            tmem_wait_ld();
-#pragma unroll
-            for (int f = 0; f < kCols; f += 16) tmem_tie16(o + f);
-            tc_fence_before();
-            bar_arrive_warp(barA);   // the next item's products may overwrite them
-            if (x < Lx) {
-                T* const rp = (T*)(first ? g.dx1 : g.dx2) + (((size_t)b * Lx + x) * heads + hx) * a.D + f0;
-#pragma unroll
-                for (int y = 0; y < kCols; y += 8) {
-                    uint32_t p[4];
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) {
-                        const float u0 = __uint_as_float(o[y + 2 * z]) * w, u1 = __uint_as_float(o[y + 2 * z + 1]) * w;
-                        p[z] = !row ? 0u : ok ? pack2<T>(u0, u1) : pack2<T>(NAN, NAN);
-                    }
-                    if (f0 + y < a.D) *reinterpret_cast<uint4*>(rp + y) = make_uint4(p[0], p[1], p[2], p[3]);
-                }
-            }
+            if (kept_b >= 0) store();   // (this warp had no tile of the item)
+            kept_b = b, kept_x = x, kept_l = lx;
             t0 += per * (DKV ? group : 1), ++done;
+        }
+        if (kept_b >= 0) store();
+        if (sums) {   // the CTA's sums, warp by warp in order
+            const int nb = n_buckets(a.edges);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) {
+                far0 += __shfl_xor_sync(0xffffffffu, far0, o);
+                far1 += __shfl_xor_sync(0xffffffffu, far1, o);
+            }
+#pragma unroll
+            for (int i = 0; i < kBuckets / 32; ++i) {
+                const int t = lane + 32 * i;
+                if (t < nb) red[warp * kBuckets + t] = bsum[i] + (t == a.edges.n ? far0 : 0.f) + (a.edges.two && t == nb - 1 ? far1 : 0.f);
+            }
+            asm volatile("bar.sync 1, 512;" ::: "memory");
+            for (int t = tid; t < nb; t += kWork) {
+                float v = 0.f;
+#pragma unroll
+                for (int k = 0; k < kWork / 32; ++k) v += red[k * kBuckets + t];
+                g.part[((size_t)hx * nb + t) * gridDim.y + blockIdx.y] = v;
+            }
         }
     }
     tc_fence_before();
@@ -546,10 +559,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kWork / 32) tmem_free(tmem, kColumns);
 }
 
-// -delta = -rowsum(dO O) and -lse in rows padded to whole tiles: 0 and -inf where no key is met.  A block takes 32
-// positions of up to 8 heads: rows are read as they lie, heads of a position together, and the sums leave by head, 32
+// -delta = -rowsum(dO O) and -lse in rows padded to whole tiles: 0 and -inf where no key is met.  A block takes 16
+// positions of up to 8 heads: rows are read as they lie, heads of a position together, and the sums leave by head, 16
 // positions together.  LANES threads a row
-constexpr int kStatRows = 32, kStatHeads = 8;
+constexpr int kStatRows = 16, kStatHeads = 8;
 template <class T, int LANES>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ AttnArgs a, const T* __restrict__ out,
                                                          const float* __restrict__ lse, const T* __restrict__ grad, int Lp,
@@ -578,7 +591,7 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
     }
     __syncthreads();
     const int h = threadIdx.x / kStatRows, i = i0 + threadIdx.x % kStatRows;
-    if (h < heads) {
+    if (h < heads && h < kStatHeads) {
         const size_t at = ((size_t)b * a.H + h0 + h) * Lp + i;
         dp[at] = -sum[h][threadIdx.x % kStatRows];
         lp[at] = i < lq ? -lse[((size_t)b * a.H + h0 + h) * a.Lq + i] : -INFINITY;
@@ -598,46 +611,24 @@ __global__ void __launch_bounds__(128) attn_dbias_kernel(const float* part, int 
     if (lane == 0) dbias[(size_t)t * H + h] = from_f<T>(s);
 }
 
-// items by falling number of streamed tiles (any order among equals)
-constexpr int kBins = 1024, kMaxOrder = 1 << 16;
-template <bool DKV>
-__device__ void order_items(const AttnArgs& a, int* order) {
-    __shared__ int first[kBins], warp_sum[32];
-    const int items = a.B * (((DKV ? a.Lk : a.Lq) + kOwn - 1) / kOwn), t = threadIdx.x;
-    auto bin = [&](int i) { return kBins - 1 - min(item_at<DKV>(a, nullptr, i).per, kBins - 1); };
-    first[t] = 0;
-    __syncthreads();
-    for (int i = t; i < items; i += 1024) atomicAdd(&first[bin(i)], 1);
-    __syncthreads();
-    const int n = first[t];
-    int sum = n;   // inclusive scan over the bins
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if ((t & 31) >= o) sum += v;
-    }
-    if ((t & 31) == 31) warp_sum[t >> 5] = sum;
-    __syncthreads();
-    for (int w = 0; w < (t >> 5); ++w) sum += warp_sum[w];
-    first[t] = sum - n;
-    __syncthreads();
-    for (int i = t; i < items; i += 1024) order[atomicAdd(&first[bin(i)], 1)] = i;
-}
 __global__ void __launch_bounds__(1024) attn_order_kernel(const __grid_constant__ AttnArgs a, int* keys, int* queries) {
-    if (blockIdx.x == 0 && keys) order_items<true>(a, keys);
-    if (blockIdx.x == 1 && queries) order_items<false>(a, queries);
+    if (blockIdx.x == 0) {
+        if (keys) order_items(a.B * ((a.Lk + kOwn - 1) / kOwn), [&](int i) { return min(item_at<true>(a, nullptr, i).per, kBins - 1); }, keys);
+    } else if (queries) {
+        order_items(a.B * ((a.Lq + kOwn - 1) / kOwn), [&](int i) { return min(item_at<false>(a, nullptr, i).per, kBins - 1); }, queries);
+    }
 }
 
 int tiles_of(int L) { return (L + kOwn - 1) / kOwn; }
 size_t stats_floats(const AttnArgs& a) { return (size_t)a.B * a.H * tiles_of(a.Lq) * kOwn; }
-size_t part_floats(const AttnArgs& a) {
-    return ((size_t)((a.edges.n + 1) << a.edges.two) * a.H * a.B * tiles_of(a.Lq) + 3) & ~(size_t)3;
-}
 // CTAs of a head: one for each owned tile, or, where each SM would see four or more of them, its share of the SMs
 long long ctas_of(const AttnArgs& a, bool dkv, int sms) {
     const long long items = (long long)a.B * tiles_of(dkv ? a.Lk : a.Lq), heads = dkv ? a.Hkv : a.H;
     if (items * heads < 4LL * sms) return items;
     return std::max<long long>(sms > heads ? sms / heads : 1, (items + kMaxItems - 1) / kMaxItems);
+}
+size_t part_floats(const AttnArgs& a, int sms) {
+    return ((size_t)((a.edges.n + 1) << a.edges.two) * a.H * ctas_of(a, false, sms) + 3) & ~(size_t)3;
 }
 // ints of its items' order, where lengths differ and CTAs take several
 size_t order_ints(const AttnArgs& a, bool dkv, int sms) {
@@ -675,7 +666,7 @@ int run(const AttnArgs& a, int dtype, const void* out, const float* lse, const v
     float* const lp = (float*)ws;
     float* const dp = lp + stats_floats(a);
     float* const part = dp + stats_floats(a);
-    int* const order = (int*)(part + (dbias ? part_floats(a) : 0));
+    int* const order = (int*)(part + (dbias ? part_floats(a, sms) : 0));
     const size_t ok = order_ints(a, true, sms), oq = order_ints(a, false, sms);
     int* const order_k = ok ? order : nullptr;
     int* const order_q = oq ? order + ok : nullptr;
@@ -727,7 +718,7 @@ int run(const AttnArgs& a, int dtype, const void* out, const float* lse, const v
         }
     }
     if (dbias) {
-        const int nb = (a.edges.n + 1) << a.edges.two, n = a.B * tiles_of(a.Lq);
+        const int nb = (a.edges.n + 1) << a.edges.two, n = a.B * tiles_of(a.Lq) ? (int)ctas_of(a, false, sms) : 0;
         if (a.bias_f32)
             attn_dbias_kernel<float><<<(nb * a.H + 3) / 4, 128, 0, st>>>(part, nb, a.H, n, (float*)dbias);
         else
@@ -751,7 +742,7 @@ static int sms_of(int* sms) {
 size_t attn_backward_bytes(const AttnArgs& a, bool dbias) {
     int sms = 0;
     if (sms_of(&sms)) return (size_t)-1;
-    return (2 * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a) : 0) + bwd::order_ints(a, true, sms) +
+    return (2 * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a, sms) : 0) + bwd::order_ints(a, true, sms) +
             bwd::order_ints(a, false, sms)) * sizeof(float);
 }
 int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const float* lse, const void* grad, void* dq,

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     constexpr int NST = Sh::kStages;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.x, row_tiles = (a.Lq + kRows - 1) / kRows, items = a.B * row_tiles;
-    const int count = (items - (int)blockIdx.y + (int)gridDim.y - 1) / (int)gridDim.y;   // of this CTA: blockIdx.y, + gridDim.y, ..
+    const int count = item_count(items, blockIdx.y, gridDim.y);   // of this CTA
 
     extern __shared__ uint8_t raw[];
     const uint32_t r0 = smem_addr(raw), base = (r0 + 1023u) & ~1023u;
@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
             *dead = 0;
-            const Item w = item_at(a, order, blockIdx.y, row_tiles);   // the first item's Q and first tile before the CTA meets
+            const Item w = item_at(a, order, item_index(0, blockIdx.y, gridDim.y), row_tiles);   // the first item's Q and first tile before the CTA meets
             if (w.tiles) {
                 load(sQ, &tmQ, w.q0, h, w.b, barQ);
                 load(sK, &tmK, 0, kh, w.b, barK);
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         tmem_alloc(smem_addr(slot), kColumns);
     } else {
         for (int e = warp < 4 ? tid : tid - 64; e < count; e += 192) {
-            const Item w = item_at(a, order, blockIdx.y + e * gridDim.y, row_tiles);
+            const Item w = item_at(a, order, item_index(e, blockIdx.y, gridDim.y), row_tiles);
             entry[e] = make_int4(w.b, w.q0, w.lq, w.lk);
             tiles[e] = w.tiles;
         }
@@ -397,28 +397,9 @@ __global__ void __launch_bounds__(kThreads, 2)
     if (warp == 4) tmem_free(tmem, kColumns);
 }
 
-// items by falling number of key tiles (any order among equals), for batches of uneven lengths
-constexpr int kBins = 1024, kMaxOrder = 1 << 16;
 __global__ void __launch_bounds__(1024) attn_order_kernel(const __grid_constant__ AttnArgs a, int* __restrict__ order) {
-    __shared__ int first[kBins], warp_sum[32];
-    const int row_tiles = (a.Lq + kRows - 1) / kRows, items = a.B * row_tiles, t = threadIdx.x;
-    first[t] = 0;
-    __syncthreads();
-    for (int i = t; i < items; i += 1024) atomicAdd(&first[kBins - 1 - min(item_at(a, nullptr, i, row_tiles).tiles, kBins - 1)], 1);
-    __syncthreads();
-    const int n = first[t];
-    int sum = n;   // inclusive scan over the bins
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, sum, o);
-        if ((t & 31) >= o) sum += v;
-    }
-    if ((t & 31) == 31) warp_sum[t >> 5] = sum;
-    __syncthreads();
-    for (int w = 0; w < (t >> 5); ++w) sum += warp_sum[w];
-    first[t] = sum - n;
-    __syncthreads();
-    for (int i = t; i < items; i += 1024) order[atomicAdd(&first[kBins - 1 - min(item_at(a, nullptr, i, row_tiles).tiles, kBins - 1)], 1)] = i;
+    const int row_tiles = (a.Lq + kRows - 1) / kRows;
+    order_items(a.B * row_tiles, [&](int i) { return min(item_at(a, nullptr, i, row_tiles).tiles, kBins - 1); }, order);
 }
 
 // a CTA for each item, or, where each place on the device (two CTAs an SM) would see four or more of them, a CTA for

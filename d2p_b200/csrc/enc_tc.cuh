@@ -243,6 +243,54 @@ __device__ __forceinline__ void fill_lut(float* lut, const AttnArgs& a, int h, i
     }
 }
 
+// Items in order of falling work, for CTAs that take several each: a stable
+// counting sort by one CTA of 1024 threads, so that which CTA takes an item never
+// changes from run to run.  bin(i): the item's work, at most kBins - 1
+constexpr int kBins = 1024, kMaxOrder = 1 << 14;
+template <class Bin>
+__device__ __forceinline__ void order_items(int items, Bin bin, int* order) {
+    __shared__ int first[kBins], warp_sum[32];
+    const int t = threadIdx.x, lane = t & 31;
+    first[t] = 0;
+    __syncthreads();
+    for (int i = t; i < items; i += 1024) atomicAdd(&first[kBins - 1 - bin(i)], 1);
+    __syncthreads();
+    const int n = first[t];
+    int sum = n;   // inclusive scan over the bins
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 31) warp_sum[t >> 5] = sum;
+    __syncthreads();
+    for (int w = 0; w < (t >> 5); ++w) sum += warp_sum[w];
+    first[t] = sum - n;
+    __syncthreads();
+    for (int base = 0; base < items; base += 1024) {
+        const int i = base + t, k = i < items ? kBins - 1 - bin(i) : -1;
+        const uint32_t same = __match_any_sync(0xffffffffu, k);
+        const int rank = __popc(same & ((1u << lane) - 1));
+        for (int w = 0; w < 32; ++w) {   // warps in turn
+            if (t >> 5 == w) {
+                const int at = k >= 0 ? first[k] : 0;
+                __syncwarp();
+                if (k >= 0) {
+                    order[at + rank] = i;
+                    if (rank == 0) first[k] = at + __popc(same);
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+// the e-th item of CTA y of n: rows of n items, every other one backwards, so that shares of falling work come out even
+__device__ __forceinline__ int item_index(int e, int y, int n) { return e * n + (e & 1 ? n - 1 - y : y); }
+__device__ __forceinline__ int item_count(int items, int y, int n) {
+    const int rows = items / n;
+    return rows + (item_index(rows, y, n) < items);
+}
+
 // [B, L, heads, D] rows with element strides s (batch, position, head) as a 4-D
 // tensor (D, position, head, batch) in boxes of 64 elements x rows
 bool rows_map(CUtensorMap* tm, int dtype, const void* base, int B, int L, int heads, int D, const long long* s, int rows);
