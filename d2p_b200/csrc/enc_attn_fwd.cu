@@ -237,14 +237,49 @@ __global__ void __launch_bounds__(kThreads, 2)
             before = lut[0], after = lut[lut_entries(reach) - 1];
             mul_before = fabsf(before) < 2147483648.f ? c : 1e-30f, mul_after = fabsf(after) < 2147483648.f ? c : 1e-30f;
         }
+        // An item's rows are finished behind the next one's first maximum, which covers the wait for its last product: O /
+        // l, a row a thread, whole 32-byte sectors
+        int kept = -1;
+        float kept_m = 0.f, kept_l = 0.f;
+        auto finish = [&]() {
+            ok = ok && bar_wait_warp(barO, (tt - 1) & 1, dead);
+            tc_fence_after();
+            const int4 w = entry[kept];   // b, q0, lq, lk
+            const int i = w.y + tid;
+            const bool some = i < w.z && (kept_l > 0.f || kept_l != kept_l);
+            const float s = !ok ? NAN : (some ? 1.f / kept_l : 0.f);
+            T* const orow = out + (((size_t)w.x * a.Lq + i) * a.H + h) * a.D;
+#pragma unroll 1
+            for (int x = 0; x < DP; x += 16) {
+                uint32_t o[16];
+                tmem_ld16(tO + trow + x, o);
+                tmem_wait_ld();
+                tmem_tie16(o);
+                if (i < a.Lq) {
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        uint32_t p[4];
+#pragma unroll
+                        for (int z = 0; z < 4; ++z) {
+                            const float u0 = __uint_as_float(o[8 * y + 2 * z]), u1 = __uint_as_float(o[8 * y + 2 * z + 1]);
+                            p[z] = s == 0.f ? 0u : pack2<T>(ok ? u0 * s : s, ok ? u1 * s : s);   // a dead row is zero whatever it held
+                        }
+                        if (x + 8 * y < a.D) *reinterpret_cast<uint4*>(orow + x + 8 * y) = make_uint4(p[0], p[1], p[2], p[3]);
+                    }
+                }
+            }
+            if (lse && i < a.Lq)
+                lse[((size_t)w.x * a.H + h) * a.Lq + i] = some ? kept_m - Softmax<T>::kShift + log2f(kept_l) : INFINITY;
+            tc_fence_before();   // the next item's first product overwrites O after this warp's first P of it
+            kept = -1;
+        };
         for (int e = 0; e < count; ++e) {
             const int4 en = entry[e];
             // (from one lane for all, so that the branches on them are known to be the warp's)
             const int lku = __shfl_sync(0xffffffffu, en.w, 0), offu = __shfl_sync(0xffffffffu, a.causal ? en.w - en.z : 0, 0);
             const Item w = {en.x, __shfl_sync(0xffffffffu, en.y, 0), en.z, lku, offu, __shfl_sync(0xffffffffu, tiles[e], 0)};
             if (w.tiles == 0) continue;
-            const int i = w.q0 + tid, pos = i + w.off, lk = w.lk;
-            T* const orow = out + (((size_t)w.b * a.Lq + i) * a.H + h) * a.D;
+            const int pos = w.q0 + tid + w.off, lk = w.lk;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < w.tiles && ok; ++j, ++tt) {
                 const int k0 = j * kRows;
@@ -308,6 +343,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     l *= f;
                 }
                 const bool rescale = __any_sync(0xffffffffu, raise) && j > 0;
+                if (kept >= 0) finish();   // (the item before)
                 // the product before reads P's columns and adds to O
                 if (j > 0 && (Sh::kApart || rescale)) {
                     if (!(ok = bar_wait_warp(barO, (tt - 1) & 1, dead))) break;
@@ -361,36 +397,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                 tc_fence_before();
                 bar_arrive_warp(barP);
             }
-            const bool some = i < w.lq && (l > 0.f || l != l);
-            ok = ok && bar_wait_warp(barO, (tt - 1) & 1, dead);
-            tc_fence_after();
-            const float s = !ok ? NAN : (some ? 1.f / l : 0.f);
-            // O / l, a row a thread: whole 32-byte sectors
-#pragma unroll 1
-            for (int x = 0; x < DP; x += 32) {
-                uint32_t o[32];
-                if (ok) {
-                    tmem_ld32(tO + trow + x, o);
-                    tmem_wait_ld();
-                    tmem_tie32(o);
-                }
-                if (i < a.Lq) {
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        uint32_t p[4];
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const float u0 = __uint_as_float(o[8 * y + 2 * z]), u1 = __uint_as_float(o[8 * y + 2 * z + 1]);
-                            p[z] = s == 0.f ? 0u : pack2<T>(ok ? u0 * s : s, ok ? u1 * s : s);   // a dead row is zero whatever it held
-                        }
-                        if (x + 8 * y < a.D) *reinterpret_cast<uint4*>(orow + x + 8 * y) = make_uint4(p[0], p[1], p[2], p[3]);
-                    }
-                }
-            }
-            if (lse && i < a.Lq)
-                lse[((size_t)w.b * a.H + h) * a.Lq + i] = some ? m - Softmax<T>::kShift + log2f(l) : INFINITY;
-            tc_fence_before();   // the next item's first product overwrites O after this warp's first P of it
+            kept = e, kept_m = m, kept_l = l;
         }
+        if (kept >= 0) finish();
     }
     tc_fence_before();
     __syncthreads();
