@@ -241,7 +241,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t tm = uniform(tmem), uA1 = tm + 128 * NB, uA2 = DKV ? uA1 + DP : uA1;
         bool ok = true;
         int t = 0, i = 0;   // tiles and items (with work) so far
-        constexpr uint32_t idS = mma_desc<T>(128, kStep, false), idA = mma_desc<T>(128, DP, true);
+        // (steps past the head's size are left out)
+        const int steps = (a.D + 15) / 16;
+        const uint32_t idS = mma_desc<T>(128, kStep, false), idA = mma_desc<T>(128, 16 * steps, true);
         auto scores = [&](int t, uint32_t dX) {
             const int s = t % NST, buf = t % NB;
             if (!bar_wait_warp(barY + 8 * s, (t / NST) & 1, dead)) return false;
@@ -252,7 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int k = 0; k < DP / 16; ++k)
-                    if (lead) mma_ss(d + 64 * w, dX + (w * Sh::kX + (k / 4) * kChunkX + (k % 4) * 32) / 16,
+                    if (lead && k < steps) mma_ss(d + 64 * w, dX + (w * Sh::kX + (k / 4) * kChunkX + (k % 4) * 32) / 16,
                                      dY + (w * Sh::kY + (k / 4) * kChunkY + (k % 4) * 32) / 16, idS, k != 0);
             if (lead) tc_commit(barS + 8 * buf);
             return true;

@@ -1,8 +1,8 @@
 // enc_attn_fwd.cu -- attention forward on the fifth-generation tensor cores.
 //
-// A CTA takes 128 query rows of a head and runs over the keys in tiles of 128.
-// S = Q K^T (tcgen05, both operands in shared memory, K-major) lands in 128 TMEM
-// columns; a warpgroup reads it, one row a thread, adds the bias, and takes the
+// A CTA takes 128 query rows of a head and runs over the keys in tiles of 128 (64
+// for heads above 64).  S = Q K^T (tcgen05, both operands in shared memory,
+// K-major) lands in TMEM; a warpgroup reads it, one row a thread, adds the bias, and takes the
 // softmax in base 2 with a running reference m: p = 2^(s - m), l = sum p.  P goes
 // back to TMEM in 16 bits and is operand A of O += P V (V from shared memory,
 // contraction down its rows).  m is raised, and O and l rescaled, only when a
@@ -25,29 +25,35 @@ namespace fwd {
 
 constexpr int kThreads = 256;   // a softmax warpgroup; the warps of S, of O, of the copies and of the empty row tiles
 constexpr int kRows = 128;
-constexpr int kColumns = 256;   // TMEM: S 128, O up to 128; two CTAs a SM
+constexpr int kColumns = 256;   // TMEM of a CTA; two CTAs a SM
 constexpr int kChunk = kRows * 128;
 constexpr int kMaxItems = 128;  // row tiles a CTA takes at most
 // registers: a softmax thread holds a row's 128 scores.  The two warpgroups' shares must fit what the CTA is launched with
 constexpr int kRegs = 128, kRegsSoftmax = 208, kRegsOther = 48;
 static_assert(kRegsSoftmax + kRegsOther <= 2 * kRegs, "register split");
 
+// Heads of up to 64: S 128 columns, O 64, P 64 of its own, so that the next S is formed while this one's exponentials
+// are taken.  Above, O takes 128: two buffers of 64 keys' S, each overwritten by its own P, do the same (tiles of 128 keys
+// with one buffer: 2015 clocks a tile and SM where the products need 1024)
 template <int DP>
 struct Shape {
-    static constexpr int kChunks = DP / 64;
-    static constexpr int kTile = kChunks * kChunk;
-    static constexpr int kStages = DP == 64 ? 2 : 1;   // K and V tiles in flight: one of each for 128 elements (two CTAs an SM)
-    static constexpr int kBars = 6 + 4 * kStages;
-    // P has TMEM columns of its own, so that the next S is formed while this one's exponentials are taken; for 128
-    // elements there is no room and P overwrites S (that shape is bound by its products as it is)
     static constexpr bool kApart = DP == 64;
-    static constexpr size_t smem(int lut) { return 1024 + (size_t)kTile * (1 + 2 * kStages) + kBars * 8 + 16 + kMaxItems * 20 + (size_t)lut * 4; }
+    static constexpr int kKeys = kApart ? 128 : 64, kBuffers = kApart ? 1 : 2;
+    static constexpr int kColO = 128, kColP = kApart ? 192 : 0;
+    static constexpr int kChunks = DP / 64;
+    static constexpr int kTile = kChunks * kChunk;                                // Q
+    static constexpr int kChunkKV = kKeys * 128, kTileKV = kChunks * kChunkKV;    // a K or V tile
+    static constexpr int kStages = 2;                                             // K and V tiles in flight
+    static constexpr int kBars = 4 + 3 * kBuffers + 4 * kStages;
+    static constexpr size_t kTiles = kTile + 2 * (size_t)kStages * kTileKV;
+    static constexpr size_t smem(int lut) { return 1024 + kTiles + kBars * 8 + 32 + kMaxItems * 20 + (size_t)lut * 4; }
 };
 
 // one row tile of a problem: its rows and the key tiles that any of them meets
 struct Item {
     int b, q0, lq, lk, off, tiles;
 };
+template <int KEYS>
 __device__ __forceinline__ Item item_at(const AttnArgs& a, const int* order, int index, int row_tiles) {
     Item w;
     if (order) index = order[index];
@@ -59,7 +65,7 @@ __device__ __forceinline__ Item item_at(const AttnArgs& a, const int* order, int
     w.off = a.causal ? w.lk - w.lq : 0;
     const int last = min(w.q0 + kRows, w.lq) - 1;   // the tile's last live row
     const int keys = w.q0 < w.lq ? (a.causal ? min(w.lk, last + w.off + 1) : w.lk) : 0;
-    w.tiles = keys > 0 ? (keys + kRows - 1) / kRows : 0;
+    w.tiles = keys > 0 ? (keys + KEYS - 1) / KEYS : 0;
     return w;
 }
 template <class T, int DP, bool BIAS>
@@ -68,7 +74,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs a, T* __restrict__ out,
                     float* __restrict__ lse, const int* __restrict__ order) {
     using Sh = Shape<DP>;
-    constexpr int NST = Sh::kStages;
+    constexpr int NST = Sh::kStages, NB = Sh::kBuffers, KT = Sh::kKeys;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.x, row_tiles = (a.Lq + kRows - 1) / kRows, items = a.B * row_tiles;
     const int count = item_count(items, blockIdx.y, gridDim.y);   // of this CTA
@@ -76,36 +82,40 @@ __global__ void __launch_bounds__(kThreads, 2)
     extern __shared__ uint8_t raw[];
     const uint32_t r0 = smem_addr(raw), base = (r0 + 1023u) & ~1023u;
     uint8_t* const gbase = raw + (base - r0);
-    const uint32_t sQ = base, sK = base + Sh::kTile, sV = sK + NST * Sh::kTile;
-    uint64_t* const bars = reinterpret_cast<uint64_t*>(gbase + (size_t)Sh::kTile * (1 + 2 * NST));
-    const uint32_t barQ = smem_addr(bars), barS = barQ + 8, barP = barQ + 16, barO = barQ + 24, barR = barQ + 32,
-                   barQE = barQ + 40, barK = barQ + 48, barV = barK + 8 * NST, barKE = barV + 8 * NST, barVE = barKE + 8 * NST;
-    volatile int* const dead = reinterpret_cast<volatile int*>(bars + Sh::kBars);
-    uint32_t* const slot = reinterpret_cast<uint32_t*>(bars + Sh::kBars) + 1;
-    int4* const entry = reinterpret_cast<int4*>(bars + Sh::kBars + 2);       // b, q0, lq, lk of an item
+    const uint32_t sQ = base, sK = base + Sh::kTile, sV = sK + NST * Sh::kTileKV;
+    uint64_t* const bars = reinterpret_cast<uint64_t*>(gbase + Sh::kTiles);
+    // Q there, Q free; O's product done, S read (S and P apart); S there, P there, P free of a buffer; K, V there, free
+    const uint32_t barQ = smem_addr(bars), barQE = barQ + 8, barO = barQ + 16, barR = barQ + 24, barS = barQ + 32,
+                   barP = barS + 8 * NB, barPE = barP + 8 * NB, barK = barPE + 8 * NB, barV = barK + 8 * NST,
+                   barKE = barV + 8 * NST, barVE = barKE + 8 * NST;
+    uint8_t* const after_bars = gbase + (Sh::kTiles + Sh::kBars * 8 + 15) / 16 * 16;
+    volatile int* const dead = reinterpret_cast<volatile int*>(after_bars);
+    uint32_t* const slot = reinterpret_cast<uint32_t*>(after_bars) + 1;
+    int4* const entry = reinterpret_cast<int4*>(after_bars + 16);            // b, q0, lq, lk of an item
     int* const tiles = reinterpret_cast<int*>(entry + kMaxItems);            // and the key tiles that its rows meet
     float* const lut = reinterpret_cast<float*>(tiles + kMaxItems);
     const int reach = BIAS ? reach_of(a.edges) : 0;
 
     const int kh = h / (a.H / a.Hkv);
-    auto load = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, int b, uint32_t bar) {
-        bar_expect(bar, Sh::kTile);
+    auto load = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, int b, uint32_t bar, int chunk) {
+        bar_expect(bar, Sh::kChunks * chunk);
 #pragma unroll
-        for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * kChunk, tm, 64 * c, row, head, b, bar);
+        for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * chunk, tm, 64 * c, row, head, b, bar);
     };
     if (warp == 5) {
         if (lane == 0) {
-            bar_init(barQ, 1), bar_init(barS, 1), bar_init(barP, 4), bar_init(barO, 1), bar_init(barR, 4), bar_init(barQE, 1);
+            bar_init(barQ, 1), bar_init(barQE, 1), bar_init(barO, 1), bar_init(barR, 4);
+            for (int s = 0; s < NB; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 4), bar_init(barPE + 8 * s, 1);
             for (int s = 0; s < NST; ++s)
                 bar_init(barK + 8 * s, 1), bar_init(barV + 8 * s, 1), bar_init(barKE + 8 * s, 1), bar_init(barVE + 8 * s, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
             *dead = 0;
-            const Item w = item_at(a, order, item_index(0, blockIdx.y, gridDim.y), row_tiles);   // the first item's Q and first tile before the CTA meets
+            const Item w = item_at<KT>(a, order, item_index(0, blockIdx.y, gridDim.y), row_tiles);   // the first item's Q and first tile before the CTA meets
             if (w.tiles) {
-                load(sQ, &tmQ, w.q0, h, w.b, barQ);
-                load(sK, &tmK, 0, kh, w.b, barK);
-                load(sV, &tmV, 0, kh, w.b, barV);
+                load(sQ, &tmQ, w.q0, h, w.b, barQ, kChunk);
+                load(sK, &tmK, 0, kh, w.b, barK, Sh::kChunkKV);
+                load(sV, &tmV, 0, kh, w.b, barV, Sh::kChunkKV);
             }
         }
         __syncwarp();
@@ -113,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         tmem_alloc(smem_addr(slot), kColumns);
     } else {
         for (int e = warp < 4 ? tid : tid - 64; e < count; e += 192) {
-            const Item w = item_at(a, order, item_index(e, blockIdx.y, gridDim.y), row_tiles);
+            const Item w = item_at<KT>(a, order, item_index(e, blockIdx.y, gridDim.y), row_tiles);
             entry[e] = make_int4(w.b, w.q0, w.lq, w.lk);
             tiles[e] = w.tiles;
         }
@@ -123,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot, tO = tmem + 128, tP = tmem + (Sh::kApart ? 192 : 0);
+    const uint32_t tmem = *slot, tO = tmem + Sh::kColO;
 
     if (warp >= 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
@@ -147,14 +157,14 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (n == 0) continue;
                 const int4 e = entry[i];
                 if (q > 0 && !(ok = bar_wait(barQE, (q - 1) & 1, dead))) break;
-                if (i > 0) load(sQ, &tmQ, e.y, h, e.x, barQ);   // (the first one's is under way)
+                if (i > 0) load(sQ, &tmQ, e.y, h, e.x, barQ, kChunk);   // (the first one's is under way)
                 ++q;
                 for (int j = 0; j < n; ++j, ++t) {
                     const int s = t % NST;
                     if (t >= NST && !(ok = bar_wait(barKE + 8 * s, (t / NST - 1) & 1, dead))) break;
-                    if (i + j > 0) load(sK + s * Sh::kTile, &tmK, j * kRows, kh, e.x, barK + 8 * s);
+                    if (i + j > 0) load(sK + s * Sh::kTileKV, &tmK, j * KT, kh, e.x, barK + 8 * s, Sh::kChunkKV);
                     if (t >= NST && !(ok = bar_wait(barVE + 8 * s, (t / NST - 1) & 1, dead))) break;
-                    if (i + j > 0) load(sV + s * Sh::kTile, &tmV, j * kRows, kh, e.x, barV + 8 * s);
+                    if (i + j > 0) load(sV + s * Sh::kTileKV, &tmV, j * KT, kh, e.x, barV + 8 * s, Sh::kChunkKV);
                 }
             }
             if (!ok || *dead) {   // a wait gave up: what is in flight ends (bounded) before the CTA does
@@ -168,55 +178,51 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         __syncwarp();
     } else {
-        // Products.  Where P has columns of its own one warp forms S and one O, so that neither's waits and issues stand
-        // before the other's; else one does both in turn.  A whole warp runs this, its operands' words in uniform
-        // registers; one lane issues
+        // Products: one warp forms S and one O, so that neither's waits and issues stand before the other's.  A whole warp
+        // runs this, its operands' words in uniform registers; one lane issues.  Steps past the head's size are left out
         const bool lead = elect_one();
-        const uint32_t uS = uniform(tmem), uO = uS + 128, uP = uS + (Sh::kApart ? 192 : 0);
-        constexpr uint32_t idS = mma_desc<T>(128, 128, false), idO = mma_desc<T>(128, DP, true);
+        const uint32_t uS = uniform(tmem), uO = uS + Sh::kColO, uP = uS + Sh::kColP;
+        const int steps = (a.D + 15) / 16;
         bool ok = true;
         int t = 0, q = 0;   // tiles and items begun
-        auto scores = [&](int t) {
-            const int s = t % NST;
-            if (!bar_wait_warp(barK + 8 * s, (t / NST) & 1, dead)) return false;
-            tc_fence_after();
-            const uint32_t dQ = desc_along(sQ), dK = desc_along(sK + s * Sh::kTile);
-#pragma unroll
-            for (int k = 0; k < DP / 16; ++k) {
-                const uint32_t o = ((k / 4) * kChunk + (k % 4) * 32) / 16;
-                if (lead) mma_ss(uS, dQ + o, dK + o, idS, k != 0);
-            }
-            if (lead) tc_commit(barS), tc_commit(barKE + 8 * s);
-            return true;
-        };
-        if (Sh::kApart && warp == 4) {
+        if (warp == 4) {
+            constexpr uint32_t idS = mma_desc<T>(128, KT, false);
+            const uint32_t dQ = desc_along(sQ);
             for (int e = 0; ok && e < count; ++e) {
                 const int n = (int)uniform(tiles[e]);
                 if (n == 0) continue;
                 if (!(ok = bar_wait_warp(barQ, q++ & 1, dead))) break;
-                for (int j = 0; j < n; ++j, ++t)   // S's columns are free once the one before is in registers
-                    if (!(ok = (t == 0 || bar_wait_warp(barR, (t - 1) & 1, dead)) && scores(t))) break;
+                for (int j = 0; j < n; ++j, ++t) {
+                    const int s = t % NST, buf = t % NB;
+                    if (!(ok = bar_wait_warp(barK + 8 * s, (t / NST) & 1, dead))) break;
+                    // S's columns are free once the one before is in registers, or its P has been multiplied
+                    if (Sh::kApart && t > 0 && !(ok = bar_wait_warp(barR, (t - 1) & 1, dead))) break;
+                    if (!Sh::kApart && t >= NB && !(ok = bar_wait_warp(barPE + 8 * buf, (t / NB - 1) & 1, dead))) break;
+                    tc_fence_after();
+                    const uint32_t dK = desc_along(sK + s * Sh::kTileKV), d = uS + buf * KT;
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k)
+                        if (lead && k < steps)
+                            mma_ss(d, dQ + ((k / 4) * kChunk + (k % 4) * 32) / 16, dK + ((k / 4) * Sh::kChunkKV + (k % 4) * 32) / 16, idS, k != 0);
+                    if (lead) tc_commit(barS + 8 * buf), tc_commit(barKE + 8 * s);
+                }
                 if (lead) tc_commit(barQE);
             }
-        } else if (warp == (Sh::kApart ? 7 : 4)) {
+        } else if (warp == 7) {
+            const uint32_t idO = mma_desc<T>(128, 16 * steps, true);
             for (int e = 0; ok && e < count; ++e) {
                 const int n = (int)uniform(tiles[e]);
                 if (n == 0) continue;
-                if (!Sh::kApart && !(ok = bar_wait_warp(barQ, q++ & 1, dead) && scores(t))) break;
-                if (!Sh::kApart && n == 1 && lead) tc_commit(barQE);
                 for (int j = 0; j < n; ++j, ++t) {
-                    const int s = t % NST;
-                    if (!(ok = bar_wait_warp(barV + 8 * s, (t / NST) & 1, dead) && bar_wait_warp(barP, t & 1, dead))) break;
+                    const int s = t % NST, buf = t % NB;
+                    if (!(ok = bar_wait_warp(barV + 8 * s, (t / NST) & 1, dead) && bar_wait_warp(barP + 8 * buf, (t / NB) & 1, dead))) break;
                     tc_fence_after();
-                    const uint32_t dV = desc_down(sV + s * Sh::kTile, kChunk);
+                    const uint32_t dV = desc_down(sV + s * Sh::kTileKV, Sh::kChunkKV), p = uP + buf * KT;
 #pragma unroll
-                    for (int k = 0; k < kRows / 16; ++k)
-                        if (lead) mma_ts(uO, uP + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
+                    for (int k = 0; k < KT / 16; ++k)
+                        if (lead) mma_ts(uO, p + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
                     if (lead) tc_commit(barO), tc_commit(barVE + 8 * s);
-                    if (!Sh::kApart && j + 1 < n) {
-                        if (!(ok = scores(t + 1))) break;
-                        if (j + 2 == n && lead) tc_commit(barQE);
-                    }
+                    if (!Sh::kApart && lead) tc_commit(barPE + 8 * buf);
                 }
             }
             if (!ok && lead) atomicAdd(&g_gave_up, 1ull);
@@ -250,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             const float s = !ok ? NAN : (some ? 1.f / kept_l : 0.f);
             T* const orow = out + (((size_t)w.x * a.Lq + i) * a.H + h) * a.D;
 #pragma unroll 1
-            for (int x = 0; x < DP; x += 16) {
+            for (int x = 0; x < a.D; x += 16) {
                 uint32_t o[16];
                 tmem_ld16(tO + trow + x, o);
                 tmem_wait_ld();
@@ -282,15 +288,17 @@ __global__ void __launch_bounds__(kThreads, 2)
             const int pos = w.q0 + tid + w.off, lk = w.lk;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < w.tiles && ok; ++j, ++tt) {
-                const int k0 = j * kRows;
-                if (!(ok = bar_wait_warp(barS, tt & 1, dead))) break;
+                const int k0 = j * KT, buf = tt % NB;
+                const uint32_t tS = tmem + trow + buf * KT, tP = tmem + trow + Sh::kColP + buf * KT;
+                if (!(ok = bar_wait_warp(barS + 8 * buf, (tt / NB) & 1, dead))) break;
                 tc_fence_after();
-                uint32_t v[128];
+                constexpr int kBlocks = KT / 32;
+                uint32_t v[KT];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) tmem_ld32(tmem + trow + 32 * x, v + 32 * x);
+                for (int x = 0; x < kBlocks; ++x) tmem_ld32(tS + 32 * x, v + 32 * x);
                 tmem_wait_ld();
 #pragma unroll
-                for (int x = 0; x < 4; ++x) tmem_tie32(v + 32 * x);
+                for (int x = 0; x < kBlocks; ++x) tmem_tie32(v + 32 * x);
                 if (Sh::kApart) {
                     tc_fence_before();
                     bar_arrive_warp(barR);
@@ -298,15 +306,15 @@ __global__ void __launch_bounds__(kThreads, 2)
                 float* const t = reinterpret_cast<float*>(v);
                 // a block's scores in base 2 are mul t + add: with the bias past the last edge (one value) or without any
                 // they stay as they are until the exponential; near the diagonal the bias is added here
-                float mul[4], add[4];
+                float mul[kBlocks], add[kBlocks];
 #pragma unroll
-                for (int x = 0; x < 4; ++x) mul[x] = c, add[x] = 0.f;
+                for (int x = 0; x < kBlocks; ++x) mul[x] = c, add[x] = 0.f;
                 if (BIAS) {
                     const float* const lp = lut_row(lut, reach, k0 - pos + reach + kPad);
                     // (from one lane for all, so that the branches are known to be the warp's)
                     const int dmin = __shfl_sync(0xffffffffu, k0 - (w.q0 + 32 * warp + 31 + w.off), 0);   // of the warp's 32 rows and the first 32 keys
 #pragma unroll
-                    for (int x = 0; x < 4; ++x) {
+                    for (int x = 0; x < kBlocks; ++x) {
                         const int lo = dmin + 32 * x;
                         add[x] = lo >= reach ? after : before, mul[x] = lo >= reach ? mul_after : mul_before;
                         if (lo < reach && lo + 62 > -reach) {
@@ -320,14 +328,14 @@ __global__ void __launch_bounds__(kThreads, 2)
                         }
                     }
                 }
-                if (k0 + kRows > lk || (a.causal && k0 + kRows - 1 > w.q0 + w.off)) {
+                if (k0 + KT > lk || (a.causal && k0 + KT - 1 > w.q0 + w.off)) {
                     const int lim = (a.causal ? min(lk - 1, pos) : lk - 1) - k0;
 #pragma unroll
-                    for (int x = 0; x < 128; ++x) t[x] = x <= lim ? t[x] : -INFINITY;
+                    for (int x = 0; x < KT; ++x) t[x] = x <= lim ? t[x] : -INFINITY;
                 }
                 float top = -INFINITY;
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
+                for (int x = 0; x < kBlocks; ++x) {
                     float mx = fmaxf(t[32 * x], t[32 * x + 1]), my = fmaxf(t[32 * x + 2], t[32 * x + 3]);
 #pragma unroll
                     for (int y = 32 * x + 4; y < 32 * x + 32; y += 4)
@@ -351,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
                 if (rescale) {   // O's rows of this warp
 #pragma unroll 1
-                    for (int x = 0; x < DP; x += 32) {
+                    for (int x = 0; x < a.D; x += 32) {
                         uint32_t o[32];
                         tmem_ld32(tO + trow + x, o);
                         tmem_wait_ld();
@@ -365,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 const float ref = (m == -INFINITY ? 0.f : m) - Softmax<T>::kShift;
                 Two sum[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
 #pragma unroll
-                for (int x = 0; x < 128; x += 32) {
+                for (int x = 0; x < KT; x += 32) {
                     uint32_t p[16];
                     const Two u(mul[x / 32], mul[x / 32]), v0(add[x / 32] - ref, add[x / 32] - ref);
 #pragma unroll
@@ -376,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                         sum[(y / 2) & 1] = add2(sum[(y / 2) & 1], Two(e0, e1));
                         p[y / 2] = pack2<T>(e0, e1);
                     }
-                    tmem_st16(tP + trow + x / 2, p);
+                    tmem_st16(tP + x / 2, p);
                 }
                 {
                     float s0, s1;
@@ -384,18 +392,17 @@ __global__ void __launch_bounds__(kThreads, 2)
                     l += s0 + s1;
                 }
                 const int live = lk - k0;
-                if (live < kRows) {   // the keys' last tile: rows of V past them to zero
+                if (live < KT) {   // the keys' last tile: rows of V past them to zero
                     if (!(ok = bar_wait_warp(barV + 8 * (tt % NST), (tt / NST) & 1, dead))) break;
-                    for (int e = tid; e < (kRows - live) * 8 * Sh::kChunks; e += 128) {
-                        const int ch = e / ((kRows - live) * 8), r = e % ((kRows - live) * 8);
-                        *reinterpret_cast<uint4*>(gbase + (sV - base) + (tt % NST) * Sh::kTile + ch * kChunk + live * 128 + r * 16) =
-                            make_uint4(0, 0, 0, 0);
-                    }
+                    const int units = (KT - live) * 8;
+                    for (int e = tid; e < units * Sh::kChunks; e += 128)
+                        *reinterpret_cast<uint4*>(gbase + (sV - base) + (tt % NST) * Sh::kTileKV + (e / units) * Sh::kChunkKV + live * 128 +
+                                                  (e % units) * 16) = make_uint4(0, 0, 0, 0);
                     fence_async_smem();
                 }
                 tmem_wait_st();
                 tc_fence_before();
-                bar_arrive_warp(barP);
+                bar_arrive_warp(barP + 8 * buf);
             }
             kept = e, kept_m = m, kept_l = l;
         }
@@ -408,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 
 __global__ void __launch_bounds__(1024) attn_order_kernel(const __grid_constant__ AttnArgs a, int* __restrict__ order) {
     const int row_tiles = (a.Lq + kRows - 1) / kRows;
-    order_items(a.B * row_tiles, [&](int i) { return min(item_at(a, nullptr, i, row_tiles).tiles, kBins - 1); }, order);
+    order_items(a.B * row_tiles, [&](int i) { return min(item_at<128>(a, nullptr, i, row_tiles).tiles, kBins - 1); }, order);
 }
 
 // a CTA for each item, or, where each place on the device (two CTAs an SM) would see four or more of them, a CTA for
@@ -443,8 +450,8 @@ int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaSt
     CUtensorMap q, k, v;
     if (!rows_map(&q, dtype, a.q, a.B, a.Lq, a.H, a.D, a.qs, kRows)) return D2P_ERR_INVALID_ARGUMENT;
     if (a.Lk == 0) k = v = q;   // never read
-    else if (!rows_map(&k, dtype, a.k, a.B, a.Lk, a.Hkv, a.D, a.ks, kRows) ||
-             !rows_map(&v, dtype, a.v, a.B, a.Lk, a.Hkv, a.D, a.vs, kRows))
+    else if (!rows_map(&k, dtype, a.k, a.B, a.Lk, a.Hkv, a.D, a.ks, Sh::kKeys) ||
+             !rows_map(&v, dtype, a.v, a.B, a.Lk, a.Hkv, a.D, a.vs, Sh::kKeys))
         return D2P_ERR_INVALID_ARGUMENT;
     const int lut = BIAS ? lut_size(reach_of(a.edges)) : 0;
     // at least a third of the SM's shared memory: no more than two CTAs (2 x 256 TMEM columns), so no allocation waits
