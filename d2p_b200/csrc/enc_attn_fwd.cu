@@ -44,7 +44,7 @@ struct Shape {
     static constexpr int kTile = kChunks * kChunk;                                // Q
     static constexpr int kChunkKV = kKeys * 128, kTileKV = kChunks * kChunkKV;    // a K or V tile
     static constexpr int kStages = 2;                                             // K and V tiles in flight
-    static constexpr int kBars = 4 + 3 * kBuffers + 4 * kStages;
+    static constexpr int kBars = 3 + 3 * kBuffers + 4 * kStages;
     static constexpr size_t kTiles = kTile + 2 * (size_t)kStages * kTileKV;
     static constexpr size_t smem(int lut) { return 1024 + kTiles + kBars * 8 + 32 + kMaxItems * 20 + (size_t)lut * 4; }
 };
@@ -84,8 +84,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint8_t* const gbase = raw + (base - r0);
     const uint32_t sQ = base, sK = base + Sh::kTile, sV = sK + NST * Sh::kTileKV;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(gbase + Sh::kTiles);
-    // Q there, Q free; O's product done, S read (S and P apart); S there, P there, P free of a buffer; K, V there, free
-    const uint32_t barQ = smem_addr(bars), barQE = barQ + 8, barO = barQ + 16, barR = barQ + 24, barS = barQ + 32,
+    // Q there, Q free; S read (S and P apart); of a buffer S there, P there, its product done; K, V there, free
+    const uint32_t barQ = smem_addr(bars), barQE = barQ + 8, barR = barQ + 16, barS = barQ + 24,
                    barP = barS + 8 * NB, barPE = barP + 8 * NB, barK = barPE + 8 * NB, barV = barK + 8 * NST,
                    barKE = barV + 8 * NST, barVE = barKE + 8 * NST;
     uint8_t* const after_bars = gbase + (Sh::kTiles + Sh::kBars * 8 + 15) / 16 * 16;
@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     };
     if (warp == 5) {
         if (lane == 0) {
-            bar_init(barQ, 1), bar_init(barQE, 1), bar_init(barO, 1), bar_init(barR, 4);
+            bar_init(barQ, 1), bar_init(barQE, 1), bar_init(barR, 4);
             for (int s = 0; s < NB; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 4), bar_init(barPE + 8 * s, 1);
             for (int s = 0; s < NST; ++s)
                 bar_init(barK + 8 * s, 1), bar_init(barV + 8 * s, 1), bar_init(barKE + 8 * s, 1), bar_init(barVE + 8 * s, 1);
@@ -221,8 +221,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                     for (int k = 0; k < KT / 16; ++k)
                         if (lead) mma_ts(uO, p + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
-                    if (lead) tc_commit(barO), tc_commit(barVE + 8 * s);
-                    if (!Sh::kApart && lead) tc_commit(barPE + 8 * buf);
+                    if (lead) tc_commit(barPE + 8 * buf), tc_commit(barVE + 8 * s);
                 }
             }
             if (!ok && lead) atomicAdd(&g_gave_up, 1ull);
@@ -245,10 +244,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         // An item's rows are finished behind the next one's first maximum, which covers the wait for its last product: O /
         // l, a row a thread, whole 32-byte sectors
+        // tile t's product done, by its buffer's barrier: of that one the phase before is always over (S t was formed after
+        // it), while a barrier for all products could be two phases behind, which its parity does not tell
+        auto product = [&](int t) { return bar_wait_warp(barPE + 8 * (t % NB), (t / NB) & 1, dead); };
         int kept = -1;
         float kept_m = 0.f, kept_l = 0.f;
         auto finish = [&]() {
-            ok = ok && bar_wait_warp(barO, (tt - 1) & 1, dead);
+            ok = ok && product(tt - 1);
             tc_fence_after();
             const int4 w = entry[kept];   // b, q0, lq, lk
             const int i = w.y + tid;
@@ -354,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (kept >= 0) finish();   // (the item before)
                 // the product before reads P's columns and adds to O
                 if (j > 0 && (Sh::kApart || rescale)) {
-                    if (!(ok = bar_wait_warp(barO, (tt - 1) & 1, dead))) break;
+                    if (!(ok = product(tt - 1))) break;
                     tc_fence_after();
                 }
                 if (rescale) {   // O's rows of this warp

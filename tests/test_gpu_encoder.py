@@ -280,6 +280,27 @@ def test_attention_is_repeatable(d2p, cuda_device):
             assert torch.equal(a[n], b[n]), n
 
 
+@pytest.mark.parametrize("B,L,H,Hkv,D,causal,ragged", [
+    (2, 2048, 16, 4, 128, True, False), (1, 4096, 8, 8, 128, False, False), (2, 2048, 16, 16, 64, True, False),
+    (64, 512, 8, 2, 128, True, True), (64, 512, 8, 8, 64, False, True), (96, 300, 8, 4, 80, False, True)])
+def test_attention_on_a_full_device_is_repeatable(d2p, cuda_device, B, L, H, Hkv, D, causal, ragged):
+    """Enough work for CTAs to take several row tiles, and for every wait to matter: the same bits again and again."""
+    q, k, v, do, bias = inputs(B, L, L, H, Hkv, D, torch.bfloat16, cuda_device, 32, seed=B)
+    lengths = None
+    if ragged:
+        ls = [(7 * b * L) // (8 * B) for b in range(B)]
+        lengths = torch.tensor([[x, min(L, x + b % 3)] for b, x in enumerate(ls)], dtype=torch.int32, device=cuda_device)
+    a = run_attention(d2p, q, k, v, do, bias, lengths, causal)
+    for _ in range(8):
+        b = run_attention(d2p, q, k, v, do, bias, lengths, causal)
+        for n in a:
+            assert torch.equal(a[n], b[n]), n
+    picked = [0, B // 2, B - 1]
+    part = lengths[picked] if ragged else None
+    val, tol = reference(q[picked], k[picked], v[picked], bias, part, causal, D ** -0.5, 128, do[picked])
+    compare({n: a[n][picked] for n in ("out", "dq", "dk", "dv")}, val, tol)
+
+
 def test_attention_float32_bias_and_out_of_range_lengths(d2p, cuda_device):
     q, k, v, do, bias = inputs(2, 140, 150, 2, 2, 64, torch.bfloat16, cuda_device, 32, bias_dtype=torch.float32)
     wild = torch.tensor([[1000, 1000], [-3, 4]], dtype=torch.int32, device=cuda_device)
@@ -530,6 +551,19 @@ def test_dropout_rate_and_edges(d2p, cuda_device):
     assert torch.equal(d2p.dropout_add(odd[1:], odd[1:], 0.4, 9), d2p.dropout_add(odd[1:].clone(), odd[1:].clone(), 0.4, 9))
     m = torch.randn(30, 50, device=cuda_device)
     assert torch.equal(d2p.dropout_add(m.t(), None, 0.4, 9), d2p.dropout_add(m.t().contiguous(), None, 0.4, 9))
+
+
+def test_no_wait_gave_up(d2p, cuda_device):
+    """Every bounded wait of the attention kernels so far in this process ended by what it waited for."""
+    q, k, v, do, bias = inputs(2, 300, 300, 4, 2, 64, torch.bfloat16, cuda_device, 16)
+    run_attention(d2p, q, k, v, do, bias, None, False)
+    torch.cuda.synchronize()
+    lib = ctypes.CDLL(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "d2p_b200", "libd2p_b200.so"))
+    n = ctypes.c_ulonglong(77)
+    lib.d2p_attention_gave_up.restype = ctypes.c_int
+    lib.d2p_attention_gave_up.argtypes = [ctypes.POINTER(ctypes.c_ulonglong)]
+    assert lib.d2p_attention_gave_up(ctypes.byref(n)) == 0
+    assert n.value == 0
 
 
 # ---------------------------------------------------------------------------- the C ABI's refusals, the kernels that run
