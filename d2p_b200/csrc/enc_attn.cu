@@ -54,17 +54,18 @@ size_t d2p_attention_forward_workspace_bytes(const d2p_attention_args* p) {
     return a.B == 0 || a.Lq == 0 || few_rows(a) ? 0 : enc::attn_forward_bytes(a);
 }
 
-int d2p_attention_forward(const d2p_attention_args* p, void* out, float* lse, void* workspace, size_t workspace_bytes,
+int d2p_attention_forward(const d2p_attention_args* p, void* out, float* lse, void* rest, void* workspace, size_t workspace_bytes,
                           void* stream) {
     enc::AttnArgs a;
     const int rc = enc::attn_args(p, &a);
     if (rc) return rc;
     if (a.B == 0 || a.Lq == 0) return D2P_OK;
-    if (!out || ((uintptr_t)out & 15) || ((uintptr_t)workspace & 15)) return D2P_ERR_INVALID_ARGUMENT;
-    if (few_rows(a)) return enc::attn_forward_tokens(a, p->dtype, out, lse, (cudaStream_t)stream);
+    if (!out || (((uintptr_t)out | (uintptr_t)rest | (uintptr_t)workspace) & 15)) return D2P_ERR_INVALID_ARGUMENT;
+    if (rest && !a.bias) return D2P_ERR_INVALID_ARGUMENT;
+    if (few_rows(a)) return enc::attn_forward_tokens(a, p->dtype, out, lse, rest, (cudaStream_t)stream);
     const size_t need = enc::attn_forward_bytes(a);
     if (need && (!workspace || workspace_bytes < need)) return D2P_ERR_WORKSPACE_TOO_SMALL;
-    return enc::attn_forward_tiles(a, p->dtype, out, lse, workspace, (cudaStream_t)stream);
+    return enc::attn_forward_tiles(a, p->dtype, out, lse, rest, workspace, (cudaStream_t)stream);
 }
 
 size_t d2p_attention_backward_workspace_bytes(const d2p_attention_args* p, int want_dbias) {
@@ -73,19 +74,19 @@ size_t d2p_attention_backward_workspace_bytes(const d2p_attention_args* p, int w
     return enc::attn_backward_bytes(a, want_dbias != 0);
 }
 
-int d2p_attention_backward(const d2p_attention_args* p, const void* out, const float* lse, const void* grad, void* dq,
-                           void* dk, void* dv, void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
+int d2p_attention_backward(const d2p_attention_args* p, const void* out, const void* rest, const float* lse,
+                           const void* grad, void* dq, void* dk, void* dv, void* dbias, void* workspace, size_t workspace_bytes, void* stream) {
     enc::AttnArgs a;
     const int rc = enc::attn_args(p, &a);
     if (rc) return rc;
     if (dbias && !a.bias) return D2P_ERR_INVALID_ARGUMENT;
     const bool rows = a.B && a.Lq, keys = a.B && a.Lk;
     if ((rows && (!out || !lse || !grad || !dq)) || (keys && (!dk || !dv))) return D2P_ERR_INVALID_ARGUMENT;
-    if (((uintptr_t)out | (uintptr_t)grad | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) & 15)
+    if (((uintptr_t)out | (uintptr_t)rest | (uintptr_t)grad | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) & 15)
         return D2P_ERR_INVALID_ARGUMENT;
     const size_t need = enc::attn_backward_bytes(a, dbias != nullptr);
     if (need && (!workspace || workspace_bytes < need)) return D2P_ERR_WORKSPACE_TOO_SMALL;
-    return enc::attn_backward_tiles(a, p->dtype, out, lse, grad, dq, dk, dv, dbias, workspace, (cudaStream_t)stream);
+    return enc::attn_backward_tiles(a, p->dtype, out, rest, lse, grad, dq, dk, dv, dbias, workspace, (cudaStream_t)stream);
 }
 
 int d2p_attention_gave_up(unsigned long long* n) {

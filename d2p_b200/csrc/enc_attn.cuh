@@ -58,14 +58,14 @@ struct Softmax<__half> {
 
 // checks of the C entry points; fills *a
 int attn_args(const d2p_attention_args* p, AttnArgs* a);
-// out and lse (or null) by tiles of 128 query rows (enc_attn_fwd.cu)
-int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaStream_t st);
+// out, and lse and rest (what rounding took from out; null: not wanted) by tiles of 128 query rows (enc_attn_fwd.cu)
+int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st);
 size_t attn_forward_bytes(const AttnArgs& a);
 // the same for at most 16 query rows of a key head, split over the keys (enc_attn_token.cu)
-int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st);
+int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, cudaStream_t st);
 // the gradients (enc_attn_bwd.cu) and their workspace
 size_t attn_backward_bytes(const AttnArgs& a, bool dbias);
-int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const float* lse, const void* grad, void* dq,
+int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const void* rest, const float* lse, const void* grad, void* dq,
                         void* dk, void* dv, void* dbias, void* ws, cudaStream_t st);
 // CTAs of the current device one of whose bounded waits gave up, since the library was loaded
 int attn_forward_gave_up(unsigned long long* n);

@@ -25,6 +25,11 @@
 // after the other, in order of their work, and the next one's copies and scores
 // begin while this one's results leave.
 //
+// The bias's gradient sums dS over many rows, and a row's dS sum to nothing: what
+// delta is off by would show there whole where one bucket holds most of a row's
+// weight (1 % of the sum with delta from the plain output).  For it the forward
+// forms O from P in twice 16 bits and keeps what rounding O took.
+//
 // The query pass also sums dS by relative position.  Along a diagonal of a
 // warp's 32 x 32 block the sum moves one lane per column (one shuffle each), the
 // 63 sums are scanned, and each lane takes its buckets as differences of the
@@ -65,7 +70,7 @@ struct Shape {
 // after the tiles: the bias by position, then (query pass) the diagonals' stage of each warp and the buckets' ranges
 __host__ __device__ inline size_t extra(bool bias, bool dkv, int reach) {
     if (!bias) return 0;
-    return 4 * (size_t)lut_size(reach) + (dkv ? 0 : 4 * (size_t)(16 * 72 + 16 * kBuckets + 2 * kBuckets));
+    return 4 * (size_t)lut_size(reach) + (dkv ? 0 : 4 * (size_t)(16 * 144 + 16 * kBuckets + 2 * kBuckets));
 }
 // at least 116 KB: one CTA an SM, since it takes the whole TMEM (no allocation waits)
 template <int DP, bool BIAS>
@@ -139,8 +144,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     int2* const span = reinterpret_cast<int2*>(entry + kMaxItems);           // and y0, per
     float* const lut = reinterpret_cast<float*>(span + kMaxItems);
     const int reach = BIAS ? reach_of(a.edges) : 0;
-    float* const diag = lut + lut_size(reach);                        // [16][72] a warp's diagonals, scanned in place
-    float* const red = diag + 16 * 72;                                // [16][kBuckets]
+    float* const diag = lut + lut_size(reach);                        // [16][144] a warp's diagonals, and their scan
+    float* const red = diag + 16 * 144;                               // [16][kBuckets]
     int* const range = reinterpret_cast<int*>(red + 16 * kBuckets);   // [kBuckets][2] positions of a bucket
     const bool sums = !DKV && BIAS && g.part;
 
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t trow = (uint32_t)(32 * w4) << 16;
         const float c = a.scale * kLog2e;
         bool ok = true;
-        float* const dw = diag + warp * 72;
+        float* const dw = diag + warp * 144;
         int t0 = 0, done = 0;   // tiles and items (with work) so far
         float far0 = 0.f, far1 = 0.f, bsum[kBuckets / 32];   // dS by position, over all the CTA's items
 #pragma unroll
@@ -368,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ask(0);
         for (int e = 0; e < count; ++e) {
             const int4 en = entry[e];
-            const float rl = nl, rd = nd;
+            const float rl = nl, rd = nd;   // -lse, -delta
             ask(e + 1);
             // (from one lane for all, so that the branches on them are known to be the warp's)
             const int x0 = __shfl_sync(0xffffffffu, en.y, 0), lq = __shfl_sync(0xffffffffu, en.z, 0), lk = __shfl_sync(0xffffffffu, en.w, 0);
@@ -507,18 +512,19 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 const float u = __shfl_up_sync(0xffffffffu, t, o);
                                 if (lane >= o) t += u;
                             }
+                            // pre[e]: the sum of the diagonals d in [lo, lo + e)
+                            float* const pre = dw + 72;
+                            pre[2 * lane + 1] = t - s1 + s0, pre[2 * lane + 2] = t;
+                            if (lane == 0) pre[0] = 0.f;
                             __syncwarp();
-                            dw[2 * lane + 1] = t - s1 + s0, dw[2 * lane + 2] = t;
-                            if (lane == 0) dw[0] = 0.f;
-                            __syncwarp();
-                            // entry e now holds the sum of the diagonals d in [lo, lo + e)
                             const int nb = n_buckets(a.edges);
 #pragma unroll
                             for (int i = 0; i < kBuckets / 32; ++i) {
                                 const int t2 = lane + 32 * i;
                                 if (t2 < nb) {
                                     const int e0 = max(range[2 * t2] - lo, 0), e1 = min(range[2 * t2 + 1] - lo + 1, 63);
-                                    if (e0 < e1) bsum[i] += dw[e1] - dw[e0];
+                                    // (narrow ones as they are: a difference carries the rounding of all before it)
+                                    if (e0 < e1) bsum[i] += e1 - e0 <= 2 ? dw[e0] + (e1 - e0 == 2 ? dw[e0 + 1] : 0.f) : pre[e1] - pre[e0];
                                 }
                             }
                             __syncwarp();
@@ -561,12 +567,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kWork / 32) tmem_free(tmem, kColumns);
 }
 
-// -delta = -rowsum(dO O) and -lse in rows padded to whole tiles: 0 and -inf where no key is met.  A block takes 16
+// -delta = -rowsum(dO O) and -lse in rows padded to whole tiles: 0 and -inf where no key is met.  O with what its
+// rounding took, where it is there.  A block takes 16
 // positions of up to 8 heads: rows are read as they lie, heads of a position together, and the sums leave by head, 16
 // positions together.  LANES threads a row
 constexpr int kStatRows = 16, kStatHeads = 8;
 template <class T, int LANES>
-__global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ AttnArgs a, const T* __restrict__ out,
+__global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ AttnArgs a, const T* __restrict__ out, const T* __restrict__ rest,
                                                          const float* __restrict__ lse, const T* __restrict__ grad, int Lp,
                                                          float* __restrict__ lp, float* __restrict__ dp) {
     __shared__ float sum[kStatHeads][kStatRows + 1];
@@ -586,6 +593,11 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
             load8<T>(grad + at, g);
 #pragma unroll
             for (int x = 0; x < 8; ++x) d = fmaf(o[x], g[x], d);
+            if (rest) {
+                load8<T>(rest + at, o);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) d = fmaf(o[x], g[x], d);
+            }
         }
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
@@ -662,7 +674,7 @@ int launch_pass(const Args& g, bool dkv, const CUtensorMap* tm, long long ctas, 
 }
 
 template <class T>
-int run(const AttnArgs& a, int dtype, const void* out, const float* lse, const void* grad, void* dq, void* dk, void* dv,
+int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const float* lse, const void* grad, void* dq, void* dk, void* dv,
         void* dbias, void* ws, int sms, cudaStream_t st) {
     const int Lp = tiles_of(a.Lq) * kOwn;
     float* const lp = (float*)ws;
@@ -679,8 +691,8 @@ int run(const AttnArgs& a, int dtype, const void* out, const float* lse, const v
     }
     if (a.B && a.Lq) {
         const dim3 grid(Lp / kStatRows, (a.H + kStatHeads - 1) / kStatHeads, a.B);
-        if (a.D <= 64) attn_stats_kernel<T, 8><<<grid, 256, 0, st>>>(a, (const T*)out, lse, (const T*)grad, Lp, lp, dp);
-        else attn_stats_kernel<T, 16><<<grid, 256, 0, st>>>(a, (const T*)out, lse, (const T*)grad, Lp, lp, dp);
+        if (a.D <= 64) attn_stats_kernel<T, 8><<<grid, 256, 0, st>>>(a, (const T*)out, (const T*)rest, lse, (const T*)grad, Lp, lp, dp);
+        else attn_stats_kernel<T, 16><<<grid, 256, 0, st>>>(a, (const T*)out, (const T*)rest, lse, (const T*)grad, Lp, lp, dp);
         if ((rc = (int)cudaGetLastError())) return rc;
     }
     if (a.B && (a.Lq || a.Lk)) {
@@ -747,13 +759,13 @@ size_t attn_backward_bytes(const AttnArgs& a, bool dbias) {
     return (2 * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a, sms) : 0) + bwd::order_ints(a, true, sms) +
             bwd::order_ints(a, false, sms)) * sizeof(float);
 }
-int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const float* lse, const void* grad, void* dq,
+int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const void* rest, const float* lse, const void* grad, void* dq,
                         void* dk, void* dv, void* dbias, void* ws, cudaStream_t st) {
     int sms = 0;
     const int rc = sms_of(&sms);
     if (rc) return rc;
-    return dtype == D2P_DTYPE_BF16 ? bwd::run<__nv_bfloat16>(a, dtype, out, lse, grad, dq, dk, dv, dbias, ws, sms, st)
-                                   : bwd::run<__half>(a, dtype, out, lse, grad, dq, dk, dv, dbias, ws, sms, st);
+    return dtype == D2P_DTYPE_BF16 ? bwd::run<__nv_bfloat16>(a, dtype, out, rest, lse, grad, dq, dk, dv, dbias, ws, sms, st)
+                                   : bwd::run<__half>(a, dtype, out, rest, lse, grad, dq, dk, dv, dbias, ws, sms, st);
 }
 
 }  // namespace enc

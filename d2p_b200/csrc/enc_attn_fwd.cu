@@ -34,10 +34,12 @@ static_assert(kRegsSoftmax + kRegsOther <= 2 * kRegs, "register split");
 
 // Heads of up to 64: S 128 columns, O 64, P 64 of its own, so that the next S is formed while this one's exponentials
 // are taken.  Above, O takes 128: two buffers of 64 keys' S, each overwritten by its own P, do the same (tiles of 128 keys
-// with one buffer: 2015 clocks a tile and SM where the products need 1024)
-template <int DP>
+// with one buffer: 2015 clocks a tile and SM where the products need 1024).  REST: P in twice 16 bits, the second half
+// behind the first in the buffer, for an O as exact as fp32 sums give it, and what rounding O took kept: for the
+// gradient of the bias, whose sums cancel
+template <int DP, bool REST>
 struct Shape {
-    static constexpr bool kApart = DP == 64;
+    static constexpr bool kApart = DP == 64 && !REST;
     static constexpr int kKeys = kApart ? 128 : 64, kBuffers = kApart ? 1 : 2;
     static constexpr int kColO = 128, kColP = kApart ? 192 : 0;
     static constexpr int kChunks = DP / 64;
@@ -68,12 +70,12 @@ __device__ __forceinline__ Item item_at(const AttnArgs& a, const int* order, int
     w.tiles = keys > 0 ? (keys + KEYS - 1) / KEYS : 0;
     return w;
 }
-template <class T, int DP, bool BIAS>
+template <class T, int DP, bool BIAS, bool REST>
 __global__ void __launch_bounds__(kThreads, 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs a, T* __restrict__ out,
-                    float* __restrict__ lse, const int* __restrict__ order) {
-    using Sh = Shape<DP>;
+                    float* __restrict__ lse, T* __restrict__ rest, const int* __restrict__ order) {
+    using Sh = Shape<DP, REST>;
     constexpr int NST = Sh::kStages, NB = Sh::kBuffers, KT = Sh::kKeys;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int h = blockIdx.x, row_tiles = (a.Lq + kRows - 1) / kRows, items = a.B * row_tiles;
@@ -142,9 +144,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (tiles[e]) continue;
             const int4 w = entry[e];
             const int rows = min(kRows, a.Lq - w.y), units = a.D / 8;
-            for (int x = lane; x < rows * units; x += 32)
-                *reinterpret_cast<uint4*>(out + (((size_t)w.x * a.Lq + w.y + x / units) * a.H + h) * a.D + (x % units) * 8) =
-                    make_uint4(0, 0, 0, 0);
+            for (int x = lane; x < rows * units; x += 32) {
+                const size_t at = (((size_t)w.x * a.Lq + w.y + x / units) * a.H + h) * a.D + (x % units) * 8;
+                *reinterpret_cast<uint4*>(out + at) = make_uint4(0, 0, 0, 0);
+                if (REST) *reinterpret_cast<uint4*>(rest + at) = make_uint4(0, 0, 0, 0);
+            }
             if (lse)
                 for (int x = lane; x < rows; x += 32) lse[((size_t)w.x * a.H + h) * a.Lq + w.y + x] = INFINITY;
         }
@@ -221,6 +225,11 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
                     for (int k = 0; k < KT / 16; ++k)
                         if (lead) mma_ts(uO, p + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
+                    if (REST) {
+#pragma unroll
+                        for (int k = 0; k < KT / 16; ++k)
+                            if (lead) mma_ts(uO, p + KT / 2 + 8 * k, dV + k * (2048 / 16), idO, true);
+                    }
                     if (lead) tc_commit(barPE + 8 * buf), tc_commit(barVE + 8 * s);
                 }
             }
@@ -256,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             const int i = w.y + tid;
             const bool some = i < w.z && (kept_l > 0.f || kept_l != kept_l);
             const float s = !ok ? NAN : (some ? 1.f / kept_l : 0.f);
-            T* const orow = out + (((size_t)w.x * a.Lq + i) * a.H + h) * a.D;
+            const size_t at = (((size_t)w.x * a.Lq + i) * a.H + h) * a.D;
 #pragma unroll 1
             for (int x = 0; x < a.D; x += 16) {
                 uint32_t o[16];
@@ -266,13 +275,17 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (i < a.Lq) {
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
-                        uint32_t p[4];
+                        uint32_t p[4], q[4];
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
-                            const float u0 = __uint_as_float(o[8 * y + 2 * z]), u1 = __uint_as_float(o[8 * y + 2 * z + 1]);
-                            p[z] = s == 0.f ? 0u : pack2<T>(ok ? u0 * s : s, ok ? u1 * s : s);   // a dead row is zero whatever it held
+                            const float u0 = ok ? __uint_as_float(o[8 * y + 2 * z]) * s : s, u1 = ok ? __uint_as_float(o[8 * y + 2 * z + 1]) * s : s;
+                            p[z] = s == 0.f ? 0u : pack2<T>(u0, u1);   // a dead row is zero whatever it held
+                            q[z] = REST && s != 0.f ? rest2<T>(u0, u1, p[z]) : 0u;
                         }
-                        if (x + 8 * y < a.D) *reinterpret_cast<uint4*>(orow + x + 8 * y) = make_uint4(p[0], p[1], p[2], p[3]);
+                        if (x + 8 * y < a.D) {
+                            *reinterpret_cast<uint4*>(out + at + x + 8 * y) = make_uint4(p[0], p[1], p[2], p[3]);
+                            if (REST) *reinterpret_cast<uint4*>(rest + at + x + 8 * y) = make_uint4(q[0], q[1], q[2], q[3]);
+                        }
                     }
                 }
             }
@@ -376,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 Two sum[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
 #pragma unroll
                 for (int x = 0; x < KT; x += 32) {
-                    uint32_t p[16];
+                    uint32_t p[16], p2[16];
                     const Two u(mul[x / 32], mul[x / 32]), v0(add[x / 32] - ref, add[x / 32] - ref);
 #pragma unroll
                     for (int y = 0; y < 32; y += 2) {
@@ -385,8 +398,10 @@ __global__ void __launch_bounds__(kThreads, 2)
                         e0 = ex2(e0), e1 = ex2(e1);
                         sum[(y / 2) & 1] = add2(sum[(y / 2) & 1], Two(e0, e1));
                         p[y / 2] = pack2<T>(e0, e1);
+                        if (REST) p2[y / 2] = rest2<T>(e0, e1, p[y / 2]);
                     }
                     tmem_st16(tP + x / 2, p);
+                    if (REST) tmem_st16(tP + KT / 2 + x / 2, p2);
                 }
                 {
                     float s0, s1;
@@ -432,19 +447,19 @@ bool ordered(const AttnArgs& a, int sms) {
     return (a.lengths || a.causal) && stays(a, sms) && (long long)a.B * ((a.Lq + kRows - 1) / kRows) <= kMaxOrder;
 }
 
-template <class T, int DP, bool BIAS>
-int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaStream_t st) {
-    using Sh = Shape<DP>;
+template <class T, int DP, bool BIAS, bool REST>
+int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
+    using Sh = Shape<DP, REST>;
     static DeviceSetup setup;
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
     int rc = device_setup(setup, dev, [] {
         cudaFuncAttributes at;   // the register split above counts on the launch's share
-        cudaError_t e = cudaFuncGetAttributes(&at, attn_fwd_kernel<T, DP, BIAS>);
+        cudaError_t e = cudaFuncGetAttributes(&at, attn_fwd_kernel<T, DP, BIAS, REST>);
         if (e == cudaSuccess && at.numRegs < (kRegsSoftmax + kRegsOther + 1) / 2) e = cudaErrorLaunchOutOfResources;
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attn_fwd_kernel<T, DP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            e = cudaFuncSetAttribute(attn_fwd_kernel<T, DP, BIAS, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)Sh::smem(lut_size(kMaxReach)));
         return (int)e;
     }, &sms);
@@ -466,14 +481,19 @@ int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaSt
         order = (int*)ws;
         attn_order_kernel<<<1, 1024, 0, st>>>(a, order);
     }
-    attn_fwd_kernel<T, DP, BIAS><<<dim3(a.H, (unsigned)ctas), kThreads, smem, st>>>(q, k, v, a, (T*)out, lse, order);
+    attn_fwd_kernel<T, DP, BIAS, REST><<<dim3(a.H, (unsigned)ctas), kThreads, smem, st>>>(q, k, v, a, (T*)out, lse, (T*)rest, order);
     return (int)cudaGetLastError();
 }
 
 template <class T>
-int pick(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaStream_t st) {
-    if (a.D <= 64) return a.bias ? launch<T, 64, true>(a, dtype, out, lse, ws, st) : launch<T, 64, false>(a, dtype, out, lse, ws, st);
-    return a.bias ? launch<T, 128, true>(a, dtype, out, lse, ws, st) : launch<T, 128, false>(a, dtype, out, lse, ws, st);
+int pick(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
+    if (a.D <= 64)
+        return !a.bias ? launch<T, 64, false, false>(a, dtype, out, lse, rest, ws, st)
+               : rest  ? launch<T, 64, true, true>(a, dtype, out, lse, rest, ws, st)
+                       : launch<T, 64, true, false>(a, dtype, out, lse, rest, ws, st);
+    return !a.bias ? launch<T, 128, false, false>(a, dtype, out, lse, rest, ws, st)
+           : rest  ? launch<T, 128, true, true>(a, dtype, out, lse, rest, ws, st)
+                   : launch<T, 128, true, false>(a, dtype, out, lse, rest, ws, st);
 }
 
 }  // namespace fwd
@@ -512,8 +532,8 @@ size_t attn_forward_bytes(const AttnArgs& a) {
     if (cudaGetDevice(&dev) != cudaSuccess || device_setup(setup, dev, [] { return 0; }, &sms)) return (size_t)-1;
     return fwd::ordered(a, sms) ? (size_t)a.B * ((a.Lq + fwd::kRows - 1) / fwd::kRows) * sizeof(int) : 0;
 }
-int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, void* ws, cudaStream_t st) {
-    return dtype == D2P_DTYPE_BF16 ? fwd::pick<__nv_bfloat16>(a, dtype, out, lse, ws, st) : fwd::pick<__half>(a, dtype, out, lse, ws, st);
+int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
+    return dtype == D2P_DTYPE_BF16 ? fwd::pick<__nv_bfloat16>(a, dtype, out, lse, rest, ws, st) : fwd::pick<__half>(a, dtype, out, lse, rest, ws, st);
 }
 
 }  // namespace enc

@@ -77,7 +77,7 @@ __device__ __forceinline__ int bucket_of(const Edges& e, int d) {
 
 template <class T, int DP>
 __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_constant__ AttnArgs a, T* __restrict__ out,
-                                                                float* __restrict__ lse) {
+                                                                float* __restrict__ lse, T* __restrict__ rest) {
     using Sh = Shape<DP>;
     constexpr int NST = Sh::kStages, CH = DP / 8;   // 16-byte units of a row
     extern __shared__ __align__(128) uint8_t sm[];
@@ -215,6 +215,10 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
         for (int y = 0; y < kKeys / 16; ++y) {
             const uint32_t pa[4] = {pack2<T>(p[0][4 * y], p[0][4 * y + 1]), pack2<T>(p[1][4 * y], p[1][4 * y + 1]),
                                     pack2<T>(p[0][4 * y + 2], p[0][4 * y + 3]), pack2<T>(p[1][4 * y + 2], p[1][4 * y + 3])};
+            uint32_t pl[4];   // what rounding took from them, where out's rest is wanted
+            if (rest)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) pl[x] = rest2<T>(p[x & 1][4 * y + 2 * (x >> 1)], p[x & 1][4 * y + 2 * (x >> 1) + 1], pa[x]);
 #pragma unroll
             for (int x = 0; x < DP / 16; ++x) {   // matrices: keys 0-7 / 8-15 (lane >> 3 & 1) by elements 0-7 / 8-15 (lane >> 4)
                 const int r = 16 * y + (lane & 7) + (((lane >> 3) & 1) << 3), c = 2 * x + (lane >> 4);
@@ -222,6 +226,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
                 ldmatrix4<true>(e, vs + r * (DP * 2) + ((c ^ (r & 7)) << 4));
                 mma16816<T>(o[2 * x], pa, e[0], e[1]);
                 mma16816<T>(o[2 * x + 1], pa, e[2], e[3]);
+                if (rest) mma16816<T>(o[2 * x], pl, e[0], e[1]), mma16816<T>(o[2 * x + 1], pl, e[2], e[3]);
             }
         }
         __syncwarp();
@@ -256,7 +261,10 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
         const int i = r / G, h = kh * G + r % G;
         const bool some = (sum > 0.f || sum != sum) && i < lq;
         const float w = some ? 1.f / sum : 0.f;
-        *reinterpret_cast<uint32_t*>(out + (((size_t)b * a.Lq + i) * a.H + h) * a.D + d) = some ? pack2<T>(x * w, y * w) : 0u;
+        const size_t at = (((size_t)b * a.Lq + i) * a.H + h) * a.D + d;
+        const uint32_t p = some ? pack2<T>(x * w, y * w) : 0u;
+        *reinterpret_cast<uint32_t*>(out + at) = p;
+        if (rest) *reinterpret_cast<uint32_t*>(rest + at) = some ? rest2<T>(x * w, y * w, p) : 0u;
         if (lse && d == 0) lse[((size_t)b * a.H + h) * a.Lq + i] = some ? top - Softmax<T>::kShift + log2f(sum) : INFINITY;
     };
     for (int e = tid; e < rows * units; e += 32 * kWarps) {
@@ -300,7 +308,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
 }
 
 template <class T, int DP>
-int launch(const AttnArgs& a, void* out, float* lse, cudaStream_t st) {
+int launch(const AttnArgs& a, void* out, float* lse, void* rest, cudaStream_t st) {
     using Sh = Shape<DP>;
     constexpr int smem = Sh::kRing > Sh::kJoin ? Sh::kRing : Sh::kJoin;
     static DeviceSetup setup;
@@ -324,15 +332,15 @@ int launch(const AttnArgs& a, void* out, float* lse, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr, cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, attn_token_kernel<T, DP>, a, (T*)out, lse);
+    return (int)cudaLaunchKernelEx(&cfg, attn_token_kernel<T, DP>, a, (T*)out, lse, (T*)rest);
 }
 
 }  // namespace tok
 
-int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, cudaStream_t st) {
+int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, cudaStream_t st) {
     if (dtype == D2P_DTYPE_BF16)
-        return a.D <= 64 ? tok::launch<__nv_bfloat16, 64>(a, out, lse, st) : tok::launch<__nv_bfloat16, 128>(a, out, lse, st);
-    return a.D <= 64 ? tok::launch<__half, 64>(a, out, lse, st) : tok::launch<__half, 128>(a, out, lse, st);
+        return a.D <= 64 ? tok::launch<__nv_bfloat16, 64>(a, out, lse, rest, st) : tok::launch<__nv_bfloat16, 128>(a, out, lse, rest, st);
+    return a.D <= 64 ? tok::launch<__half, 64>(a, out, lse, rest, st) : tok::launch<__half, 128>(a, out, lse, rest, st);
 }
 
 }  // namespace enc

@@ -47,6 +47,19 @@ __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// what that rounding took from a and b, in the same type; p: the two rounded
+template <class T>
+__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t p);
+template <>
+__device__ __forceinline__ uint32_t rest2<__nv_bfloat16>(float a, float b, uint32_t p) {
+    return pack2<__nv_bfloat16>(a - __uint_as_float(p << 16), b - __uint_as_float(p & 0xffff0000u));
+}
+template <>
+__device__ __forceinline__ uint32_t rest2<__half>(float a, float b, uint32_t p) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&p));
+    return pack2<__half>(a - f.x, b - f.y);
+}
+
 // eight consecutive elements at a 16-byte boundary
 template <class T>
 __device__ __forceinline__ void load8(const T* p, float* v) {

@@ -1052,28 +1052,30 @@ void attn_fill(Attn& f, const Tensor& q, const Tensor& k, const Tensor& v, const
     }
 }
 
-std::tuple<Tensor, Tensor> attention_forward_cuda(const Tensor& q, const Tensor& k, const Tensor& v,
-                                                  const c10::optional<Tensor>& bias, const c10::optional<Tensor>& lengths,
-                                                  at::IntArrayRef edges, double scale, bool causal, bool want_lse) {
+std::tuple<Tensor, Tensor, Tensor> attention_forward_cuda(const Tensor& q, const Tensor& k, const Tensor& v,
+                                                          const c10::optional<Tensor>& bias,
+                                                          const c10::optional<Tensor>& lengths, at::IntArrayRef edges,
+                                                          double scale, bool causal, bool want_lse, bool want_rest) {
     TORCH_CHECK(q.is_cuda(), "attention: q, k and v must be CUDA tensors");
     const c10::cuda::CUDAGuard guard(q.device());
     Attn f;
     attn_fill(f, q, k, v, bias, lengths, edges, scale, causal);
     Tensor out = torch::empty({q.size(0), q.size(1), q.size(2), q.size(3)}, q.options());
     Tensor lse = torch::empty({want_lse ? q.size(0) : 0, q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    Tensor rest = torch::empty({want_rest ? q.size(0) : 0, q.size(1), q.size(2), q.size(3)}, q.options());
     const size_t n = d2p_attention_forward_workspace_bytes(&f.a);
     TORCH_CHECK(n != static_cast<size_t>(-1), "attention: problem not supported");
     Tensor ws = n ? torch::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte)) : Tensor();
     check_rc(d2p_attention_forward(&f.a, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
-                                   n ? ws.data_ptr() : nullptr, n, cur_stream()),
+                                   want_rest ? rest.data_ptr() : nullptr, n ? ws.data_ptr() : nullptr, n, cur_stream()),
              "d2p_attention_forward");
-    return {out, lse};
+    return {out, lse, rest};
 }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(
     const Tensor& grad, const Tensor& q, const Tensor& k, const Tensor& v, const c10::optional<Tensor>& bias,
     const c10::optional<Tensor>& lengths, at::IntArrayRef edges, double scale, bool causal, const Tensor& out,
-    const Tensor& lse, bool want_bias) {
+    const Tensor& lse, const c10::optional<Tensor>& rest, bool want_bias) {
     TORCH_CHECK(q.is_cuda(), "attention: q, k and v must be CUDA tensors");
     const c10::cuda::CUDAGuard guard(q.device());
     Attn f;
@@ -1085,6 +1087,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(
                     lse.size(0) == q.size(0) && lse.size(1) == q.size(2) && lse.size(2) == q.size(1),
                 "attention_backward: lse must be the forward's fp32 [B, H, Lq]");
     TORCH_CHECK(!want_bias || f.bias.defined(), "attention_backward: no bias to take the gradient of");
+    Tensor rs;
+    if (rest.has_value() && rest->defined()) {
+        TORCH_CHECK(rest->sizes() == q.sizes() && rest->scalar_type() == q.scalar_type() && rest->device() == q.device(),
+                    "attention_backward: rest must have q's shape, dtype and device");
+        rs = packed16(*rest);
+    }
     const Tensor g = packed16(grad), o = packed16(out), L = lse.contiguous();
     Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
     Tensor dv = torch::empty(v.sizes(), v.options());
@@ -1092,8 +1100,8 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(
     const size_t n = d2p_attention_backward_workspace_bytes(&f.a, want_bias);
     TORCH_CHECK(n != static_cast<size_t>(-1), "attention_backward: problem not supported");
     Tensor ws = torch::empty({static_cast<int64_t>(n > 0 ? n : 1)}, q.options().dtype(at::kByte));
-    check_rc(d2p_attention_backward(&f.a, o.data_ptr(), L.data_ptr<float>(), g.data_ptr(), dq.data_ptr(), dk.data_ptr(),
-                                    dv.data_ptr(), want_bias ? db.data_ptr() : nullptr, ws.data_ptr(), n, cur_stream()),
+    check_rc(d2p_attention_backward(&f.a, o.data_ptr(), rs.defined() ? rs.data_ptr() : nullptr, L.data_ptr<float>(),
+                                    g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), want_bias ? db.data_ptr() : nullptr, ws.data_ptr(), n, cur_stream()),
              "d2p_attention_backward");
     return {dq, dk, dv, db};
 }
@@ -1204,14 +1212,14 @@ OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor()
 Tensor undef(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
-std::tuple<Tensor, Tensor> call_attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
+std::tuple<Tensor, Tensor, Tensor> call_attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
                                                   const OptTensor& lengths, at::IntArrayRef edges, double scale, bool causal,
-                                                  bool want_lse) {
+                                                  bool want_lse, bool want_rest) {
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("d2p_b200::attention_forward", "")
-                         .typed<std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
-                                                           const OptTensor&, at::IntArrayRef, double, bool, bool)>();
-    return op.call(q, k, v, bias, lengths, edges, scale, causal, want_lse);
+                         .typed<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                                                                   const OptTensor&, at::IntArrayRef, double, bool, bool, bool)>();
+    return op.call(q, k, v, bias, lengths, edges, scale, causal, want_lse, want_rest);
 }
 
 class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
@@ -1219,12 +1227,14 @@ class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
     static Tensor forward(AutogradContext* ctx, const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
                           const OptTensor& lengths, at::IntArrayRef edges, double scale, bool causal) {
         at::AutoDispatchBelowADInplaceOrView guard;
-        auto r = call_attention_forward(q, k, v, bias, lengths, edges, scale, causal, true);
-        ctx->save_for_backward({q, k, v, undef(bias), undef(lengths), std::get<0>(r), std::get<1>(r)});
+        const bool want_bias = bias.has_value() && wants_grad(*bias);
+        auto r = call_attention_forward(q, k, v, bias, lengths, edges, scale, causal, true, want_bias);
+        ctx->save_for_backward({q, k, v, undef(bias), undef(lengths), std::get<0>(r), std::get<1>(r),
+                                want_bias ? std::get<2>(r) : Tensor()});
         ctx->saved_data["edges"] = edges.vec();
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["causal"] = causal;
-        ctx->saved_data["want_bias"] = bias.has_value() && wants_grad(*bias);
+        ctx->saved_data["want_bias"] = want_bias;
         return std::get<0>(r);
     }
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
@@ -1232,12 +1242,12 @@ class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
                              .findSchemaOrThrow("d2p_b200::attention_backward", "")
                              .typed<std::tuple<Tensor, Tensor, Tensor, Tensor>(
                                  const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
-                                 const OptTensor&, at::IntArrayRef, double, bool, const Tensor&, const Tensor&, bool)>();
+                                 const OptTensor&, at::IntArrayRef, double, bool, const Tensor&, const Tensor&, const OptTensor&, bool)>();
         auto s = ctx->get_saved_variables();
         const std::vector<int64_t> edges = ctx->saved_data["edges"].toIntVector();
         const bool want_bias = ctx->saved_data["want_bias"].toBool();
         auto r = op.call(grads[0], s[0], s[1], s[2], opt(s[3]), opt(s[4]), edges, ctx->saved_data["scale"].toDouble(),
-                         ctx->saved_data["causal"].toBool(), s[5], s[6], want_bias);
+                         ctx->saved_data["causal"].toBool(), s[5], s[6], opt(s[7]), want_bias);
         return {std::get<0>(r), std::get<1>(r), std::get<2>(r), want_bias ? std::get<3>(r) : Tensor(),
                 Tensor(), Tensor(), Tensor(), Tensor()};
     }
@@ -1248,11 +1258,11 @@ Tensor attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, con
     if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(undef(bias))))
         return AttentionFunction::apply(q, k, v, bias, lengths, edges, scale, causal);
     at::AutoDispatchBelowADInplaceOrView guard;
-    return std::get<0>(call_attention_forward(q, k, v, bias, lengths, edges, scale, causal, false));
+    return std::get<0>(call_attention_forward(q, k, v, bias, lengths, edges, scale, causal, false, false));
 }
 Tensor attention_cuda(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias, const OptTensor& lengths,
                       at::IntArrayRef edges, double scale, bool causal) {
-    return std::get<0>(attention_forward_cuda(q, k, v, bias, lengths, edges, scale, causal, false));
+    return std::get<0>(attention_forward_cuda(q, k, v, bias, lengths, edges, scale, causal, false, false));
 }
 
 std::tuple<Tensor, Tensor> call_norm_rope_forward(const Tensor& q, const Tensor& k, const Tensor& qw, const Tensor& kw,
@@ -1335,8 +1345,8 @@ TORCH_LIBRARY_FRAGMENT(d2p_b200, m) {
     m.def("embed_grad_scores(Tensor marginals, Tensor grad_value, float scale) -> Tensor");
     // what a user calls (with gradients), and the parts they are made of
     m.def("attention(Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal) -> Tensor");
-    m.def("attention_forward(Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal, bool want_lse) -> (Tensor, Tensor)");
-    m.def("attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal, Tensor out, Tensor lse, bool want_bias) -> (Tensor, Tensor, Tensor, Tensor)");
+    m.def("attention_forward(Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal, bool want_lse, bool want_rest) -> (Tensor, Tensor, Tensor)");
+    m.def("attention_backward(Tensor grad, Tensor q, Tensor k, Tensor v, Tensor? bias, Tensor? lengths, int[] bucket_edges, float scale, bool causal, Tensor out, Tensor lse, Tensor? rest, bool want_bias) -> (Tensor, Tensor, Tensor, Tensor)");
     m.def("qk_norm_rope(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor)");
     m.def("qk_norm_rope_forward(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor)");
     m.def("qk_norm_rope_backward(Tensor grad_q, Tensor grad_k, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor, Tensor, Tensor)");

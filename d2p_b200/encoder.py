@@ -164,16 +164,16 @@ def dropout_add(
     return _ops_dropout_add(x, residual, float(p), int(seed), int(offset))
 
 
-def _attention_forward_fake(q, k, v, bias, lengths, bucket_edges, scale, causal, want_lse):
+def _attention_forward_fake(q, k, v, bias, lengths, bucket_edges, scale, causal, want_lse, want_rest):
     lse = q.new_empty((q.shape[0] if want_lse else 0, q.shape[2], q.shape[1]), dtype=torch.float32)
-    return q.new_empty(q.shape), lse
+    return q.new_empty(q.shape), lse, q.new_empty((q.shape[0] if want_rest else 0, *q.shape[1:]))
 
 
 def _attention_fake(q, k, v, bias, lengths, bucket_edges, scale, causal):
     return q.new_empty(q.shape)
 
 
-def _attention_backward_fake(grad, q, k, v, bias, lengths, bucket_edges, scale, causal, out, lse, want_bias):
+def _attention_backward_fake(grad, q, k, v, bias, lengths, bucket_edges, scale, causal, out, lse, rest, want_bias):
     db = bias.new_empty(bias.shape) if want_bias else q.new_empty((0, 0))
     return q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape), db
 

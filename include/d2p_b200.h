@@ -336,19 +336,22 @@ typedef struct {
     int causal;
     float scale; /* positive */
 } d2p_attention_args;
-/* out [B, Lq, H, D] contiguous, the inputs' type; lse [B, H, Lq] fp32 or NULL:
- * what the backward pass takes (log2 of the sum of exponentials, +inf in rows
- * with no allowed key). */
+/* out [B, Lq, H, D] contiguous, the inputs' type.  For the backward pass: lse [B,
+ * H, Lq] fp32 or NULL (log2 of the sum of exponentials, +inf in rows with no
+ * allowed key), and rest, like out, or NULL: for the gradient of the bias (needs
+ * one), whose sums cancel, out is formed from unrounded probabilities and what its
+ * own rounding took is kept.
+ * Large batches of uneven lengths take a small workspace. */
 D2P_API size_t d2p_attention_forward_workspace_bytes(const d2p_attention_args* args);
-D2P_API int d2p_attention_forward(const d2p_attention_args* args, void* out, float* lse, void* workspace,
-                                  size_t workspace_bytes, void* stream);
+D2P_API int d2p_attention_forward(const d2p_attention_args* args, void* out, float* lse, void* rest,
+                                  void* workspace, size_t workspace_bytes, void* stream);
 /* Gradients of the above with the probabilities recomputed: grad, out [B, Lq, H,
- * D] contiguous, lse from the forward call; dq, dk, dv contiguous in the inputs'
+ * D] contiguous, lse and rest (or NULL) from the forward call; dq, dk, dv contiguous in the inputs'
  * type (zero outside the lengths); dbias [num_buckets, H] in bias_dtype, or NULL.
  * Deterministic: no atomics. */
 D2P_API size_t d2p_attention_backward_workspace_bytes(const d2p_attention_args* args, int want_dbias);
-D2P_API int d2p_attention_backward(const d2p_attention_args* args, const void* out, const float* lse, const void* grad,
-                                   void* dq, void* dk, void* dv, void* dbias, void* workspace, size_t workspace_bytes,
+D2P_API int d2p_attention_backward(const d2p_attention_args* args, const void* out, const void* rest, const float* lse,
+                                   const void* grad, void* dq, void* dk, void* dv, void* dbias, void* workspace, size_t workspace_bytes,
                                    void* stream);
 /* CTAs of the attention kernels on the current device, since the library was
  * loaded, one of whose bounded waits gave up; the rows such a CTA owns are NaN.
