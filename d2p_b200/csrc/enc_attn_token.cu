@@ -75,7 +75,7 @@ __device__ __forceinline__ int bucket_of(const Edges& e, int d) {
     return lo + ((e.two && d > 0) ? e.n + 1 : 0);
 }
 
-template <class T, int DP>
+template <class T, int DP, bool REST>
 __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_constant__ AttnArgs a, T* __restrict__ out,
                                                                 float* __restrict__ lse, T* __restrict__ rest) {
     using Sh = Shape<DP>;
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
             const uint32_t pa[4] = {pack2<T>(p[0][4 * y], p[0][4 * y + 1]), pack2<T>(p[1][4 * y], p[1][4 * y + 1]),
                                     pack2<T>(p[0][4 * y + 2], p[0][4 * y + 3]), pack2<T>(p[1][4 * y + 2], p[1][4 * y + 3])};
             uint32_t pl[4];   // what rounding took from them, where out's rest is wanted
-            if (rest)
+            if (REST)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) pl[x] = rest2<T>(p[x & 1][4 * y + 2 * (x >> 1)], p[x & 1][4 * y + 2 * (x >> 1) + 1], pa[x]);
 #pragma unroll
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
                 ldmatrix4<true>(e, vs + r * (DP * 2) + ((c ^ (r & 7)) << 4));
                 mma16816<T>(o[2 * x], pa, e[0], e[1]);
                 mma16816<T>(o[2 * x + 1], pa, e[2], e[3]);
-                if (rest) mma16816<T>(o[2 * x], pl, e[0], e[1]), mma16816<T>(o[2 * x + 1], pl, e[2], e[3]);
+                if (REST) mma16816<T>(o[2 * x], pl, e[0], e[1]), mma16816<T>(o[2 * x + 1], pl, e[2], e[3]);
             }
         }
         __syncwarp();
@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
         const size_t at = (((size_t)b * a.Lq + i) * a.H + h) * a.D + d;
         const uint32_t p = some ? pack2<T>(x * w, y * w) : 0u;
         *reinterpret_cast<uint32_t*>(out + at) = p;
-        if (rest) *reinterpret_cast<uint32_t*>(rest + at) = some ? rest2<T>(x * w, y * w, p) : 0u;
+        if (REST) *reinterpret_cast<uint32_t*>(rest + at) = some ? rest2<T>(x * w, y * w, p) : 0u;
         if (lse && d == 0) lse[((size_t)b * a.H + h) * a.Lq + i] = some ? top - Softmax<T>::kShift + log2f(sum) : INFINITY;
     };
     for (int e = tid; e < rows * units; e += 32 * kWarps) {
@@ -307,7 +307,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
     cluster.sync();   // the sets are read from other CTAs
 }
 
-template <class T, int DP>
+template <class T, int DP, bool REST>
 int launch(const AttnArgs& a, void* out, float* lse, void* rest, cudaStream_t st) {
     using Sh = Shape<DP>;
     constexpr int smem = Sh::kRing > Sh::kJoin ? Sh::kRing : Sh::kJoin;
@@ -316,8 +316,8 @@ int launch(const AttnArgs& a, void* out, float* lse, void* rest, cudaStream_t st
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
     int rc = device_setup(setup, dev, [] {
-        cudaError_t e = cudaFuncSetAttribute(attn_token_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_token_kernel<T, DP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        cudaError_t e = cudaFuncSetAttribute(attn_token_kernel<T, DP, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_token_kernel<T, DP, REST>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         return (int)e;
     }, &sms);
     if (rc) return rc;
@@ -332,15 +332,18 @@ int launch(const AttnArgs& a, void* out, float* lse, void* rest, cudaStream_t st
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr, cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, attn_token_kernel<T, DP>, a, (T*)out, lse, (T*)rest);
+    return (int)cudaLaunchKernelEx(&cfg, attn_token_kernel<T, DP, REST>, a, (T*)out, lse, (T*)rest);
 }
 
 }  // namespace tok
 
+template <class T>
+static int pick_token(const AttnArgs& a, void* out, float* lse, void* rest, cudaStream_t st) {
+    if (a.D <= 64) return rest ? tok::launch<T, 64, true>(a, out, lse, rest, st) : tok::launch<T, 64, false>(a, out, lse, rest, st);
+    return rest ? tok::launch<T, 128, true>(a, out, lse, rest, st) : tok::launch<T, 128, false>(a, out, lse, rest, st);
+}
 int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, cudaStream_t st) {
-    if (dtype == D2P_DTYPE_BF16)
-        return a.D <= 64 ? tok::launch<__nv_bfloat16, 64>(a, out, lse, rest, st) : tok::launch<__nv_bfloat16, 128>(a, out, lse, rest, st);
-    return a.D <= 64 ? tok::launch<__half, 64>(a, out, lse, rest, st) : tok::launch<__half, 128>(a, out, lse, rest, st);
+    return dtype == D2P_DTYPE_BF16 ? pick_token<__nv_bfloat16>(a, out, lse, rest, st) : pick_token<__half>(a, out, lse, rest, st);
 }
 
 }  // namespace enc

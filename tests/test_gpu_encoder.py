@@ -609,3 +609,15 @@ def test_operators_refuse(d2p, cuda_device):
             op(*args)
     with pytest.raises(RuntimeError):
         torch.ops.d2p_b200.dropout_add(q, q.float(), 0.1, 1, 0)
+
+
+def test_example_trains(cuda_device):
+    """examples/encode_align.py: the four operators and the alignment in one training loop."""
+    import importlib.util
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "encode_align.py")
+    spec = importlib.util.spec_from_file_location("encode_align", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    losses = module.train(60, report=None)
+    assert all(math.isfinite(x) for x in losses) and sum(losses[-10:]) < 0.5 * sum(losses[:10])
