@@ -31,6 +31,7 @@ int attn_args(const d2p_attention_args* p, AttnArgs* a) {
         if (p->q_stride[i] % 8 || p->k_stride[i] % 8 || p->v_stride[i] % 8) return D2P_ERR_INVALID_ARGUMENT;
         a->qs[i] = p->q_stride[i], a->ks[i] = p->k_stride[i], a->vs[i] = p->v_stride[i];
     }
+    if (((uintptr_t)p->lengths & 3) || ((uintptr_t)p->bias & (a->bias_f32 ? 3 : 1))) return D2P_ERR_INVALID_ARGUMENT;
     a->lengths = p->lengths;
     a->B = p->B, a->Lq = p->Lq, a->Lk = p->Lk, a->H = p->H, a->Hkv = p->Hkv, a->D = p->D, a->causal = p->causal != 0;
     a->scale = p->scale;
@@ -60,7 +61,7 @@ int d2p_attention_forward(const d2p_attention_args* p, void* out, float* lse, vo
     const int rc = enc::attn_args(p, &a);
     if (rc) return rc;
     if (a.B == 0 || a.Lq == 0) return D2P_OK;
-    if (!out || (((uintptr_t)out | (uintptr_t)rest | (uintptr_t)workspace) & 15)) return D2P_ERR_INVALID_ARGUMENT;
+    if (!out || (((uintptr_t)out | (uintptr_t)rest | (uintptr_t)workspace) & 15) || ((uintptr_t)lse & 3)) return D2P_ERR_INVALID_ARGUMENT;
     if (rest && !a.bias) return D2P_ERR_INVALID_ARGUMENT;
     if (few_rows(a)) return enc::attn_forward_tokens(a, p->dtype, out, lse, rest, (cudaStream_t)stream);
     const size_t need = enc::attn_forward_bytes(a);
@@ -84,6 +85,7 @@ int d2p_attention_backward(const d2p_attention_args* p, const void* out, const v
     if ((rows && (!out || !lse || !grad || !dq)) || (keys && (!dk || !dv))) return D2P_ERR_INVALID_ARGUMENT;
     if (((uintptr_t)out | (uintptr_t)rest | (uintptr_t)grad | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv | (uintptr_t)workspace) & 15)
         return D2P_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)lse & 3) || ((uintptr_t)dbias & (a.bias_f32 ? 3 : 1))) return D2P_ERR_INVALID_ARGUMENT;
     const size_t need = enc::attn_backward_bytes(a, dbias != nullptr);
     if (need && (!workspace || workspace_bytes < need)) return D2P_ERR_WORKSPACE_TOO_SMALL;
     return enc::attn_backward_tiles(a, p->dtype, out, rest, lse, grad, dq, dk, dv, dbias, workspace, (cudaStream_t)stream);

@@ -54,6 +54,9 @@ constexpr int kMaxItems = 64;   // owned tiles a CTA takes at most
 
 template <int DP, bool DKV>
 __host__ __device__ constexpr int buffers() { return DKV && DP == 128 ? 2 : 3; }
+// barriers of the scores: a warpgroup pair waits for every other tile, and of each barrier it has to have seen the phase
+// before, or the parity would not tell the two apart; with three buffers that takes one for each buffer and pair
+__host__ __device__ constexpr int score_bars(int nb) { return nb == 2 ? 2 : 6; }
 
 template <int DP, bool BIAS>
 struct Shape {
@@ -63,7 +66,7 @@ struct Shape {
     static constexpr int kStage = 2 * kY + 1024;                  // keeps the tiles at 1024-byte boundaries
     static constexpr int kOwned = DP == 64 ? 2 : 1;                          // owned tiles in shared memory: the next one's copies early
     static constexpr int kStages = DP == 64 ? 6 : BIAS ? 3 : 4;              // (the bias by position takes up to 35 KB)
-    static constexpr int kBars = 2 * kOwned + 2 + 2 * kStages + 9;
+    static constexpr int kBars = 2 * kOwned + 2 + 2 * kStages + 12;
     static constexpr size_t kTiles = 2 * (size_t)kOwned * kX + (size_t)kStages * kStage;
     static constexpr size_t fixed() { return 1024 + kTiles + kBars * 8 + 32 + kMaxItems * 24; }
 };
@@ -123,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const __grid_constant__ CUtensorMap tmY1, const __grid_constant__ CUtensorMap tmY2,
                     const __grid_constant__ Args g) {
     using Sh = Shape<DP, BIAS>;
-    constexpr int NST = Sh::kStages, NB = buffers<DP, DKV>(), NX = Sh::kOwned;
+    constexpr int NST = Sh::kStages, NB = buffers<DP, DKV>(), NS = score_bars(NB), NX = Sh::kOwned;
     const AttnArgs& a = g.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int hx = blockIdx.x, group = a.H / a.Hkv;
@@ -136,7 +139,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t sY = base + 2 * NX * Sh::kX;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(gb + Sh::kTiles);
     const uint32_t barX = smem_addr(bars), barXE = barX + 8 * NX, barF = barXE + 8 * NX, barA = barF + 8, barY = barA + 8,
-                   barE = barY + 8 * NST, barS = barE + 8 * NST, barP = barS + 24, barPE = barP + 24;
+                   barE = barY + 8 * NST, barS = barE + 8 * NST, barP = barS + 8 * NS, barPE = barP + 24;
     uint8_t* const after = gb + (Sh::kTiles + Sh::kBars * 8 + 15) / 16 * 16;
     volatile int* const dead = reinterpret_cast<volatile int*>(after);
     uint32_t* const slot = reinterpret_cast<uint32_t*>(after) + 1;
@@ -180,7 +183,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int s = 0; s < NX; ++s) bar_init(barX + 8 * s, 1), bar_init(barXE + 8 * s, 1);
             bar_init(barF, 1), bar_init(barA, kWork / 32);
             for (int s = 0; s < NST; ++s) bar_init(barY + 8 * s, 1), bar_init(barE + 8 * s, 1);
-            for (int s = 0; s < NB; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 8), bar_init(barPE + 8 * s, 1);
+            for (int s = 0; s < NS; ++s) bar_init(barS + 8 * s, 1);
+            for (int s = 0; s < NB; ++s) bar_init(barP + 8 * s, 8), bar_init(barPE + 8 * s, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
             *dead = 0;
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int k = 0; k < DP / 16; ++k)
                     if (lead && k < steps) mma_ss(d + 64 * w, dX + (w * Sh::kX + (k / 4) * kChunkX + (k % 4) * 32) / 16,
                                      dY + (w * Sh::kY + (k / 4) * kChunkY + (k % 4) * 32) / 16, idS, k != 0);
-            if (lead) tc_commit(barS + 8 * buf);
+            if (lead) tc_commit(barS + 8 * (t % NS));
             return true;
         };
         if (kApart && warp == kWork / 32) {
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // (after a wait that gave up a warp still meets its partners at the barriers above)
                     // (the streamed tile's own barrier: the keys pass reads the row statistics that came with it)
                     ok = ok && (!DKV || bar_wait_warp(barY + 8 * s, (t / NST) & 1, dead)) &&
-                         bar_wait_warp(barS + 8 * buf, (t / NB) & 1, dead);
+                         bar_wait_warp(barS + 8 * (t % NS), (t / NS) & 1, dead);
                     if (!ok) continue;
                     tc_fence_after();
                     const int col0 = 32 * half, yc = yb + col0;

@@ -13,7 +13,6 @@ namespace d2pb {
 namespace enc {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
 template <class T>
 __device__ __forceinline__ float to_f(T v);

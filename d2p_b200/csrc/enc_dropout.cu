@@ -116,6 +116,7 @@ extern "C" int d2p_dropout_add(const void* x, const void* residual, int dtype, u
     if (!(p >= 0.0 && p < 1.0)) return D2P_ERR_INVALID_ARGUMENT;
     if (n == 0) return D2P_OK;
     if (!x || !y) return D2P_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)x | (uintptr_t)residual | (uintptr_t)y) & (dtype == D2P_DTYPE_F32 ? 3 : 1)) return D2P_ERR_INVALID_ARGUMENT;
     static DeviceSetup setup;
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);

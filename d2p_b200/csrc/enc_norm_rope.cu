@@ -187,7 +187,7 @@ __global__ void __launch_bounds__(kThreadsNR, sizeof(T) == 4 ? 1 : 2) norm_rope_
             const long long db = dtok / a.L;
             const long long hs = a.xs[part][2];
             const T *px, *pg;   // the row asked for next
-            bool live, ahead;   // whether this unit, and the one asked for, is one there is
+            bool live, ahead, there;   // whether this unit, and the one asked for, is one there is; this lane's, and any
             auto seek = [&]() {
                 ahead = on && b < a.B;
                 const long long tok = b * a.L + l;
@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kThreadsNR, sizeof(T) == 4 ? 1 : 2) norm_rope_
                 }
                 const int h0 = set * span;
                 T* py = (T*)a.y[part] + ((b * a.L + l) * H + h0) * a.D;
-                live = ahead;
+                live = ahead, there = b < a.B;
                 for (int k = 0; k < span; ++k, py += a.D) {
                     xs = nx;
                     gs = ng;
@@ -246,7 +246,8 @@ __global__ void __launch_bounds__(kThreadsNR, sizeof(T) == 4 ? 1 : 2) norm_rope_
                     float q = 0.f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) q = fmaf(x[i], x[i], q);
-                    const float r = rsqrtf(group_sum<G>(q) * invD + a.eps);
+                    // (a place without a row adds nothing to dw, with eps = 0 too)
+                    const float sq = group_sum<G>(q), r = there && h0 + k < H ? rsqrtf(sq * invD + a.eps) : 0.f;
                     float g[16];
                     gs.get(g);
                     float dot = 0.f;
@@ -374,6 +375,13 @@ static int norm_rope_check(const d2p_norm_rope_args* p) {
     if (p->D < 16 || p->D > 256 || p->D % 16 || p->R < 0 || p->R > p->D || p->R % 16) return D2P_ERR_INVALID_ARGUMENT;
     if (p->R > 0 && (!p->cos || !p->sin || p->P <= 0)) return D2P_ERR_INVALID_ARGUMENT;
     if (!p->positions && p->R > 0 && p->L > p->P) return D2P_ERR_INVALID_ARGUMENT;
+    if (!(p->eps >= 0.f)) return D2P_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->q_weight | (uintptr_t)p->k_weight | (uintptr_t)p->cos | (uintptr_t)p->sin) & 15)
+        return D2P_ERR_INVALID_ARGUMENT;
+    if ((uintptr_t)p->positions & (p->positions_int64 ? 7 : 3)) return D2P_ERR_INVALID_ARGUMENT;
+    const int unit = p->dtype == D2P_DTYPE_F32 ? 4 : 8;
+    for (int i = 0; i < 3; ++i)
+        if (p->q_stride[i] % unit || p->k_stride[i] % unit) return D2P_ERR_INVALID_ARGUMENT;
     return D2P_OK;
 }
 static enc::NormRopeArgs norm_rope_args(const d2p_norm_rope_args* p) {
@@ -410,6 +418,7 @@ int d2p_norm_rope_forward(const d2p_norm_rope_args* p, void* q_out, void* k_out,
     if (p->B == 0 || p->L == 0 || (p->H == 0 && p->Hkv == 0)) return D2P_OK;
     if ((p->H && (!p->q || !q_out)) || (p->Hkv && (!p->k || !k_out)) || !p->q_weight || !p->k_weight)
         return D2P_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)q_out | (uintptr_t)k_out) & 15) return D2P_ERR_INVALID_ARGUMENT;
     int sms = 0;
     if ((rc = norm_rope_sms(&sms))) return rc;
     enc::NormRopeArgs a = norm_rope_args(p);
@@ -430,6 +439,7 @@ int d2p_norm_rope_backward(const d2p_norm_rope_args* p, const void* dq_out, cons
     if (!p->q_weight || !p->k_weight || !dq_weight || !dk_weight || !workspace) return D2P_ERR_INVALID_ARGUMENT;
     if (p->B && p->L && ((p->H && (!p->q || !dq_out || !dq)) || (p->Hkv && (!p->k || !dk_out || !dk))))
         return D2P_ERR_INVALID_ARGUMENT;
+    if (((uintptr_t)dq_out | (uintptr_t)dk_out | (uintptr_t)dq | (uintptr_t)dk | (uintptr_t)workspace) & 15) return D2P_ERR_INVALID_ARGUMENT;
     int sms = 0;
     if ((rc = norm_rope_sms(&sms))) return rc;
     enc::NormRopeArgs a = norm_rope_args(p);

@@ -73,12 +73,6 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* tm, in
         "l"((unsigned long long)tm), "r"(x), "r"(row), "r"(head), "r"(b), "r"(bar)
         : "memory");
 }
-__device__ __forceinline__ void tma_store(const CUtensorMap* tm, int x, int row, int head, int b, uint32_t src) {
-    asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
-                     (unsigned long long)tm),
-                 "r"(x), "r"(row), "r"(head), "r"(b), "r"(src)
-                 : "memory");
-}
 
 __device__ __forceinline__ void tmem_alloc(uint32_t slot, int columns) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");

@@ -24,9 +24,11 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/library.h>
 #include <torch/types.h>
 
+#include <algorithm>
 #include <limits>
 #include <vector>
 
@@ -1211,6 +1213,13 @@ using OptTensor = c10::optional<Tensor>;
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor undef(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+// gradients that are not themselves differentiable: with create_graph they carry a node that says so when it is reached
+tensor_list once(tensor_list grads, const tensor_list& from, const char* what) {
+    if (!at::GradMode::is_enabled() || std::none_of(from.begin(), from.end(), wants_grad)) return grads;
+    for (Tensor& g : grads)
+        if (g.defined()) g = g.detach().set_requires_grad(true);
+    return torch::autograd::DelayedError(std::string(what) + ": its gradients cannot be differentiated again", (int64_t)grads.size())(std::move(grads));
+}
 
 std::tuple<Tensor, Tensor, Tensor> call_attention_forward(const Tensor& q, const Tensor& k, const Tensor& v, const OptTensor& bias,
                                                   const OptTensor& lengths, at::IntArrayRef edges, double scale, bool causal,
@@ -1246,10 +1255,15 @@ class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
         auto s = ctx->get_saved_variables();
         const std::vector<int64_t> edges = ctx->saved_data["edges"].toIntVector();
         const bool want_bias = ctx->saved_data["want_bias"].toBool();
-        auto r = op.call(grads[0], s[0], s[1], s[2], opt(s[3]), opt(s[4]), edges, ctx->saved_data["scale"].toDouble(),
-                         ctx->saved_data["causal"].toBool(), s[5], s[6], opt(s[7]), want_bias);
-        return {std::get<0>(r), std::get<1>(r), std::get<2>(r), want_bias ? std::get<3>(r) : Tensor(),
-                Tensor(), Tensor(), Tensor(), Tensor()};
+        std::tuple<Tensor, Tensor, Tensor, Tensor> r;
+        {
+            at::AutoDispatchBelowADInplaceOrView guard;
+            r = op.call(grads[0], s[0], s[1], s[2], opt(s[3]), opt(s[4]), edges, ctx->saved_data["scale"].toDouble(),
+                        ctx->saved_data["causal"].toBool(), s[5], s[6], opt(s[7]), want_bias);
+        }
+        return once({std::get<0>(r), std::get<1>(r), std::get<2>(r), want_bias ? std::get<3>(r) : Tensor(),
+                     Tensor(), Tensor(), Tensor(), Tensor()},
+                    {grads[0], s[0], s[1], s[2], s[3]}, "attention");
     }
 };
 
@@ -1291,8 +1305,13 @@ class NormRopeFunction : public torch::autograd::Function<NormRopeFunction> {
                                  const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                                  const Tensor&, const Tensor&, const OptTensor&, double)>();
         auto s = ctx->get_saved_variables();
-        auto r = op.call(grads[0], grads[1], s[0], s[1], s[2], s[3], s[4], s[5], opt(s[6]), ctx->saved_data["eps"].toDouble());
-        return {std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), Tensor(), Tensor(), Tensor(), Tensor()};
+        std::tuple<Tensor, Tensor, Tensor, Tensor> r;
+        {
+            at::AutoDispatchBelowADInplaceOrView guard;
+            r = op.call(grads[0], grads[1], s[0], s[1], s[2], s[3], s[4], s[5], opt(s[6]), ctx->saved_data["eps"].toDouble());
+        }
+        return once({std::get<0>(r), std::get<1>(r), std::get<2>(r), std::get<3>(r), Tensor(), Tensor(), Tensor(), Tensor()},
+                    {grads[0], grads[1], s[0], s[1], s[2], s[3]}, "qk_norm_rope");
     }
 };
 
@@ -1313,6 +1332,8 @@ Tensor call_dropout(const Tensor& x, const OptTensor& residual, double p, int64_
     return op.call(x, residual, p, seed, offset);
 }
 
+Tensor dropout_add_autograd(const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset);
+
 class DropoutFunction : public torch::autograd::Function<DropoutFunction> {
    public:
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset) {
@@ -1325,10 +1346,10 @@ class DropoutFunction : public torch::autograd::Function<DropoutFunction> {
         return call_dropout(x, residual, p, seed, offset);
     }
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
-        Tensor dx;
+        Tensor dx;   // (linear in the gradient: the operator itself, differentiable as it is)
         if (ctx->saved_data["dx"].toBool())
-            dx = call_dropout(grads[0], OptTensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
-                              ctx->saved_data["offset"].toInt());
+            dx = dropout_add_autograd(grads[0], OptTensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
+                                      ctx->saved_data["offset"].toInt());
         return {dx, ctx->saved_data["dr"].toBool() ? grads[0] : Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };

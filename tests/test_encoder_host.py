@@ -175,6 +175,7 @@ def attention_args(**over):
     ({"scale": 0.0}, 1001), ({"scale": float("nan")}, 1001), ({"q": 4097}, 1001), ({"k": None}, 1001),
     ({"q_stride": (ctypes.c_longlong * 3)(512, 100, 64)}, 1001), ({"bias": 4096, "n_edges": 64}, 1001),
     ({"bias": 4096, "n_edges": 2, "bucket_edges": (ctypes.c_int * 2)(3, 2)}, 1001), ({"bias": 4096, "bias_dtype": 2}, 1001),
+    ({"lengths": 4098}, 1001), ({"bias": 4098}, 1001),
     ({"B": 70000}, 1003), ({"B": 0}, 0), ({"Lq": 0}, 0)])
 def test_c_abi_checks_attention(lib, over, code):
     f = lib.d2p_attention_forward
@@ -204,3 +205,31 @@ def test_c_abi_checks_outputs(lib):
     assert d(None, None, 0, 0, 0.5, 1, 1, None, None) == 0
     assert d(None, None, 0, 4, 0.5, 1, 1, None, None) == 1001
     assert d(None, None, 0, 0, 1.5, 1, 1, None, None) == 1001
+    assert d(4097, None, 1, 4, 0.5, 1, 1, 4096, None) == 1001                   # off an element's boundary
+    assert d(4096, None, 0, 4, 0.5, 1, 1, 4098, None) == 1001
+
+
+class NormRopeArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k")] + [("q_stride", ctypes.c_longlong * 3), ("k_stride", ctypes.c_longlong * 3)] + [
+        (n, ctypes.c_void_p) for n in ("q_weight", "k_weight", "cos", "sin", "positions")] + [("position_batch_stride", ctypes.c_longlong)] + [
+        (n, ctypes.c_int) for n in ("positions_int64", "P", "B", "L", "H", "Hkv", "D", "R", "dtype", "weight_dtype")] + [("eps", ctypes.c_float)]
+
+
+@pytest.mark.parametrize("over", [
+    {"D": 24}, {"D": 272}, {"R": 80}, {"R": 8}, {"L": 9}, {"cos": None}, {"q": 4104}, {"q_weight": 4100}, {"sin": 4104}, {"eps": -1.0},
+    {"eps": float("nan")}, {"q_stride": (ctypes.c_longlong * 3)(512, 132, 64)}, {"positions": 4098}, {"B": -1}])
+def test_c_abi_checks_norm_rope(lib, over):
+    a = NormRopeArgs(q=4096, k=4096, q_weight=4096, k_weight=4096, cos=4096, sin=4096, P=8, B=1, L=4, H=2, Hkv=1, D=64, R=64, dtype=1,
+                     weight_dtype=1, eps=1e-6)
+    for n in ("q_stride", "k_stride"):
+        setattr(a, n, (ctypes.c_longlong * 3)(512, 128, 64))
+    for n, v in over.items():
+        setattr(a, n, v)
+    f = lib.d2p_norm_rope_forward
+    f.restype = ctypes.c_int
+    f.argtypes = [ctypes.POINTER(NormRopeArgs)] + [ctypes.c_void_p] * 3
+    assert f(ctypes.byref(a), 4096, 4096, None) == 1001
+    b = lib.d2p_norm_rope_backward
+    b.restype = ctypes.c_int
+    b.argtypes = [ctypes.POINTER(NormRopeArgs)] + [ctypes.c_void_p] * 7 + [ctypes.c_size_t, ctypes.c_void_p]
+    assert b(ctypes.byref(a), *[4096] * 7, 1 << 30, None) == 1001

@@ -286,6 +286,37 @@ def test_attention_strided_views(d2p, cuda_device):
     assert torch.equal(out, d2p.attention(*c, causal=True))
 
 
+def test_attention_of_broadcast_inputs(d2p, cuda_device):
+    """Keys and values expanded over the batch and over heads: copied, and their gradients summed where they came from."""
+    q, k, v, do, bias = inputs(3, 70, 90, 4, 2, 64, torch.bfloat16, cuda_device, 8)
+    k1, v1 = k[:1, :, :1].clone().requires_grad_(True), v[:1, :, :1].clone().requires_grad_(True)
+    d2p.attention(q, k1.expand_as(k), v1.expand_as(v), bias=bias.clone().requires_grad_(True)).backward(do)   # (as below)
+    got = run_attention(d2p, q, k1.detach().expand_as(k).contiguous(), v1.detach().expand_as(v).contiguous(), do, bias, None, False)
+    for leaf, name in ((k1, "dk"), (v1, "dv")):   # (a sum of six bf16 terms, itself rounded once or per axis)
+        want = got[name].double().sum((0, 2), keepdim=True)
+        mag = got[name].double().abs().sum((0, 2), keepdim=True)
+        assert ((leaf.grad.double() - want).abs() <= 2 * U[torch.bfloat16] * mag + 1e-7).all()
+
+
+def test_second_derivatives(d2p, cuda_device):
+    """Attention's and the norms' gradients say that they are not differentiable; dropout's is the operator itself."""
+    q, k, v, do, _ = inputs(1, 20, 20, 2, 2, 64, torch.bfloat16, cuda_device)
+    leaf = q.clone().requires_grad_(True)
+    (dq,) = torch.autograd.grad(d2p.attention(leaf, k, v), leaf, do, create_graph=True)
+    assert torch.equal(dq.detach(), run_attention(d2p, q, k, v, do, None, None, False)["dq"])
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        dq.float().sum().backward()
+    w, ang = torch.ones(64, device=cuda_device), torch.rand(20, 32, device=cuda_device)
+    (dq,) = torch.autograd.grad(d2p.qk_norm_rope(leaf, k, w.bfloat16(), w.bfloat16(), ang.cos(), ang.sin())[0], leaf, do, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        dq.float().sum().backward()
+    x, g = torch.randn(999, device=cuda_device, requires_grad=True), torch.randn(999, device=cuda_device, requires_grad=True)
+    y = d2p.dropout_add(x, None, 0.3, 5)
+    (dx,) = torch.autograd.grad(y, x, g, create_graph=True)
+    (dg,) = torch.autograd.grad(dx, g, x.detach())
+    assert torch.equal(dg, y.detach())
+
+
 def test_attention_is_repeatable(d2p, cuda_device):
     q, k, v, do, bias = inputs(4, 500, 480, 4, 2, 64, torch.bfloat16, cuda_device, 32)
     a = run_attention(d2p, q, k, v, do, bias, None, False)
@@ -492,6 +523,24 @@ def test_qk_norm_rope_positions_are_held_in_the_table(d2p, cuda_device):
     assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
     e = d2p.qk_norm_rope(q[:, :0], q[:, :0], w, w, ang.cos(), ang.sin())
     assert e[0].shape == (1, 0, 2, 32)
+
+
+@pytest.mark.parametrize("B,L,H,Hkv", [(1, 3, 2, 1), (2, 7, 3, 2), (40, 300, 6, 5)])
+def test_qk_norm_rope_without_eps(d2p, cuda_device, B, L, H, Hkv):
+    """With eps = 0 a group of threads without a row would divide by zero: the weights' gradients take nothing from it."""
+    g = torch.Generator().manual_seed(L)
+    D = 48
+    x = [torch.randn(B, L, h, D, generator=g).to(torch.bfloat16).to(cuda_device).requires_grad_(True) for h in (H, Hkv)]
+    w = [torch.rand(D, generator=g).to(cuda_device).requires_grad_(True) for _ in range(2)]
+    ang = torch.rand(L, 8, generator=g).to(cuda_device)
+    y = d2p.qk_norm_rope(*x, *w, ang.cos(), ang.sin(), eps=0.0)
+    gr = [torch.randn(B, L, h, D, generator=g).to(torch.bfloat16).to(cuda_device) for h in (H, Hkv)]
+    torch.autograd.backward(y, gr)
+    pos = torch.arange(L, device=cuda_device).expand(B, L)
+    for i in range(2):   # (tolerances: test_qk_norm_rope's)
+        ref = rope_reference(x[i].detach(), w[i].detach(), ang.cos(), ang.sin(), pos, 0.0, gr[i])
+        assert ((x[i].grad.double() - ref[2]).abs() <= U[torch.bfloat16] * ref[2].abs() + 4e-6 * ref[3] + 1e-7).all()
+        assert ((w[i].grad.double() - ref[4]).abs() <= U[torch.float32] * ref[4].abs() + 4e-6 * ref[5] + 1e-7).all()
 
 
 def test_qk_norm_rope_zero_rows_and_empty_batches(d2p, cuda_device):
