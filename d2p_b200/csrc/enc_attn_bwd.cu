@@ -421,6 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         else c1 = min(c1, 1 - d0);
                     }
                     const bool edge = __any_sync(0xffffffffu, c0 > 0 || c1 < 32);
+                    bool live_block = true;
                     float run = 0.f, all = 0.f;   // the diagonals under way; the sum of a block in one bucket
                     // (forms without the masks and without the bias by position: a block needs them rarely)
                     auto block = [&](auto edge_c, auto near_c) {
@@ -483,7 +484,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (DKV) tmem_st16(tS + col0, sv);
                         tmem_st16(tD + col0, dv);
                     };
-                    if (BIAS && near) {
+                    if (!__any_sync(0xffffffffu, c0 < c1)) {   // the whole block masked: zeros, whatever S holds
+                        uint32_t zero[16];
+#pragma unroll
+                        for (int y = 0; y < 16; ++y) zero[y] = 0u;
+                        if (DKV) tmem_st16(tS + col0, zero);
+                        tmem_st16(tD + col0, zero);
+                        live_block = false;
+                    } else if (BIAS && near) {
                         if (edge) block(std::true_type{}, std::true_type{});
                         else block(std::false_type{}, std::true_type{});
                     } else {
@@ -504,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     tc_fence_before();
                     bar_arrive_warp(barP + 8 * buf);
                     if (kept_b >= 0) store();   // the item before
-                    if (sums) {
+                    if (sums && live_block) {
                         if (near) {
                             dw[62 - lane] = run;   // the diagonals still under way; lane 31's is in place
                             __syncwarp();

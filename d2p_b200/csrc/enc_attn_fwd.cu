@@ -215,20 +215,20 @@ __global__ void __launch_bounds__(kThreads, 2)
         } else if (warp == 7) {
             const uint32_t idO = mma_desc<T>(128, 16 * steps, true);
             for (int e = 0; ok && e < count; ++e) {
-                const int n = (int)uniform(tiles[e]);
+                const int n = (int)uniform(tiles[e]), lk = (int)uniform(entry[e].w);
                 if (n == 0) continue;
                 for (int j = 0; j < n; ++j, ++t) {
-                    const int s = t % NST, buf = t % NB;
+                    const int s = t % NST, buf = t % NB, ks = lk - j * KT <= KT / 2 ? KT / 32 : KT / 16;   // steps with keys
                     if (!(ok = bar_wait_warp(barV + 8 * s, (t / NST) & 1, dead) && bar_wait_warp(barP + 8 * buf, (t / NB) & 1, dead))) break;
                     tc_fence_after();
                     const uint32_t dV = desc_down(sV + s * Sh::kTileKV, Sh::kChunkKV), p = uP + buf * KT;
 #pragma unroll
                     for (int k = 0; k < KT / 16; ++k)
-                        if (lead) mma_ts(uO, p + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
+                        if (lead && k < ks) mma_ts(uO, p + 8 * k, dV + k * (2048 / 16), idO, (j | k) != 0);
                     if (REST) {
 #pragma unroll
                         for (int k = 0; k < KT / 16; ++k)
-                            if (lead) mma_ts(uO, p + KT / 2 + 8 * k, dV + k * (2048 / 16), idO, true);
+                            if (lead && k < ks) mma_ts(uO, p + KT / 2 + 8 * k, dV + k * (2048 / 16), idO, true);
                     }
                     if (lead) tc_commit(barPE + 8 * buf), tc_commit(barVE + 8 * s);
                 }
@@ -308,6 +308,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 if (!(ok = bar_wait_warp(barS + 8 * buf, (tt / NB) & 1, dead))) break;
                 tc_fence_after();
                 constexpr int kBlocks = KT / 32;
+                const bool half = lk - k0 <= KT / 2;   // no key in the tile's second half: left out, here and in the product
                 uint32_t v[KT];
 #pragma unroll
                 for (int x = 0; x < kBlocks; ++x) tmem_ld32(tS + 32 * x, v + 32 * x);
@@ -330,6 +331,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     const int dmin = __shfl_sync(0xffffffffu, k0 - (w.q0 + 32 * warp + 31 + w.off), 0);   // of the warp's 32 rows and the first 32 keys
 #pragma unroll
                     for (int x = 0; x < kBlocks; ++x) {
+                        if (2 * x >= kBlocks && half) break;
                         const int lo = dmin + 32 * x;
                         add[x] = lo >= reach ? after : before, mul[x] = lo >= reach ? mul_after : mul_before;
                         if (lo < reach && lo + 62 > -reach) {
@@ -351,6 +353,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 float top = -INFINITY;
 #pragma unroll
                 for (int x = 0; x < kBlocks; ++x) {
+                    if (2 * x >= kBlocks && half) break;
                     float mx = fmaxf(t[32 * x], t[32 * x + 1]), my = fmaxf(t[32 * x + 2], t[32 * x + 3]);
 #pragma unroll
                     for (int y = 32 * x + 4; y < 32 * x + 32; y += 4)
@@ -389,6 +392,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 Two sum[2] = {Two(0.f, 0.f), Two(0.f, 0.f)};
 #pragma unroll
                 for (int x = 0; x < KT; x += 32) {
+                    if (2 * x >= KT && half) break;
                     uint32_t p[16], p2[16];
                     const Two u(mul[x / 32], mul[x / 32]), v0(add[x / 32] - ref, add[x / 32] - ref);
 #pragma unroll
