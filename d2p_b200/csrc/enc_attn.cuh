@@ -48,21 +48,42 @@ __device__ __forceinline__ void problem_lengths(const AttnArgs& a, int b, int* l
 // the softmax's running reference is raised when a row's maximum passes it by
 // more than kSlack (2^kSlack stays in range of the 16-bit types)
 template <class T>
-struct Softmax {   // fp16: probabilities start at 2^8, so that small ones stay above its subnormals
-    static constexpr float kShift = 0.f, kSlack = 8.f;
+struct Softmax {   // fp16: probabilities are held 2^8 times as large, so that small ones stay above its subnormals
+    static constexpr float kShift = 0.f, kSlack = 8.f, kDown = 1.f;   // kDown: 2^-kShift
 };
 template <>
 struct Softmax<__half> {
-    static constexpr float kShift = 8.f, kSlack = 7.f;
+    static constexpr float kShift = 8.f, kSlack = 7.f, kDown = 1.f / 256.f;
 };
 
 // checks of the C entry points; fills *a
 int attn_args(const d2p_attention_args* p, AttnArgs* a);
+// Where rows are few and keys many, the keys are split and the splits' results joined by a second launch.  Of split s,
+// row i of head h: sum of p v at o + set D, with set = ((b H + h) splits + s) Lq + i, its reference and sum of p in ml[set]
+constexpr int kMaxParts = 64;
+struct Parts {
+    float* o;
+    float2* ml;
+    int splits;                   // 1: no splits, results written at once
+    __host__ __device__ size_t set(const AttnArgs& a, int b, int h, int s, int i) const {
+        return (((size_t)b * a.H + h) * splits + s) * a.Lq + i;
+    }
+};
+inline size_t parts_bytes(const AttnArgs& a, int splits) {   // (rows of o stay at 16-byte boundaries)
+    return splits > 1 ? (size_t)a.B * a.H * splits * a.Lq * (a.D * sizeof(float) + sizeof(float2)) : 0;
+}
+inline Parts parts_at(const AttnArgs& a, int splits, void* ws) {
+    Parts p = {(float*)ws, nullptr, splits};
+    if (splits > 1) p.ml = (float2*)(p.o + (size_t)a.B * a.H * splits * a.Lq * a.D);
+    return p;
+}
+int attn_join(const AttnArgs& a, int dtype, const Parts& p, void* out, float* lse, void* rest, cudaStream_t st);
 // out, and lse and rest (what rounding took from out; null: not wanted) by tiles of 128 query rows (enc_attn_fwd.cu)
 int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st);
 size_t attn_forward_bytes(const AttnArgs& a);
 // the same for at most 16 query rows of a key head, split over the keys (enc_attn_token.cu)
-int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, cudaStream_t st);
+int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st);
+size_t attn_tokens_bytes(const AttnArgs& a);
 // the gradients (enc_attn_bwd.cu) and their workspace
 size_t attn_backward_bytes(const AttnArgs& a, bool dbias);
 int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const void* rest, const float* lse, const void* grad, void* dq,

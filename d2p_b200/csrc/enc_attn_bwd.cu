@@ -84,7 +84,7 @@ size_t smem_bytes(bool dkv, int reach) {
 
 struct Args {
     AttnArgs a;
-    const float* lse;      // [B, H, Lp] padded copies, negated: -inf and 0 in dead rows
+    const float* lse;      // [B, H, Lp] padded copies, negated: kShift - lse and -delta kDown; -inf and 0 in dead rows
     const float* delta;
     int Lp;
     void* dx1;             // keys pass: dv; query pass: unused
@@ -338,7 +338,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             ok = ok && bar_wait_warp(barF, (done - 1) & 1, dead);
             tc_fence_after();
             const bool row = kept_x < kept_l, first = DKV && pair == 0;
-            const float w = first ? 1.f : a.scale;
+            const float w = first ? Softmax<T>::kDown : a.scale;
             const int f0 = DKV ? half * (DP / 2) : (warp >> 2) * (DP / 4);
             constexpr int kCols = DKV ? DP / 2 : DP / 4;
             const uint32_t acc = (first ? tA1 : tA2) + trow;
@@ -458,8 +458,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int z = 0; z < 4; ++z) pv[z] = ex2(pv[z]);
                             const Two d0(__uint_as_float(dv[y]), __uint_as_float(dv[y + 1])), d1(__uint_as_float(dv[y + 2]), __uint_as_float(dv[y + 3]));
-                            mul2(Two(pv[0], pv[1]), add2(d0, Two(E.x, E.y))).get(gv, gv + 1);
-                            mul2(Two(pv[2], pv[3]), add2(d1, Two(E.z, E.w))).get(gv + 2, gv + 3);
+                            // (P is 2^kShift times as large here, dS is as it is)
+                            const Two w(Softmax<T>::kDown, Softmax<T>::kDown), E0(E.x, E.y), E1(E.z, E.w);
+                            mul2(Two(pv[0], pv[1]), Softmax<T>::kShift == 0.f ? add2(d0, E0) : fma2(d0, w, E0)).get(gv, gv + 1);
+                            mul2(Two(pv[2], pv[3]), Softmax<T>::kShift == 0.f ? add2(d1, E1) : fma2(d1, w, E1)).get(gv + 2, gv + 3);
 #pragma unroll
                             for (int z = 0; z < 4; ++z) {
                                 const int col = y + z;
@@ -579,7 +581,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == kWork / 32) tmem_free(tmem, kColumns);
 }
 
-// -delta = -rowsum(dO O) and -lse in rows padded to whole tiles: 0 and -inf where no key is met.  O with what its
+// -delta = -rowsum(dO O) (times kDown) and kShift - lse in rows padded to whole tiles: 0 and -inf where no key is met.  O with what its
 // rounding took, where it is there.  A block takes 16
 // positions of up to 8 heads: rows are read as they lie, heads of a position together, and the sums leave by head, 16
 // positions together.  LANES threads a row
@@ -619,8 +621,8 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
     const int h = threadIdx.x / kStatRows, i = i0 + threadIdx.x % kStatRows;
     if (h < heads && h < kStatHeads) {
         const size_t at = ((size_t)b * a.H + h0 + h) * Lp + i;
-        dp[at] = -sum[h][threadIdx.x % kStatRows];
-        lp[at] = i < lq ? -lse[((size_t)b * a.H + h0 + h) * a.Lq + i] : -INFINITY;
+        dp[at] = -sum[h][threadIdx.x % kStatRows] * Softmax<T>::kDown;
+        lp[at] = i < lq ? Softmax<T>::kShift - lse[((size_t)b * a.H + h0 + h) * a.Lq + i] : -INFINITY;
     }
 }
 

@@ -74,7 +74,7 @@ template <class T, int DP, bool BIAS, bool REST>
 __global__ void __launch_bounds__(kThreads, 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs a, T* __restrict__ out,
-                    float* __restrict__ lse, T* __restrict__ rest, const int* __restrict__ order) {
+                    float* __restrict__ lse, T* __restrict__ rest, const int* __restrict__ order, const __grid_constant__ Parts part) {
     using Sh = Shape<DP, REST>;
     constexpr int NST = Sh::kStages, NB = Sh::kBuffers, KT = Sh::kKeys;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -93,6 +93,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     uint8_t* const after_bars = gbase + (Sh::kTiles + Sh::kBars * 8 + 15) / 16 * 16;
     volatile int* const dead = reinterpret_cast<volatile int*>(after_bars);
     uint32_t* const slot = reinterpret_cast<uint32_t*>(after_bars) + 1;
+    int* const from = reinterpret_cast<int*>(after_bars) + 2;                // this split's first key tile
     int4* const entry = reinterpret_cast<int4*>(after_bars + 16);            // b, q0, lq, lk of an item
     int* const tiles = reinterpret_cast<int*>(entry + kMaxItems);            // and the key tiles that its rows meet
     float* const lut = reinterpret_cast<float*>(tiles + kMaxItems);
@@ -104,6 +105,12 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
         for (int c = 0; c < Sh::kChunks; ++c) tma_load(dst + c * chunk, tm, 64 * c, row, head, b, bar);
     };
+    // this split's part of an item's key tiles: the first, how many (a CTA of a split takes one item)
+    auto share = [&](int n) {
+        if (part.splits == 1) return make_int2(0, n);
+        const int per = (n + part.splits - 1) / part.splits, t = min(n, (int)blockIdx.z * per);
+        return make_int2(t, min(per, n - t));
+    };
     if (warp == 5) {
         if (lane == 0) {
             bar_init(barQ, 1), bar_init(barQE, 1), bar_init(barR, 4);
@@ -114,10 +121,12 @@ __global__ void __launch_bounds__(kThreads, 2)
             fence_async_smem();
             *dead = 0;
             const Item w = item_at<KT>(a, order, item_index(0, blockIdx.y, gridDim.y), row_tiles);   // the first item's Q and first tile before the CTA meets
-            if (w.tiles) {
+            const int2 r = share(w.tiles);
+            *from = r.x;
+            if (r.y) {
                 load(sQ, &tmQ, w.q0, h, w.b, barQ, kChunk);
-                load(sK, &tmK, 0, kh, w.b, barK, Sh::kChunkKV);
-                load(sV, &tmV, 0, kh, w.b, barV, Sh::kChunkKV);
+                load(sK, &tmK, r.x * KT, kh, w.b, barK, Sh::kChunkKV);
+                load(sV, &tmV, r.x * KT, kh, w.b, barV, Sh::kChunkKV);
             }
         }
         __syncwarp();
@@ -127,7 +136,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         for (int e = warp < 4 ? tid : tid - 64; e < count; e += 192) {
             const Item w = item_at<KT>(a, order, item_index(e, blockIdx.y, gridDim.y), row_tiles);
             entry[e] = make_int4(w.b, w.q0, w.lq, w.lk);
-            tiles[e] = w.tiles;
+            tiles[e] = share(w.tiles).y;
         }
         __syncwarp();
         if (BIAS) fill_lut<T>(lut, a, h, reach, warp < 4 ? warp : warp - 2, 6);
@@ -144,6 +153,10 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (tiles[e]) continue;
             const int4 w = entry[e];
             const int rows = min(kRows, a.Lq - w.y), units = a.D / 8;
+            if (part.splits > 1) {
+                for (int x = lane; x < rows; x += 32) part.ml[part.set(a, w.x, h, blockIdx.z, w.y + x)] = make_float2(-INFINITY, 0.f);
+                continue;
+            }
             for (int x = lane; x < rows * units; x += 32) {
                 const size_t at = (((size_t)w.x * a.Lq + w.y + x / units) * a.H + h) * a.D + (x % units) * 8;
                 *reinterpret_cast<uint4*>(out + at) = make_uint4(0, 0, 0, 0);
@@ -155,6 +168,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     } else if (warp == 5) {   // copies
         if (lane == 0) {
             bool ok = true;
+            const int j0 = *from;
             int t = 0, q = 0;   // tiles and items asked for
             for (int i = 0; ok && i < count; ++i) {
                 const int n = tiles[i];
@@ -166,9 +180,9 @@ __global__ void __launch_bounds__(kThreads, 2)
                 for (int j = 0; j < n; ++j, ++t) {
                     const int s = t % NST;
                     if (t >= NST && !(ok = bar_wait(barKE + 8 * s, (t / NST - 1) & 1, dead))) break;
-                    if (i + j > 0) load(sK + s * Sh::kTileKV, &tmK, j * KT, kh, e.x, barK + 8 * s, Sh::kChunkKV);
+                    if (i + j > 0) load(sK + s * Sh::kTileKV, &tmK, (j0 + j) * KT, kh, e.x, barK + 8 * s, Sh::kChunkKV);
                     if (t >= NST && !(ok = bar_wait(barVE + 8 * s, (t / NST - 1) & 1, dead))) break;
-                    if (i + j > 0) load(sV + s * Sh::kTileKV, &tmV, j * KT, kh, e.x, barV + 8 * s, Sh::kChunkKV);
+                    if (i + j > 0) load(sV + s * Sh::kTileKV, &tmV, (j0 + j) * KT, kh, e.x, barV + 8 * s, Sh::kChunkKV);
                 }
             }
             if (!ok || *dead) {   // a wait gave up: what is in flight ends (bounded) before the CTA does
@@ -215,7 +229,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         } else if (warp == 7) {
             const uint32_t idO = mma_desc<T>(128, 16 * steps, true);
             for (int e = 0; ok && e < count; ++e) {
-                const int n = (int)uniform(tiles[e]), lk = (int)uniform(entry[e].w);
+                const int n = (int)uniform(tiles[e]), lk = (int)uniform(entry[e].w) - (int)uniform(*from) * KT;
                 if (n == 0) continue;
                 for (int j = 0; j < n; ++j, ++t) {
                     const int s = t % NST, buf = t % NB, ks = lk - j * KT <= KT / 2 ? KT / 32 : KT / 16;   // steps with keys
@@ -243,6 +257,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float c = a.scale * kLog2e;
         bool ok = true;
         int tt = 0;   // tiles so far
+        const int j0 = __shfl_sync(0xffffffffu, *from, 0);
         // the bias past the last edge on either side, and what multiplies the scores there: it is added last, and one so
         // large that it swallows the scores near the diagonal, where it is added first, has to do so there too (the
         // factor leaves a masked -inf what it is)
@@ -264,6 +279,25 @@ __global__ void __launch_bounds__(kThreads, 2)
             const int4 w = entry[kept];   // b, q0, lq, lk
             const int i = w.y + tid;
             const bool some = i < w.z && (kept_l > 0.f || kept_l != kept_l);
+            if (part.splits > 1) {   // sums as they are, for the join
+                const size_t set = part.set(a, w.x, h, blockIdx.z, min(i, a.Lq - 1));
+#pragma unroll 1
+                for (int x = 0; x < a.D; x += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(tO + trow + x, o);
+                    tmem_wait_ld();
+                    tmem_tie16(o);
+                    if (i < a.Lq) {
+#pragma unroll
+                        for (int y = 0; y < 16; y += 4)
+                            if (x + y < a.D) *reinterpret_cast<uint4*>(part.o + set * a.D + x + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
+                    }
+                }
+                if (i < a.Lq) part.ml[set] = !ok ? make_float2(0.f, NAN) : some ? make_float2(kept_m, kept_l) : make_float2(-INFINITY, 0.f);
+                tc_fence_before();
+                kept = -1;
+                return;
+            }
             const float s = !ok ? NAN : (some ? 1.f / kept_l : 0.f);
             const size_t at = (((size_t)w.x * a.Lq + i) * a.H + h) * a.D;
 #pragma unroll 1
@@ -303,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             const int pos = w.q0 + tid + w.off, lk = w.lk;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < w.tiles && ok; ++j, ++tt) {
-                const int k0 = j * KT, buf = tt % NB;
+                const int k0 = (j0 + j) * KT, buf = tt % NB;
                 const uint32_t tS = tmem + trow + buf * KT, tP = tmem + trow + Sh::kColP + buf * KT;
                 if (!(ok = bar_wait_warp(barS + 8 * buf, (tt / NB) & 1, dead))) break;
                 tc_fence_after();
@@ -446,6 +480,13 @@ long long stays(const AttnArgs& a, int sms) {
     if (items * a.H < 4 * places) return 0;
     return std::max<long long>(places > a.H ? places / a.H : 1, (items + kMaxItems - 1) / kMaxItems);
 }
+// splits of the keys where the row tiles leave half the places free or more, each at least 256 keys.  Below 1024 the
+// join costs what they save (2 x 512 x 512, 8 heads: 12.8 us whole, 15.9 split); 11 x 17 x 3766, 2 heads of 80: 54 us
+// whole, 14.6 split; 3 x 689 x 3951, 4 heads of 80: 57 and 31
+int splits_of(const AttnArgs& a, int sms) {
+    const long long ctas = (long long)a.B * ((a.Lq + kRows - 1) / kRows) * a.H, places = 2LL * sms;
+    return 2 * ctas > places || a.Lk < 1024 ? 1 : (int)std::min<long long>(std::min<long long>(places / ctas, a.Lk / 256), kMaxParts);
+}
 // whether its items are put in order first: lengths differ, and the shares with them (ragged, 180 us unordered)
 bool ordered(const AttnArgs& a, int sms) {
     return (a.lengths || a.causal) && stays(a, sms) && (long long)a.B * ((a.Lq + kRows - 1) / kRows) <= kMaxOrder;
@@ -485,8 +526,10 @@ int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void
         order = (int*)ws;
         attn_order_kernel<<<1, 1024, 0, st>>>(a, order);
     }
-    attn_fwd_kernel<T, DP, BIAS, REST><<<dim3(a.H, (unsigned)ctas), kThreads, smem, st>>>(q, k, v, a, (T*)out, lse, (T*)rest, order);
-    return (int)cudaGetLastError();
+    const Parts part = parts_at(a, splits_of(a, sms), ws);
+    attn_fwd_kernel<T, DP, BIAS, REST><<<dim3(a.H, (unsigned)ctas, part.splits), kThreads, smem, st>>>(q, k, v, a, (T*)out, lse, (T*)rest, order, part);
+    rc = (int)cudaGetLastError();
+    return rc || part.splits == 1 ? rc : attn_join(a, dtype, part, out, lse, rest, st);
 }
 
 template <class T>
@@ -534,6 +577,7 @@ size_t attn_forward_bytes(const AttnArgs& a) {
     static DeviceSetup setup;
     int dev = 0, sms = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || device_setup(setup, dev, [] { return 0; }, &sms)) return (size_t)-1;
+    if (fwd::splits_of(a, sms) > 1) return parts_bytes(a, fwd::splits_of(a, sms));
     return fwd::ordered(a, sms) ? (size_t)a.B * ((a.Lq + fwd::kRows - 1) / fwd::kRows) * sizeof(int) : 0;
 }
 int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {

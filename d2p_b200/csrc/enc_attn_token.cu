@@ -8,9 +8,13 @@
 // keys are split over the CTAs of a cluster and over a CTA's warps; a warp takes
 // 16 keys at a time through its own ring of shared memory (cp.async, so no
 // barrier in the loop) with a running maximum and sum, and the partial results
-// join in shared memory, then through the cluster's: one launch, no workspace,
+// join in shared memory, then through the cluster's (one launch, no workspace) or,
+// where there are more splits than a cluster holds, by a second launch; always in
 // a fixed order.
 #include <cooperative_groups.h>
+
+#include <algorithm>
+#include <type_traits>
 
 #include "enc_attn.cuh"
 
@@ -77,7 +81,7 @@ __device__ __forceinline__ int bucket_of(const Edges& e, int d) {
 
 template <class T, int DP, bool REST>
 __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_constant__ AttnArgs a, T* __restrict__ out,
-                                                                float* __restrict__ lse, T* __restrict__ rest) {
+                                                                float* __restrict__ lse, T* __restrict__ rest, const __grid_constant__ Parts part) {
     using Sh = Shape<DP>;
     constexpr int NST = Sh::kStages, CH = DP / 8;   // 16-byte units of a row
     extern __shared__ __align__(128) uint8_t sm[];
@@ -280,12 +284,17 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
         }
         if (splits == 1) {
             finish(r, d, x, y, top, sum);
+        } else if (part.o) {
+            const int i = r / G;
+            const size_t set = part.set(a, b, kh * G + r % G, split, i);
+            *reinterpret_cast<float2*>(part.o + set * a.D + d) = make_float2(x, y);
+            if (d == 0) part.ml[set] = make_float2(top, sum);
         } else {
             *reinterpret_cast<float2*>(jo + (kWarps * kRowsM + r) * kPitch + d) = make_float2(x, y);
             if (d == 0) jm[kWarps * kRowsM + r] = top, jl[kWarps * kRowsM + r] = sum;
         }
     }
-    if (splits == 1) return;
+    if (splits == 1 || part.o) return;
     cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
     // every CTA finishes its part of the rows from all the cluster's sets: their weights first, then the sums
@@ -307,8 +316,26 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
     cluster.sync();   // the sets are read from other CTAs
 }
 
+int resident(const AttnArgs& a) { return a.D <= 64 ? Shape<64>::kResident : Shape<128>::kResident; }
+// CTAs of a cluster that share a problem's keys
+int cluster_of(const AttnArgs& a, int sms) {
+    int splits = 1;
+    while (splits < kMaxSplits && (long long)a.B * a.Hkv * splits < (long long)resident(a) * sms && (long long)a.Lk > (long long)splits * kMinRounds * kWarps * kKeys)
+        splits *= 2;
+    return splits;
+}
+// more splits than a cluster holds, joined by a second launch: for long caches of few heads.  Clusters of 16 also find no
+// place for all at once.  One token, us by a cluster / by parts: 2 x 8 heads of 128, 27248 keys 71 / 42; 1 x 4 of 128, 32768
+// keys 38 / 18, 4096 keys 9.5 / 9.0; 11 x 2 of 64, 17687 keys 27.6 / 21.6; 1 x 2 of 64, 2900 keys 6.7 / 8.1
+int parts_of(const AttnArgs& a, int sms) {
+    if (a.Lk < 4096 || cluster_of(a, sms) < kMaxSplits) return 1;
+    const long long places = (long long)resident(a) * sms / ((long long)a.B * a.Hkv), most = a.Lk / (kMinRounds * kWarps * kKeys);
+    const long long n = std::min(std::min(places, most), (long long)kMaxParts);
+    return n > kMaxSplits ? (int)n : 1;
+}
+
 template <class T, int DP, bool REST>
-int launch(const AttnArgs& a, void* out, float* lse, void* rest, cudaStream_t st) {
+int launch(const AttnArgs& a, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
     using Sh = Shape<DP>;
     constexpr int smem = Sh::kRing > Sh::kJoin ? Sh::kRing : Sh::kJoin;
     static DeviceSetup setup;
@@ -323,27 +350,34 @@ int launch(const AttnArgs& a, void* out, float* lse, void* rest, cudaStream_t st
     if (rc) return rc;
     // CTAs for every place there is, as far as the keys go round; 32 x 16 heads of 64, 4096 keys: 105 us (5.1 TB/s) with
     // two CTAs a problem, 119 with one of larger steps; 8 x 8 heads of 128, 8192 keys: 63 us with places for all, 84 with twice as many
-    int splits = 1;
-    while (splits < kMaxSplits && (long long)a.B * a.Hkv * splits < (long long)Sh::kResident * sms && (long long)a.Lk > (long long)splits * kMinRounds * kWarps * kKeys)
-        splits *= 2;
+    const Parts part = parts_at(a, parts_of(a, sms), parts_of(a, sms) > 1 ? ws : nullptr);
+    const int splits = part.splits > 1 ? part.splits : cluster_of(a, sms);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(splits, a.Hkv, a.B), cfg.blockDim = dim3(32 * kWarps), cfg.dynamicSmemBytes = smem, cfg.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr, cfg.numAttrs = 1;
-    return (int)cudaLaunchKernelEx(&cfg, attn_token_kernel<T, DP, REST>, a, (T*)out, lse, (T*)rest);
+    cfg.attrs = attr, cfg.numAttrs = part.splits > 1 ? 0 : 1;
+    e = cudaLaunchKernelEx(&cfg, attn_token_kernel<T, DP, REST>, a, (T*)out, lse, (T*)rest, part);
+    if (e != cudaSuccess || part.splits == 1) return (int)e;
+    return attn_join(a, std::is_same<T, __half>::value ? D2P_DTYPE_F16 : D2P_DTYPE_BF16, part, out, lse, rest, st);
 }
 
 }  // namespace tok
 
 template <class T>
-static int pick_token(const AttnArgs& a, void* out, float* lse, void* rest, cudaStream_t st) {
-    if (a.D <= 64) return rest ? tok::launch<T, 64, true>(a, out, lse, rest, st) : tok::launch<T, 64, false>(a, out, lse, rest, st);
-    return rest ? tok::launch<T, 128, true>(a, out, lse, rest, st) : tok::launch<T, 128, false>(a, out, lse, rest, st);
+static int pick_token(const AttnArgs& a, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
+    if (a.D <= 64) return rest ? tok::launch<T, 64, true>(a, out, lse, rest, ws, st) : tok::launch<T, 64, false>(a, out, lse, rest, ws, st);
+    return rest ? tok::launch<T, 128, true>(a, out, lse, rest, ws, st) : tok::launch<T, 128, false>(a, out, lse, rest, ws, st);
 }
-int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, cudaStream_t st) {
-    return dtype == D2P_DTYPE_BF16 ? pick_token<__nv_bfloat16>(a, out, lse, rest, st) : pick_token<__half>(a, out, lse, rest, st);
+int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
+    return dtype == D2P_DTYPE_BF16 ? pick_token<__nv_bfloat16>(a, out, lse, rest, ws, st) : pick_token<__half>(a, out, lse, rest, ws, st);
+}
+size_t attn_tokens_bytes(const AttnArgs& a) {
+    static DeviceSetup setup;
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || device_setup(setup, dev, [] { return 0; }, &sms)) return (size_t)-1;
+    return parts_bytes(a, tok::parts_of(a, sms));
 }
 
 }  // namespace enc

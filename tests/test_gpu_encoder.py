@@ -170,6 +170,33 @@ def test_attention_and_gradients(d2p, cuda_device, case):
     compare(run_attention(d2p, q, k, v, do, bias, lengths, causal, md), val, tol)
 
 
+SPLIT = [   # few rows and many keys: the keys split over CTAs, the splits' results joined
+    (2, 40, 3000, 2, 1, 64, BF, True, 32, 128, [[40, 3000], [17, 700]]),
+    (1, 130, 2500, 2, 2, 128, FP, False, 16, 64, [[130, 2100]]),
+    (1, 300, 4000, 1, 1, 64, FP, True, 0, 128, None),
+    (2, 90, 1030, 4, 4, 80, BF, False, 0, 128, [[90, 1030], [40, 1]]),
+    (3, 1, 9000, 4, 2, 64, BF, True, 16, 200, [[1, 9000], [1, 300], [0, 5]]),
+    (1, 2, 20000, 4, 1, 128, FP, False, 0, 128, None),
+    (2, 1, 5000, 3, 3, 40, BF, True, 32, 64, [[1, 4999], [1, 0]]),
+]
+
+
+@pytest.mark.parametrize("case", SPLIT, ids=["-".join(str(x).replace("torch.", "") for x in c[:9]) for c in SPLIT])
+def test_attention_split_keys(d2p, cuda_device, case):
+    B, Lq, Lk, H, Hkv, D, dtype, causal, nb, dist, lengths = case
+    q, k, v, do, bias = inputs(B, Lq, Lk, H, Hkv, D, dtype, cuda_device, nb, seed=Lk)
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device=cuda_device)
+    if lengths is not None:
+        for b, (lq, lk) in enumerate(lengths):   # what lies outside is never used
+            q[b, lq:], do[b, lq:], k[b, lk:], v[b, lk:] = math.nan, math.nan, math.inf, math.nan
+    val, tol = reference(q, k, v, bias, ln, causal, D ** -0.5, dist, do)
+    got = run_attention(d2p, q, k, v, do, bias, ln, causal, dist)
+    compare(got, val, tol)
+    alone = d2p.attention(q, k, v, bias=bias, lengths=ln, causal=causal, max_distance=dist)
+    compare({"out": alone}, val, tol)
+    assert torch.equal(alone, d2p.attention(q, k, v, bias=bias, lengths=ln, causal=causal, max_distance=dist))
+
+
 def test_reference_gradients_by_differences(cuda_device):
     """The fp64 formulas the gradients are judged by, against central differences of the fp64 output."""
     q, k, v, do, bias = inputs(1, 6, 7, 2, 1, 8, torch.bfloat16, cuda_device, 8, seed=3)
