@@ -38,6 +38,13 @@ int attn_args(const d2p_attention_args* p, AttnArgs* a) {
     return D2P_OK;
 }
 
+int attn_sms(int* sms) {
+    static DeviceSetup setup;
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    return e != cudaSuccess ? (int)e : device_setup(setup, dev, [] { return 0; }, sms);
+}
+
 // The splits' sums in a fixed order, each in the frame of the largest reference: WARPS warps a row, each every WARPS-th
 // split, four elements a lane.  Eight where there are many splits, whose loads would follow one another
 template <class T, int WARPS>
@@ -133,7 +140,6 @@ int d2p_attention_forward(const d2p_attention_args* p, void* out, float* lse, vo
     if (rc) return rc;
     if (a.B == 0 || a.Lq == 0) return D2P_OK;
     if (!out || (((uintptr_t)out | (uintptr_t)rest | (uintptr_t)workspace) & 15) || ((uintptr_t)lse & 3)) return D2P_ERR_INVALID_ARGUMENT;
-    if (rest && !a.bias) return D2P_ERR_INVALID_ARGUMENT;
     const size_t need = few_rows(a) ? enc::attn_tokens_bytes(a) : enc::attn_forward_bytes(a);
     if (need && (!workspace || workspace_bytes < need)) return D2P_ERR_WORKSPACE_TOO_SMALL;
     if (few_rows(a)) return enc::attn_forward_tokens(a, p->dtype, out, lse, rest, workspace, (cudaStream_t)stream);

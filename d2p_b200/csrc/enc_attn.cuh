@@ -56,6 +56,8 @@ struct Softmax<__half> {
     static constexpr float kShift = 8.f, kSlack = 7.f, kDown = 1.f / 256.f;
 };
 
+// SMs of the current device
+int attn_sms(int* sms);
 // checks of the C entry points; fills *a
 int attn_args(const d2p_attention_args* p, AttnArgs* a);
 // Where rows are few and keys many, the keys are split and the splits' results joined by a second launch.  Of split s,

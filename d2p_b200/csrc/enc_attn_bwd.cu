@@ -28,7 +28,8 @@
 // The bias's gradient sums dS over many rows, and a row's dS sum to nothing: what
 // delta is off by would show there whole where one bucket holds most of a row's
 // weight (1 % of the sum with delta from the plain output).  For it the forward
-// forms O from P in twice 16 bits and keeps what rounding O took.
+// forms O from P in twice 16 bits and keeps what rounding O took.  Without a bias
+// it keeps the latter alone: short rows' dQ and dK are off by a sixth less.
 //
 // The query pass also sums dS by relative position.  Along a diagonal of a
 // warp's 32 x 32 block the sum moves one lane per column (one shuffle each), the
@@ -760,23 +761,16 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
 
 int attn_backward_gave_up(unsigned long long* n) { return (int)cudaMemcpyFromSymbol(n, g_gave_up, sizeof(*n)); }
 
-static int sms_of(int* sms) {
-    static DeviceSetup setup;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e != cudaSuccess) return (int)e;
-    return device_setup(setup, dev, [] { return 0; }, sms);
-}
 size_t attn_backward_bytes(const AttnArgs& a, bool dbias) {
     int sms = 0;
-    if (sms_of(&sms)) return (size_t)-1;
+    if (attn_sms(&sms)) return (size_t)-1;
     return (2 * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a, sms) : 0) + bwd::order_ints(a, true, sms) +
             bwd::order_ints(a, false, sms)) * sizeof(float);
 }
 int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const void* rest, const float* lse, const void* grad, void* dq,
                         void* dk, void* dv, void* dbias, void* ws, cudaStream_t st) {
     int sms = 0;
-    const int rc = sms_of(&sms);
+    const int rc = attn_sms(&sms);
     if (rc) return rc;
     return dtype == D2P_DTYPE_BF16 ? bwd::run<__nv_bfloat16>(a, dtype, out, rest, lse, grad, dq, dk, dv, dbias, ws, sms, st)
                                    : bwd::run<__half>(a, dtype, out, rest, lse, grad, dq, dk, dv, dbias, ws, sms, st);

@@ -70,7 +70,9 @@ __device__ __forceinline__ Item item_at(const AttnArgs& a, const int* order, int
     w.tiles = keys > 0 ? (keys + KEYS - 1) / KEYS : 0;
     return w;
 }
-template <class T, int DP, bool BIAS, bool REST>
+// KEEP: what rounding O took is kept, for the gradients.  SPLIT: the keys split over blockIdx.z, the sums for the join (a form
+// of its own: as branches these cost heads of 128 4 %)
+template <class T, int DP, bool BIAS, bool REST, bool KEEP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 2)
     attn_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                     const __grid_constant__ CUtensorMap tmV, const __grid_constant__ AttnArgs a, T* __restrict__ out,
@@ -107,7 +109,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     };
     // this split's part of an item's key tiles: the first, how many (a CTA of a split takes one item)
     auto share = [&](int n) {
-        if (part.splits == 1) return make_int2(0, n);
+        if (!SPLIT) return make_int2(0, n);
         const int per = (n + part.splits - 1) / part.splits, t = min(n, (int)blockIdx.z * per);
         return make_int2(t, min(per, n - t));
     };
@@ -122,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             *dead = 0;
             const Item w = item_at<KT>(a, order, item_index(0, blockIdx.y, gridDim.y), row_tiles);   // the first item's Q and first tile before the CTA meets
             const int2 r = share(w.tiles);
-            *from = r.x;
+            if (SPLIT) *from = r.x;
             if (r.y) {
                 load(sQ, &tmQ, w.q0, h, w.b, barQ, kChunk);
                 load(sK, &tmK, r.x * KT, kh, w.b, barK, Sh::kChunkKV);
@@ -153,14 +155,14 @@ __global__ void __launch_bounds__(kThreads, 2)
             if (tiles[e]) continue;
             const int4 w = entry[e];
             const int rows = min(kRows, a.Lq - w.y), units = a.D / 8;
-            if (part.splits > 1) {
+            if (SPLIT) {
                 for (int x = lane; x < rows; x += 32) part.ml[part.set(a, w.x, h, blockIdx.z, w.y + x)] = make_float2(-INFINITY, 0.f);
                 continue;
             }
             for (int x = lane; x < rows * units; x += 32) {
                 const size_t at = (((size_t)w.x * a.Lq + w.y + x / units) * a.H + h) * a.D + (x % units) * 8;
                 *reinterpret_cast<uint4*>(out + at) = make_uint4(0, 0, 0, 0);
-                if (REST) *reinterpret_cast<uint4*>(rest + at) = make_uint4(0, 0, 0, 0);
+                if (KEEP) *reinterpret_cast<uint4*>(rest + at) = make_uint4(0, 0, 0, 0);
             }
             if (lse)
                 for (int x = lane; x < rows; x += 32) lse[((size_t)w.x * a.H + h) * a.Lq + w.y + x] = INFINITY;
@@ -168,7 +170,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     } else if (warp == 5) {   // copies
         if (lane == 0) {
             bool ok = true;
-            const int j0 = *from;
+            const int j0 = SPLIT ? *from : 0;
             int t = 0, q = 0;   // tiles and items asked for
             for (int i = 0; ok && i < count; ++i) {
                 const int n = tiles[i];
@@ -229,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         } else if (warp == 7) {
             const uint32_t idO = mma_desc<T>(128, 16 * steps, true);
             for (int e = 0; ok && e < count; ++e) {
-                const int n = (int)uniform(tiles[e]), lk = (int)uniform(entry[e].w) - (int)uniform(*from) * KT;
+                const int n = (int)uniform(tiles[e]), lk = (int)uniform(entry[e].w) - (SPLIT ? (int)uniform(*from) * KT : 0);
                 if (n == 0) continue;
                 for (int j = 0; j < n; ++j, ++t) {
                     const int s = t % NST, buf = t % NB, ks = lk - j * KT <= KT / 2 ? KT / 32 : KT / 16;   // steps with keys
@@ -257,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float c = a.scale * kLog2e;
         bool ok = true;
         int tt = 0;   // tiles so far
-        const int j0 = __shfl_sync(0xffffffffu, *from, 0);
+        const int j0 = SPLIT ? __shfl_sync(0xffffffffu, *from, 0) : 0;
         // the bias past the last edge on either side, and what multiplies the scores there: it is added last, and one so
         // large that it swallows the scores near the diagonal, where it is added first, has to do so there too (the
         // factor leaves a masked -inf what it is)
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             const int4 w = entry[kept];   // b, q0, lq, lk
             const int i = w.y + tid;
             const bool some = i < w.z && (kept_l > 0.f || kept_l != kept_l);
-            if (part.splits > 1) {   // sums as they are, for the join
+            if (SPLIT) {   // sums as they are, for the join
                 const size_t set = part.set(a, w.x, h, blockIdx.z, min(i, a.Lq - 1));
 #pragma unroll 1
                 for (int x = 0; x < a.D; x += 16) {
@@ -314,11 +316,11 @@ __global__ void __launch_bounds__(kThreads, 2)
                         for (int z = 0; z < 4; ++z) {
                             const float u0 = ok ? __uint_as_float(o[8 * y + 2 * z]) * s : s, u1 = ok ? __uint_as_float(o[8 * y + 2 * z + 1]) * s : s;
                             p[z] = s == 0.f ? 0u : pack2<T>(u0, u1);   // a dead row is zero whatever it held
-                            q[z] = REST && s != 0.f ? rest2<T>(u0, u1, p[z]) : 0u;
+                            q[z] = KEEP && s != 0.f ? rest2<T>(u0, u1, p[z]) : 0u;
                         }
                         if (x + 8 * y < a.D) {
                             *reinterpret_cast<uint4*>(out + at + x + 8 * y) = make_uint4(p[0], p[1], p[2], p[3]);
-                            if (REST) *reinterpret_cast<uint4*>(rest + at + x + 8 * y) = make_uint4(q[0], q[1], q[2], q[3]);
+                            if (KEEP) *reinterpret_cast<uint4*>(rest + at + x + 8 * y) = make_uint4(q[0], q[1], q[2], q[3]);
                         }
                     }
                 }
@@ -492,7 +494,7 @@ bool ordered(const AttnArgs& a, int sms) {
     return (a.lengths || a.causal) && stays(a, sms) && (long long)a.B * ((a.Lq + kRows - 1) / kRows) <= kMaxOrder;
 }
 
-template <class T, int DP, bool BIAS, bool REST>
+template <class T, int DP, bool BIAS, bool REST, bool KEEP, bool SPLIT>
 int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
     using Sh = Shape<DP, REST>;
     static DeviceSetup setup;
@@ -501,10 +503,10 @@ int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void
     if (e != cudaSuccess) return (int)e;
     int rc = device_setup(setup, dev, [] {
         cudaFuncAttributes at;   // the register split above counts on the launch's share
-        cudaError_t e = cudaFuncGetAttributes(&at, attn_fwd_kernel<T, DP, BIAS, REST>);
+        cudaError_t e = cudaFuncGetAttributes(&at, attn_fwd_kernel<T, DP, BIAS, REST, KEEP, SPLIT>);
         if (e == cudaSuccess && at.numRegs < (kRegsSoftmax + kRegsOther + 1) / 2) e = cudaErrorLaunchOutOfResources;
         if (e == cudaSuccess)
-            e = cudaFuncSetAttribute(attn_fwd_kernel<T, DP, BIAS, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+            e = cudaFuncSetAttribute(attn_fwd_kernel<T, DP, BIAS, REST, KEEP, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)Sh::smem(lut_size(kMaxReach)));
         return (int)e;
     }, &sms);
@@ -527,20 +529,25 @@ int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void
         attn_order_kernel<<<1, 1024, 0, st>>>(a, order);
     }
     const Parts part = parts_at(a, splits_of(a, sms), ws);
-    attn_fwd_kernel<T, DP, BIAS, REST><<<dim3(a.H, (unsigned)ctas, part.splits), kThreads, smem, st>>>(q, k, v, a, (T*)out, lse, (T*)rest, order, part);
+    attn_fwd_kernel<T, DP, BIAS, REST, KEEP, SPLIT><<<dim3(a.H, (unsigned)ctas, part.splits), kThreads, smem, st>>>(q, k, v, a, (T*)out, lse, (T*)rest, order, part);
     rc = (int)cudaGetLastError();
     return rc || part.splits == 1 ? rc : attn_join(a, dtype, part, out, lse, rest, st);
 }
 
+template <class T, int DP, bool BIAS, bool REST, bool KEEP>
+int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, int sms, cudaStream_t st) {
+    return splits_of(a, sms) > 1 ? launch<T, DP, BIAS, REST, false, true>(a, dtype, out, lse, rest, ws, st)
+                                 : launch<T, DP, BIAS, REST, KEEP, false>(a, dtype, out, lse, rest, ws, st);
+}
+template <class T, int DP>
+int pick(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, int sms, cudaStream_t st) {
+    if (a.bias)
+        return rest ? launch<T, DP, true, true, true>(a, dtype, out, lse, rest, ws, sms, st) : launch<T, DP, true, false, false>(a, dtype, out, lse, rest, ws, sms, st);
+    return rest ? launch<T, DP, false, false, true>(a, dtype, out, lse, rest, ws, sms, st) : launch<T, DP, false, false, false>(a, dtype, out, lse, rest, ws, sms, st);
+}
 template <class T>
-int pick(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
-    if (a.D <= 64)
-        return !a.bias ? launch<T, 64, false, false>(a, dtype, out, lse, rest, ws, st)
-               : rest  ? launch<T, 64, true, true>(a, dtype, out, lse, rest, ws, st)
-                       : launch<T, 64, true, false>(a, dtype, out, lse, rest, ws, st);
-    return !a.bias ? launch<T, 128, false, false>(a, dtype, out, lse, rest, ws, st)
-           : rest  ? launch<T, 128, true, true>(a, dtype, out, lse, rest, ws, st)
-                   : launch<T, 128, true, false>(a, dtype, out, lse, rest, ws, st);
+int pick(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, int sms, cudaStream_t st) {
+    return a.D <= 64 ? pick<T, 64>(a, dtype, out, lse, rest, ws, sms, st) : pick<T, 128>(a, dtype, out, lse, rest, ws, sms, st);
 }
 
 }  // namespace fwd
@@ -574,14 +581,16 @@ bool rows_map(CUtensorMap* tm, int dtype, const void* base, int B, int L, int he
 int attn_forward_gave_up(unsigned long long* n) { return (int)cudaMemcpyFromSymbol(n, g_gave_up, sizeof(*n)); }
 
 size_t attn_forward_bytes(const AttnArgs& a) {
-    static DeviceSetup setup;
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || device_setup(setup, dev, [] { return 0; }, &sms)) return (size_t)-1;
+    int sms = 0;
+    if (attn_sms(&sms)) return (size_t)-1;
     if (fwd::splits_of(a, sms) > 1) return parts_bytes(a, fwd::splits_of(a, sms));
     return fwd::ordered(a, sms) ? (size_t)a.B * ((a.Lq + fwd::kRows - 1) / fwd::kRows) * sizeof(int) : 0;
 }
 int attn_forward_tiles(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
-    return dtype == D2P_DTYPE_BF16 ? fwd::pick<__nv_bfloat16>(a, dtype, out, lse, rest, ws, st) : fwd::pick<__half>(a, dtype, out, lse, rest, ws, st);
+    int sms = 0;
+    const int rc = attn_sms(&sms);
+    if (rc) return rc;
+    return dtype == D2P_DTYPE_BF16 ? fwd::pick<__nv_bfloat16>(a, dtype, out, lse, rest, ws, sms, st) : fwd::pick<__half>(a, dtype, out, lse, rest, ws, sms, st);
 }
 
 }  // namespace enc

@@ -374,9 +374,8 @@ int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, voi
     return dtype == D2P_DTYPE_BF16 ? pick_token<__nv_bfloat16>(a, out, lse, rest, ws, st) : pick_token<__half>(a, out, lse, rest, ws, st);
 }
 size_t attn_tokens_bytes(const AttnArgs& a) {
-    static DeviceSetup setup;
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || device_setup(setup, dev, [] { return 0; }, &sms)) return (size_t)-1;
+    int sms = 0;
+    if (attn_sms(&sms)) return (size_t)-1;
     return parts_bytes(a, tok::parts_of(a, sms));
 }
 

@@ -1237,9 +1237,9 @@ class AttentionFunction : public torch::autograd::Function<AttentionFunction> {
                           const OptTensor& lengths, at::IntArrayRef edges, double scale, bool causal) {
         at::AutoDispatchBelowADInplaceOrView guard;
         const bool want_bias = bias.has_value() && wants_grad(*bias);
-        auto r = call_attention_forward(q, k, v, bias, lengths, edges, scale, causal, true, want_bias);
+        auto r = call_attention_forward(q, k, v, bias, lengths, edges, scale, causal, true, true);
         ctx->save_for_backward({q, k, v, undef(bias), undef(lengths), std::get<0>(r), std::get<1>(r),
-                                want_bias ? std::get<2>(r) : Tensor()});
+                                std::get<2>(r)});
         ctx->saved_data["edges"] = edges.vec();
         ctx->saved_data["scale"] = scale;
         ctx->saved_data["causal"] = causal;

@@ -338,10 +338,10 @@ typedef struct {
 } d2p_attention_args;
 /* out [B, Lq, H, D] contiguous, the inputs' type.  For the backward pass: lse [B,
  * H, Lq] fp32 or NULL (log2 of the sum of exponentials, +inf in rows with no
- * allowed key), and rest, like out, or NULL: for the gradient of the bias (needs
- * one), whose sums cancel, out is formed from unrounded probabilities and what its
- * own rounding took is kept.
- * Large batches of uneven lengths take a small workspace. */
+ * allowed key), and rest, like out, or NULL: what rounding took from out, for a
+ * more exact row sum of grad out; with a bias, out is then also formed from
+ * probabilities in twice 16 bits, since the sums of the bias's gradient cancel.
+ * Large batches of uneven lengths, and few rows over many keys, take a workspace. */
 D2P_API size_t d2p_attention_forward_workspace_bytes(const d2p_attention_args* args);
 D2P_API int d2p_attention_forward(const d2p_attention_args* args, void* out, float* lse, void* rest,
                                   void* workspace, size_t workspace_bytes, void* stream);

@@ -197,7 +197,8 @@ def test_c_abi_checks_outputs(lib):
     a = attention_args()
     assert f(ctypes.byref(a), None, None, None, None, 0, None) == 1001          # no output
     assert f(ctypes.byref(a), 4100, None, None, None, 0, None) == 1001          # output off a 16-byte boundary
-    assert f(ctypes.byref(a), 4096, None, 4096, None, 0, None) == 1001          # rest without a bias
+    assert f(ctypes.byref(a), 4096, None, 4104, None, 0, None) == 1001          # rest off one
+    assert f(ctypes.byref(a), 4096, 4098, None, None, 0, None) == 1001          # lse off a word
     d = lib.d2p_dropout_add
     d.restype = ctypes.c_int
     d.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_ulonglong, ctypes.c_double, ctypes.c_ulonglong,
