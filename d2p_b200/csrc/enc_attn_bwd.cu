@@ -351,17 +351,18 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int f = 0; f < kCols; f += 16) tmem_tie16(o + f);
             tc_fence_before();
             bar_arrive_warp(barA);   // the next item's products may overwrite them
+            const bool whole = a.D % 16 == 0 && (((uintptr_t)g.dx1 | (uintptr_t)g.dx2) & 31) == 0;
             if (kept_x < Lx) {
                 T* const rp = (T*)(first ? g.dx1 : g.dx2) + (((size_t)kept_b * Lx + kept_x) * heads + hx) * a.D + f0;
 #pragma unroll
-                for (int y = 0; y < kCols; y += 8) {
-                    uint32_t p[4];
+                for (int y = 0; y < kCols; y += 16) {
+                    uint32_t p[8];
 #pragma unroll
-                    for (int z = 0; z < 4; ++z) {
+                    for (int z = 0; z < 8; ++z) {
                         const float u0 = __uint_as_float(o[y + 2 * z]) * w, u1 = __uint_as_float(o[y + 2 * z + 1]) * w;
                         p[z] = !row ? 0u : ok ? pack2<T>(u0, u1) : pack2<T>(NAN, NAN);
                     }
-                    if (f0 + y < a.D) *reinterpret_cast<uint4*>(rp + y) = make_uint4(p[0], p[1], p[2], p[3]);
+                    if (f0 + y < a.D) store16(rp + y, p, a.D - f0 - y, whole);
                 }
             }
             kept_b = -1;

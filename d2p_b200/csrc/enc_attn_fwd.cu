@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 return;
             }
             const float s = !ok ? NAN : (some ? 1.f / kept_l : 0.f);
+            const bool whole = a.D % 16 == 0 && (((uintptr_t)out | (uintptr_t)rest) & 31) == 0;
             const size_t at = (((size_t)w.x * a.Lq + i) * a.H + h) * a.D;
 #pragma unroll 1
             for (int x = 0; x < a.D; x += 16) {
@@ -309,20 +310,15 @@ __global__ void __launch_bounds__(kThreads, 2)
                 tmem_wait_ld();
                 tmem_tie16(o);
                 if (i < a.Lq) {
+                    uint32_t p[8], q[8];
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) {
-                        uint32_t p[4], q[4];
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const float u0 = ok ? __uint_as_float(o[8 * y + 2 * z]) * s : s, u1 = ok ? __uint_as_float(o[8 * y + 2 * z + 1]) * s : s;
-                            p[z] = s == 0.f ? 0u : pack2<T>(u0, u1);   // a dead row is zero whatever it held
-                            q[z] = KEEP && s != 0.f ? rest2<T>(u0, u1, p[z]) : 0u;
-                        }
-                        if (x + 8 * y < a.D) {
-                            *reinterpret_cast<uint4*>(out + at + x + 8 * y) = make_uint4(p[0], p[1], p[2], p[3]);
-                            if (KEEP) *reinterpret_cast<uint4*>(rest + at + x + 8 * y) = make_uint4(q[0], q[1], q[2], q[3]);
-                        }
+                    for (int z = 0; z < 8; ++z) {
+                        const float u0 = ok ? __uint_as_float(o[2 * z]) * s : s, u1 = ok ? __uint_as_float(o[2 * z + 1]) * s : s;
+                        p[z] = s == 0.f ? 0u : pack2<T>(u0, u1);   // a dead row is zero whatever it held
+                        q[z] = KEEP && s != 0.f ? rest2<T>(u0, u1, p[z]) : 0u;
                     }
+                    store16(out + at + x, p, a.D - x, whole);
+                    if (KEEP) store16(rest + at + x, q, a.D - x, whole);
                 }
             }
             if (lse && i < a.Lq)

@@ -164,6 +164,16 @@ __device__ __forceinline__ void tmem_tie16(uint32_t* v) { asm volatile("" : ENC_
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// sixteen 16-bit elements, of which the first `n` (8 or 16) are stored; whole: at a 32-byte boundary, one store a sector
+__device__ __forceinline__ void store16(void* to, const uint32_t* p, int n, bool whole) {
+    if (whole) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), ENC_R8(p, 0) : "memory");
+    } else {
+        reinterpret_cast<uint4*>(to)[0] = make_uint4(p[0], p[1], p[2], p[3]);
+        if (n > 8) reinterpret_cast<uint4*>(to)[1] = make_uint4(p[4], p[5], p[6], p[7]);
+    }
+}
+
 // two fp32 operations in one instruction
 struct Two {
     uint64_t v;
