@@ -31,6 +31,12 @@
 // forms O from P in twice 16 bits and keeps what rounding O took.  Without a bias
 // it keeps the latter alone: short rows' dQ and dK are off by a sixth less.
 //
+// Measured: 2 x 4096 causal, 16/4 heads of 128: keys 252 us, queries 183: 790
+// TFLOP/s counted as the gradients' 5 products, 1100 as the 7 taken; 64 x 512, 8
+// heads of 64: 227 us together.  Bound by the products' pipe (two thirds to three
+// quarters busy) and, for heads of 64, by the exponentials and the 16-bit stores of
+// P and dS to TMEM.
+//
 // The query pass also sums dS by relative position.  Along a diagonal of a
 // warp's 32 x 32 block the sum moves one lane per column (one shuffle each), the
 // 63 sums are scanned, and each lane takes its buckets as differences of the

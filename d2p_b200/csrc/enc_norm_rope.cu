@@ -10,6 +10,10 @@
 // memory.  A thread holds 16 elements of a row as two 8-element units that are
 // each other's rotation partners, so the rotation needs no exchange, and D / 16
 // threads (rounded up to a power of two) share the row's sums by shuffles.
+//
+// Measured, 64 x 512 tokens, 8 + 8 heads of 64, bf16: forward 34 us (142 MB: 4.2
+// TB/s), backward 56 us (210 MB: 3.7 TB/s) and 4 us for the weights' sums; a
+// token of 32 sequences 5 us, latency.
 #include "enc_common.cuh"
 
 namespace d2pb {

@@ -68,6 +68,7 @@ def attention(
     are copied).  ``lengths`` [B, 2] int32: (queries, keys) of each problem, clamped to the padded sizes on the
     device; rows past them are zero, and what q, k, v hold there is never used.  ``causal`` aligns the last query
     with the last key (query i at position i + lk - lq) and masks later keys; a row left without keys is zero.
+    (A NaN or infinity in a live key's v reaches masked rows of its tile too, as 0 x inf does in the plain product.)
     ``bias`` [num_buckets, H] (q's dtype or float32) adds bias[bucket, h] by relative position
     (``relative_bucket_edges``; two-sided unless causal).  ``scale`` defaults to 1 / sqrt(D) and must be positive.
     """
