@@ -98,6 +98,7 @@ struct Args {
     void* dx2;             // dk or dq
     float* part;           // query pass: [H][buckets][CTAs of a head] sums of dS, or null
     const int* order;      // items in order of their work, or null
+    int beside;            // query pass: launched after the keys pass, whose results it does not need
 };
 
 // one owned tile: its rows [x0, x0 + 128) of problem b, and the streamed rows [y0, ..) in `per` tiles that any of them meets
@@ -140,6 +141,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int Lx = DKV ? a.Lk : a.Lq, heads = DKV ? a.Hkv : a.H, row_tiles = (Lx + kOwn - 1) / kOwn, items = a.B * row_tiles;
     const int count = item_count(items, blockIdx.y, gridDim.y);   // of this CTA
 
+    // The queries pass begins where the keys pass leaves SMs free: that one's CTAs have all begun, and so have waited for the
+    // statistics and the order.  It ends after that one has ended (the wait at its end), for those who read the results
+    if (DKV || !g.beside) wait_ahead();
+    if (DKV) let_next();
     extern __shared__ uint8_t raw[];
     const uint32_t r0 = smem_addr(raw), base = (r0 + 1023u) & ~1023u;
     uint8_t* const gb = raw + (base - r0);
@@ -587,6 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     if (warp == kWork / 32) tmem_free(tmem, kColumns);
+    if (!DKV) wait_ahead();
 }
 
 // -delta = -rowsum(dO O) (times kDown) and kShift - lse in rows padded to whole tiles: 0 and -inf where no key is met.  O with what its
@@ -598,6 +604,7 @@ template <class T, int LANES>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ AttnArgs a, const T* __restrict__ out, const T* __restrict__ rest,
                                                          const float* __restrict__ lse, const T* __restrict__ grad, int Lp,
                                                          float* __restrict__ lp, float* __restrict__ dp) {
+    let_next();
     __shared__ float sum[kStatHeads][kStatRows + 1];
     const int lane = threadIdx.x % LANES, i0 = blockIdx.x * kStatRows, h0 = blockIdx.y * kStatHeads, b = blockIdx.z;
     const int heads = min(kStatHeads, a.H - h0);
@@ -632,6 +639,7 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
         dp[at] = -sum[h][threadIdx.x % kStatRows] * Softmax<T>::kDown;
         lp[at] = i < lq ? Softmax<T>::kShift - lse[((size_t)b * a.H + h0 + h) * a.Lq + i] : -INFINITY;
     }
+    wait_ahead();   // (the order is not read here, but by the passes, which wait for this launch alone)
 }
 
 // dbias[t][h]: one warp each, the CTAs' sums in a fixed order
@@ -648,6 +656,7 @@ __global__ void __launch_bounds__(128) attn_dbias_kernel(const float* part, int 
 }
 
 __global__ void __launch_bounds__(1024) attn_order_kernel(const __grid_constant__ AttnArgs a, int* keys, int* queries) {
+    let_next();
     if (blockIdx.x == 0) {
         if (keys) order_items(a.B * ((a.Lk + kOwn - 1) / kOwn), [&](int i) { return min(item_at<true>(a, nullptr, i).per, kBins - 1); }, keys);
     } else if (queries) {
@@ -685,8 +694,8 @@ int launch_pass(const Args& g, const CUtensorMap* tm, long long ctas, cudaStream
     if (rc) return rc;
     const int reach = BIAS ? reach_of(g.a.edges) : 0;
     const size_t smem = smem_bytes<DP, BIAS>(DKV, reach);
-    attn_bwd_kernel<T, DP, BIAS, DKV><<<dim3(DKV ? g.a.Hkv : g.a.H, (unsigned)ctas), kThreads, smem, st>>>(tm[0], tm[1], tm[2], tm[3], g);
-    return (int)cudaGetLastError();
+    return launch_early(true, attn_bwd_kernel<T, DP, BIAS, DKV>, dim3(DKV ? g.a.Hkv : g.a.H, (unsigned)ctas), kThreads, smem, st, tm[0], tm[1], tm[2],
+                        tm[3], g);
 }
 template <class T, int DP>
 int launch_pass(const Args& g, bool dkv, const CUtensorMap* tm, long long ctas, cudaStream_t st) {
@@ -713,9 +722,10 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
     }
     if (a.B && a.Lq) {
         const dim3 grid(Lp / kStatRows, (a.H + kStatHeads - 1) / kStatHeads, a.B);
-        if (a.D <= 64) attn_stats_kernel<T, 8><<<grid, 256, 0, st>>>(a, (const T*)out, (const T*)rest, lse, (const T*)grad, Lp, lp, dp);
-        else attn_stats_kernel<T, 16><<<grid, 256, 0, st>>>(a, (const T*)out, (const T*)rest, lse, (const T*)grad, Lp, lp, dp);
-        if ((rc = (int)cudaGetLastError())) return rc;
+        // (beside the order: what it reads was there before that launch)
+        rc = launch_early(ok || oq, a.D <= 64 ? attn_stats_kernel<T, 8> : attn_stats_kernel<T, 16>, grid, 256, 0, st, a, (const T*)out, (const T*)rest,
+                          lse, (const T*)grad, Lp, lp, dp);
+        if (rc) return rc;
     }
     if (a.B && (a.Lq || a.Lk)) {
         // maps of the rows there are; an axis without rows is never read
@@ -737,7 +747,7 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
             }
         }
         if (!fine) return D2P_ERR_INVALID_ARGUMENT;
-        Args g = {a, lp, dp, Lp, nullptr, nullptr, nullptr, nullptr};
+        Args g = {a, lp, dp, Lp, nullptr, nullptr, nullptr, nullptr, 0};
         if (a.Lk) {
             g.dx1 = dv, g.dx2 = dk, g.order = order_k;
             const CUtensorMap tm[4] = {own[2], own[3], str[0], str[1]};
@@ -746,7 +756,7 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
             if (rc) return rc;
         }
         if (a.Lq) {
-            g.dx1 = nullptr, g.dx2 = dq, g.part = dbias ? part : nullptr, g.order = order_q;
+            g.dx1 = nullptr, g.dx2 = dq, g.part = dbias ? part : nullptr, g.order = order_q, g.beside = a.Lk > 0;
             const CUtensorMap tm[4] = {own[0], own[1], str[2], str[3]};
             const long long n = ctas_of(a, false, sms);
             rc = a.D <= 64 ? launch_pass<T, 64>(g, false, tm, n, st) : launch_pass<T, 128>(g, false, tm, n, st);

@@ -130,6 +130,7 @@ __global__ void __launch_bounds__(kThreads, 2)
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
             *dead = 0;
+            wait_ahead();   // (the items' order)
             const Item w = item_at<KT>(a, order, item_index(0, blockIdx.y, gridDim.y), row_tiles);   // the first item's Q and first tile before the CTA meets
             const int2 r = share(w.tiles);
             if (SPLIT) *from = r.x;
@@ -143,13 +144,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     } else if (warp == 4) {
         tmem_alloc(smem_addr(slot), kColumns);
     } else {
+        if (BIAS) fill_lut<T>(lut, a, h, reach, warp < 4 ? warp : warp - 2, 6);
+        wait_ahead();
         for (int e = warp < 4 ? tid : tid - 64; e < count; e += 192) {
             const Item w = item_at<KT>(a, order, item_index(e, blockIdx.y, gridDim.y), row_tiles);
             entry[e] = make_int4(w.b, w.q0, w.lq, w.lk);
             tiles[e] = share(w.tiles).y;
         }
-        __syncwarp();
-        if (BIAS) fill_lut<T>(lut, a, h, reach, warp < 4 ? warp : warp - 2, 6);
     }
     tc_fence_before();
     __syncthreads();
@@ -475,6 +476,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 __global__ void __launch_bounds__(1024) attn_order_kernel(const __grid_constant__ AttnArgs a, int* __restrict__ order) {
+    let_next();
     const int row_tiles = (a.Lq + kRows - 1) / kRows;
     order_items(a.B * row_tiles, [&](int i) { return min(item_at<128>(a, nullptr, i, row_tiles).tiles, kBins - 1); }, order);
 }
@@ -534,8 +536,8 @@ int launch(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void
         attn_order_kernel<<<1, 1024, 0, st>>>(a, order);
     }
     const Parts part = parts_at(a, splits_of(a, sms), ws);
-    attn_fwd_kernel<T, DP, BIAS, REST, KEEP, SPLIT><<<dim3(a.H, (unsigned)ctas, part.splits), kThreads, smem, st>>>(q, k, v, a, (T*)out, lse, (T*)rest, order, part);
-    rc = (int)cudaGetLastError();
+    rc = launch_early(order != nullptr, attn_fwd_kernel<T, DP, BIAS, REST, KEEP, SPLIT>, dim3(a.H, (unsigned)ctas, part.splits), kThreads, smem, st, q,
+                      k, v, a, (T*)out, lse, (T*)rest, (const int*)order, part);
     return rc || part.splits == 1 ? rc : attn_join(a, dtype, part, out, lse, rest, st);
 }
 

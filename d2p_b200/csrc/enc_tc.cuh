@@ -247,6 +247,21 @@ __device__ __forceinline__ void fill_lut(float* lut, const AttnArgs& a, int h, i
     }
 }
 
+// Launches that begin before the one ahead has ended (programmatic): what that one writes is read after the wait, which
+// does nothing in an ordinary launch
+__device__ __forceinline__ void wait_ahead() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <class... P, class... A>
+int launch_early(bool early, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid, cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = early ? 1 : 0;
+    return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Items in order of falling work, for CTAs that take several each: a stable
 // counting sort by one CTA of 1024 threads, so that which CTA takes an item never
 // changes from run to run.  bin(i): the item's work, at most kBins - 1
