@@ -31,9 +31,8 @@
 // forms O from P in twice 16 bits and keeps what rounding O took.  Without a bias
 // it keeps the latter alone: short rows' dQ and dK are off by a sixth less.
 //
-// Measured: 2 x 4096 causal, 16/4 heads of 128: keys 252 us, queries 183: 790
-// TFLOP/s counted as the gradients' 5 products, 1100 as the 7 taken; 64 x 512, 8
-// heads of 64: 227 us together.  Bound by the products' pipe (two thirds to three
+// Measured: 2 x 4096 causal, 16/4 heads of 128: 441 us, 780 TFLOP/s counted as the
+// gradients' 5 products, 1090 as the 7 taken; 64 x 512, 8 heads of 64: 205 us.  Bound by the products' pipe (two thirds to three
 // quarters busy) and, for heads of 64, by the exponentials and the 16-bit stores of
 // P and dS to TMEM.
 //
@@ -142,7 +141,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int count = item_count(items, blockIdx.y, gridDim.y);   // of this CTA
 
     // The queries pass begins where the keys pass leaves SMs free: that one's CTAs have all begun, and so have waited for the
-    // statistics and the order.  It ends after that one has ended (the wait at its end), for those who read the results
+    // statistics and the order.  It ends after that one has ended (the wait at its end), for those who read the results.
+    // 1 x 4096 causal, 16/4 heads of 128, whose 128 items of keys leave SMs free: both passes 370 us one after the other, 260 so
     if (DKV || !g.beside) wait_ahead();
     if (DKV) let_next();
     extern __shared__ uint8_t raw[];
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_before();
     __syncthreads();
     if (warp == kWork / 32) tmem_free(tmem, kColumns);
-    if (!DKV) wait_ahead();
+    if (!DKV && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) wait_ahead();   // (one CTA is enough, and leaves the others' SMs free)
 }
 
 // -delta = -rowsum(dO O) (times kDown) and kShift - lse in rows padded to whole tiles: 0 and -inf where no key is met.  O with what its
@@ -639,7 +639,8 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
         dp[at] = -sum[h][threadIdx.x % kStatRows] * Softmax<T>::kDown;
         lp[at] = i < lq ? Softmax<T>::kShift - lse[((size_t)b * a.H + h0 + h) * a.Lq + i] : -INFINITY;
     }
-    wait_ahead();   // (the order is not read here, but by the passes, which wait for this launch alone)
+    // (the order is not read here, but by the passes, which wait for this launch alone: one block ends after it)
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) wait_ahead();
 }
 
 // dbias[t][h]: one warp each, the CTAs' sums in a fixed order
