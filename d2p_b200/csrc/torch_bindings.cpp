@@ -22,6 +22,7 @@
 //    [B,2] tensor with a host->device copy.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -977,6 +978,8 @@ Tensor embed_grad_scores_cuda(const Tensor& marginals, const Tensor& grad_value,
 // relative position bias and its gradients, head norms with the position
 // rotation, dropout with the residual
 // =============================================================================
+// an output or workspace, without the dispatcher's way to it (these calls' host time counts: five a backward pass)
+Tensor fresh(at::IntArrayRef sizes, const at::TensorOptions& options) { return Tensor(at::detail::empty_cuda(sizes, options)); }
 int enc_dtype(const Tensor& t, const char* what, bool f32) {
     if (t.scalar_type() == at::kBFloat16) return D2P_DTYPE_BF16;
     if (t.scalar_type() == at::kHalf) return D2P_DTYPE_F16;
@@ -1062,12 +1065,12 @@ std::tuple<Tensor, Tensor, Tensor> attention_forward_cuda(const Tensor& q, const
     const c10::cuda::CUDAGuard guard(q.device());
     Attn f;
     attn_fill(f, q, k, v, bias, lengths, edges, scale, causal);
-    Tensor out = torch::empty({q.size(0), q.size(1), q.size(2), q.size(3)}, q.options());
-    Tensor lse = torch::empty({want_lse ? q.size(0) : 0, q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
-    Tensor rest = torch::empty({want_rest ? q.size(0) : 0, q.size(1), q.size(2), q.size(3)}, q.options());
+    Tensor out = fresh({q.size(0), q.size(1), q.size(2), q.size(3)}, q.options());
+    Tensor lse = fresh({want_lse ? q.size(0) : 0, q.size(2), q.size(1)}, q.options().dtype(at::kFloat));
+    Tensor rest = fresh({want_rest ? q.size(0) : 0, q.size(1), q.size(2), q.size(3)}, q.options());
     const size_t n = d2p_attention_forward_workspace_bytes(&f.a);
     TORCH_CHECK(n != static_cast<size_t>(-1), "attention: problem not supported");
-    Tensor ws = n ? torch::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte)) : Tensor();
+    Tensor ws = n ? fresh({static_cast<int64_t>(n)}, q.options().dtype(at::kByte)) : Tensor();
     check_rc(d2p_attention_forward(&f.a, out.data_ptr(), want_lse ? lse.data_ptr<float>() : nullptr,
                                    want_rest ? rest.data_ptr() : nullptr, n ? ws.data_ptr() : nullptr, n, cur_stream()),
              "d2p_attention_forward");
@@ -1096,12 +1099,12 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attention_backward_cuda(
         rs = packed16(*rest);
     }
     const Tensor g = packed16(grad), o = packed16(out), L = lse.contiguous();
-    Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
-    Tensor dv = torch::empty(v.sizes(), v.options());
-    Tensor db = want_bias ? torch::empty(f.bias.sizes(), f.bias.options()) : torch::empty({0, 0}, q.options());
+    Tensor dq = fresh(q.sizes(), q.options()), dk = fresh(k.sizes(), k.options());
+    Tensor dv = fresh(v.sizes(), v.options());
+    Tensor db = want_bias ? fresh(f.bias.sizes(), f.bias.options()) : fresh({0, 0}, q.options());
     const size_t n = d2p_attention_backward_workspace_bytes(&f.a, want_bias);
     TORCH_CHECK(n != static_cast<size_t>(-1), "attention_backward: problem not supported");
-    Tensor ws = torch::empty({static_cast<int64_t>(n > 0 ? n : 1)}, q.options().dtype(at::kByte));
+    Tensor ws = fresh({static_cast<int64_t>(n > 0 ? n : 1)}, q.options().dtype(at::kByte));
     check_rc(d2p_attention_backward(&f.a, o.data_ptr(), rs.defined() ? rs.data_ptr() : nullptr, L.data_ptr<float>(),
                                     g.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), want_bias ? db.data_ptr() : nullptr, ws.data_ptr(), n, cur_stream()),
              "d2p_attention_backward");
@@ -1160,7 +1163,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope_cuda(const Tensor& q, const Tensor& k, c
     const c10::cuda::CUDAGuard guard(q.device());
     NormRope f;
     norm_rope_fill(f, q, k, qw, kw, cos, sin, positions, eps);
-    Tensor yq = torch::empty(q.sizes(), q.options()), yk = torch::empty(k.sizes(), k.options());
+    Tensor yq = fresh(q.sizes(), q.options()), yk = fresh(k.sizes(), k.options());
     check_rc(d2p_norm_rope_forward(&f.a, yq.data_ptr(), yk.data_ptr(), cur_stream()), "d2p_norm_rope_forward");
     return {yq, yk};
 }
@@ -1176,11 +1179,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> qk_norm_rope_backward_cuda(
                     gk.scalar_type() == q.scalar_type() && gq.device() == q.device() && gk.device() == q.device(),
                 "qk_norm_rope_backward: gradients must have the shape, dtype and device of q and k");
     const Tensor g0 = packed16(gq), g1 = packed16(gk);
-    Tensor dq = torch::empty(q.sizes(), q.options()), dk = torch::empty(k.sizes(), k.options());
-    Tensor dqw = torch::empty(qw.sizes(), qw.options()), dkw = torch::empty(kw.sizes(), kw.options());
+    Tensor dq = fresh(q.sizes(), q.options()), dk = fresh(k.sizes(), k.options());
+    Tensor dqw = fresh(qw.sizes(), qw.options()), dkw = fresh(kw.sizes(), kw.options());
     const size_t n = d2p_norm_rope_workspace_bytes(&f.a);
     TORCH_CHECK(n != static_cast<size_t>(-1), "qk_norm_rope_backward: problem not supported");
-    Tensor ws = torch::empty({static_cast<int64_t>(n)}, q.options().dtype(at::kByte));
+    Tensor ws = fresh({static_cast<int64_t>(n)}, q.options().dtype(at::kByte));
     check_rc(d2p_norm_rope_backward(&f.a, g0.data_ptr(), g1.data_ptr(), dq.data_ptr(), dk.data_ptr(), dqw.data_ptr(),
                                     dkw.data_ptr(), ws.data_ptr(), n, cur_stream()),
              "d2p_norm_rope_backward");
@@ -1200,7 +1203,7 @@ Tensor dropout_add_cuda(const Tensor& x, const c10::optional<Tensor>& residual, 
                     "dropout_add: residual must have x's shape, dtype and device");
         rc = residual->contiguous();
     }
-    Tensor y = torch::empty(x.sizes(), x.options());
+    Tensor y = fresh(x.sizes(), x.options());
     check_rc(d2p_dropout_add(xc.data_ptr(), rc.defined() ? rc.data_ptr() : nullptr, dt, (unsigned long long)x.numel(), p,
                              (unsigned long long)seed, (unsigned long long)offset, y.data_ptr(), cur_stream()),
              "d2p_dropout_add");
