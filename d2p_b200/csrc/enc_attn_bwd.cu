@@ -3,10 +3,12 @@
 //   P = 2^(s - lse),  dP = dO V^T,  dS = P (dP - delta),  delta = rowsum(dO O),
 //   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K,  dbias = buckets' sums of dS.
 //
-// Two passes of one kernel, a CTA taking 128 rows that it owns at a time, so that
+// Two passes in one launch, a CTA taking 128 rows that it owns at a time, so that
 // every sum stays in the CTA's accumulators and no atomics are needed: the key pass
 // (DKV) owns 128 keys and streams 64 queries at a time of every head that shares
-// them, the query pass owns 128 queries and streams 64 keys.  With X1, X2 the
+// them, the query pass owns 128 queries and streams 64 keys.  The queries pass's
+// CTAs come after the keys pass's in the grid and so take the SMs that these leave
+// free; neither reads what the other writes.  With X1, X2 the
 // owned and Y1, Y2 the streamed rows (keys pass: K, V / Q, dO; query pass: Q, dO
 // / K, V) both are
 //   S = X1 Y1^T,  dP = X2 Y2^T  (two 64-column products into TMEM),
@@ -40,6 +42,8 @@
 // warp's 32 x 32 block the sum moves one lane per column (one shuffle each), the
 // 63 sums are scanned, and each lane takes its buckets as differences of the
 // scan: registers only, in a fixed order.
+#include <limits.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -77,14 +81,13 @@ struct Shape {
     static constexpr size_t fixed() { return 1024 + kTiles + kBars * 8 + 32 + kMaxItems * 24; }
 };
 // after the tiles: the bias by position, then (query pass) the diagonals' stage of each warp and the buckets' ranges
-__host__ __device__ inline size_t extra(bool bias, bool dkv, int reach) {
-    if (!bias) return 0;
-    return 4 * (size_t)lut_size(reach) + (dkv ? 0 : 4 * (size_t)(16 * 144 + 16 * kBuckets + 2 * kBuckets));
+__host__ __device__ inline size_t extra(bool bias, int reach) {
+    return bias ? 4 * (size_t)(lut_size(reach) + 16 * 144 + 16 * kBuckets + 2 * kBuckets) : 0;
 }
 // at least 116 KB: one CTA an SM, since it takes the whole TMEM (no allocation waits)
 template <int DP, bool BIAS>
-size_t smem_bytes(bool dkv, int reach) {
-    const size_t n = Shape<DP, BIAS>::fixed() + extra(BIAS, dkv, reach);
+size_t smem_bytes(int reach) {
+    const size_t n = Shape<DP, BIAS>::fixed() + extra(BIAS, reach);
     return n < 116 * 1024 ? 116 * 1024 : n;
 }
 
@@ -93,11 +96,13 @@ struct Args {
     const float* lse;      // [B, H, Lp] padded copies, negated: kShift - lse and -delta kDown; -inf and 0 in dead rows
     const float* delta;
     int Lp;
-    void* dx1;             // keys pass: dv; query pass: unused
-    void* dx2;             // dk or dq
+    void *dv, *dk, *dq;
     float* part;           // query pass: [H][buckets][CTAs of a head] sums of dS, or null
-    const int* order;      // items in order of their work, or null
-    int beside;            // query pass: launched after the keys pass, whose results it does not need
+    const int *order_k, *order_q;   // the passes' items in order of their work, or null
+    int ctas_k, ctas_q;    // CTAs of a head (0: no such pass)
+};
+struct Maps {              // 128 rows for those a CTA owns, 64 for those it streams
+    CUtensorMap q, grad, k, v;
 };
 
 // one owned tile: its rows [x0, x0 + 128) of problem b, and the streamed rows [y0, ..) in `per` tiles that any of them meets
@@ -127,24 +132,20 @@ __device__ __forceinline__ Item item_at(const AttnArgs& a, const int* order, int
 }
 
 // rows of X past the lengths never reach a sum of another row; rows of Y do (0 x NaN), and are zeroed in shared memory
+// CTA y of the `ys` of head hx
 template <class T, int DP, bool BIAS, bool DKV>
-__global__ void __launch_bounds__(kThreads, 1)
-    attn_bwd_kernel(const __grid_constant__ CUtensorMap tmX1, const __grid_constant__ CUtensorMap tmX2,
-                    const __grid_constant__ CUtensorMap tmY1, const __grid_constant__ CUtensorMap tmY2,
-                    const __grid_constant__ Args g) {
+__device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUtensorMap& tmX2, const CUtensorMap& tmY1,
+                                              const CUtensorMap& tmY2, const Args& g, const int hx, const int y_cta, const int y_ctas) {
     using Sh = Shape<DP, BIAS>;
     constexpr int NST = Sh::kStages, NB = buffers<DP, DKV>(), NS = score_bars(NB), NX = Sh::kOwned;
     const AttnArgs& a = g.a;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int hx = blockIdx.x, group = a.H / a.Hkv;
+    const int group = a.H / a.Hkv;
+    const int* const order = DKV ? g.order_k : g.order_q;
+    void *const dx1 = g.dv, *const dx2 = DKV ? g.dk : g.dq;   // (the query pass has one result)
     const int Lx = DKV ? a.Lk : a.Lq, heads = DKV ? a.Hkv : a.H, row_tiles = (Lx + kOwn - 1) / kOwn, items = a.B * row_tiles;
-    const int count = item_count(items, blockIdx.y, gridDim.y);   // of this CTA
+    const int count = item_count(items, y_cta, y_ctas);   // of this CTA
 
-    // The queries pass begins where the keys pass leaves SMs free: that one's CTAs have all begun, and so have waited for the
-    // statistics and the order.  It ends after that one has ended (the wait at its end), for those who read the results.
-    // 1 x 4096 causal, 16/4 heads of 128, whose 128 items of keys leave SMs free: both passes 370 us one after the other, 260 so
-    if (DKV || !g.beside) wait_ahead();
-    if (DKV) let_next();
     extern __shared__ uint8_t raw[];
     const uint32_t r0 = smem_addr(raw), base = (r0 + 1023u) & ~1023u;
     uint8_t* const gb = raw + (base - r0);
@@ -200,7 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
             *dead = 0;
-            const Item w = item_at<DKV>(a, g.order, item_index(0, blockIdx.y, gridDim.y));
+            const Item w = item_at<DKV>(a, order, item_index(0, y_cta, y_ctas));
             if (w.per) {
                 own(0, w.b, w.x0);
                 stream(0, w.b, w.y0, DKV ? hx * group : hx / group);
@@ -211,7 +212,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_alloc(smem_addr(slot), kColumns);
     } else if (warp < kWork / 32) {
         for (int e = tid; e < count; e += kWork) {
-            const Item w = item_at<DKV>(a, g.order, item_index(e, blockIdx.y, gridDim.y));
+            const Item w = item_at<DKV>(a, order, item_index(e, y_cta, y_ctas));
             entry[e] = make_int4(w.b, w.x0, w.lq, w.lk);
             span[e] = make_int2(w.y0, w.per);
         }
@@ -362,9 +363,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int f = 0; f < kCols; f += 16) tmem_tie16(o + f);
             tc_fence_before();
             bar_arrive_warp(barA);   // the next item's products may overwrite them
-            const bool whole = a.D % 16 == 0 && (((uintptr_t)g.dx1 | (uintptr_t)g.dx2) & 31) == 0;
+            const bool whole = a.D % 16 == 0 && (((uintptr_t)dx1 | (uintptr_t)dx2) & 31) == 0;
             if (kept_x < Lx) {
-                T* const rp = (T*)(first ? g.dx1 : g.dx2) + (((size_t)kept_b * Lx + kept_x) * heads + hx) * a.D + f0;
+                T* const rp = (T*)(first ? dx1 : dx2) + (((size_t)kept_b * Lx + kept_x) * heads + hx) * a.D + f0;
 #pragma unroll
                 for (int y = 0; y < kCols; y += 16) {
                     uint32_t p[8];
@@ -400,8 +401,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int rows = min(kOwn, Lx - x0), units = a.D / 8;
                 for (int v = tid; v < rows * units; v += kWork) {
                     const size_t at = (((size_t)b * Lx + x0 + v / units) * heads + hx) * a.D + (v % units) * 8;
-                    *reinterpret_cast<uint4*>((T*)g.dx2 + at) = make_uint4(0, 0, 0, 0);
-                    if (DKV) *reinterpret_cast<uint4*>((T*)g.dx1 + at) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>((T*)dx2 + at) = make_uint4(0, 0, 0, 0);
+                    if (DKV) *reinterpret_cast<uint4*>((T*)dx1 + at) = make_uint4(0, 0, 0, 0);
                 }
                 continue;
             }
@@ -585,14 +586,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                 float v = 0.f;
 #pragma unroll
                 for (int k = 0; k < kWork / 32; ++k) v += red[k * kBuckets + t];
-                g.part[((size_t)hx * nb + t) * gridDim.y + blockIdx.y] = v;
+                g.part[((size_t)hx * nb + t) * y_ctas + y_cta] = v;
             }
         }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == kWork / 32) tmem_free(tmem, kColumns);
-    if (!DKV && blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1) wait_ahead();   // (one CTA is enough, and leaves the others' SMs free)
+}
+
+// Both passes wait for the statistics and the order at their start: what these wrote is theirs to read only after that wait.
+// 1 x 4096 causal, 16/4 heads of 128, whose 128 items of keys leave SMs free: 285 us, 370 as two launches one after the other
+template <class T, int DP, bool BIAS>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_bwd_kernel(const __grid_constant__ Maps own, const __grid_constant__ Maps str, const __grid_constant__ Args g) {
+    wait_ahead();   // (the statistics and the order)
+    const int keys = g.ctas_k * g.a.Hkv;
+    if ((int)blockIdx.x < keys) {
+        attn_bwd_pass<T, DP, BIAS, true>(own.k, own.v, str.q, str.grad, g, blockIdx.x % g.a.Hkv, blockIdx.x / g.a.Hkv, g.ctas_k);
+    } else {
+        const int at = blockIdx.x - keys;
+        attn_bwd_pass<T, DP, BIAS, false>(own.q, own.grad, str.k, str.v, g, at % g.a.H, at / g.a.H, g.ctas_q);
+    }
 }
 
 // -delta = -rowsum(dO O) (times kDown) and kShift - lse in rows padded to whole tiles: 0 and -inf where no key is met.  O with what its
@@ -682,27 +697,20 @@ size_t order_ints(const AttnArgs& a, bool dkv, int sms) {
     return (a.lengths || a.causal) && ctas_of(a, dkv, sms) < items && items <= kMaxOrder ? (size_t)(items + 3) & ~(size_t)3 : 0;
 }
 
-template <class T, int DP, bool BIAS, bool DKV>
-int launch_pass(const Args& g, const CUtensorMap* tm, long long ctas, cudaStream_t st) {
+template <class T, int DP, bool BIAS>
+int launch_passes(const Args& g, const Maps& own, const Maps& str, cudaStream_t st) {
     static DeviceSetup setup;
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
     int rc = device_setup(setup, dev, [] {
-        return (int)cudaFuncSetAttribute(attn_bwd_kernel<T, DP, BIAS, DKV>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem_bytes<DP, BIAS>(DKV, kMaxReach));
+        return (int)cudaFuncSetAttribute(attn_bwd_kernel<T, DP, BIAS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<DP, BIAS>(kMaxReach));
     }, &sms);
     if (rc) return rc;
-    const int reach = BIAS ? reach_of(g.a.edges) : 0;
-    const size_t smem = smem_bytes<DP, BIAS>(DKV, reach);
-    return launch_early(true, attn_bwd_kernel<T, DP, BIAS, DKV>, dim3(DKV ? g.a.Hkv : g.a.H, (unsigned)ctas), kThreads, smem, st, tm[0], tm[1], tm[2],
-                        tm[3], g);
-}
-template <class T, int DP>
-int launch_pass(const Args& g, bool dkv, const CUtensorMap* tm, long long ctas, cudaStream_t st) {
-    if (ctas > 65535) return D2P_ERR_TOO_LARGE;
-    if (g.a.bias) return dkv ? launch_pass<T, DP, true, true>(g, tm, ctas, st) : launch_pass<T, DP, true, false>(g, tm, ctas, st);
-    return dkv ? launch_pass<T, DP, false, true>(g, tm, ctas, st) : launch_pass<T, DP, false, false>(g, tm, ctas, st);
+    const long long ctas = (long long)g.ctas_k * g.a.Hkv + (long long)g.ctas_q * g.a.H;
+    if (ctas > INT_MAX) return D2P_ERR_TOO_LARGE;
+    return launch_early(true, attn_bwd_kernel<T, DP, BIAS>, dim3((unsigned)ctas), kThreads, smem_bytes<DP, BIAS>(BIAS ? reach_of(g.a.edges) : 0), st, own,
+                        str, g);
 }
 
 template <class T>
@@ -731,38 +739,23 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
     if (a.B && (a.Lq || a.Lk)) {
         // maps of the rows there are; an axis without rows is never read
         const long long gs[3] = {(long long)a.Lq * a.H * a.D, (long long)a.H * a.D, a.D};
-        CUtensorMap own[4] = {}, str[4] = {};   // q, dO, k, v
+        Maps own = {}, str = {};
         bool fine = true;
-        if (a.Lq) {
-            for (int w = 0; w < 2; ++w) {
-                CUtensorMap* const m = w ? str : own;
-                fine = fine && rows_map(m, dtype, a.q, a.B, a.Lq, a.H, a.D, a.qs, w ? kStep : kOwn) &&
-                     rows_map(m + 1, dtype, grad, a.B, a.Lq, a.H, a.D, gs, w ? kStep : kOwn);
-            }
-        }
-        if (a.Lk) {
-            for (int w = 0; w < 2; ++w) {
-                CUtensorMap* const m = w ? str : own;
-                fine = fine && rows_map(m + 2, dtype, a.k, a.B, a.Lk, a.Hkv, a.D, a.ks, w ? kStep : kOwn) &&
-                     rows_map(m + 3, dtype, a.v, a.B, a.Lk, a.Hkv, a.D, a.vs, w ? kStep : kOwn);
-            }
+        for (int w = 0; w < 2; ++w) {
+            Maps& m = w ? str : own;
+            const int rows = w ? kStep : kOwn;
+            if (a.Lq)
+                fine = fine && rows_map(&m.q, dtype, a.q, a.B, a.Lq, a.H, a.D, a.qs, rows) && rows_map(&m.grad, dtype, grad, a.B, a.Lq, a.H, a.D, gs, rows);
+            if (a.Lk)
+                fine = fine && rows_map(&m.k, dtype, a.k, a.B, a.Lk, a.Hkv, a.D, a.ks, rows) && rows_map(&m.v, dtype, a.v, a.B, a.Lk, a.Hkv, a.D, a.vs, rows);
         }
         if (!fine) return D2P_ERR_INVALID_ARGUMENT;
-        Args g = {a, lp, dp, Lp, nullptr, nullptr, nullptr, nullptr, 0};
-        if (a.Lk) {
-            g.dx1 = dv, g.dx2 = dk, g.order = order_k;
-            const CUtensorMap tm[4] = {own[2], own[3], str[0], str[1]};
-            const long long n = ctas_of(a, true, sms);
-            rc = a.D <= 64 ? launch_pass<T, 64>(g, true, tm, n, st) : launch_pass<T, 128>(g, true, tm, n, st);
-            if (rc) return rc;
-        }
-        if (a.Lq) {
-            g.dx1 = nullptr, g.dx2 = dq, g.part = dbias ? part : nullptr, g.order = order_q, g.beside = a.Lk > 0;
-            const CUtensorMap tm[4] = {own[0], own[1], str[2], str[3]};
-            const long long n = ctas_of(a, false, sms);
-            rc = a.D <= 64 ? launch_pass<T, 64>(g, false, tm, n, st) : launch_pass<T, 128>(g, false, tm, n, st);
-            if (rc) return rc;
-        }
+        const long long nk = a.Lk ? ctas_of(a, true, sms) : 0, nq = a.Lq ? ctas_of(a, false, sms) : 0;
+        if (nk > INT_MAX || nq > INT_MAX) return D2P_ERR_TOO_LARGE;
+        const Args g = {a, lp, dp, Lp, dv, dk, dq, dbias ? part : nullptr, order_k, order_q, (int)nk, (int)nq};
+        if (a.D <= 64) rc = a.bias ? launch_passes<T, 64, true>(g, own, str, st) : launch_passes<T, 64, false>(g, own, str, st);
+        else rc = a.bias ? launch_passes<T, 128, true>(g, own, str, st) : launch_passes<T, 128, false>(g, own, str, st);
+        if (rc) return rc;
     }
     if (dbias) {
         const int nb = (a.edges.n + 1) << a.edges.two, n = a.B * tiles_of(a.Lq) ? (int)ctas_of(a, false, sms) : 0;
