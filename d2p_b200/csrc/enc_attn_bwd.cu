@@ -27,6 +27,11 @@
 // after the other, in order of their work, and the next one's copies and scores
 // begin while this one's results leave.
 //
+// In fp16 the operand dS is held 2^k times as large, k by problem and key head so that it fits: |dS| is at most 2 |dO| |V|
+// (largest norms of a row), and 2^k of that lies in [2^14, 2^15).  As it is, a small gradient's dS lies
+// among fp16's subnormals, whose spacing then shows in dQ and dK (dO around 2^-16: 7591 of 128000 entries of dQ past what
+// the results' own rounding explains), and a large one's may pass 65504.
+//
 // The bias's gradient sums dS over many rows, and a row's dS sum to nothing: what
 // delta is off by would show there whole where one bucket holds most of a row's
 // weight (1 % of the sum with delta from the plain output).  For it the forward
@@ -68,6 +73,14 @@ __host__ __device__ constexpr int buffers() { return DKV && DP == 128 ? 2 : 3; }
 // before, or the parity would not tell the two apart; with three buffers that takes one for each buffer and pair
 __host__ __device__ constexpr int score_bars(int nb) { return nb == 2 ? 2 : 6; }
 
+// 2^k and 2^-k for what dS is at most; nothing is scaled where that is zero or not finite
+__device__ __forceinline__ float2 ds_scale(float grad_top, float v_top) {
+    const float most = 2.f * grad_top * v_top;
+    if (!(most > 0.f && most < INFINITY)) return make_float2(1.f, 1.f);
+    const int k = min(max(14 - ilogbf(most), -100), 60);
+    return make_float2(ldexpf(1.f, k), ldexpf(1.f, -k));
+}
+
 template <int DP, bool BIAS>
 struct Shape {
     static constexpr int kChunks = DP / 64;
@@ -98,6 +111,7 @@ struct Args {
     int Lp;
     void *dv, *dk, *dq;
     float* part;           // query pass: [H][buckets][CTAs of a head] sums of dS, or null
+    const float *grad_top, *v_top;  // fp16: [B][Hkv] largest norms of dO's (of the heads that share a key head) and V's rows
     const int *order_k, *order_q;   // the passes' items in order of their work, or null
     int ctas_k, ctas_q;    // CTAs of a head (0: no such pass)
 };
@@ -346,12 +360,14 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
         // An item's results are stored after this warp's first tile of the next one, whose work covers the wait for the
         // last products.  keys pass: half of dV's or dK's columns a warpgroup; query pass: a quarter of dQ's.  A row a
         // thread, whole 32-byte sectors
+        constexpr bool kScaled = std::is_same<T, __half>::value;   // (bf16 has fp32's range)
         int kept_b = -1, kept_x = 0, kept_l = 0;   // problem, this thread's row, rows there are
+        float kept_down = 1.f;                     // and 2^-k of its dS
         auto store = [&]() {
             ok = ok && bar_wait_warp(barF, (done - 1) & 1, dead);
             tc_fence_after();
             const bool row = kept_x < kept_l, first = DKV && pair == 0;
-            const float w = first ? Softmax<T>::kDown : a.scale;
+            const float w = first ? Softmax<T>::kDown : kScaled ? a.scale * kept_down : a.scale;
             const int f0 = DKV ? half * (DP / 2) : (warp >> 2) * (DP / 4);
             constexpr int kCols = DKV ? DP / 2 : DP / 4;
             const uint32_t acc = (first ? tA1 : tA2) + trow;
@@ -405,6 +421,12 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                     if (DKV) *reinterpret_cast<uint4*>((T*)dx1 + at) = make_uint4(0, 0, 0, 0);
                 }
                 continue;
+            }
+            float up = 1.f, down = 1.f;
+            if (kScaled) {
+                const size_t at = (size_t)b * a.Hkv + (DKV ? hx : hx / group);
+                const float2 s = ds_scale(g.grad_top[at], g.v_top[at]);
+                up = s.x, down = s.y;
             }
             for (int head = 0; head < (DKV ? group : 1); ++head) {
                 if (BIAS && DKV && group > 1) {   // keys pass: the bias of the group's next head, once every warp is past the one before
@@ -472,10 +494,12 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
 #pragma unroll
                             for (int z = 0; z < 4; ++z) pv[z] = ex2(pv[z]);
                             const Two d0(__uint_as_float(dv[y]), __uint_as_float(dv[y + 1])), d1(__uint_as_float(dv[y + 2]), __uint_as_float(dv[y + 3]));
-                            // (P is 2^kShift times as large here, dS is as it is)
-                            const Two w(Softmax<T>::kDown, Softmax<T>::kDown), E0(E.x, E.y), E1(E.z, E.w);
-                            mul2(Two(pv[0], pv[1]), Softmax<T>::kShift == 0.f ? add2(d0, E0) : fma2(d0, w, E0)).get(gv, gv + 1);
-                            mul2(Two(pv[2], pv[3]), Softmax<T>::kShift == 0.f ? add2(d1, E1) : fma2(d1, w, E1)).get(gv + 2, gv + 3);
+                            // (fp16: P is 2^kShift times as large here, delta that much less, and dS 2^k times as large)
+                            const float w = Softmax<T>::kDown * up;
+                            Two E0(E.x, E.y), E1(E.z, E.w);
+                            if (kScaled) E0 = mul2(E0, Two(up, up)), E1 = mul2(E1, Two(up, up));
+                            mul2(Two(pv[0], pv[1]), kScaled ? fma2(d0, Two(w, w), E0) : add2(d0, E0)).get(gv, gv + 1);
+                            mul2(Two(pv[2], pv[3]), kScaled ? fma2(d1, Two(w, w), E1) : add2(d1, E1)).get(gv + 2, gv + 3);
 #pragma unroll
                             for (int z = 0; z < 4; ++z) {
                                 const int col = y + z;
@@ -552,20 +576,20 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                                 if (t2 < nb) {
                                     const int e0 = max(range[2 * t2] - lo, 0), e1 = min(range[2 * t2 + 1] - lo + 1, 63);
                                     // (narrow ones as they are: a difference carries the rounding of all before it)
-                                    if (e0 < e1) bsum[i] += e1 - e0 <= 2 ? dw[e0] + (e1 - e0 == 2 ? dw[e0 + 1] : 0.f) : pre[e1] - pre[e0];
+                                    if (e0 < e1) bsum[i] += down * (e1 - e0 <= 2 ? dw[e0] + (e1 - e0 == 2 ? dw[e0 + 1] : 0.f) : pre[e1] - pre[e0]);
                                 }
                             }
                             __syncwarp();
                         } else if (lo >= reach) {
-                            far1 += all;
+                            far1 += down * all;
                         } else {
-                            far0 += all;
+                            far0 += down * all;
                         }
                     }
                 }
             }
             if (kept_b >= 0) store();   // (this warp had no tile of the item)
-            kept_b = b, kept_x = x, kept_l = lx;
+            kept_b = b, kept_x = x, kept_l = lx, kept_down = down;
             t0 += per * (DKV ? group : 1), ++done;
         }
         if (kept_b >= 0) store();
@@ -618,9 +642,10 @@ constexpr int kStatRows = 16, kStatHeads = 8;
 template <class T, int LANES>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ AttnArgs a, const T* __restrict__ out, const T* __restrict__ rest,
                                                          const float* __restrict__ lse, const T* __restrict__ grad, int Lp,
-                                                         float* __restrict__ lp, float* __restrict__ dp) {
+                                                         float* __restrict__ lp, float* __restrict__ dp, unsigned* __restrict__ grad_top) {
     let_next();
-    __shared__ float sum[kStatHeads][kStatRows + 1];
+    constexpr bool kScaled = std::is_same<T, __half>::value;
+    __shared__ float sum[kStatHeads][kStatRows + 1], norm[kScaled ? kStatHeads : 1][kStatRows + 1];
     const int lane = threadIdx.x % LANES, i0 = blockIdx.x * kStatRows, h0 = blockIdx.y * kStatHeads, b = blockIdx.z;
     const int heads = min(kStatHeads, a.H - h0);
     int lq, lk;
@@ -629,14 +654,14 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
 #pragma unroll
     for (int k = 0; k < kStatRows * kStatHeads / kStride; ++k) {
         const int row = k * kStride + threadIdx.x / LANES, i = i0 + row / kStatHeads, h = row % kStatHeads;
-        float d = 0.f;
+        float d = 0.f, n = 0.f;
         if (i < lq && h < heads && 8 * lane < a.D) {
             const size_t at = (((size_t)b * a.Lq + i) * a.H + h0 + h) * a.D + 8 * lane;
             float o[8], g[8];
             load8<T>(out + at, o);
             load8<T>(grad + at, g);
 #pragma unroll
-            for (int x = 0; x < 8; ++x) d = fmaf(o[x], g[x], d);
+            for (int x = 0; x < 8; ++x) d = fmaf(o[x], g[x], d), n = fmaf(g[x], g[x], n);
             if (rest) {
                 load8<T>(rest + at, o);
 #pragma unroll
@@ -644,10 +669,20 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
             }
         }
 #pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+        for (int o = LANES / 2; o > 0; o >>= 1) {
+            d += __shfl_xor_sync(0xffffffffu, d, o);
+            if (kScaled) n += __shfl_xor_sync(0xffffffffu, n, o);
+        }
         if (lane == 0) sum[h][row / kStatHeads] = d;
+        if (kScaled && lane == 0) norm[h][row / kStatHeads] = n;
     }
     __syncthreads();
+    if (kScaled && threadIdx.x < heads) {   // (NaN is above every number here)
+        unsigned top = 0;
+#pragma unroll
+        for (int x = 0; x < kStatRows; ++x) top = max(top, __float_as_uint(sqrtf(norm[threadIdx.x][x])));
+        atomicMax(grad_top + (size_t)b * a.Hkv + (h0 + threadIdx.x) / (a.H / a.Hkv), top);
+    }
     const int h = threadIdx.x / kStatRows, i = i0 + threadIdx.x % kStatRows;
     if (h < heads && h < kStatHeads) {
         const size_t at = ((size_t)b * a.H + h0 + h) * Lp + i;
@@ -656,6 +691,32 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
     }
     // (the order is not read here, but by the passes, which wait for this launch alone: one block ends after it)
     if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) wait_ahead();
+}
+
+// the largest norm of V's live rows of each problem and key head, LANES threads a row (fp16)
+template <int LANES>
+__global__ void __launch_bounds__(256) attn_v_top_kernel(const __grid_constant__ AttnArgs a, unsigned* __restrict__ v_top) {
+    const int lane = threadIdx.x % LANES, kh = blockIdx.y, b = blockIdx.z;
+    int lq, lk;
+    problem_lengths(a, b, &lq, &lk);
+    const __half* const v = (const __half*)a.v + b * a.vs[0] + kh * a.vs[2] + 8 * lane;
+    constexpr int kStride = 256 / LANES;
+    unsigned top = 0;
+    for (int j0 = blockIdx.x * kStride; j0 < lk; j0 += gridDim.x * kStride) {
+        const int j = j0 + threadIdx.x / LANES;
+        float n = 0.f;
+        if (j < lk && 8 * lane < a.D) {
+            float x[8];
+            load8<__half>(v + (long long)j * a.vs[1], x);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) n = fmaf(x[i], x[i], n);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+        top = max(top, __float_as_uint(sqrtf(n)));
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0 && top) atomicMax(v_top + (size_t)b * a.Hkv + kh, top);
 }
 
 // dbias[t][h]: one warp each, the CTAs' sums in a fixed order
@@ -691,6 +752,7 @@ long long ctas_of(const AttnArgs& a, bool dkv, int sms) {
 size_t part_floats(const AttnArgs& a, int sms) {
     return ((size_t)((a.edges.n + 1) << a.edges.two) * a.H * ctas_of(a, false, sms) + 3) & ~(size_t)3;
 }
+size_t top_floats(const AttnArgs& a) { return ((size_t)2 * a.B * a.Hkv + 3) & ~(size_t)3; }
 // ints of its items' order, where lengths differ and CTAs take several
 size_t order_ints(const AttnArgs& a, bool dkv, int sms) {
     const long long items = (long long)a.B * tiles_of(dkv ? a.Lk : a.Lq);
@@ -720,11 +782,21 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
     float* const lp = (float*)ws;
     float* const dp = lp + stats_floats(a);
     float* const part = dp + stats_floats(a);
-    int* const order = (int*)(part + (dbias ? part_floats(a, sms) : 0));
+    float* const top = part + (dbias ? part_floats(a, sms) : 0);
+    int* const order = (int*)(top + top_floats(a));
     const size_t ok = order_ints(a, true, sms), oq = order_ints(a, false, sms);
     int* const order_k = ok ? order : nullptr;
     int* const order_q = oq ? order + ok : nullptr;
     int rc = 0;
+    if (std::is_same<T, __half>::value && a.B) {
+        if ((rc = (int)cudaMemsetAsync(top, 0, top_floats(a) * sizeof(float), st))) return rc;
+        if (a.Lk) {
+            const dim3 grid((unsigned)std::min(std::max(8LL * sms / ((long long)a.B * a.Hkv), 1LL), (a.Lk + 31LL) / 32), a.Hkv, a.B);
+            if (a.D <= 64) attn_v_top_kernel<8><<<grid, 256, 0, st>>>(a, (unsigned*)top + (size_t)a.B * a.Hkv);
+            else attn_v_top_kernel<16><<<grid, 256, 0, st>>>(a, (unsigned*)top + (size_t)a.B * a.Hkv);
+            if ((rc = (int)cudaGetLastError())) return rc;
+        }
+    }
     if (ok || oq) {
         attn_order_kernel<<<2, 1024, 0, st>>>(a, order_k, order_q);
         if ((rc = (int)cudaGetLastError())) return rc;
@@ -733,7 +805,7 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
         const dim3 grid(Lp / kStatRows, (a.H + kStatHeads - 1) / kStatHeads, a.B);
         // (beside the order: what it reads was there before that launch)
         rc = launch_early(ok || oq, a.D <= 64 ? attn_stats_kernel<T, 8> : attn_stats_kernel<T, 16>, grid, 256, 0, st, a, (const T*)out, (const T*)rest,
-                          lse, (const T*)grad, Lp, lp, dp);
+                          lse, (const T*)grad, Lp, lp, dp, (unsigned*)top);
         if (rc) return rc;
     }
     if (a.B && (a.Lq || a.Lk)) {
@@ -752,7 +824,7 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
         if (!fine) return D2P_ERR_INVALID_ARGUMENT;
         const long long nk = a.Lk ? ctas_of(a, true, sms) : 0, nq = a.Lq ? ctas_of(a, false, sms) : 0;
         if (nk > INT_MAX || nq > INT_MAX) return D2P_ERR_TOO_LARGE;
-        const Args g = {a, lp, dp, Lp, dv, dk, dq, dbias ? part : nullptr, order_k, order_q, (int)nk, (int)nq};
+        const Args g = {a, lp, dp, Lp, dv, dk, dq, dbias ? part : nullptr, top, top + (size_t)a.B * a.Hkv, order_k, order_q, (int)nk, (int)nq};
         if (a.D <= 64) rc = a.bias ? launch_passes<T, 64, true>(g, own, str, st) : launch_passes<T, 64, false>(g, own, str, st);
         else rc = a.bias ? launch_passes<T, 128, true>(g, own, str, st) : launch_passes<T, 128, false>(g, own, str, st);
         if (rc) return rc;
@@ -775,7 +847,7 @@ int attn_backward_gave_up(unsigned long long* n) { return (int)cudaMemcpyFromSym
 size_t attn_backward_bytes(const AttnArgs& a, bool dbias) {
     int sms = 0;
     if (attn_sms(&sms)) return (size_t)-1;
-    return (2 * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a, sms) : 0) + bwd::order_ints(a, true, sms) +
+    return (2 * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a, sms) : 0) + bwd::top_floats(a) + bwd::order_ints(a, true, sms) +
             bwd::order_ints(a, false, sms)) * sizeof(float);
 }
 int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const void* rest, const float* lse, const void* grad, void* dq,
