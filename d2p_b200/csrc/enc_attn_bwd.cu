@@ -45,8 +45,9 @@
 //
 // The query pass also sums dS by relative position.  Along a diagonal of a
 // warp's 32 x 32 block the sum moves one lane per column (one shuffle each), the
-// 63 sums are scanned, and each lane takes its buckets as differences of the
-// scan: registers only, in a fixed order.
+// 63 sums are scanned within the buckets they belong to, and each lane takes its
+// buckets' last entries, in a fixed order.  (Differences of one scan over all carry
+// the rounding of the buckets before: one of no weight got 2^-20 rather than nothing.)
 #include <limits.h>
 
 #include <algorithm>
@@ -66,6 +67,7 @@ constexpr int kColumns = 512;   // TMEM: buffers of 64 columns of S and 64 of dP
 constexpr int kChunkX = kOwn * 128, kChunkY = kStep * 128;
 constexpr int kBuckets = 2 * (kMaxEdges + 1);
 constexpr int kMaxItems = 64;   // owned tiles a CTA takes at most
+constexpr int kStartWords = (2 * (kMaxReach + kPad) + 1 + 31) / 32 + 2;   // a bit for each position that begins a bucket, read 64 at a time
 
 template <int DP, bool DKV>
 __host__ __device__ constexpr int buffers() { return DKV && DP == 128 ? 2 : 3; }
@@ -95,7 +97,7 @@ struct Shape {
 };
 // after the tiles: the bias by position, then (query pass) the diagonals' stage of each warp and the buckets' ranges
 __host__ __device__ inline size_t extra(bool bias, int reach) {
-    return bias ? 4 * (size_t)(lut_size(reach) + 16 * 144 + 16 * kBuckets + 2 * kBuckets) : 0;
+    return bias ? 4 * (size_t)(lut_size(reach) + 16 * 144 + 16 * kBuckets + 2 * kBuckets + kStartWords) : 0;
 }
 // at least 116 KB: one CTA an SM, since it takes the whole TMEM (no allocation waits)
 template <int DP, bool BIAS>
@@ -177,6 +179,7 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
     float* const diag = lut + lut_size(reach);                        // [16][144] a warp's diagonals, and their scan
     float* const red = diag + 16 * 144;                               // [16][kBuckets]
     int* const range = reinterpret_cast<int*>(red + 16 * kBuckets);   // [kBuckets][2] positions of a bucket
+    uint32_t* const starts = reinterpret_cast<uint32_t*>(range + 2 * kBuckets);   // [kStartWords] bit d + reach + kPad: a bucket begins at d
     const bool sums = !DKV && BIAS && g.part;
 
     auto copy = [&](uint32_t dst, const CUtensorMap* tm, int row, int head, int b, uint32_t bar, int chunk) {
@@ -237,6 +240,14 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                 const int2 v = bucket_range(a.edges, t, 1 << 29);
                 range[2 * t] = v.x, range[2 * t + 1] = v.y;
             }
+        if (sums && warp == 0) {
+            for (int t = lane; t < kStartWords; t += 32) starts[t] = 0u;
+            __syncwarp();
+            for (int t = lane; t < n_buckets(a.edges); t += 32) {
+                const int at = bucket_range(a.edges, t, 1 << 29).x + reach + kPad;
+                if (at >= 0) atomicOr(starts + (at >> 5), 1u << (at & 31));
+            }
+        }
     }
     tc_fence_before();
     __syncthreads();
@@ -556,18 +567,22 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                         if (near) {
                             dw[62 - lane] = run;   // the diagonals still under way; lane 31's is in place
                             __syncwarp();
-                            // the 63 sums (and a zero) scanned: lane l takes 2 l and 2 l + 1
-                            const float s0 = dw[2 * lane], s1 = s0 + (lane < 31 ? dw[2 * lane + 1] : 0.f);
-                            float t = s1;
+                            // the 63 sums (and a zero): lane l takes 2 l and 2 l + 1, and scans from where their buckets begin
+                            const float s0 = dw[2 * lane], s1 = lane < 31 ? dw[2 * lane + 1] : 0.f;
+                            const int at = lo + reach + kPad + (lane < 16 ? 0 : 32);
+                            const uint32_t begin = __funnelshift_r(starts[at >> 5], starts[(at >> 5) + 1], at & 31) >> ((2 * lane) & 31);
+                            const uint32_t from = (__ballot_sync(0xffffffffu, (begin & 3u) != 0) | 1u) & (0xffffffffu >> (31 - lane));
+                            const int first = 31 - __clz(from);   // the lane in which this one's last bucket begins
+                            float t = begin & 2u ? s1 : s0 + s1;
 #pragma unroll
                             for (int o = 1; o < 32; o <<= 1) {
                                 const float u = __shfl_up_sync(0xffffffffu, t, o);
-                                if (lane >= o) t += u;
+                                if (lane - o >= first) t += u;
                             }
-                            // pre[e]: the sum of the diagonals d in [lo, lo + e)
-                            float* const pre = dw + 72;
-                            pre[2 * lane + 1] = t - s1 + s0, pre[2 * lane + 2] = t;
-                            if (lane == 0) pre[0] = 0.f;
+                            const float u = __shfl_up_sync(0xffffffffu, t, 1);
+                            // sum[e]: of the diagonals up to lo + e that lie in its bucket
+                            float* const sum = dw + 72;
+                            sum[2 * lane] = begin & 1u || lane == 0 ? s0 : u + s0, sum[2 * lane + 1] = t;
                             __syncwarp();
                             const int nb = n_buckets(a.edges);
 #pragma unroll
@@ -575,8 +590,7 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                                 const int t2 = lane + 32 * i;
                                 if (t2 < nb) {
                                     const int e0 = max(range[2 * t2] - lo, 0), e1 = min(range[2 * t2 + 1] - lo + 1, 63);
-                                    // (narrow ones as they are: a difference carries the rounding of all before it)
-                                    if (e0 < e1) bsum[i] += down * (e1 - e0 <= 2 ? dw[e0] + (e1 - e0 == 2 ? dw[e0 + 1] : 0.f) : pre[e1] - pre[e0]);
+                                    if (e0 < e1) bsum[i] += down * sum[e1 - 1];
                                 }
                             }
                             __syncwarp();
