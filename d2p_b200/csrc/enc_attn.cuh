@@ -37,6 +37,33 @@ __device__ __forceinline__ float bias_log2(const AttnArgs& a, int bucket, int h)
     return fabsf(b) < INFINITY ? fminf(fmaxf(b, -1e30f), 1e30f) * kLog2e : b;
 }
 
+// positions d of bucket t, clipped to +-far
+__device__ __forceinline__ int2 bucket_range(const Edges& e, int t, int far) {
+    const int side = e.n + 1, u = t < side ? t : t - side;
+    const int lo = u ? e.e[u - 1] : 0, hi = u < e.n ? e.e[u] - 1 : far;
+    if (t >= side) return make_int2(max(lo, 1), min(hi, far));
+    return make_int2(-min(hi, far), !e.two && u == 0 ? far : -lo);
+}
+// A row's scores are formed in fp32 less its base, the largest bias of its keys where that is kLargeBias or more in base 2
+// (else zero): beside a bias of 1e9 the scores, and beside a reference of 1e9 the logarithm of the sum, would be lost, in
+// one kernel here and in another there.  Every kernel takes the same base, and lse is less it too
+constexpr float kLargeBias = 256.f;
+__device__ __forceinline__ bool large_bias(float b) { return fabsf(b) >= kLargeBias && fabsf(b) < INFINITY; }
+// of query position `pos` whose keys are those before `keys`; lane `first` of `lanes` that share the row's buckets
+template <class T>
+__device__ __forceinline__ float row_top(const AttnArgs& a, int h, int pos, int keys, int first = 0, int lanes = 1) {
+    float top = -INFINITY;
+    for (int t = first; t < n_buckets(a.edges); t += lanes) {
+        const int2 r = bucket_range(a.edges, t, 1 << 30);
+        if (r.y >= -pos && r.x < keys - pos) top = fmaxf(top, bias_log2<T>(a, t, h));
+    }
+    return top;
+}
+__device__ __forceinline__ float base_of(float top) { return large_bias(top) ? top : 0.f; }
+// what multiplies a row's scores: a base of 2^56 and more swallows them (in 64 bits too), which leaves its keys equal (the
+// factor leaves a masked -inf what it is)
+__device__ __forceinline__ float score_factor(float base, float c) { return fabsf(base) < 72057594037927936.f ? c : 1e-30f; }
+
 __device__ __forceinline__ void problem_lengths(const AttnArgs& a, int b, int* lq, int* lk) {
     *lq = a.Lq, *lk = a.Lk;
     if (a.lengths) {

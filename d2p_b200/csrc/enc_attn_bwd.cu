@@ -110,6 +110,7 @@ struct Args {
     AttnArgs a;
     const float* lse;      // [B, H, Lp] padded copies, negated: kShift - lse and -delta kDown; -inf and 0 in dead rows
     const float* delta;
+    const float* base;     // of the rows, where there is a bias: 0 in dead rows
     int Lp;
     void *dv, *dk, *dq;
     float* part;           // query pass: [H][buckets][CTAs of a head] sums of dS, or null
@@ -208,6 +209,7 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                     : "memory");
         }
     };
+    bool large = false;   // whether rows of these heads have bases
     if (warp == kWork / 32 + 2) {   // barriers, and the first item's copies before the CTA meets
         if (lane == 0) {
             for (int s = 0; s < NX; ++s) bar_init(barX + 8 * s, 1), bar_init(barXE + 8 * s, 1);
@@ -234,7 +236,9 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
             span[e] = make_int2(w.y0, w.per);
         }
         __syncwarp();
-        if (BIAS && (!DKV || group == 1)) fill_lut<T>(lut, a, hx, reach, warp, kWork / 32);
+        if (BIAS && (!DKV || group == 1)) large = fill_lut<T>(lut, a, hx, reach, warp, kWork / 32);
+        if (BIAS && DKV && group > 1)
+            for (int t = tid; t < group * n_buckets(a.edges); t += kWork) large |= large_bias(bias_log2<T>(a, t / group, hx * group + t % group));
         if (sums)
             for (int t = tid; t < n_buckets(a.edges); t += kWork) {
                 const int2 v = bucket_range(a.edges, t, 1 << 29);
@@ -250,7 +254,7 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
         }
     }
     tc_fence_before();
-    __syncthreads();
+    large = __syncthreads_or(large);
     tc_fence_after();
     const uint32_t tmem = *slot, tA1 = tmem + 128 * NB, tA2 = DKV ? tA1 + DP : tA1;
 
@@ -415,6 +419,9 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                 nl = g.lse[at], nd = g.delta[at];
             }
         };
+        // LARGE: rows have bases.  A loop of its own (in the same one the others took a tenth longer)
+        auto items = [&](auto large_c) {
+        constexpr bool LARGE = decltype(large_c)::value;
         ask(0);
         for (int e = 0; e < count; ++e) {
             const int4 en = entry[e];
@@ -476,8 +483,7 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                         // four columns' entries at lp +- y: the keys pass meets them in falling order
                         const float* const lp = lut_row(lut, reach, d0 + reach + kPad - (DKV ? 3 : 0));
                         const float flat = BIAS && !NEAR ? (lo >= reach ? lut[lut_entries(reach) - 1] : lut[0]) : 0.f;
-                        // (a value that swallows the scores near the diagonal has to do so here, where it is added last)
-                        const float mul = fabsf(flat) < 2147483648.f ? c : 1e-30f;
+                        const float* const bases = LARGE ? g.base + ((size_t)b * a.H + (DKV ? hx * group + head : hx)) * g.Lp + (DKV ? yc : x) : nullptr;
                         uint32_t sv[32], dv[32];
                         tmem_ld32(tS + col0, sv);
                         tmem_ld32(tD + col0, dv);
@@ -493,12 +499,21 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                             float pv[4], gv[4];
                             Two t0(__uint_as_float(sv[y]), __uint_as_float(sv[y + 1])), t1(__uint_as_float(sv[y + 2]), __uint_as_float(sv[y + 3]));
                             const Two L0(L.x, L.y), L1(L.z, L.w);
-                            if (BIAS && NEAR) {
+                            if (LARGE) {
+                                const float4 R = DKV ? *reinterpret_cast<const float4*>(bases + y) : make_float4(*bases, *bases, *bases, *bases);
+                                float4 e = make_float4(flat, flat, flat, flat);
+                                if (NEAR) {
+                                    e = *reinterpret_cast<const float4*>(DKV ? lp - y : lp + y);
+                                    if (DKV) e = make_float4(e.w, e.z, e.y, e.x);
+                                }
+                                t0 = add2(fma2(t0, Two(score_factor(R.x, c), score_factor(R.y, c)), Two(e.x - R.x, e.y - R.y)), L0);
+                                t1 = add2(fma2(t1, Two(score_factor(R.z, c), score_factor(R.w, c)), Two(e.z - R.z, e.w - R.w)), L1);
+                            } else if (BIAS && NEAR) {
                                 const float4 e = *reinterpret_cast<const float4*>(DKV ? lp - y : lp + y);
                                 t0 = add2(fma2(t0, Two(c, c), DKV ? Two(e.w, e.z) : Two(e.x, e.y)), L0);
                                 t1 = add2(fma2(t1, Two(c, c), DKV ? Two(e.y, e.x) : Two(e.z, e.w)), L1);
                             } else {
-                                const Two m(mul, mul), f(flat, flat);
+                                const Two m(c, c), f(flat, flat);
                                 t0 = fma2(t0, m, BIAS ? add2(f, L0) : L0), t1 = fma2(t1, m, BIAS ? add2(f, L1) : L1);
                             }
                             t0.get(pv, pv + 1), t1.get(pv + 2, pv + 3);
@@ -543,11 +558,11 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                         tmem_st16(tD + col0, zero);
                         live_block = false;
                     } else if (BIAS && near) {
-                        if (edge) block(std::true_type{}, std::true_type{});
-                        else block(std::false_type{}, std::true_type{});
+                        if (LARGE || edge) block(std::true_type{}, std::true_type{});
+                        else block(std::integral_constant<bool, LARGE>{}, std::true_type{});
                     } else {
-                        if (edge) block(std::true_type{}, std::false_type{});
-                        else block(std::false_type{}, std::false_type{});
+                        if (LARGE || edge) block(std::true_type{}, std::false_type{});
+                        else block(std::integral_constant<bool, LARGE>{}, std::false_type{});
                     }
                     const int live = ly - yb;
                     if (live < kStep) {   // rows of Y past the length to zero, for the products that sum over them
@@ -606,6 +621,9 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
             kept_b = b, kept_x = x, kept_l = lx, kept_down = down;
             t0 += per * (DKV ? group : 1), ++done;
         }
+        };
+        if (!BIAS || __builtin_expect(!large, 1)) items(std::false_type{});
+        else items(std::integral_constant<bool, BIAS>{});
         if (kept_b >= 0) store();
         if (sums) {   // the CTA's sums, warp by warp in order
             const int nb = n_buckets(a.edges);
@@ -648,7 +666,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// -delta = -rowsum(dO O) (times kDown) and kShift - lse in rows padded to whole tiles: 0 and -inf where no key is met.  O with what its
+// -delta = -rowsum(dO O) (times kDown) and kShift - lse in rows padded to whole tiles: 0 and -inf where no key is met; and the
+// rows' bases, where there is a bias.  O with what its
 // rounding took, where it is there.  A block takes 16
 // positions of up to 8 heads: rows are read as they lie, heads of a position together, and the sums leave by head, 16
 // positions together.  LANES threads a row
@@ -656,7 +675,8 @@ constexpr int kStatRows = 16, kStatHeads = 8;
 template <class T, int LANES>
 __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__ AttnArgs a, const T* __restrict__ out, const T* __restrict__ rest,
                                                          const float* __restrict__ lse, const T* __restrict__ grad, int Lp,
-                                                         float* __restrict__ lp, float* __restrict__ dp, unsigned* __restrict__ grad_top) {
+                                                         float* __restrict__ lp, float* __restrict__ dp, float* __restrict__ bp,
+                                                         unsigned* __restrict__ grad_top) {
     let_next();
     constexpr bool kScaled = std::is_same<T, __half>::value;
     __shared__ float sum[kStatHeads][kStatRows + 1], norm[kScaled ? kStatHeads : 1][kStatRows + 1];
@@ -690,7 +710,10 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
         if (lane == 0) sum[h][row / kStatHeads] = d;
         if (kScaled && lane == 0) norm[h][row / kStatHeads] = n;
     }
-    __syncthreads();
+    bool large = false;
+    if (bp)
+        for (int x = threadIdx.x; x < heads * n_buckets(a.edges); x += 256) large |= large_bias(bias_log2<T>(a, x / heads, h0 + x % heads));
+    large = __syncthreads_or(large);
     if (kScaled && threadIdx.x < heads) {   // (NaN is above every number here)
         unsigned top = 0;
 #pragma unroll
@@ -701,6 +724,10 @@ __global__ void __launch_bounds__(256) attn_stats_kernel(const __grid_constant__
     if (h < heads && h < kStatHeads) {
         const size_t at = ((size_t)b * a.H + h0 + h) * Lp + i;
         dp[at] = -sum[h][threadIdx.x % kStatRows] * Softmax<T>::kDown;
+        if (bp) {
+            const int pos = i + (a.causal ? lk - lq : 0);
+            bp[at] = large && i < lq ? base_of(row_top<T>(a, h0 + h, pos, a.causal ? min(lk, pos + 1) : lk)) : 0.f;
+        }
         lp[at] = i < lq ? Softmax<T>::kShift - lse[((size_t)b * a.H + h0 + h) * a.Lq + i] : -INFINITY;
     }
     // (the order is not read here, but by the passes, which wait for this launch alone: one block ends after it)
@@ -795,7 +822,8 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
     const int Lp = tiles_of(a.Lq) * kOwn;
     float* const lp = (float*)ws;
     float* const dp = lp + stats_floats(a);
-    float* const part = dp + stats_floats(a);
+    float* const bp = a.bias ? dp + stats_floats(a) : nullptr;
+    float* const part = dp + (a.bias ? 2 : 1) * stats_floats(a);
     float* const top = part + (dbias ? part_floats(a, sms) : 0);
     int* const order = (int*)(top + top_floats(a));
     const size_t ok = order_ints(a, true, sms), oq = order_ints(a, false, sms);
@@ -819,7 +847,7 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
         const dim3 grid(Lp / kStatRows, (a.H + kStatHeads - 1) / kStatHeads, a.B);
         // (beside the order: what it reads was there before that launch)
         rc = launch_early(ok || oq, a.D <= 64 ? attn_stats_kernel<T, 8> : attn_stats_kernel<T, 16>, grid, 256, 0, st, a, (const T*)out, (const T*)rest,
-                          lse, (const T*)grad, Lp, lp, dp, (unsigned*)top);
+                          lse, (const T*)grad, Lp, lp, dp, bp, (unsigned*)top);
         if (rc) return rc;
     }
     if (a.B && (a.Lq || a.Lk)) {
@@ -838,7 +866,7 @@ int run(const AttnArgs& a, int dtype, const void* out, const void* rest, const f
         if (!fine) return D2P_ERR_INVALID_ARGUMENT;
         const long long nk = a.Lk ? ctas_of(a, true, sms) : 0, nq = a.Lq ? ctas_of(a, false, sms) : 0;
         if (nk > INT_MAX || nq > INT_MAX) return D2P_ERR_TOO_LARGE;
-        const Args g = {a, lp, dp, Lp, dv, dk, dq, dbias ? part : nullptr, top, top + (size_t)a.B * a.Hkv, order_k, order_q, (int)nk, (int)nq};
+        const Args g = {a, lp, dp, bp, Lp, dv, dk, dq, dbias ? part : nullptr, top, top + (size_t)a.B * a.Hkv, order_k, order_q, (int)nk, (int)nq};
         if (a.D <= 64) rc = a.bias ? launch_passes<T, 64, true>(g, own, str, st) : launch_passes<T, 64, false>(g, own, str, st);
         else rc = a.bias ? launch_passes<T, 128, true>(g, own, str, st) : launch_passes<T, 128, false>(g, own, str, st);
         if (rc) return rc;
@@ -861,7 +889,7 @@ int attn_backward_gave_up(unsigned long long* n) { return (int)cudaMemcpyFromSym
 size_t attn_backward_bytes(const AttnArgs& a, bool dbias) {
     int sms = 0;
     if (attn_sms(&sms)) return (size_t)-1;
-    return (2 * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a, sms) : 0) + bwd::top_floats(a) + bwd::order_ints(a, true, sms) +
+    return ((a.bias ? 3 : 2) * bwd::stats_floats(a) + (dbias ? bwd::part_floats(a, sms) : 0) + bwd::top_floats(a) + bwd::order_ints(a, true, sms) +
             bwd::order_ints(a, false, sms)) * sizeof(float);
 }
 int attn_backward_tiles(const AttnArgs& a, int dtype, const void* out, const void* rest, const float* lse, const void* grad, void* dq,

@@ -23,6 +23,7 @@
 // the fp32 pipes: 366 us, but 424 with the bias).  256 x 512, 8 heads of 64: 222
 // us, with the bias 273: an item's end costs as much as one more tile.
 #include <algorithm>
+#include <type_traits>
 
 #include "enc_tc.cuh"
 
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int per = (n + part.splits - 1) / part.splits, t = min(n, (int)blockIdx.z * per);
         return make_int2(t, min(per, n - t));
     };
+    bool large = false;   // whether rows of this head have bases
     if (warp == 5) {
         if (lane == 0) {
             bar_init(barQ, 1), bar_init(barQE, 1), bar_init(barR, 4);
@@ -144,7 +146,7 @@ __global__ void __launch_bounds__(kThreads, 2)
     } else if (warp == 4) {
         tmem_alloc(smem_addr(slot), kColumns);
     } else {
-        if (BIAS) fill_lut<T>(lut, a, h, reach, warp < 4 ? warp : warp - 2, 6);
+        if (BIAS) large = fill_lut<T>(lut, a, h, reach, warp < 4 ? warp : warp - 2, 6);
         wait_ahead();
         for (int e = warp < 4 ? tid : tid - 64; e < count; e += 192) {
             const Item w = item_at<KT>(a, order, item_index(e, blockIdx.y, gridDim.y), row_tiles);
@@ -153,7 +155,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
     }
     tc_fence_before();
-    __syncthreads();
+    large = __syncthreads_or(large);
     tc_fence_after();
     const uint32_t tmem = *slot, tO = tmem + Sh::kColO;
 
@@ -269,14 +271,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         bool ok = true;
         int tt = 0;   // tiles so far
         const int j0 = SPLIT ? __shfl_sync(0xffffffffu, *from, 0) : 0;
-        // the bias past the last edge on either side, and what multiplies the scores there: it is added last, and one so
-        // large that it swallows the scores near the diagonal, where it is added first, has to do so there too (the
-        // factor leaves a masked -inf what it is)
-        float before = 0.f, after = 0.f, mul_before = c, mul_after = c;
-        if (BIAS) {
-            before = lut[0], after = lut[lut_entries(reach) - 1];
-            mul_before = fabsf(before) < 2147483648.f ? c : 1e-30f, mul_after = fabsf(after) < 2147483648.f ? c : 1e-30f;
-        }
+        float before = 0.f, after = 0.f;   // the bias past the last edge on either side
+        if (BIAS) before = lut[0], after = lut[lut_entries(reach) - 1];
         // An item's rows are finished behind the next one's first maximum, which covers the wait for its last product: O /
         // l, a row a thread, whole 32-byte sectors
         // tile t's product done, by its buffer's barrier: of that one the phase before is always over (S t was formed after
@@ -335,6 +331,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             tc_fence_before();   // the next item's first product overwrites O after this warp's first P of it
             kept = -1;
         };
+        // LARGE: rows have bases.  A loop of its own (in the same one the others took a tenth longer)
+        auto items = [&](auto large_c) {
+        constexpr bool LARGE = decltype(large_c)::value;
         for (int e = 0; e < count; ++e) {
             const int4 en = entry[e];
             // (from one lane for all, so that the branches on them are known to be the warp's)
@@ -342,6 +341,11 @@ __global__ void __launch_bounds__(kThreads, 2)
             const Item w = {en.x, __shfl_sync(0xffffffffu, en.y, 0), en.z, lku, offu, __shfl_sync(0xffffffffu, tiles[e], 0)};
             if (w.tiles == 0) continue;
             const int pos = w.q0 + tid + w.off, lk = w.lk;
+            float rb = 0.f, rc = c;   // this row's base, what multiplies its scores
+            if (LARGE && w.q0 + tid < w.lq) {
+                rb = base_of(row_top<T>(a, h, pos, a.causal ? min(lk, pos + 1) : lk));
+                rc = score_factor(rb, c);
+            }
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < w.tiles && ok; ++j, ++tt) {
                 const int k0 = (j0 + j) * KT, buf = tt % NB;
@@ -374,16 +378,23 @@ __global__ void __launch_bounds__(kThreads, 2)
                     for (int x = 0; x < kBlocks; ++x) {
                         if (2 * x >= kBlocks && half) break;
                         const int lo = dmin + 32 * x;
-                        add[x] = lo >= reach ? after : before, mul[x] = lo >= reach ? mul_after : mul_before;
-                        if (lo < reach && lo + 62 > -reach) {
+                        add[x] = (lo >= reach ? after : before) - rb;
+                        const bool near = lo < reach && lo + 62 > -reach;
+                        if (LARGE && near) {   // (the scores themselves, so that their maximum is one of them and no exponent is above 0)
+#pragma unroll
+                            for (int y = 32 * x; y < 32 * x + 32; ++y) t[y] = fmaf(t[y], rc, lp[y] - rb);
+                        } else if (LARGE) {
+#pragma unroll
+                            for (int y = 32 * x; y < 32 * x + 32; ++y) t[y] = fmaf(t[y], rc, add[x]);
+                        } else if (near) {
 #pragma unroll
                             for (int y = 32 * x; y < 32 * x + 32; y += 4) {
                                 const float4 e = *reinterpret_cast<const float4*>(lp + y);
                                 fma2(Two(t[y], t[y + 1]), Two(c, c), Two(e.x, e.y)).get(t + y, t + y + 1);
                                 fma2(Two(t[y + 2], t[y + 3]), Two(c, c), Two(e.z, e.w)).get(t + y + 2, t + y + 3);
                             }
-                            mul[x] = 1.f, add[x] = 0.f;
                         }
+                        if (LARGE || near) mul[x] = 1.f, add[x] = 0.f;
                     }
                 }
                 if (k0 + KT > lk || (a.causal && k0 + KT - 1 > w.q0 + w.off)) {
@@ -468,6 +479,9 @@ __global__ void __launch_bounds__(kThreads, 2)
             }
             kept = e, kept_m = m, kept_l = l;
         }
+        };
+        if (!BIAS || __builtin_expect(!large, 1)) items(std::false_type{});
+        else items(std::integral_constant<bool, BIAS>{});
         if (kept >= 0) finish();
     }
     tc_fence_before();

@@ -159,11 +159,23 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
 
+    const float c2 = a.scale * kLog2e;
+    float rb[2] = {0.f, 0.f}, rc[2] = {c2, c2};   // the rows' bases, what multiplies their scores
+    if (a.bias) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {   // (a row's four lanes share its buckets)
+            float top = live[w] ? row_top<T>(a, head[w], qi[w] + off, lim[w], t, 4) : -INFINITY;
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            rb[w] = base_of(top), rc[w] = score_factor(rb[w], c2);
+            before[w] -= rb[w], after[w] -= rb[w];
+        }
+    }
+
     float o[DP / 8][4];
 #pragma unroll
     for (int x = 0; x < DP / 8; ++x) o[x][0] = o[x][1] = o[x][2] = o[x][3] = 0.f;
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-    const float c2 = a.scale * kLog2e;
     for (int it = 0; it < n; ++it) {
         asm volatile("cp.async.wait_group %0;" ::"n"(NST - 2) : "memory");
         __syncwarp();
@@ -196,9 +208,9 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
 #pragma unroll
             for (int j = 0; j < kKeys / 4; ++j) {
                 const int key = at + 8 * (j >> 1) + 2 * t + (j & 1);
-                float v = s[j >> 1][2 * w + (j & 1)] * c2;
+                float v = s[j >> 1][2 * w + (j & 1)] * rc[w];
                 if (one) v += flat;
-                else if (live[w]) v += bias_log2<T>(a, bucket_of(a.edges, key - pos), head[w]);
+                else if (live[w]) v += bias_log2<T>(a, bucket_of(a.edges, key - pos), head[w]) - rb[w];
                 p[w][j] = key < lim[w] ? v : -INFINITY;
                 top = fmaxf(top, p[w][j]);
             }

@@ -219,21 +219,17 @@ __device__ __forceinline__ const float* lut_row(const float* lut, int reach, int
     return lut + (at & 3) * lut_pitch(reach) + (at & ~3);
 }
 
-// positions d of bucket t, clipped to +-far
-__device__ __forceinline__ int2 bucket_range(const Edges& e, int t, int far) {
-    const int side = e.n + 1, u = t < side ? t : t - side;
-    const int lo = u ? e.e[u - 1] : 0, hi = u < e.n ? e.e[u] - 1 : far;
-    if (t >= side) return make_int2(max(lo, 1), min(hi, far));
-    return make_int2(-min(hi, far), !e.two && u == 0 ? far : -lo);
-}
 // fills lut for head h by `warps` warps, a bucket each in turn: its value is
-// fetched once, its positions are consecutive
+// fetched once, its positions are consecutive.  Returns whether any is large, so that rows have bases
 template <class T>
-__device__ __forceinline__ void fill_lut(float* lut, const AttnArgs& a, int h, int reach, int warp, int warps) {
+__device__ __forceinline__ bool fill_lut(float* lut, const AttnArgs& a, int h, int reach, int warp, int warps) {
     const int lane = threadIdx.x & 31, nb = n_buckets(a.edges), far = reach + kPad;
     float mine[(kMaxEdges + 1) / 16];
 #pragma unroll
     for (int i = 0; i < (kMaxEdges + 1) / 16; ++i) mine[i] = lane + 32 * i < nb ? bias_log2<T>(a, lane + 32 * i, h) : 0.f;
+    bool large = false;
+#pragma unroll
+    for (int i = 0; i < (kMaxEdges + 1) / 16; ++i) large |= large_bias(mine[i]);
     for (int t = warp; t < nb; t += warps) {
         float v = mine[0];
 #pragma unroll
@@ -245,6 +241,7 @@ __device__ __forceinline__ void fill_lut(float* lut, const AttnArgs& a, int h, i
             for (int k = 0; k < 4; ++k)
                 if (d + far >= k) lut[k * lut_pitch(reach) + d + far - k] = v;
     }
+    return __any_sync(0xffffffffu, large);
 }
 
 // Launches that begin before the one ahead has ended (programmatic): what that one writes is read after the wait, which

@@ -337,7 +337,8 @@ typedef struct {
     float scale; /* positive */
 } d2p_attention_args;
 /* out [B, Lq, H, D] contiguous, the inputs' type.  For the backward pass: lse [B,
- * H, Lq] fp32 or NULL (log2 of the sum of exponentials, +inf in rows with no
+ * H, Lq] fp32 or NULL (log2 of the sum of exponentials, less the largest bias of
+ * the row's keys in base 2 where that is 256 or more in size; +inf in rows with no
  * allowed key), and rest, like out, or NULL: what rounding took from out, for a
  * more exact row sum of grad out; with a bias, out is then also formed from
  * probabilities in twice 16 bits, since the sums of the bias's gradient cancel.
