@@ -1,9 +1,13 @@
 // enc_attn.cu -- the C entry points of attention over a ragged batch: checks of
 // the arguments, and which kernels take them.
+#include <atomic>
+
 #include "enc_attn.cuh"
 
 namespace d2pb {
 namespace enc {
+
+static std::atomic<int> wait_polls{kWaitLimit};
 
 int attn_args(const d2p_attention_args* p, AttnArgs* a) {
     if (!p || p->B < 0 || p->Lq < 0 || p->Lk < 0 || p->H <= 0 || p->Hkv <= 0 || p->H % p->Hkv) return D2P_ERR_INVALID_ARGUMENT;
@@ -34,7 +38,7 @@ int attn_args(const d2p_attention_args* p, AttnArgs* a) {
     if (((uintptr_t)p->lengths & 3) || ((uintptr_t)p->bias & (a->bias_f32 ? 3 : 1))) return D2P_ERR_INVALID_ARGUMENT;
     a->lengths = p->lengths;
     a->B = p->B, a->Lq = p->Lq, a->Lk = p->Lk, a->H = p->H, a->Hkv = p->Hkv, a->D = p->D, a->causal = p->causal != 0;
-    a->scale = p->scale;
+    a->scale = p->scale, a->polls = wait_polls.load(std::memory_order_relaxed);
     return D2P_OK;
 }
 
@@ -167,6 +171,8 @@ int d2p_attention_backward(const d2p_attention_args* p, const void* out, const v
     if (need && (!workspace || workspace_bytes < need)) return D2P_ERR_WORKSPACE_TOO_SMALL;
     return enc::attn_backward_tiles(a, p->dtype, out, rest, lse, grad, dq, dk, dv, dbias, workspace, (cudaStream_t)stream);
 }
+
+int d2p_attention_wait_limit(int polls) { return enc::wait_polls.exchange(polls < 0 ? enc::kWaitLimit : polls); }
 
 int d2p_attention_gave_up(unsigned long long* n) {
     if (!n) return D2P_ERR_INVALID_ARGUMENT;

@@ -24,7 +24,9 @@ struct AttnArgs {
     const int* lengths;
     int B, Lq, Lk, H, Hkv, D, causal;
     float scale;                  // of the natural scores
+    int polls;                    // of a wait before it gives up
 };
+constexpr int kWaitLimit = 1 << 21;
 
 __device__ __forceinline__ int n_buckets(const Edges& e) { return (e.n + 1) << e.two; }
 

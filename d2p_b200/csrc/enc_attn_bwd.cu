@@ -91,7 +91,7 @@ struct Shape {
     static constexpr int kStage = 2 * kY + 1024;                  // keeps the tiles at 1024-byte boundaries
     static constexpr int kOwned = DP == 64 ? 2 : 1;                          // owned tiles in shared memory: the next one's copies early
     static constexpr int kStages = DP == 64 ? 6 : BIAS ? 3 : 4;              // (the bias by position takes up to 35 KB)
-    static constexpr int kBars = 2 * kOwned + 2 + 2 * kStages + 12;
+    static constexpr int kBars = 2 * kOwned + 4 + 2 * kStages + 12;
     static constexpr size_t kTiles = 2 * (size_t)kOwned * kX + (size_t)kStages * kStage;
     static constexpr size_t fixed() { return 1024 + kTiles + kBars * 8 + 32 + kMaxItems * 24; }
 };
@@ -169,10 +169,11 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
     const uint32_t sY = base + 2 * NX * Sh::kX;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(gb + Sh::kTiles);
     const uint32_t barX = smem_addr(bars), barXE = barX + 8 * NX, barF = barXE + 8 * NX, barA = barF + 8, barY = barA + 8,
-                   barE = barY + 8 * NST, barS = barE + 8 * NST, barP = barS + 8 * NS, barPE = barP + 24;
+                   barE = barY + 8 * NST, barS = barE + 8 * NST, barP = barS + 8 * NS, barPE = barP + 24, barD = barPE + 24;   // (D: the products' end, after a wait that gave up)
     uint8_t* const after = gb + (Sh::kTiles + Sh::kBars * 8 + 15) / 16 * 16;
-    volatile int* const dead = reinterpret_cast<volatile int*>(after);
+    const Dead dead = {reinterpret_cast<volatile int*>(after), a.polls};
     uint32_t* const slot = reinterpret_cast<uint32_t*>(after) + 1;
+    int* const asked = reinterpret_cast<int*>(after) + 2;                    // items (with work) and streamed tiles whose copies were issued
     int4* const entry = reinterpret_cast<int4*>(after + 16);                 // b, x0, lq, lk of an item
     int2* const span = reinterpret_cast<int2*>(entry + kMaxItems);           // and y0, per
     float* const lut = reinterpret_cast<float*>(span + kMaxItems);
@@ -213,13 +214,13 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
     if (warp == kWork / 32 + 2) {   // barriers, and the first item's copies before the CTA meets
         if (lane == 0) {
             for (int s = 0; s < NX; ++s) bar_init(barX + 8 * s, 1), bar_init(barXE + 8 * s, 1);
-            bar_init(barF, 1), bar_init(barA, kWork / 32);
+            bar_init(barF, 1), bar_init(barA, kWork / 32), bar_init(barD, 1), bar_init(barD + 8, 1);
             for (int s = 0; s < NST; ++s) bar_init(barY + 8 * s, 1), bar_init(barE + 8 * s, 1);
             for (int s = 0; s < NS; ++s) bar_init(barS + 8 * s, 1);
             for (int s = 0; s < NB; ++s) bar_init(barP + 8 * s, 8), bar_init(barPE + 8 * s, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
-            *dead = 0;
+            *dead.flag = 0;
             const Item w = item_at<DKV>(a, order, item_index(0, y_cta, y_ctas));
             if (w.per) {
                 own(0, w.b, w.x0);
@@ -275,11 +276,7 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                         if (e + t > 0) stream(t, b, y0 + step * kStep, DKV ? hx * group + k : hx / group);
                     }
             }
-            if (!ok || *dead) {   // what is in flight ends (bounded) before the CTA does
-                volatile int none = 0;
-                for (int x = max(0, i - NX); x < i; ++x) bar_wait(barX + 8 * (x % NX), (x / NX) & 1, &none);
-                for (int x = max(0, t - NST); x < t; ++x) bar_wait(barY + 8 * (x % NST), (x / NST) & 1, &none);
-            }
+            asked[0] = i, asked[1] = t;
         }
         __syncwarp();
     } else if (warp >= kWork / 32) {
@@ -358,7 +355,6 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                 if (lead) tc_commit(barF);
                 ++i;
             }
-            if (!ok && lead) atomicAdd(&g_gave_up, 1ull);
         }
         __syncwarp();
     } else {   // P and dS of a tile
@@ -635,7 +631,7 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
 #pragma unroll
             for (int i = 0; i < kBuckets / 32; ++i) {
                 const int t = lane + 32 * i;
-                if (t < nb) red[warp * kBuckets + t] = bsum[i] + (t == a.edges.n ? far0 : 0.f) + (a.edges.two && t == nb - 1 ? far1 : 0.f);
+                if (t < nb) red[warp * kBuckets + t] = !ok ? NAN : bsum[i] + (t == a.edges.n ? far0 : 0.f) + (a.edges.two && t == nb - 1 ? far1 : 0.f);
             }
             asm volatile("bar.sync 1, 512;" ::: "memory");
             for (int t = tid; t < nb; t += kWork) {
@@ -648,6 +644,18 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
     }
     tc_fence_before();
     __syncthreads();
+    if (*dead.flag) {   // a wait gave up: what is in flight ends (bounded) before the CTA does
+        if (warp < kWork / 32) tmem_wait_st();
+        if (warp == kWork / 32 || warp == kWork / 32 + 1) tc_drain(barD + 8 * (warp - kWork / 32));
+        if (warp == kWork / 32 + 2 && lane == 0) {
+            int none = 0;
+            const Dead end = {&none, kWaitLimit};
+            for (int x = max(0, asked[0] - NX); x < asked[0]; ++x) bar_wait(barX + 8 * (x % NX), (x / NX) & 1, end);
+            for (int x = max(0, asked[1] - NST); x < asked[1]; ++x) bar_wait(barY + 8 * (x % NST), (x / NST) & 1, end);
+            atomicAdd(&g_gave_up, 1ull);
+        }
+        __syncthreads();
+    }
     if (warp == kWork / 32) tmem_free(tmem, kColumns);
 }
 

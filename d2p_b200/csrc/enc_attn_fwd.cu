@@ -55,9 +55,9 @@ struct Shape {
     static constexpr int kTile = kChunks * kChunk;                                // Q
     static constexpr int kChunkKV = kKeys * 128, kTileKV = kChunks * kChunkKV;    // a K or V tile
     static constexpr int kStages = 2;                                             // K and V tiles in flight
-    static constexpr int kBars = 3 + 3 * kBuffers + 4 * kStages;
+    static constexpr int kBars = 5 + 3 * kBuffers + 4 * kStages;
     static constexpr size_t kTiles = kTile + 2 * (size_t)kStages * kTileKV;
-    static constexpr size_t smem(int lut) { return 1024 + kTiles + kBars * 8 + 32 + kMaxItems * 20 + (size_t)lut * 4; }
+    static constexpr size_t smem(int lut) { return 1024 + kTiles + kBars * 8 + 48 + kMaxItems * 20 + (size_t)lut * 4; }
 };
 
 // one row tile of a problem: its rows and the key tiles that any of them meets
@@ -100,12 +100,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     // Q there, Q free; S read (S and P apart); of a buffer S there, P there, its product done; K, V there, free
     const uint32_t barQ = smem_addr(bars), barQE = barQ + 8, barR = barQ + 16, barS = barQ + 24,
                    barP = barS + 8 * NB, barPE = barP + 8 * NB, barK = barPE + 8 * NB, barV = barK + 8 * NST,
-                   barKE = barV + 8 * NST, barVE = barKE + 8 * NST;
+                   barKE = barV + 8 * NST, barVE = barKE + 8 * NST, barD = barVE + 8 * NST;   // (D: the products' end, after a wait that gave up)
     uint8_t* const after_bars = gbase + (Sh::kTiles + Sh::kBars * 8 + 15) / 16 * 16;
-    volatile int* const dead = reinterpret_cast<volatile int*>(after_bars);
+    const Dead dead = {reinterpret_cast<volatile int*>(after_bars), a.polls};
     uint32_t* const slot = reinterpret_cast<uint32_t*>(after_bars) + 1;
     int* const from = reinterpret_cast<int*>(after_bars) + 2;                // this split's first key tile
-    int4* const entry = reinterpret_cast<int4*>(after_bars + 16);            // b, q0, lq, lk of an item
+    int* const asked = reinterpret_cast<int*>(after_bars) + 4;               // copies issued: Q, K, V
+    int4* const entry = reinterpret_cast<int4*>(after_bars + 32);            // b, q0, lq, lk of an item
     int* const tiles = reinterpret_cast<int*>(entry + kMaxItems);            // and the key tiles that its rows meet
     float* const lut = reinterpret_cast<float*>(tiles + kMaxItems);
     const int reach = BIAS ? reach_of(a.edges) : 0;
@@ -125,13 +126,13 @@ __global__ void __launch_bounds__(kThreads, 2)
     bool large = false;   // whether rows of this head have bases
     if (warp == 5) {
         if (lane == 0) {
-            bar_init(barQ, 1), bar_init(barQE, 1), bar_init(barR, 4);
+            bar_init(barQ, 1), bar_init(barQE, 1), bar_init(barR, 4), bar_init(barD, 1), bar_init(barD + 8, 1);
             for (int s = 0; s < NB; ++s) bar_init(barS + 8 * s, 1), bar_init(barP + 8 * s, 4), bar_init(barPE + 8 * s, 1);
             for (int s = 0; s < NST; ++s)
                 bar_init(barK + 8 * s, 1), bar_init(barV + 8 * s, 1), bar_init(barKE + 8 * s, 1), bar_init(barVE + 8 * s, 1);
             asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
             fence_async_smem();
-            *dead = 0;
+            *dead.flag = 0;
             wait_ahead();   // (the items' order)
             const Item w = item_at<KT>(a, order, item_index(0, blockIdx.y, gridDim.y), row_tiles);   // the first item's Q and first tile before the CTA meets
             const int2 r = share(w.tiles);
@@ -182,7 +183,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (lane == 0) {
             bool ok = true;
             const int j0 = SPLIT ? *from : 0;
-            int t = 0, q = 0;   // tiles and items asked for
+            int t = 0, q = 0, asked_k = 0, asked_v = 0;   // tiles and items asked for
             for (int i = 0; ok && i < count; ++i) {
                 const int n = tiles[i];
                 if (n == 0) continue;
@@ -194,18 +195,13 @@ __global__ void __launch_bounds__(kThreads, 2)
                     const int s = t % NST;
                     if (t >= NST && !(ok = bar_wait(barKE + 8 * s, (t / NST - 1) & 1, dead))) break;
                     if (i + j > 0) load(sK + s * Sh::kTileKV, &tmK, (j0 + j) * KT, kh, e.x, barK + 8 * s, Sh::kChunkKV);
+                    asked_k = t + 1;
                     if (t >= NST && !(ok = bar_wait(barVE + 8 * s, (t / NST - 1) & 1, dead))) break;
                     if (i + j > 0) load(sV + s * Sh::kTileKV, &tmV, (j0 + j) * KT, kh, e.x, barV + 8 * s, Sh::kChunkKV);
+                    asked_v = t + 1;
                 }
             }
-            if (!ok || *dead) {   // a wait gave up: what is in flight ends (bounded) before the CTA does
-                volatile int none = 0;
-                if (q) bar_wait(barQ, (q - 1) & 1, &none);
-                for (int x = max(t - NST, 0); x < t; ++x) {
-                    bar_wait(barK + 8 * (x % NST), (x / NST) & 1, &none);
-                    bar_wait(barV + 8 * (x % NST), (x / NST) & 1, &none);
-                }
-            }
+            asked[0] = q, asked[1] = asked_k, asked[2] = asked_v;
         }
         __syncwarp();
     } else {
@@ -260,7 +256,6 @@ __global__ void __launch_bounds__(kThreads, 2)
                     if (lead) tc_commit(barPE + 8 * buf), tc_commit(barVE + 8 * s);
                 }
             }
-            if (!ok && lead) atomicAdd(&g_gave_up, 1ull);
         }
         __syncwarp();
     }
@@ -278,10 +273,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         // tile t's product done, by its buffer's barrier: of that one the phase before is always over (S t was formed after
         // it), while a barrier for all products could be two phases behind, which its parity does not tell
         auto product = [&](int t) { return bar_wait_warp(barPE + 8 * (t % NB), (t / NB) & 1, dead); };
-        int kept = -1;
+        int kept = -1, item = 0;   // the item that waits for it, and the one begun
         float kept_m = 0.f, kept_l = 0.f;
         auto finish = [&]() {
-            ok = ok && product(tt - 1);
+            if (!(ok = product(tt - 1))) return;
             tc_fence_after();
             const int4 w = entry[kept];   // b, q0, lq, lk
             const int i = w.y + tid;
@@ -300,12 +295,12 @@ __global__ void __launch_bounds__(kThreads, 2)
                             if (x + y < a.D) *reinterpret_cast<uint4*>(part.o + set * a.D + x + y) = make_uint4(o[y], o[y + 1], o[y + 2], o[y + 3]);
                     }
                 }
-                if (i < a.Lq) part.ml[set] = !ok ? make_float2(0.f, NAN) : some ? make_float2(kept_m, kept_l) : make_float2(-INFINITY, 0.f);
+                if (i < a.Lq) part.ml[set] = some ? make_float2(kept_m, kept_l) : make_float2(-INFINITY, 0.f);
                 tc_fence_before();
                 kept = -1;
                 return;
             }
-            const float s = !ok ? NAN : (some ? 1.f / kept_l : 0.f);
+            const float s = some ? 1.f / kept_l : 0.f;
             const bool whole = a.D % 16 == 0 && (((uintptr_t)out | (uintptr_t)rest) & 31) == 0;
             const size_t at = (((size_t)w.x * a.Lq + i) * a.H + h) * a.D;
 #pragma unroll 1
@@ -318,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                     uint32_t p[8], q[8];
 #pragma unroll
                     for (int z = 0; z < 8; ++z) {
-                        const float u0 = ok ? __uint_as_float(o[2 * z]) * s : s, u1 = ok ? __uint_as_float(o[2 * z + 1]) * s : s;
+                        const float u0 = __uint_as_float(o[2 * z]) * s, u1 = __uint_as_float(o[2 * z + 1]) * s;
                         p[z] = s == 0.f ? 0u : pack2<T>(u0, u1);   // a dead row is zero whatever it held
                         q[z] = KEEP && s != 0.f ? rest2<T>(u0, u1, p[z]) : 0u;
                     }
@@ -334,11 +329,11 @@ __global__ void __launch_bounds__(kThreads, 2)
         // LARGE: rows have bases.  A loop of its own (in the same one the others took a tenth longer)
         auto items = [&](auto large_c) {
         constexpr bool LARGE = decltype(large_c)::value;
-        for (int e = 0; e < count; ++e) {
-            const int4 en = entry[e];
+        for (; item < count; ++item) {
+            const int4 en = entry[item];
             // (from one lane for all, so that the branches on them are known to be the warp's)
             const int lku = __shfl_sync(0xffffffffu, en.w, 0), offu = __shfl_sync(0xffffffffu, a.causal ? en.w - en.z : 0, 0);
-            const Item w = {en.x, __shfl_sync(0xffffffffu, en.y, 0), en.z, lku, offu, __shfl_sync(0xffffffffu, tiles[e], 0)};
+            const Item w = {en.x, __shfl_sync(0xffffffffu, en.y, 0), en.z, lku, offu, __shfl_sync(0xffffffffu, tiles[item], 0)};
             if (w.tiles == 0) continue;
             const int pos = w.q0 + tid + w.off, lk = w.lk;
             float rb = 0.f, rc = c;   // this row's base, what multiplies its scores
@@ -422,6 +417,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                 }
                 const bool rescale = __any_sync(0xffffffffu, raise) && j > 0;
                 if (kept >= 0) finish();   // (the item before)
+                if (!ok) break;
                 // the product before reads P's columns and adds to O
                 if (j > 0 && (Sh::kApart || rescale)) {
                     if (!(ok = product(tt - 1))) break;
@@ -477,15 +473,46 @@ __global__ void __launch_bounds__(kThreads, 2)
                 tc_fence_before();
                 bar_arrive_warp(barP + 8 * buf);
             }
-            kept = e, kept_m = m, kept_l = l;
+            if (!ok) break;
+            kept = item, kept_m = m, kept_l = l;
         }
         };
         if (!BIAS || __builtin_expect(!large, 1)) items(std::false_type{});
         else items(std::integral_constant<bool, BIAS>{});
-        if (kept >= 0) finish();
+        if (ok && kept >= 0) finish();
+        if (!ok) {   // a wait gave up: NaN in this warp's rows of the items from there on
+            for (int e = kept >= 0 ? kept : item; e < count; ++e) {
+                const int4 w = entry[e];
+                const int i = w.y + tid;
+                if (tiles[e] == 0 || i >= a.Lq) continue;
+                if (SPLIT) {
+                    part.ml[part.set(a, w.x, h, blockIdx.z, i)] = make_float2(0.f, NAN);
+                    continue;
+                }
+                const size_t at = (((size_t)w.x * a.Lq + i) * a.H + h) * a.D;
+                for (int x = 0; x < a.D; ++x) {
+                    out[at + x] = from_f<T>(NAN);
+                    if (KEEP) rest[at + x] = from_f<T>(NAN);
+                }
+                if (lse) lse[((size_t)w.x * a.H + h) * a.Lq + i] = NAN;
+            }
+        }
     }
     tc_fence_before();
     __syncthreads();
+    if (*dead.flag) {   // a wait gave up: what is in flight ends (bounded) before the CTA does
+        if (warp < 4) tmem_wait_st();
+        if (warp == 4 || warp == 7) tc_drain(barD + (warp == 7 ? 8 : 0));
+        if (warp == 5 && lane == 0) {
+            int none = 0;
+            const Dead end = {&none, kWaitLimit};
+            if (asked[0]) bar_wait(barQ, (asked[0] - 1) & 1, end);
+            for (int x = max(asked[1] - NST, 0); x < asked[1]; ++x) bar_wait(barK + 8 * (x % NST), (x / NST) & 1, end);
+            for (int x = max(asked[2] - NST, 0); x < asked[2]; ++x) bar_wait(barV + 8 * (x % NST), (x / NST) & 1, end);
+            atomicAdd(&g_gave_up, 1ull);
+        }
+        __syncthreads();
+    }
     if (warp == 4) tmem_free(tmem, kColumns);
 }
 

@@ -14,9 +14,7 @@
 namespace d2pb {
 namespace enc {
 
-static __device__ unsigned long long g_gave_up;   // CTAs one of whose waits gave up (their rows are NaN)
-
-constexpr int kWaitLimit = 1 << 21;   // polls before a wait gives up
+static __device__ unsigned long long g_gave_up;   // CTAs one of whose waits gave up (rows whose results did not come are NaN)
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
@@ -34,10 +32,14 @@ __device__ __forceinline__ void bar_arrive_warp(uint32_t bar) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) bar_arrive(bar);
 }
-// waits for the phase of the given parity; *dead is the CTA's flag that some
-// wait gave up (then every other wait ends as well)
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-    for (int it = 0; it < kWaitLimit; ++it) {
+// the CTA's flag that some wait gave up (then every other wait ends as well), and the polls before one does
+struct Dead {
+    volatile int* flag;
+    int polls;
+};
+// waits for the phase of the given parity
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, const Dead& dead) {
+    for (int it = 0; it < dead.polls; ++it) {
         uint32_t done;
         asm volatile(
             "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
@@ -45,14 +47,14 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
             : "r"(bar), "r"(parity)
             : "memory");
         if (done) return true;
-        if ((it & 255) == 255 && *dead) return false;
+        if ((it & 255) == 255 && *dead.flag) return false;
     }
-    *dead = 1;
+    *dead.flag = 1;
     return false;
 }
 
 // the same for a whole warp, one answer for its lanes
-__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* dead) {
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, const Dead& dead) {
     return __all_sync(0xffffffffu, bar_wait(bar, parity, dead));
 }
 
@@ -85,6 +87,15 @@ __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence:
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// after a wait that gave up, by the warp that issued products (its elected lane): those under way end (bounded) before TMEM is freed
+__device__ __forceinline__ void tc_drain(uint32_t bar) {
+    int none = 0;
+    if (elect_one()) {
+        tc_commit(bar);
+        bar_wait(bar, 0, Dead{&none, kWaitLimit});
+    }
+    __syncwarp();
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

@@ -355,9 +355,13 @@ D2P_API int d2p_attention_backward(const d2p_attention_args* args, const void* o
                                    const void* grad, void* dq, void* dk, void* dv, void* dbias, void* workspace, size_t workspace_bytes,
                                    void* stream);
 /* CTAs of the attention kernels on the current device, since the library was
- * loaded, one of whose bounded waits gave up; the rows such a CTA owns are NaN.
- * Synchronises with the device. */
+ * loaded, one of whose bounded waits gave up.  Rows (of the outputs or of a
+ * gradient) whose results did not come are NaN, and so is a bias's gradient any of
+ * whose sums did not.  Synchronises with the device. */
 D2P_API int d2p_attention_gave_up(unsigned long long* n);
+/* For tests of that path: polls of a wait before it gives up, in calls of this
+ * process from now on (negative: the default).  Returns the former number. */
+D2P_API int d2p_attention_wait_limit(int polls);
 
 /* RMS norms of queries and keys for each head with the position rotation.
  * q [B, L, H, D], k [B, L, Hkv, D] with element strides of batch, position and
