@@ -1216,6 +1216,11 @@ using OptTensor = c10::optional<Tensor>;
 OptTensor opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 Tensor undef(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
 bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+// forward-mode derivatives: the nodes below refuse them, and so does the way past them, which would drop a tangent in silence
+void no_tangents(const char* what, std::initializer_list<Tensor> inputs) {
+    for (const Tensor& t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), what, ": forward-mode derivatives are not implemented");
+}
 // gradients that are not themselves differentiable: with create_graph they carry a node that says so when it is reached
 tensor_list once(tensor_list grads, const tensor_list& from, const char* what) {
     if (!at::GradMode::is_enabled() || std::none_of(from.begin(), from.end(), wants_grad)) return grads;
@@ -1274,6 +1279,7 @@ Tensor attention_autograd(const Tensor& q, const Tensor& k, const Tensor& v, con
                           at::IntArrayRef edges, double scale, bool causal) {
     if (at::GradMode::is_enabled() && (wants_grad(q) || wants_grad(k) || wants_grad(v) || wants_grad(undef(bias))))
         return AttentionFunction::apply(q, k, v, bias, lengths, edges, scale, causal);
+    no_tangents("attention", {q, k, v, undef(bias)});
     at::AutoDispatchBelowADInplaceOrView guard;
     return std::get<0>(call_attention_forward(q, k, v, bias, lengths, edges, scale, causal, false, false));
 }
@@ -1324,6 +1330,7 @@ std::tuple<Tensor, Tensor> qk_norm_rope_autograd(const Tensor& q, const Tensor& 
         auto r = NormRopeFunction::apply(q, k, qw, kw, cos, sin, positions, eps);
         return {r[0], r[1]};
     }
+    no_tangents("qk_norm_rope", {q, k, qw, kw, cos, sin});
     at::AutoDispatchBelowADInplaceOrView guard;
     return call_norm_rope_forward(q, k, qw, kw, cos, sin, positions, eps);
 }
@@ -1360,6 +1367,7 @@ class DropoutFunction : public torch::autograd::Function<DropoutFunction> {
 Tensor dropout_add_autograd(const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset) {
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(undef(residual))))
         return DropoutFunction::apply(x, residual, p, seed, offset);
+    no_tangents("dropout_add", {x, undef(residual)});
     at::AutoDispatchBelowADInplaceOrView guard;
     return call_dropout(x, residual, p, seed, offset);
 }
