@@ -1335,18 +1335,19 @@ std::tuple<Tensor, Tensor> qk_norm_rope_autograd(const Tensor& q, const Tensor& 
     return call_norm_rope_forward(q, k, qw, kw, cos, sin, positions, eps);
 }
 
-Tensor call_dropout(const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset) {
+// (seed and offset stay symbols under tracing: an offset of its own each step is no other graph)
+Tensor call_dropout(const Tensor& x, const OptTensor& residual, double p, const c10::SymInt& seed, const c10::SymInt& offset) {
     static auto op = c10::Dispatcher::singleton()
                          .findSchemaOrThrow("d2p_b200::dropout_add_forward", "")
-                         .typed<Tensor(const Tensor&, const OptTensor&, double, int64_t, int64_t)>();
+                         .typed<Tensor(const Tensor&, const OptTensor&, double, c10::SymInt, c10::SymInt)>();
     return op.call(x, residual, p, seed, offset);
 }
 
-Tensor dropout_add_autograd(const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset);
+Tensor dropout_add_autograd(const Tensor& x, const OptTensor& residual, double p, c10::SymInt seed, c10::SymInt offset);
 
 class DropoutFunction : public torch::autograd::Function<DropoutFunction> {
    public:
-    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset) {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const OptTensor& residual, double p, c10::SymInt seed, c10::SymInt offset) {
         at::AutoDispatchBelowADInplaceOrView guard;
         ctx->saved_data["p"] = p;
         ctx->saved_data["seed"] = seed;
@@ -1358,13 +1359,13 @@ class DropoutFunction : public torch::autograd::Function<DropoutFunction> {
     static tensor_list backward(AutogradContext* ctx, tensor_list grads) {
         Tensor dx;   // (linear in the gradient: the operator itself, differentiable as it is)
         if (ctx->saved_data["dx"].toBool())
-            dx = dropout_add_autograd(grads[0], OptTensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
-                                      ctx->saved_data["offset"].toInt());
+            dx = dropout_add_autograd(grads[0], OptTensor(), ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toSymInt(),
+                                      ctx->saved_data["offset"].toSymInt());
         return {dx, ctx->saved_data["dr"].toBool() ? grads[0] : Tensor(), Tensor(), Tensor(), Tensor()};
     }
 };
 
-Tensor dropout_add_autograd(const Tensor& x, const OptTensor& residual, double p, int64_t seed, int64_t offset) {
+Tensor dropout_add_autograd(const Tensor& x, const OptTensor& residual, double p, c10::SymInt seed, c10::SymInt offset) {
     if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(undef(residual))))
         return DropoutFunction::apply(x, residual, p, seed, offset);
     no_tangents("dropout_add", {x, undef(residual)});
@@ -1382,8 +1383,8 @@ TORCH_LIBRARY_FRAGMENT(d2p_b200, m) {
     m.def("qk_norm_rope(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor)");
     m.def("qk_norm_rope_forward(Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor)");
     m.def("qk_norm_rope_backward(Tensor grad_q, Tensor grad_k, Tensor q, Tensor k, Tensor q_weight, Tensor k_weight, Tensor cos, Tensor sin, Tensor? positions, float eps) -> (Tensor, Tensor, Tensor, Tensor)");
-    m.def("dropout_add(Tensor x, Tensor? residual, float p, int seed, int offset) -> Tensor");
-    m.def("dropout_add_forward(Tensor x, Tensor? residual, float p, int seed, int offset) -> Tensor");
+    m.def("dropout_add(Tensor x, Tensor? residual, float p, SymInt seed, SymInt offset) -> Tensor");
+    m.def("dropout_add_forward(Tensor x, Tensor? residual, float p, SymInt seed, SymInt offset) -> Tensor");
 }
 TORCH_LIBRARY_IMPL(d2p_b200, CUDA, m) {
     m.impl("embed_scores", embed_scores_cuda);

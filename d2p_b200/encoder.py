@@ -162,7 +162,9 @@ def dropout_add(
     for name, value in (("seed", seed), ("offset", offset)):
         if not 0 <= value < 2 ** 63:
             raise ValueError(f"dropout_add: {name} must be in [0, 2^63), got {value}")
-    return _ops_dropout_add(x, residual, float(p), int(seed), int(offset))
+    # (symbols of a trace stay what they are)
+    seed, offset = (v if isinstance(v, torch.SymInt) else int(v) for v in (seed, offset))
+    return _ops_dropout_add(x, residual, float(p), seed, offset)
 
 
 def _attention_forward_fake(q, k, v, bias, lengths, bucket_edges, scale, causal, want_lse, want_rest):
