@@ -1030,6 +1030,7 @@ void attn_fill(Attn& f, const Tensor& q, const Tensor& k, const Tensor& v, const
     a.dtype = enc_dtype(q, "attention", false);
     a.B = checked_dim(q.size(0), "attention batch"), a.Lq = checked_dim(q.size(1), "attention Lq");
     a.Lk = checked_dim(k.size(1), "attention Lk"), a.H = checked_dim(q.size(2), "attention heads");
+    TORCH_CHECK(a.B <= 65535 && a.H <= 65535, "attention: at most 65535 problems and heads a call, got ", a.B, " and ", a.H);
     a.Hkv = (int)k.size(2), a.D = (int)q.size(3);
     a.causal = causal, a.scale = (float)scale;
     f.q = rows16(q), f.k = rows16(k), f.v = rows16(v);

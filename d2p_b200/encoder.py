@@ -21,6 +21,7 @@ _ops_attention = torch.ops.d2p_b200.attention.default
 _ops_qk_norm_rope = torch.ops.d2p_b200.qk_norm_rope.default
 _ops_dropout_add = torch.ops.d2p_b200.dropout_add.default
 
+_MAX_PROBLEMS = 65535   # of a launch's grid
 _MAX_REACH = 1024
 _MAX_SIDE = 64
 
@@ -64,7 +65,7 @@ def attention(
     """softmax(scale q k^T + bias) v over a ragged batch: [B, Lq, H, D], with gradients to q, k, v and bias.
 
     q [B, Lq, H, D], k and v [B, Lk, Hkv, D], bfloat16 or float16, D a multiple of 8 up to 128; H is a multiple
-    of Hkv, query head h reads key head ``h // (H // Hkv)``.  Any strides (rows that are not whole 16-byte units
+    of Hkv, query head h reads key head ``h // (H // Hkv)``; B and H up to 65535.  Any strides (rows that are not whole 16-byte units
     are copied).  ``lengths`` [B, 2] int32: (queries, keys) of each problem, clamped to the padded sizes on the
     device; rows past them are zero, and what q, k, v hold there is never used.  ``causal`` aligns the last query
     with the last key (query i at position i + lk - lq) and masks later keys; a row left without keys is zero.
@@ -78,6 +79,8 @@ def attention(
         raise TypeError("attention: q, k and v must all be bfloat16 or all float16")
     if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2]:
         raise ValueError("attention: the heads of q must be a multiple of those of k and v")
+    if q.shape[0] > _MAX_PROBLEMS or q.shape[2] > _MAX_PROBLEMS:
+        raise ValueError(f"attention: at most {_MAX_PROBLEMS} problems and heads a call, got {q.shape[0]} and {q.shape[2]}")
     if not 8 <= q.shape[3] <= 128 or q.shape[3] % 8:
         raise ValueError(f"attention: the head size must be a multiple of 8, at most 128, got {q.shape[3]}")
     scale = 1.0 / math.sqrt(q.shape[3]) if scale is None else float(scale)

@@ -310,7 +310,8 @@ D2P_API int d2p_embed_grad_scores(const float* marginals, const float* grad_valu
 /* Attention over a ragged batch.  q [B, Lq, H, D], k and v [B, Lk, Hkv, D] with
  * element strides of batch, position and head (the last axis contiguous; base
  * addresses and strides whole 16-byte units), bf16 or fp16; D a multiple of 8,
- * at most 128; H a multiple of Hkv (query head h reads key head h / (H / Hkv)).
+ * at most 128; H a multiple of Hkv (query head h reads key head h / (H / Hkv));
+ * B and H at most 65535, Lq and Lk at most 2^30 (else D2P_ERR_TOO_LARGE).
  * lengths [B, 2] int32 (lq, lk), clamped to [0, Lq] x [0, Lk], or NULL.
  * Query i stands at position i, or i + lk - lq when causal; with d = j - that
  * position, key j is allowed where i < lq, j < lk and (not causal or d <= 0), and
