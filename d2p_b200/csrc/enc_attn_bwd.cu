@@ -352,6 +352,7 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                         if (it + NB == max(n, NB) && lead) tc_commit(barXE + 8 * xs);   // the owned tile's last use
                     }
                 }
+                if (!ok) break;   // (sums without their last products must not pass for whole ones)
                 if (lead) tc_commit(barF);
                 ++i;
             }
