@@ -452,9 +452,11 @@ __device__ __forceinline__ void attn_bwd_pass(const CUtensorMap& tmX1, const CUt
                 for (int step = (pair ^ (t0 + head * per)) & 1; step < per; step += 2) {   // this pair's tiles of the head
                     const int t = t0 + head * per + step, s = t % NST, buf = t % NB, yb = y0 + step * kStep;
                     // (after a wait that gave up a warp still meets its partners at the barriers above)
-                    // (the streamed tile's own barrier: the keys pass reads the row statistics that came with it)
-                    ok = ok && (!DKV || bar_wait_warp(barY + 8 * s, (t / NST) & 1, dead)) &&
-                         bar_wait_warp(barS + 8 * (t % NS), (t / NS) & 1, dead);
+                    // (the streamed tile's own barrier: the keys pass reads the row statistics that came with it.  After the scores',
+                    // which were formed behind it: a pair sees a stage's phases two apart where there are three stages, and the
+                    // parity alone would not tell this one from the last but one)
+                    ok = ok && bar_wait_warp(barS + 8 * (t % NS), (t / NS) & 1, dead) &&
+                         (!DKV || bar_wait_warp(barY + 8 * s, (t / NST) & 1, dead));
                     if (!ok) continue;
                     tc_fence_after();
                     const int col0 = 32 * half, yc = yb + col0;
