@@ -4,7 +4,7 @@
 //   dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K,  dbias = buckets' sums of dS.
 //
 // Two passes in one launch, a CTA taking 128 rows that it owns at a time, so that
-// every sum stays in the CTA's accumulators and no atomics are needed: the key pass
+// every sum stays in the CTA's accumulators and none is atomic: the key pass
 // (DKV) owns 128 keys and streams 64 queries at a time of every head that shares
 // them, the query pass owns 128 queries and streams 64 keys.  The queries pass's
 // CTAs come after the keys pass's in the grid and so take the SMs that these leave
@@ -38,10 +38,14 @@
 // forms O from P in twice 16 bits and keeps what rounding O took.  Without a bias
 // it keeps the latter alone: short rows' dQ and dK are off by a sixth less.
 //
-// Measured: 2 x 4096 causal, 16/4 heads of 128: 441 us, 780 TFLOP/s counted as the
-// gradients' 5 products, 1090 as the 7 taken; 64 x 512, 8 heads of 64: 205 us.  Bound by the products' pipe (two thirds to three
-// quarters busy) and, for heads of 64, by the exponentials and the 16-bit stores of
-// P and dS to TMEM.
+// P and dS in 16 bits are the tensor cores' operands, of the type of the rows they
+// multiply: an entry is off by as much as one of those is; all sums are fp32.
+//
+// Measured: 2 x 4096 causal, 16/4 heads of 128: 463 us (statistics and order 26
+// more), 740 TFLOP/s counted as the gradients' 5 products, 1040 as the 7 taken;
+// 64 x 512, 8 heads of 64: 193 us and 18, in fp16 210 and 30.  No pipe is full: at 1 x 4096 the
+// products' unit is busy 71 % of the time, its tensor pipe 53 (S and dP, 64 columns
+// wide, take both operands from shared memory), the exponentials' 30.
 //
 // The query pass also sums dS by relative position.  Along a diagonal of a
 // warp's 32 x 32 block the sum moves one lane per column (one shuffle each), the

@@ -15,13 +15,17 @@
 // after the other of its head: the copies and scores of the next begin while this
 // one's results leave, and the bias by position is laid out once.
 //
-// Measured: 4 x 4096, 8 heads of 128: 250 us, 1100 TFLOP/s (two thirds of what a
-// large library product reaches), bound by the products' pipe together with the
-// exponentials.  8 x 4096, 8 heads of 64: 387 us, 710 TFLOP/s, with the bias 431:
-// a tile's 128 x 128 exponentials alone take 1024 clocks of the 1650, the rest is
-// the softmax warps' own chain of waits (a quarter of the exponentials moved to
-// the fp32 pipes: 366 us, but 424 with the bias).  256 x 512, 8 heads of 64: 222
-// us, with the bias 273: an item's end costs as much as one more tile.
+// P in 16 bits is the tensor cores' operand, of V's own type: an entry is off by as
+// much as one of V is; l sums what it was rounded from, in fp32.
+//
+// Measured: 4 x 4096, 8 heads of 128: 259 us, 1060 TFLOP/s (two thirds of what a
+// large library product reaches).  No pipe is full there: the products' unit is
+// busy 64 % of the time and its tensor pipe 50 (S takes both operands from shared
+// memory), the exponentials' pipe 50.  8 x 4096, 8 heads of 64: 404 us, 680
+// TFLOP/s, with the bias 447: the softmax warps' own chain of waits (a quarter of
+// the exponentials moved to the fp32 pipes gained 5 % without the bias, nothing
+// with it).  256 x 512, 8 heads of 64: 229 us, with the bias 281: an item's end
+// costs as much as one more tile.
 #include <algorithm>
 #include <type_traits>
 

@@ -12,10 +12,12 @@
 // where there are more splits than a cluster holds, by a second launch; always in
 // a fixed order.
 //
-// Measured: one token, 32 x 16 heads of 64, 4096 keys each: 90 us, 6.0 TB/s of keys
-// and values (0.91 of a copy's rate); 8 x 8 key heads of 128, 8192 keys: 52 us, 5.2
-// TB/s; ragged caches of up to 4096: 73 us, 4.2 TB/s (the last CTAs' share).  One
-// short cache (513 keys): 6 us, latency.
+// P in 16 bits is the operand, as in the tiles' kernel.
+//
+// Measured: one token, 32 x 16 heads of 64, 4096 keys each: 93 us, 5.8 TB/s of keys
+// and values (0.88 of a copy's rate); 8 x 8 key heads of 128, 8192 keys: 53 us, 5.1
+// TB/s; ragged caches of up to 4096 with the bias: 76 us, 4.0 TB/s (the last CTAs'
+// share).  One short cache (513 keys): 7 us, latency.
 #include <cooperative_groups.h>
 
 #include <algorithm>

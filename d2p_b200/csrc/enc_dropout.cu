@@ -8,17 +8,17 @@
 // the word is at least floor(p 2^32).  A dropped element is selected away, not
 // multiplied by zero, so infinities and NaN in dropped places do not reach y.
 //
-// Measured, 131072 x 256 bf16: with a residual 41 us (201 MB: 4.9 TB/s), without 38
-// us.  Bound by the generator's wide multiplies: 33 us of them at their issue rate.
+// Measured, 131072 x 256 bf16: with a residual 42 us (201 MB: 4.8 TB/s), without 39
+// us (134 MB: 3.4 TB/s).  So not the bytes bound it but the generator's arithmetic:
+// the integer pipe is 60 % busy, the multiplies' 54, and issue waits on both.
 #include "enc_common.cuh"
 
 namespace d2pb {
 namespace enc {
 
-// a M in two words.  The widening multiply issues at an eighth of the plain rate
-// on this device, 16 a clock and SM, and is what bounds this kernel; the same
-// product from 16-bit halves on the plain multiply and the logic pipes costs
-// more (three of a block's products that way, when this was tried: 51 us against 46).
+// a M in two words.  The same product from 16-bit halves on the plain multiply and
+// the logic pipes costs more (three of a block's products that way, when this was
+// tried: 51 us against 46).
 template <uint32_t M>
 __device__ __forceinline__ uint2 wide(uint32_t a) {
     const uint64_t p = (uint64_t)a * M;

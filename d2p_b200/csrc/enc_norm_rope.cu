@@ -6,14 +6,15 @@
 // of the token's position (cos, sin: [P, R / 2] fp32 tables), the rest pass.
 // With g the gradient of the rotated row, u = g rotated back, t = u w:
 //   dx = r (t - xh mean(t xh)),  xh = x r,   dw = sum over rows of u xh.
-// Both passes move each element once and recompute r, so they are bound by
-// memory.  A thread holds 16 elements of a row as two 8-element units that are
+// Both passes move each element once and recompute r.  A thread holds 16 elements of a row as two 8-element units that are
 // each other's rotation partners, so the rotation needs no exchange, and D / 16
 // threads (rounded up to a power of two) share the row's sums by shuffles.
 //
-// Measured, 64 x 512 tokens, 8 + 8 heads of 64, bf16: forward 34 us (142 MB: 4.2
+// Measured, 64 x 512 tokens, 8 + 8 heads of 64, bf16: forward 34 us (142 MB: 4.1
 // TB/s), backward 56 us (210 MB: 3.7 TB/s) and 4 us for the weights' sums; a
-// token of 32 sequences 5 us, latency.
+// token of 32 sequences 5 us, latency.  Memory is not full (0.6 of a copy's rate),
+// nor are the issue slots (69 and 63 %): too few rows are asked for ahead, and the
+// forward reads the token's cosines and sines again for every head.
 #include "enc_common.cuh"
 
 namespace d2pb {

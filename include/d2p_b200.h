@@ -350,7 +350,7 @@ D2P_API int d2p_attention_forward(const d2p_attention_args* args, void* out, flo
 /* Gradients of the above with the probabilities recomputed: grad, out [B, Lq, H,
  * D] contiguous, lse and rest (or NULL) from the forward call; dq, dk, dv contiguous in the inputs'
  * type (zero outside the lengths); dbias [num_buckets, H] in bias_dtype, or NULL.
- * Deterministic: no atomics. */
+ * Deterministic. */
 D2P_API size_t d2p_attention_backward_workspace_bytes(const d2p_attention_args* args, int want_dbias);
 D2P_API int d2p_attention_backward(const d2p_attention_args* args, const void* out, const void* rest, const float* lse,
                                    const void* grad, void* dq, void* dk, void* dv, void* dbias, void* workspace, size_t workspace_bytes,
