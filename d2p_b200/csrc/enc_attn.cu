@@ -128,7 +128,7 @@ using namespace d2pb;
 extern "C" {
 
 // few query rows of a key head: tiles of 128 rows would be mostly empty, and read the keys once for each query head.  One
-// token, 32 x 4096 keys, us by tiles / by tokens: 16/16 heads of 64, ragged, 119 / 76; 16 query heads to a key head of 64 124 /
+// token, 32 x 4096 keys, us by tiles / by tokens: 16/16 heads of 64, ragged, 119 / 74; 16 query heads to a key head of 64 124 /
 // 24, of 128 144 / 45; 4 x 16384, 16/1 of 128 83 / 26.  The tokens' operand holds 16 rows: past that tiles it is (17
 // heads to one 124, 32 to one 210)
 static bool few_rows(const enc::AttnArgs& a) { return (long long)a.Lq * (a.H / a.Hkv) <= 16; }

@@ -51,11 +51,11 @@ __device__ __forceinline__ int2 bucket_range(const Edges& e, int t, int far) {
 // one kernel here and in another there.  Every kernel takes the same base, and lse is less it too
 constexpr float kLargeBias = 256.f;
 __device__ __forceinline__ bool large_bias(float b) { return fabsf(b) >= kLargeBias && fabsf(b) < INFINITY; }
-// of query position `pos` whose keys are those before `keys`; lane `first` of `lanes` that share the row's buckets
+// of query position `pos` whose keys are those before `keys`
 template <class T>
-__device__ __forceinline__ float row_top(const AttnArgs& a, int h, int pos, int keys, int first = 0, int lanes = 1) {
+__device__ __forceinline__ float row_top(const AttnArgs& a, int h, int pos, int keys) {
     float top = -INFINITY;
-    for (int t = first; t < n_buckets(a.edges); t += lanes) {
+    for (int t = 0; t < n_buckets(a.edges); ++t) {
         const int2 r = bucket_range(a.edges, t, 1 << 30);
         if (r.y >= -pos && r.x < keys - pos) top = fmaxf(top, bias_log2<T>(a, t, h));
     }

@@ -14,10 +14,11 @@
 //
 // P in 16 bits is the operand, as in the tiles' kernel.
 //
-// Measured: one token, 32 x 16 heads of 64, 4096 keys each: 93 us, 5.8 TB/s of keys
-// and values (0.88 of a copy's rate); 8 x 8 key heads of 128, 8192 keys: 53 us, 5.1
-// TB/s; ragged caches of up to 4096 with the bias: 76 us, 4.0 TB/s (the last CTAs'
-// share).  One short cache (513 keys): 7 us, latency.
+// Measured: one token, 32 x 16 heads of 64, 4096 keys each: 86 us, 6.2 TB/s of keys
+// and values (0.95 of a copy's rate); 8 x 8 key heads of 128, 8192 keys: 48 us, 5.6
+// TB/s; with 32 buckets of bias 98 us, and 74 us over ragged caches of up to 4096
+// (4.1 TB/s: the last CTAs' share).  One short cache (513 keys): 6 us, with the bias
+// 12, latency.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -86,7 +87,7 @@ __device__ __forceinline__ int bucket_of(const Edges& e, int d) {
     return lo + ((e.two && d > 0) ? e.n + 1 : 0);
 }
 
-template <class T, int DP, bool REST>
+template <class T, int DP, bool BIAS, bool REST>
 __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_constant__ AttnArgs a, T* __restrict__ out,
                                                                 float* __restrict__ lse, T* __restrict__ rest, const __grid_constant__ Parts part) {
     using Sh = Shape<DP>;
@@ -95,6 +96,10 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const int split = blockIdx.x, splits = gridDim.x, kh = blockIdx.y, b = blockIdx.z;
     const int G = a.H / a.Hkv, rows = a.Lq * G;
+    // an entry of these heads' bias a thread, asked for ahead of all else: whether any is large, and rows have bases (every
+    // row's own maximum in its place: a short cache 2 us longer)
+    float entry = 0.f;
+    if (BIAS && tid < G * n_buckets(a.edges)) entry = bias_log2<T>(a, tid / G, kh * G + tid % G);
     int lq, lk;
     problem_lengths(a, b, &lq, &lk);
     const int off = a.causal ? lk - lq : 0;
@@ -126,7 +131,7 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
         }
     const int reach = a.edges.n ? a.edges.e[a.edges.n - 1] : 1;
     float before[2] = {0.f, 0.f}, after[2] = {0.f, 0.f};   // the bias past the last edge, on either side
-    if (a.bias) {
+    if (BIAS) {
 #pragma unroll
         for (int w = 0; w < 2; ++w)
             if (live[w]) {
@@ -163,14 +168,16 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
 
     const float c2 = a.scale * kLog2e;
     float rb[2] = {0.f, 0.f}, rc[2] = {c2, c2};   // the rows' bases, what multiplies their scores
-    if (a.bias) {
+    if (BIAS) {
+        bool large = large_bias(entry);
+        for (int x = tid + 32 * kWarps; x < G * n_buckets(a.edges); x += 32 * kWarps) large |= large_bias(bias_log2<T>(a, x / G, kh * G + x % G));
+        if (__builtin_expect(__syncthreads_or(large), 0)) {
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {   // (a row's four lanes share its buckets)
-            float top = live[w] ? row_top<T>(a, head[w], qi[w] + off, lim[w], t, 4) : -INFINITY;
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            rb[w] = base_of(top), rc[w] = score_factor(rb[w], c2);
-            before[w] -= rb[w], after[w] -= rb[w];
+            for (int w = 0; w < 2; ++w) {
+                if (live[w]) rb[w] = base_of(row_top<T>(a, head[w], qi[w] + off, lim[w]));
+                rc[w] = score_factor(rb[w], c2);
+                before[w] -= rb[w], after[w] -= rb[w];
+            }
         }
     }
 
@@ -205,8 +212,8 @@ __global__ void __launch_bounds__(32 * kWarps) attn_token_kernel(const __grid_co
             const int pos = qi[w] + off;
             float top = -INFINITY;
             // past the last edge on one side the bias is one value
-            const bool one = !a.bias || at + kKeys - 1 - pos <= -reach || (a.edges.two && at - pos >= reach);
-            const float flat = !a.bias ? 0.f : at + kKeys - 1 - pos <= -reach ? before[w] : after[w];
+            const bool one = !BIAS || at + kKeys - 1 - pos <= -reach || (a.edges.two && at - pos >= reach);
+            const float flat = !BIAS ? 0.f : at + kKeys - 1 - pos <= -reach ? before[w] : after[w];
 #pragma unroll
             for (int j = 0; j < kKeys / 4; ++j) {
                 const int key = at + 8 * (j >> 1) + 2 * t + (j & 1);
@@ -355,7 +362,7 @@ int parts_of(const AttnArgs& a, int sms) {
     return n > kMaxSplits ? (int)n : 1;
 }
 
-template <class T, int DP, bool REST>
+template <class T, int DP, bool BIAS, bool REST>
 int launch(const AttnArgs& a, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
     using Sh = Shape<DP>;
     constexpr int smem = Sh::kRing > Sh::kJoin ? Sh::kRing : Sh::kJoin;
@@ -364,8 +371,8 @@ int launch(const AttnArgs& a, void* out, float* lse, void* rest, void* ws, cudaS
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return (int)e;
     int rc = device_setup(setup, dev, [] {
-        cudaError_t e = cudaFuncSetAttribute(attn_token_kernel<T, DP, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_token_kernel<T, DP, REST>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        cudaError_t e = cudaFuncSetAttribute(attn_token_kernel<T, DP, BIAS, REST>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(attn_token_kernel<T, DP, BIAS, REST>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         return (int)e;
     }, &sms);
     if (rc) return rc;
@@ -377,17 +384,21 @@ int launch(const AttnArgs& a, void* out, float* lse, void* rest, void* ws, cudaS
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = splits, attr[0].val.clusterDim.y = 1, attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr, cfg.numAttrs = part.splits > 1 ? 0 : 1;
-    e = cudaLaunchKernelEx(&cfg, attn_token_kernel<T, DP, REST>, a, (T*)out, lse, (T*)rest, part);
+    e = cudaLaunchKernelEx(&cfg, attn_token_kernel<T, DP, BIAS, REST>, a, (T*)out, lse, (T*)rest, part);
     if (e != cudaSuccess || part.splits == 1) return (int)e;
     return attn_join(a, std::is_same<T, __half>::value ? D2P_DTYPE_F16 : D2P_DTYPE_BF16, part, out, lse, rest, st);
 }
 
 }  // namespace tok
 
+template <class T, int DP>
+static int pick_token(const AttnArgs& a, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
+    if (a.bias) return rest ? tok::launch<T, DP, true, true>(a, out, lse, rest, ws, st) : tok::launch<T, DP, true, false>(a, out, lse, rest, ws, st);
+    return rest ? tok::launch<T, DP, false, true>(a, out, lse, rest, ws, st) : tok::launch<T, DP, false, false>(a, out, lse, rest, ws, st);
+}
 template <class T>
 static int pick_token(const AttnArgs& a, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
-    if (a.D <= 64) return rest ? tok::launch<T, 64, true>(a, out, lse, rest, ws, st) : tok::launch<T, 64, false>(a, out, lse, rest, ws, st);
-    return rest ? tok::launch<T, 128, true>(a, out, lse, rest, ws, st) : tok::launch<T, 128, false>(a, out, lse, rest, ws, st);
+    return a.D <= 64 ? pick_token<T, 64>(a, out, lse, rest, ws, st) : pick_token<T, 128>(a, out, lse, rest, ws, st);
 }
 int attn_forward_tokens(const AttnArgs& a, int dtype, void* out, float* lse, void* rest, void* ws, cudaStream_t st) {
     return dtype == D2P_DTYPE_BF16 ? pick_token<__nv_bfloat16>(a, out, lse, rest, ws, st) : pick_token<__half>(a, out, lse, rest, ws, st);
