@@ -71,7 +71,8 @@ def attention(
     with the last key (query i at position i + lk - lq) and masks later keys; a row left without keys is zero.
     (A NaN or infinity in a live key's v reaches masked rows of its tile too, as 0 x inf does in the plain product.)
     ``bias`` [num_buckets, H] (q's dtype or float32) adds bias[bucket, h] by relative position
-    (``relative_bucket_edges``; two-sided unless causal).  ``scale`` defaults to 1 / sqrt(D) and must be positive.
+    (``relative_bucket_edges``; two-sided unless causal).  -inf masks a bucket; a row all of whose keys carry one large
+    entry (-1e9) is the softmax of its scores.  ``scale`` defaults to 1 / sqrt(D) and must be positive.
     """
     if q.dim() != 4 or k.dim() != 4 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3]:
         raise ValueError("attention: q must be [B, Lq, H, D] and k, v [B, Lk, Hkv, D]")

@@ -56,3 +56,16 @@ def test_scores_of_their_own_within_a_masked_row(d2p, cuda_device):  # noqa: F81
     val, tol = reference(q, k, v, None, None, False, 0.75, 16, do)
     got = run_attention(d2p, q, k, v, do, flat, None, False, 16, 0.75)
     compare({n: got[n] for n in ("out", "dq", "dk", "dv")}, val, tol)
+
+
+@pytest.mark.parametrize("dtype,causal", [(BF, False), (FP, True)])
+def test_large_biases_on_a_full_device(d2p, cuda_device, dtype, causal):  # noqa: F811
+    """Several items a CTA, uneven lengths, heads with and without large entries."""
+    B, L, H, Hkv, D = 40, 500, 16, 4, 64
+    q, k, v, do, _ = inputs(B, L, L, H, Hkv, D, dtype, cuda_device, seed=3)
+    bias = table((False, -1e9), 8, H, F32, cuda_device)
+    bias[:, 6] = bias[:, 0]
+    bias[:, 9] = torch.finfo(F32).min
+    lengths = torch.tensor([[(b * 37) % (L + 1), (b * 53 + 20) % (L + 1)] for b in range(B)], dtype=torch.int32, device=cuda_device)
+    val, tol = reference(q, k, v, bias, lengths, causal, 0.5, 16, do)
+    compare(run_attention(d2p, q, k, v, do, bias, lengths, causal, 16, 0.5), val, tol)
